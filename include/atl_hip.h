@@ -492,6 +492,57 @@ int atl_tile_trajectories(const float* coef, int64_t sb, int64_t sc, int64_t sy,
 int atl_tile_trajectories_bwd(const float* gout, int64_t B, int64_t K, int64_t Hq, int64_t Wq, const float* times,
                               int64_t nt, int64_t basis, float* gcoef, hipStream_t stream);
 
+/* ---------------------------------------------------------------- sequence operators (no counterpart in the
+ * reference's extension): the layers of a recurrent model over event tokens.  Element types: 0 single precision,
+ * 1 bfloat16, 2 half precision; rows of D channels are contiguous, row strides (s*) count elements and may exceed D
+ * (or be 0).  Sums and states are single precision whatever the types; each output is rounded once. */
+
+/* out (N,D) = scale * table[ids] (table (V,D), row stride st; an id outside [0,V) is no token: zeros).  ids int64 if
+ * wide_ids, else int32. */
+int atl_embed_fwd(const void* ids, int wide_ids, int64_t N, const void* table, int64_t st, int ttype, int64_t V,
+                  int64_t D, double scale, void* out, int otype, hipStream_t stream);
+/* gtable (V,D) written (contiguous, 16-byte aligned): scale * the sum of gout over the tokens of each id, in token
+ * order (no atomic adds: the same bits on every call).  ws: atl_embed_bwd_ws_bytes bytes (-1: sizes unsupported). */
+int64_t atl_embed_bwd_ws_bytes(int64_t N, int64_t V, int64_t D);
+int atl_embed_bwd(const void* ids, int wide_ids, int64_t N, const void* gout, int64_t sgo, int otype, int64_t V,
+                  int64_t D, double scale, void* gtable, int ttype, void* ws, int64_t ws_bytes, hipStream_t stream);
+
+/* s = res + dropout_p(x), rounded to rtype (= dtype or single precision; res null: no residual, rtype = dtype);
+ * y = s / sqrt(mean(s^2) + eps) * w.  y (N,D) and s (N,D) written (s null: not stored).  Dropout keeps an element where
+ * its 16 bits of Philox4x32-10 at counter (row, 2^31 + column / 8, offset) under seed (column c: the low or high half
+ * of word (c % 8) / 2) are >= round(65536 p) and scales it by 1 / (1 - p), p rounded to that multiple of 1 / 65536.
+ * scale not null: y is e4m3, 448 y / a with a = max(max_row |y|, 1e-30), and scale (N) = a / 448.  D <= 8192. */
+int atl_rms_norm_fwd(const void* x, int64_t sx, int dtype, const void* res, int64_t sr, int rtype, const float* w,
+                     int64_t N, int64_t D, double eps, double p, uint64_t seed, uint64_t offset, void* y, void* s,
+                     float* scale, hipStream_t stream);
+/* Its backward from s (row stride ss), gy (dtype; may be null) and gs (rtype; may be null): gx (N,D) dtype, gres (N,D)
+ * rtype and gw (D) written, each unless null.  ws (for gw): atl_rms_norm_bwd_ws_bytes bytes (-1: sizes unsupported). */
+int64_t atl_rms_norm_bwd_ws_bytes(int64_t N, int64_t D);
+int atl_rms_norm_bwd(const void* s, int64_t ss, int rtype, const float* w, const void* gy, int64_t sgy, int dtype,
+                     const void* gs, int64_t sgs, int64_t N, int64_t D, double eps, double p, uint64_t seed,
+                     uint64_t offset, void* gx, void* gres, float* gw, void* ws, int64_t ws_bytes,
+                     hipStream_t stream);
+
+/* h_i = a_i h_{i-1} + w_i x_i with w = sigmoid(gate), a = exp(-dt_i softplus(gate)) (dt null: 1), per channel, within
+ * each window of tokens [start[b], start[b+1]) (start (B+1) ascends from 0 to N; empty windows allowed), from h0 (B,D)
+ * or zero.  y (N,D) = h; last (B,D) = every window's last state (an empty window's: h0 or zero).  states
+ * (atl_gated_scan_groups(N), D): the states the backward starts from, or null.  ws: atl_gated_scan_ws_bytes bytes
+ * (-1: sizes unsupported). */
+int64_t atl_gated_scan_groups(int64_t N);
+int64_t atl_gated_scan_ws_bytes(int64_t N, int64_t D, int dtype);
+int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
+                       const int64_t* start, int64_t B, const float* dt, const float* h0, void* y, float* last,
+                       float* states, void* ws, int64_t ws_bytes, hipStream_t stream);
+/* Its backward: gx, ggate (N,D) and gh0 (B,D; may be null) written, from gy (may be null) and glast (B,D; may be
+ * null). */
+int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
+                       const int64_t* start, int64_t B, const float* dt, const float* h0, const float* states,
+                       const void* gy, int64_t sgy, const float* glast, void* gx, void* ggate, float* gh0, void* ws,
+                       int64_t ws_bytes, hipStream_t stream);
+/* One token of each of N streams: state (N,D) updated in place, y (N,D) = state. */
+int atl_gated_scan_step(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
+                        const float* dt, float* state, void* y, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

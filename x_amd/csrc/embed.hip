@@ -1,0 +1,405 @@
+// Token embedding: out[i] = scale * table[ids[i]], and its gradient gtable[v] = scale * sum of gout[i] over ids[i] = v.
+// An id outside [0, V) is no token (as an event outside the image): its row is zeros and takes no gradient.
+//
+// Forward: one pass, 16 bytes of a row per lane where widths and addresses allow it.
+// Gradient: the tokens are sorted by id (a stable radix sort of (id, position), digits of up to 10 bits), so that the
+// rows of one id are one run and every sum is taken in the order of the tokens: no atomic adds, the same bits on every
+// call however often an id occurs (a hot pixel may own a tenth of a million events).  The sorted positions are cut into
+// equal chunks, so a long run is shared by many lanes: a run inside a chunk is written at once, the partial sums of runs
+// that cross chunks are joined afterwards, in order.  Sums are fp32, each row is rounded once.
+#include "scan.h"
+#include "typed.h"
+#include "../../include/atl_hip.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace atlhip {
+namespace {
+
+struct Rec { uint32_t key, idx; };
+
+__device__ __forceinline__ int64_t id_at(const void* __restrict__ ids, bool wide, int64_t i) {
+  return wide ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+}
+
+template <typename T, typename O, int V>
+__global__ void __launch_bounds__(kBlock) k_embed_fwd(const void* __restrict__ ids, bool wide, int64_t N, int64_t vocab,
+                                                      const T* __restrict__ table, int64_t st, uint32_t units,
+                                                      float scale, O* __restrict__ out, int rows) {
+  const int64_t r0 = (int64_t)blockIdx.x * rows;
+  const uint32_t items = (uint32_t)min((int64_t)rows, N - r0) * units;
+  for (uint32_t e = threadIdx.x; e < items; e += kBlock) {
+    const uint32_t r = e / units, c = (e - r * units) * V;
+    const int64_t id = id_at(ids, wide, r0 + r);
+    float v[V];
+    if (id >= 0 && id < vocab) {
+      load_f<V>(table + id * st + c, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] *= scale;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = 0.f;
+    }
+    store_f<V>(out + (r0 + r) * (int64_t)units * V + c, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- stable radix sort
+constexpr int kSortItems = 16, kSortTile = kBlock * kSortItems, kMaxDigitBits = 10;
+
+// The record at position i: of the first pass from the ids (an id that is no token sorts behind all others).
+template <bool FIRST>
+__device__ __forceinline__ Rec rec_at(const void* __restrict__ src, bool wide, int64_t vocab, int64_t i) {
+  if constexpr (FIRST) {
+    const int64_t id = id_at(src, wide, i);
+    return Rec{(uint32_t)(id >= 0 && id < vocab ? id : vocab), (uint32_t)i};
+  } else {
+    return ((const Rec*)src)[i];
+  }
+}
+
+// cnt (blocks, digits): how often each digit occurs in the block's tile.
+template <bool FIRST>
+__global__ void __launch_bounds__(kBlock) k_sort_count(const void* __restrict__ src, bool wide, int64_t vocab,
+                                                       int64_t N, int shift, int bits, int* __restrict__ cnt) {
+  __shared__ int hist[1 << kMaxDigitBits];
+  const int nd = 1 << bits;
+  for (int d = threadIdx.x; d < nd; d += kBlock) hist[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = base + k * kBlock + threadIdx.x;
+    if (i < N) atomicAdd(&hist[(rec_at<FIRST>(src, wide, vocab, i).key >> shift) & (nd - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < nd; d += kBlock) cnt[(int64_t)blockIdx.x * nd + d] = hist[d];
+}
+
+// off (digits, blocks): where the block's records of a digit go.  Each wave takes a quarter of the tile in rounds of
+// 64; a record's rank among its wave's records of the same digit is that of its lane among the lanes found equal by a
+// ballot per bit, so equal digits keep their order.
+template <bool FIRST>
+__global__ void __launch_bounds__(kBlock) k_sort_scatter(const void* __restrict__ src, bool wide, int64_t vocab,
+                                                         int64_t N, int shift, int bits, const int* __restrict__ off,
+                                                         int nblk, Rec* __restrict__ dst) {
+  constexpr int W = kBlock / kWave;
+  __shared__ int at[W][1 << kMaxDigitBits];
+  const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  for (int d = lane; d < nd; d += kWave) at[w][d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kSortTile + w * (kSortTile / W);
+  Rec rec[kSortItems];
+  int rank[kSortItems];
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = base + k * kWave + lane;
+    const bool live = i < N;
+    rec[k] = live ? rec_at<FIRST>(src, wide, vocab, i) : Rec{0, 0};
+    const int d = (rec[k].key >> shift) & (nd - 1);
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t one = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? one : ~one;
+    }
+    const int before = live ? at[w][d] : 0;
+    rank[k] = before + __popcll(same & below);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // LDS accesses of one wave take effect in order
+    if (live && (same & below) == 0) at[w][d] = before + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < nd; d += kBlock) {
+    int run = off[(int64_t)d * nblk + blockIdx.x];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int n = at[j][d];
+      at[j][d] = run;
+      run += n;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k)
+    if (base + k * kWave + lane < N) dst[at[w][(rec[k].key >> shift) & (nd - 1)] + rank[k]] = rec[k];
+}
+
+// ------------------------------------------------------------------------------------------- sums of the runs
+constexpr int kChunk = 64;            // sorted positions of a group of lanes
+constexpr int kAhead = 8;             // rows in flight
+
+// Zeros, by 16 bytes; p is aligned to them.
+__global__ void __launch_bounds__(kBlock) k_clear(uint16_t* __restrict__ p, int64_t halves) {
+  const int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  if (i + 8 <= halves) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+  else
+    for (int64_t k = i; k < halves; ++k) p[k] = 0;
+}
+
+struct RunGeo {
+  int64_t N, D, sgo, nchunk;
+  uint32_t vocab;
+  int cl2;
+  float scale;
+};
+
+// part (chunks, 2, D): the chunk's sum of a run that began before it, and of one that goes on after it.
+template <typename T, typename O, int V>
+__global__ void __launch_bounds__(kBlock) k_embed_runs(RunGeo g, const Rec* __restrict__ rec, const T* __restrict__ go,
+                                                       O* __restrict__ gt, float* __restrict__ part) {
+  const int64_t chunk = (int64_t)blockIdx.x * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
+  const int64_t c = (((int64_t)blockIdx.y << g.cl2) + (threadIdx.x & ((1 << g.cl2) - 1))) * V;
+  const int64_t p0 = chunk * kChunk, p1 = min(p0 + kChunk, g.N);
+  if (p0 >= g.N || c >= g.D) return;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = 0.f;
+  uint32_t cur = rec[p0].key;
+  bool head = p0 > 0 && rec[p0 - 1].key == cur;
+  auto flush = [&](int slot) {
+    if (slot >= 0) {
+      store_f<V>(part + (chunk * 2 + slot) * g.D + c, acc);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] *= g.scale;
+      store_f<V>(gt + cur * g.D + c, acc);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+  };
+  for (int64_t q = p0; q < p1 && cur < g.vocab; q += kAhead) {
+    Rec r[kAhead];
+    Pack<T, V> v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) r[k] = rec[min(q + k, p1 - 1)];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = load_pack<T, V>(go + (int64_t)r[k].idx * g.sgo + c);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (q + k >= p1 || cur >= g.vocab) break;
+      if (r[k].key != cur) {
+        flush(head ? 0 : -1);
+        head = false;
+        cur = r[k].key;
+        if (cur >= g.vocab) break;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += (float)v[k].e[j];
+    }
+  }
+  if (cur < g.vocab) flush(head ? 0 : p1 < g.N && rec[p1].key == cur ? 1 : -1);
+}
+
+// Joins the partial sums of the runs that cross chunks, each by the group of the chunk where the run begins: its own
+// share, then those of the chunks after it.  Runs of more than kSerial chunks are added up by the whole workgroup, a
+// stretch per group, the stretches joined in order.
+constexpr int kSerial = 16;
+template <typename O, int V>
+__global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __restrict__ rec, O* __restrict__ gt,
+                                                       const float* __restrict__ part) {
+  __shared__ int64_t long_n[kBlock], long_chunk[kBlock];
+  __shared__ float lds[kBlock * V];
+  const int lanes = 1 << g.cl2, G = kBlock >> g.cl2, gi = threadIdx.x >> g.cl2;
+  const int64_t chunk = (int64_t)blockIdx.x * G + gi;
+  const int64_t c = (((int64_t)blockIdx.y << g.cl2) + (threadIdx.x & (lanes - 1))) * V;
+  const bool live = c < g.D;
+  int64_t after = 0;                              // chunks behind this one that share its last run
+  uint32_t key = 0;
+  const int64_t p0 = chunk * kChunk, p1 = p0 + kChunk;
+  if (p1 < g.N) {
+    key = rec[p1 - 1].key;
+    const bool begins = !(p0 > 0 && rec[p0].key == key && rec[p0 - 1].key == key);
+    if (key < g.vocab && rec[p1].key == key && begins) {
+      int64_t lo = chunk + 1, hi = g.nchunk;      // the first chunk in (lo, hi) that begins with another key
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (rec[mid * kChunk].key == key) lo = mid;
+        else hi = mid;
+      }
+      after = hi - chunk - 1;
+    }
+  }
+  if (after > 0 && after <= kSerial && live) {
+    float acc[V];
+    load_f<V>(part + (chunk * 2 + 1) * g.D + c, acc);
+    for (int64_t j = chunk + 1; j <= chunk + after; ++j) {
+      float v[V];
+      load_f<V>(part + j * 2 * g.D + c, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] *= g.scale;
+    store_f<V>(gt + key * g.D + c, acc);
+  }
+  if ((threadIdx.x & (lanes - 1)) == 0) {
+    long_n[gi] = after > kSerial ? after : 0;
+    long_chunk[gi] = chunk;
+  }
+  __syncthreads();
+  for (int run = 0; run < G; ++run) {             // every thread takes the same turns
+    const int64_t n = long_n[run];
+    if (n == 0) continue;
+    const int64_t first = long_chunk[run];
+    const int64_t per = (n + G - 1) / G, j0 = first + 1 + gi * per, j1 = min(j0 + per, first + 1 + n);
+    float acc[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    if (live) {
+      if (gi == 0) load_f<V>(part + (first * 2 + 1) * g.D + c, acc);
+#pragma unroll 8
+      for (int64_t j = j0; j < j1; ++j) {
+        float v[V];
+        load_f<V>(part + j * 2 * g.D + c, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += v[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) lds[threadIdx.x * V + k] = acc[k];
+    __syncthreads();
+    if (gi == 0 && live) {
+      for (int o = 1; o < G; ++o)
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += lds[(o * lanes + threadIdx.x) * V + k];
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] *= g.scale;
+      store_f<V>(gt + (int64_t)rec[first * kChunk + kChunk - 1].key * g.D + c, acc);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------- host
+struct SortPlan {
+  int passes, bits, nblk;
+  int64_t rec_a, rec_b, cnt, off, scan, part, bytes;      // workspace offsets in bytes
+};
+
+SortPlan sort_plan(int64_t N, int64_t D, int64_t vocab) {
+  SortPlan q;
+  int total = 1;
+  while (((int64_t)1 << total) <= vocab) ++total;          // the keys are [0, vocab]
+  q.passes = (total + kMaxDigitBits - 1) / kMaxDigitBits;
+  q.bits = (total + q.passes - 1) / q.passes;
+  q.nblk = (int)((N + kSortTile - 1) / kSortTile);
+  const int64_t n = (int64_t)q.nblk << q.bits;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+  q.rec_a = take(N * 8);
+  q.rec_b = take(N * 8);
+  q.cnt = take(n * 4);
+  q.off = take((n + 1) * 4);
+  q.scan = take((scan_tiles(n) + 1) * 4);
+  q.part = take((N + kChunk - 1) / kChunk * 2 * D * 4);
+  q.bytes = at;
+  return q;
+}
+
+bool embed_ok(int64_t N, int64_t vocab, int64_t D) {
+  return N >= 0 && N < ((int64_t)1 << 31) - kSortTile && vocab >= 1 && vocab < ((int64_t)1 << 31) - 1 && D >= 1 && D <= 65536;
+}
+
+template <typename F>
+void by_one(int t, F&& f) {
+  if (t == kF32) f(float{});
+  else if (t == kBF16) f(bf16_t{});
+  else f(f16_t{});
+}
+
+template <int V, typename F>
+void by_pair(int a, int b, F&& f) {
+  by_one(a, [&](auto x) { by_one(b, [&](auto y) { f(x, y, std::integral_constant<int, V>{}); }); });
+}
+
+// Vectors of 16 bytes of the first type.
+template <typename F>
+void by_pair_vec(int a, int b, F&& f) {
+  by_one(a, [&](auto x) {
+    by_one(b, [&](auto y) { f(x, y, std::integral_constant<int, 16 / (int)sizeof(x)>{}); });
+  });
+}
+
+}  // namespace
+}  // namespace atlhip
+
+using namespace atlhip;
+
+extern "C" {
+
+int atl_embed_fwd(const void* ids, int wide_ids, int64_t N, const void* table, int64_t st, int ttype, int64_t vocab,
+                  int64_t D, double scale, void* out, int otype, hipStream_t stream) {
+  if (!embed_ok(N, vocab, D) || !dtype_ok(ttype) || !dtype_ok(otype) || st < 0) { set_error("embed_fwd: bad sizes N=%lld V=%lld D=%lld types %d, %d", (long long)N, (long long)vocab, (long long)D, ttype, otype); return 1; }
+  if (N == 0) return 0;
+  if (!ids || !table || !out) { set_error("embed_fwd: null argument"); return 1; }
+  const bool vec = D % 8 == 0 && st % 8 == 0 && aligned_to(table, 16) && aligned_to(out, 16);
+  const int V = vec ? 8 : 1;
+  const int64_t units = D / V;
+  // about 2048 pieces a workgroup, fewer where the call is too small to give every compute unit some
+  const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(2048 / units, (N + 1023) / 1024));
+  auto go = [&](auto t, auto o, auto v) {
+    using T = decltype(t);
+    using O = decltype(o);
+    hipLaunchKernelGGL((k_embed_fwd<T, O, decltype(v)::value>), dim3((unsigned)((N + rows - 1) / rows)), dim3(kBlock), 0, stream, ids,
+                       wide_ids != 0, N, vocab, (const T*)table, st, (uint32_t)units, (float)scale, (O*)out, (int)rows);
+  };
+  if (vec) by_pair<8>(ttype, otype, go);
+  else by_pair<1>(ttype, otype, go);
+  return check_launch("embed_fwd");
+}
+
+int64_t atl_embed_bwd_ws_bytes(int64_t N, int64_t vocab, int64_t D) {
+  return embed_ok(N, vocab, D) ? sort_plan(N, D, vocab).bytes : -1;
+}
+
+int atl_embed_bwd(const void* ids, int wide_ids, int64_t N, const void* gout, int64_t sgo, int otype, int64_t vocab,
+                  int64_t D, double scale, void* gtable, int ttype, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  if (!embed_ok(N, vocab, D) || !dtype_ok(ttype) || !dtype_ok(otype) || sgo < 0) { set_error("embed_bwd: bad sizes N=%lld V=%lld D=%lld types %d, %d", (long long)N, (long long)vocab, (long long)D, ttype, otype); return 1; }
+  if (!gtable || (N > 0 && (!ids || !gout || !ws))) { set_error("embed_bwd: null argument"); return 1; }
+  if (!aligned_to(gtable, 16)) { set_error("embed_bwd: gtable must be aligned to 16 bytes"); return 1; }
+  const SortPlan q = sort_plan(N, D, vocab);
+  if (N > 0 && ws_bytes < q.bytes) { set_error("embed_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)q.bytes); return 1; }
+  const int64_t halves = vocab * D * dtype_size(ttype) / 2;
+  if ((halves + kBlock * 8 - 1) / (kBlock * 8) >= ((int64_t)1 << 31)) { set_error("embed_bwd: table too large"); return 1; }
+  hipLaunchKernelGGL(k_clear, dim3(grid_for(halves, kBlock * 8)), dim3(kBlock), 0, stream, (uint16_t*)gtable, halves);
+  if (N == 0) return check_launch("embed_bwd");
+  char* w = (char*)ws;
+  const void* src = ids;
+  Rec* dst = (Rec*)(w + q.rec_a);
+  for (int pass = 0; pass < q.passes; ++pass) {
+    const int shift = pass * q.bits;
+    int* cnt = (int*)(w + q.cnt);
+    int* off = (int*)(w + q.off);
+    if (pass == 0)
+      hipLaunchKernelGGL((k_sort_count<true>), dim3(q.nblk), dim3(kBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits, cnt);
+    else
+      hipLaunchKernelGGL((k_sort_count<false>), dim3(q.nblk), dim3(kBlock), 0, stream, src, false, vocab, N, shift, q.bits, cnt);
+    scan32t(cnt, 1 << q.bits, q.nblk, (int*)(w + q.scan), off, stream);
+    if (pass == 0)
+      hipLaunchKernelGGL((k_sort_scatter<true>), dim3(q.nblk), dim3(kBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits, (const int*)off, q.nblk, dst);
+    else
+      hipLaunchKernelGGL((k_sort_scatter<false>), dim3(q.nblk), dim3(kBlock), 0, stream, src, false, vocab, N, shift, q.bits, (const int*)off, q.nblk, dst);
+    src = dst;
+    dst = dst == (Rec*)(w + q.rec_a) ? (Rec*)(w + q.rec_b) : (Rec*)(w + q.rec_a);
+  }
+  RunGeo g{};
+  g.N = N; g.D = D; g.sgo = sgo; g.vocab = (uint32_t)vocab; g.scale = (float)scale;
+  g.nchunk = (N + kChunk - 1) / kChunk;
+  const bool vec = D % 8 == 0 && sgo % 8 == 0 && aligned_to(gout, 16);
+  const int V = vec ? 16 / dtype_size(otype) : 1;
+  while ((1 << g.cl2) < kWave && ((int64_t)V << g.cl2) < D) ++g.cl2;
+  const dim3 grid((unsigned)((g.nchunk + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2)), (unsigned)((D + ((int64_t)V << g.cl2) - 1) / ((int64_t)V << g.cl2)));
+  auto go = [&](auto o, auto t, auto v) {
+    using T = decltype(o);
+    using O = decltype(t);
+    constexpr int VV = decltype(v)::value;
+    hipLaunchKernelGGL((k_embed_runs<T, O, VV>), grid, dim3(kBlock), 0, stream, g, (const Rec*)src, (const T*)gout, (O*)gtable, (float*)(w + q.part));
+    hipLaunchKernelGGL((k_embed_join<O, VV>), grid, dim3(kBlock), 0, stream, g, (const Rec*)src, (O*)gtable, (const float*)(w + q.part));
+  };
+  if (vec) by_pair_vec(otype, ttype, go);
+  else by_pair<1>(otype, ttype, go);
+  return check_launch("embed_bwd");
+}
+
+}  // extern "C"

@@ -6,6 +6,7 @@
 // weights are bit-identical to the reference's fp32 arithmetic.  Outputs that accumulate (splatted images,
 // image gradients, grid gradients) are accumulated into caller-zeroed buffers with hardware float atomics.
 #include "common.h"
+#include "philox.h"
 #include "scan.h"
 #include "bilinear.h"
 #include "traj.h"
@@ -1167,26 +1168,6 @@ __global__ void __launch_bounds__(kBlock) k_traj_gout(const float2* __restrict__
 bool dims_ok(int64_t H, int64_t W) { return H > 0 && W > 0 && H * W < (int64_t)1 << 31; }
 
 // ------------------------------------------------------------------------------------------- event noise
-// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011): a
-// counter-based generator, so every event draws its own four words from (its index, the call's offset) under
-// the seed, in any order and without state.
-struct U4 {
-  uint32_t x, y, z, w;
-};
-
-__device__ __forceinline__ U4 philox4x32_10(U4 c, uint32_t k0, uint32_t k1) {
-  constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u, kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(kM0, c.x), lo0 = kM0 * c.x;
-    const uint32_t hi1 = __umulhi(kM1, c.z), lo1 = kM1 * c.z;
-    c = U4{hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0};
-    k0 += kW0;
-    k1 += kW1;
-  }
-  return c;
-}
-
 // Dequantisation and anchor smoothing noise of the anchored score (atl/objectives/ats.py:79-84 draws them with
 // torch.rand / torch.randn): xs = xy + U(-1/2, 1/2)^2 if dequantize, else xy; xa = xs + h N(0, 1)^2 (Box-Muller
 // on the other two words) if xa is given.  One pass over the events instead of two fills and two adds.

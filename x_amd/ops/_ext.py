@@ -126,6 +126,17 @@ _SIGS = {
     "atl_warp_splat_gather_ws_bytes": [_I, _I, _I, _I, _I, _I],
     "atl_warp_splat_gather_fwd": [_P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _D, _I, _P, _P, _P, _I, _P],
     "atl_warp_splat_gather_bwd": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _D, _P, _P, _I, _P],
+    "atl_embed_fwd": [_P, _C, _I, _P, _I, _C, _I, _I, _D, _P, _C, _P],
+    "atl_embed_bwd": [_P, _C, _I, _P, _I, _C, _I, _I, _D, _P, _C, _P, _I, _P],
+    "atl_embed_bwd_ws_bytes": [_I, _I, _I],
+    "atl_rms_norm_fwd": [_P, _I, _C, _P, _I, _C, _P, _I, _I, _D, _D, ctypes.c_uint64, ctypes.c_uint64, _P, _P, _P, _P],
+    "atl_rms_norm_bwd": [_P, _I, _C, _P, _P, _I, _C, _P, _I, _I, _I, _D, _D, ctypes.c_uint64, ctypes.c_uint64, _P, _P, _P, _P, _I, _P],
+    "atl_rms_norm_bwd_ws_bytes": [_I, _I],
+    "atl_gated_scan_fwd": [_P, _I, _P, _I, _C, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P],
+    "atl_gated_scan_bwd": [_P, _I, _P, _I, _C, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P],
+    "atl_gated_scan_step": [_P, _I, _P, _I, _C, _I, _I, _P, _P, _P, _P],
+    "atl_gated_scan_groups": [_I],
+    "atl_gated_scan_ws_bytes": [_I, _I, _C],
 }
 _RESTYPE = {"atl_scan_work_size": ctypes.c_int64, "atl_grid_plan_bytes": ctypes.c_int64,
             "atl_tile_ws_bytes": ctypes.c_int64, "atl_splat_gauss_ws_bytes": ctypes.c_int64,
@@ -133,7 +144,9 @@ _RESTYPE = {"atl_scan_work_size": ctypes.c_int64, "atl_grid_plan_bytes": ctypes.
             "atl_voxel_ws_bytes": ctypes.c_int64, "atl_warp_splat_gather_ws_bytes": ctypes.c_int64,
             "atl_ats_pair_ws_bytes": ctypes.c_int64, "atl_ats_pair_bwd_ws_bytes": ctypes.c_int64, "atl_traj_field_bwd_bytes": ctypes.c_int64,
             "atl_sample_grid_bwd_rows_bytes": ctypes.c_int64, "atl_plan_sort_bytes": ctypes.c_int64,
-            "atl_image_variance_ws_bytes": ctypes.c_int64,
+            "atl_image_variance_ws_bytes": ctypes.c_int64, "atl_embed_bwd_ws_bytes": ctypes.c_int64,
+            "atl_rms_norm_bwd_ws_bytes": ctypes.c_int64, "atl_gated_scan_groups": ctypes.c_int64,
+            "atl_gated_scan_ws_bytes": ctypes.c_int64,
 "atl_last_error": ctypes.c_char_p, "atl_abi_version": ctypes.c_int}
 
 class FastGeometry(ctypes.Structure):

@@ -10,6 +10,7 @@ vectorised over a small stacked axis (the four bilinear corners, the (2R+1)^2 Ga
 * brute-force anchored leave-one-out Gaussian sums, O(M N) in anchor chunks         (reference.py:58-71)
 * trilinear polarity voxel grid                                                     (reference.py:74-86)
 * the trajectory pair sums (slice-linearised transport), O(M N)                     (no counterpart)
+* the sequence operators (embedding, residual norm, gated recurrence)              (no counterpart)
 """
 from __future__ import annotations
 
@@ -136,3 +137,84 @@ def voxel_grid(pos, t, p, b, B, C, H, W):
         flat = ((b[:, None] * C + tbl) * H + row) * W + col
         vox = vox.index_add(0, flat[ok], ((p * wt)[:, None] * cw)[ok])
     return vox.view(B, C, H, W)
+
+
+# ------------------------------------------------------------------------------------------- sequence operators
+def _wide(t):
+    """In the precision sums are kept in: float32, or the tensor's own if that is wider."""
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def embed_tokens(ids, table, scale, dtype):
+    token = (ids >= 0) & (ids < table.shape[0])
+    rows = torch.where(token.unsqueeze(-1), _wide(table)[torch.where(token, ids, 0).long()], 0.0)
+    return (rows * scale).to(dtype)
+
+
+def philox4x32_10(counter, seed):
+    """The four words (int64 tensors) of Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC 2011) at a counter of four int64
+    tensors of 32-bit values."""
+    low = 0xFFFFFFFF
+    a, b, c, d = counter
+    k0, k1 = seed & low, seed >> 32
+    for _ in range(10):
+        pa, pc = a * 0xD2511F53, c * 0xCD9E8D57
+        a, b, c, d = (pc >> 32 & low) ^ b ^ k0, pc & low, (pa >> 32 & low) ^ d ^ k1, pa & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    return a, b, c, d
+
+
+def dropout_keeps(rows, D, p, seed, offset, device="cpu"):
+    """(rows, D) truth values: where residual_rms_norm's dropout keeps an element."""
+    row = torch.arange(rows, device=device)[:, None].expand(rows, (D + 7) // 8)
+    group = torch.arange((D + 7) // 8, device=device) + 2 ** 31
+    words = philox4x32_10((row, group.expand_as(row), torch.full_like(row, offset & 0xFFFFFFFF),
+                           torch.full_like(row, offset >> 32)), seed)
+    bits = torch.stack([half for w in words for half in (w & 0xFFFF, w >> 16)], -1)
+    return bits.reshape(rows, -1)[:, :D] >= round(65536 * p)
+
+
+def residual_rms_norm(x, residual, weight, eps, p, seed, offset):
+    v = _wide(x)
+    if p > 0:
+        D = x.shape[-1]
+        keeps = dropout_keeps(x.numel() // D, D, p, seed, offset, x.device).view(x.shape)
+        v = torch.where(keeps, v * (65536.0 / (65536 - round(65536 * p))), 0.0)
+    s = (v if residual is None else _wide(residual) + v).to((x if residual is None else residual).dtype)
+    f = _wide(s)
+    y = f * torch.rsqrt(f.square().mean(-1, keepdim=True) + eps) * _wide(weight)
+    return y.to(x.dtype), s
+
+
+def residual_rms_norm_fp8(x, residual, weight, eps):
+    s = x if residual is None else (_wide(residual) + _wide(x)).to(residual.dtype)
+    f = _wide(s)
+    y = f * torch.rsqrt(f.square().mean(-1, keepdim=True) + eps) * _wide(weight)
+    top = y.abs().amax(-1, keepdim=True).clamp(min=1e-30)
+    return (y * (448.0 / top)).to(torch.float8_e4m3fn), (top / 448.0).float(), s
+
+
+def gated_scan(x, gate, start, dt, h0):
+    """Token by token from the definition, the windows side by side: step k takes the k-th token of every window."""
+    v, g = _wide(x), _wide(gate)
+    decay = torch.exp(-torch.logaddexp(g, torch.zeros_like(g)) * (1.0 if dt is None else dt[:, None]))
+    add = torch.sigmoid(g) * v
+    sizes = start[1:] - start[:-1]
+    h = v.new_zeros(sizes.shape[0], x.shape[1]) if h0 is None else _wide(h0)
+    parts, where = [], []
+    for k in range(int(sizes.max()) if sizes.numel() else 0):
+        on = sizes > k
+        at = (start[:-1] + k)[on]
+        new = decay[at] * h[on] + add[at]
+        h = h.index_put((on.nonzero()[:, 0],), new)
+        parts.append(new)
+        where.append(at)
+    y = torch.cat(parts)[torch.argsort(torch.cat(where))] if parts else torch.zeros_like(v)
+    return y.to(x.dtype), h
+
+
+def gated_scan_step(x, gate, state, dt):
+    v, g = _wide(x), _wide(gate)
+    rate = torch.logaddexp(g, torch.zeros_like(g))
+    state.copy_(torch.exp(-rate if dt is None else -rate * dt[:, None]) * state + torch.sigmoid(g) * v)
+    return state.to(x.dtype)

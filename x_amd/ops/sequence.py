@@ -1,0 +1,336 @@
+"""Operators of a recurrent model over event tokens, on the HIP library (no counterpart in the reference's package).
+
+* :func:`embed_tokens`           table rows of token ids, scaled; grad to the table, summed by sorted tokens
+* :func:`residual_rms_norm`      residual addition with dropout and RMS norm; grads to x, residual and weight
+* :func:`residual_rms_norm_fp8`  the same without dropout, the norm in 8 bits (e4m3) with a scale per row
+* :func:`gated_scan`             gated linear recurrence over ragged windows of tokens; grads to x, gate and h0
+* :func:`gated_scan_step`        its single-token form for streams, the state updated in place
+
+Tokens are rows of D channels in single, bfloat16 or half precision; sums and states are kept in single precision and
+every output is rounded once.  Rows may lie apart (a slice of a wider projection) as long as a row is contiguous; other
+layouts are copied first.  Device tensors run on the HIP kernels, CPU tensors on :mod:`x_amd.ops.reference`.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import reference as ref
+from ._ext import F32, I64, call, ext_supports, load_library, on_device, ptr, stream_of
+
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_NORM_WIDTH = 8192
+_U64 = 2 ** 64 - 1
+
+
+def _float_type(t, name: str) -> int:
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a tensor")
+    code = _CODE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _on(t, name: str, dev):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as (rows, D) with contiguous rows: a view where its strides allow it, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _grads_wanted(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _ws(nbytes: int, dev, what: str) -> torch.Tensor:
+    if nbytes < 0:
+        raise ValueError(f"{what}: sizes not supported")
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+
+
+# ------------------------------------------------------------------------------------------- embedding
+def _embed_fwd(ids, table, scale, dtype):
+    N, (V, D) = ids.numel(), table.shape
+    out = torch.empty(*ids.shape, D, dtype=dtype, device=table.device)
+    with on_device(table.device):
+        call("atl_embed_fwd", ptr(ids), int(ids.dtype == I64), N, ptr(table), table.stride(0), _CODE[table.dtype], V, D,
+             scale, ptr(out), _CODE[dtype], stream_of(table))
+    return out
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, dtype):
+        ctx.save_for_backward(ids)
+        ctx.meta = (table.shape, table.dtype, scale)
+        return _embed_fwd(ids, table, scale, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        (V, D), ttype, scale = ctx.meta
+        g = _rows(g)
+        N = ids.numel()
+        gt = torch.empty(V, D, dtype=ttype, device=g.device)
+        nbytes = int(load_library().atl_embed_bwd_ws_bytes(N, V, D))
+        ws = _ws(nbytes, g.device, "embed_tokens")
+        with on_device(g.device):
+            call("atl_embed_bwd", ptr(ids), int(ids.dtype == I64), N, ptr(g), g.stride(0), _CODE[g.dtype], V, D, scale,
+                 ptr(gt), _CODE[ttype], ptr(ws), nbytes, stream_of(g))
+        return None, gt, None, None
+
+
+def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype: torch.dtype | None = None):
+    """(\\*ids.shape, D) rows ``scale * table[ids]`` of a (V, D) table, in ``dtype`` (the table's if None).  An id outside
+    [0, V) is no token, as an event outside the image is no vote: zeros, and no gradient.  The table's gradient adds
+    the rows of one id in token order (the tokens are sorted by id, no atomic adds): equal calls give equal bits."""
+    _float_type(table, "table")
+    _on(ids, "ids", table.device)
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be (V, D), got {tuple(table.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
+    dtype = table.dtype if dtype is None else dtype
+    if dtype not in _CODE:
+        raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    scale = float(scale)
+    if not ext_supports(table):
+        return ref.embed_tokens(ids, table, scale, dtype)
+    ids, rows = ids.contiguous(), _rows(table)
+    if _grads_wanted(table):
+        return _Embed.apply(ids, rows, scale, dtype)
+    return _embed_fwd(ids, rows, scale, dtype)
+
+
+# ------------------------------------------------------------------------------------------- residual norm
+def _norm_fwd(x, res, w, eps, p, seed, offset, fp8=False):
+    """(y, s, scale) for rows x (N, D) and res (N, D) or None; s None where it would be x itself."""
+    N, D = x.shape
+    dev, rtype = x.device, (x if res is None else res).dtype
+    y = torch.empty(N, D, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
+    s = None if res is None and p == 0 else torch.empty(N, D, dtype=rtype, device=dev)
+    scale = torch.empty(N, 1, dtype=F32, device=dev) if fp8 else None
+    with on_device(dev):
+        call("atl_rms_norm_fwd", ptr(x), x.stride(0), _CODE[x.dtype], ptr(res), 0 if res is None else res.stride(0),
+             _CODE[rtype], ptr(w), N, D, eps, p, seed, offset, ptr(y), ptr(s), ptr(scale), stream_of(x))
+    return y, s, scale
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, res, w, eps, p, seed, offset):
+        rx, rr = _rows(x), None if res is None else _rows(res)
+        y, s, _ = _norm_fwd(rx, rr, w, eps, p, seed, offset)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(rx if s is None else s, w)
+        ctx.meta = (x.shape, x.dtype, None if res is None else res.shape, eps, p, seed, offset)
+        return y.view(x.shape), (None if s is None else s.view(x.shape))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gs=None):
+        s, w = ctx.saved_tensors
+        shape, xtype, rshape, eps, p, seed, offset = ctx.meta
+        want_x, want_r, want_w = ctx.needs_input_grad[:3]
+        if gy is None and gs is None:
+            return (None,) * 7
+        N, D = s.shape
+        dev = s.device
+        gy, gs = None if gy is None else _rows(gy), None if gs is None else _rows(gs)
+        same = p == 0 and xtype == s.dtype                 # then both gradients are one tensor
+        gr = torch.empty(N, D, dtype=s.dtype, device=dev) if (want_r or same) and (want_r or want_x) else None
+        gx = torch.empty(N, D, dtype=xtype, device=dev) if want_x and not same else None
+        gw = torch.empty(D, dtype=F32, device=dev) if want_w else None
+        nbytes = int(load_library().atl_rms_norm_bwd_ws_bytes(N, D)) if want_w else 0
+        ws = _ws(nbytes, dev, "residual_rms_norm") if want_w else None
+        with on_device(dev):
+            call("atl_rms_norm_bwd", ptr(s), s.stride(0), _CODE[s.dtype], ptr(w), ptr(gy),
+                 0 if gy is None else gy.stride(0), _CODE[xtype], ptr(gs), 0 if gs is None else gs.stride(0), N, D, eps,
+                 p, seed, offset, ptr(gx), ptr(gr), ptr(gw), ptr(ws), nbytes, stream_of(s))
+        gx = gr if same else gx
+        return (gx.view(shape) if want_x else None, gr.view(rshape) if want_r else None, gw, None, None, None, None)
+
+
+def _norm_args(x, residual, weight, eps, p=0.0):
+    _float_type(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be (..., D), got {tuple(x.shape)}")
+    D = x.shape[-1]
+    if D > MAX_NORM_WIDTH:
+        raise ValueError(f"rows of up to {MAX_NORM_WIDTH} channels, got {D}")
+    _on(weight, "weight", x.device)
+    _float_type(weight, "weight")
+    if weight.shape != (D,):
+        raise ValueError(f"weight must be ({D},), got {tuple(weight.shape)}")
+    if residual is not None:
+        _on(residual, "residual", x.device)
+        if residual.dtype not in (x.dtype, F32):
+            raise TypeError(f"residual must be {x.dtype} or float32, got {residual.dtype}")
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
+    eps, p = float(eps), float(p)
+    if not 0 <= eps < 1e30:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if not (0 <= p < 1 and round(p * 65536) < 65536):
+        raise ValueError(f"p must be in [0, 1 - 2^-16], got {p}")
+    return eps, round(p * 65536) / 65536
+
+
+def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6,
+                      p: float = 0.0, seed: int = 0, offset: int = 0):
+    """(y, s): the sum s = residual + dropout(x) and its root-mean-square norm y = s / sqrt(mean(s^2) + eps) * weight
+    over the last axis (of up to 8192 channels).  s has the residual's type (x's or float32) and is the next residual;
+    y has x's, and is the norm of s as it is returned.  Without a residual s is dropout(x).
+
+    Dropout zeroes an element with probability p (to the nearest 1 / 65536) and scales the others by 1 / (1 - p).  Its
+    bits come from Philox4x32-10 at counter (row, 2^31 + column // 8, ``offset``) under the key ``seed``, so equal
+    (seed, offset) give equal masks whatever the launch, the backward draws them again, and no mask is stored."""
+    eps, p = _norm_args(x, residual, weight, eps, p)
+    seed, offset = int(seed) & _U64, int(offset) & _U64
+    if not ext_supports(x):
+        return ref.residual_rms_norm(x, residual, weight, eps, p, seed, offset)
+    w = weight.to(F32).contiguous()
+    if _grads_wanted(x, residual, w):
+        y, s = _Norm.apply(x, residual, w, eps, p, seed, offset)
+    else:
+        y, s, _ = _norm_fwd(_rows(x), None if residual is None else _rows(residual), w, eps, p, seed, offset)
+        y, s = y.view(x.shape), None if s is None else s.view(x.shape)
+    return y, x if s is None else s
+
+
+def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6):
+    """(q, scale, s): :func:`residual_rms_norm` without dropout, its norm in e4m3 with a scale per row: y = q * scale,
+    scale (..., 1) = max(max |y|, 1e-30) / 448, q = 448 y / max |y| rounded to nearest.  For inference (no gradient): q
+    and scale are what a row-scaled 8-bit product takes."""
+    eps, _ = _norm_args(x, residual, weight, eps)
+    with torch.no_grad():
+        if not ext_supports(x):
+            return ref.residual_rms_norm_fp8(x, residual, weight, eps)
+        y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.to(F32).contiguous(),
+                                eps, 0.0, 0, 0, fp8=True)
+        return y.view(x.shape), scale.view(*x.shape[:-1], 1), x if s is None else s.view(x.shape)
+
+
+# ------------------------------------------------------------------------------------------- recurrence
+def _scan_fwd(x, gate, start, dt, h0, save):
+    N, D = x.shape
+    B, dev = start.numel() - 1, x.device
+    lib = load_library()
+    y = torch.empty(N, D, dtype=x.dtype, device=dev)
+    last = torch.empty(B, D, dtype=F32, device=dev)
+    nbytes = int(lib.atl_gated_scan_ws_bytes(N, D, _CODE[x.dtype]))
+    ws = _ws(nbytes, dev, "gated_scan")
+    states = torch.empty(int(lib.atl_gated_scan_groups(N)), D, dtype=F32, device=dev) if save else None
+    with on_device(dev):
+        call("atl_gated_scan_fwd", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], N, D, ptr(start), B,
+             ptr(dt), ptr(h0), ptr(y), ptr(last), ptr(states), ptr(ws), nbytes, stream_of(x))
+    return y, last, states
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, start, dt, h0):
+        y, last, states = _scan_fwd(x, gate, start, dt, h0, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, gate, start, dt, h0, states)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, glast):
+        x, gate, start, dt, h0, states = ctx.saved_tensors
+        if gy is None and glast is None:
+            return (None,) * 5
+        N, D = x.shape
+        B, dev = start.numel() - 1, x.device
+        gy = None if gy is None else _rows(gy)
+        glast = None if glast is None else glast.contiguous()
+        gx = torch.empty(N, D, dtype=x.dtype, device=dev)
+        gg = torch.empty(N, D, dtype=x.dtype, device=dev)
+        gh0 = torch.empty(B, D, dtype=F32, device=dev) if ctx.needs_input_grad[4] else None
+        nbytes = int(load_library().atl_gated_scan_ws_bytes(N, D, _CODE[x.dtype]))
+        ws = _ws(nbytes, dev, "gated_scan")
+        with on_device(dev):
+            call("atl_gated_scan_bwd", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], N, D, ptr(start),
+                 B, ptr(dt), ptr(h0), ptr(states), ptr(gy), 0 if gy is None else gy.stride(0), ptr(glast), ptr(gx),
+                 ptr(gg), ptr(gh0), ptr(ws), nbytes, stream_of(x))
+        return gx, gg, None, None, gh0
+
+
+def _scan_args(x, gate, dt):
+    _float_type(x, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be (N, D), got {tuple(x.shape)}")
+    _on(gate, "gate", x.device)
+    if gate.dtype != x.dtype or gate.shape != x.shape:
+        raise ValueError(f"gate must be like x ({tuple(x.shape)}, {x.dtype}), got {tuple(gate.shape)}, {gate.dtype}")
+    if dt is None:
+        return None
+    _on(dt, "dt", x.device)
+    if dt.shape != (x.shape[0],):
+        raise ValueError(f"dt must be ({x.shape[0]},), got {tuple(dt.shape)}")
+    if dt.requires_grad:
+        raise ValueError("no gradient flows to dt: detach it")
+    return dt.to(F32).contiguous()
+
+
+def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: torch.Tensor | None = None,
+               h0: torch.Tensor | None = None):
+    """(y, last): the gated linear recurrence
+
+        h_i = exp(-dt_i softplus(gate_i)) h_{i-1} + sigmoid(gate_i) x_i
+
+    of every channel over the tokens (N, D) of each window, from h0 (B, D) or zero.  y (N, D) holds every state in x's
+    type, last (B, D) each window's last one in float32 (an empty window's: h0 or zero), to go on from.
+
+    ``start`` (B + 1) holds the windows' first tokens and N (``EventPacket.offsets``); it must ascend from 0 to N, which
+    is not checked on the device.  ``dt`` (N,) is the gap to the token before, in units of a time constant (the first
+    token's: since h0), not negative; None stands for ones: then h is a running average.  No gradient flows to dt."""
+    dt = _scan_args(x, gate, dt)
+    N, D = x.shape
+    _on(start, "start", x.device)
+    if start.dim() != 1 or start.numel() < 1 or start.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"start must be (B + 1,) of int64 or int32, got {tuple(start.shape)}, {start.dtype}")
+    B = start.numel() - 1
+    if B == 0 and N > 0:
+        raise ValueError(f"{N} tokens but no window")
+    if h0 is not None:
+        _on(h0, "h0", x.device)
+        if h0.shape != (B, D):
+            raise ValueError(f"h0 must be ({B}, {D}), got {tuple(h0.shape)}")
+        h0 = h0.to(F32).contiguous()
+    start = start.to(I64).contiguous()
+    if not ext_supports(x):
+        return ref.gated_scan(x, gate, start, dt, h0)
+    rx, rg = _rows(x), _rows(gate)
+    if _grads_wanted(x, gate, h0):
+        return _Scan.apply(rx, rg, start, dt, h0)
+    return _scan_fwd(rx, rg, start, dt, h0, False)[:2]
+
+
+def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt: torch.Tensor | None = None):
+    """One token of each of N streams: ``state`` (N, D) float32 becomes exp(-dt softplus(gate)) state + sigmoid(gate) x in
+    place; returns it in x's type.  For inference (no gradient)."""
+    dt = _scan_args(x, gate, dt)
+    _on(state, "state", x.device)
+    if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
+        raise ValueError(f"state must be a contiguous float32 tensor of {tuple(x.shape)} without gradient, got "
+                         f"{tuple(state.shape)}, {state.dtype}")
+    with torch.no_grad():
+        if not ext_supports(x):
+            return ref.gated_scan_step(x, gate, state, dt)
+        x, gate = _rows(x), _rows(gate)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with on_device(x.device):
+            call("atl_gated_scan_step", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], x.shape[0],
+                 x.shape[1], ptr(dt), ptr(state), ptr(y), stream_of(x))
+        return y
