@@ -5,14 +5,14 @@
 // from h0 (or zero) at each window's first token.  z is the gate's rate times the time gap to the token before (1
 // where no gaps are given: then a = 1 - w and h is a running average); tokens of one time stamp (dt = 0) add up.
 //
-// The recurrence is associative in (Z, U): h_out = exp(-Z) h_in + U.  Tokens are cut into groups of kLen, a workgroup
-// holds 256 / lanes groups (a chunk); lanes run over the channels, V each.  Forward:
-//   1. k_scan_local: every group's (Z, U) and their exclusive prefixes within the chunk, and the chunk's (Z, U);
+// The recurrence is associative in (Z, U): h_out = exp(-Z) h_in + U.  Tokens are cut into groups of kLen, one thread
+// per group and V channels; a workgroup holds as many groups side by side as its threads allow (a chunk).  Forward:
+//   1. k_scan_local: every chunk's (Z, U), its groups joined in LDS;
 //   2. k_scan_carry: the state before every chunk;
-//   3. k_scan_apply: every group again from its own start state: y, the last states, and (for the backward) the
-//      start states.
-// The backward is the same recurrence from the end, C_i = a_i (gy_i + C_{i+1}), with the group's states recomputed
-// from its saved start state.  A range that holds a window's start is marked: its U alone is its outcome, whatever came
+//   3. k_scan_apply: decays and inputs once into registers, the groups joined in LDS again, then every group from its
+//      own start state: y, the last states, and (for the backward) the start states.
+// A call of one chunk needs the third alone.  The backward is the same recurrence from the end, C_i = a_i (gy_i +
+// C_{i+1}), in the same three steps, with the group's states recomputed from its saved start state.  A range that holds a window's start is marked: its U alone is its outcome, whatever came
 // before it (an infinity or NaN of one window stays there), so chunks need not know about windows.
 // States, decays and sums are fp32 whatever the tokens' type; y is rounded once.
 #include "typed.h"
@@ -24,7 +24,7 @@
 namespace atlhip {
 namespace {
 
-constexpr int kLen = 16;              // tokens of a group
+constexpr int kLen = 8;               // tokens of a group
 constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.925962991e-8f, kLn2 = 0.69314718055994530942f;
 
 // The gate's weight w, 1 - w and its rate softplus(g) in units of log 2, from one exp2, one reciprocal and one log2:
@@ -77,11 +77,13 @@ __device__ __forceinline__ float rate_of(float M, float P) {
   return M < 0.5f ? -log1pf(-M) * kLog2e : -__builtin_amdgcn_logf(P);
 }
 
+constexpr int kScanBlock = 512;
+
 struct ScanGeo {
   int64_t N, D, sx, sg, sgy;          // tokens, channels, row strides in elements
-  int64_t nchunk;
+  int64_t nchunk, cstride;            // chunks, and the distance of two channels' chunk records
   int B;
-  int cl2;                            // log2 of the lanes of a row
+  int units, G, seg;                  // threads of a row, groups of a workgroup and of a segment of them
 };
 
 // Number of entries of start[0, B) below i (start ascends), by the whole wave: 64 probes a step.
@@ -99,362 +101,575 @@ __device__ __forceinline__ int count_below(const int64_t* __restrict__ start, in
   return lo + __popcll(__ballot(lane < n && start[lo + (lane < n ? lane : 0)] < i));
 }
 
-// Where a thread works: its channels, its group and the group's tokens [i0, i1).
+// Where a thread works: its channels, its group and the group's n tokens from i0 on.
 struct Place {
-  int64_t c, group, i0, i1;
-  int gi, G;
-  bool live;                          // has channels
+  int64_t c, i0;
+  int gi, n;
+  bool live;                          // has channels and tokens
 };
 template <int V>
-__device__ __forceinline__ Place place_of(const ScanGeo& s) {
+__device__ __forceinline__ Place place_of(const ScanGeo& s, int64_t chunk) {
   Place p;
-  const int cl = threadIdx.x & ((1 << s.cl2) - 1);
-  p.gi = threadIdx.x >> s.cl2;
-  p.G = kBlock >> s.cl2;
-  p.c = (((int64_t)blockIdx.y << s.cl2) + cl) * V;
-  p.group = (int64_t)blockIdx.x * p.G + p.gi;
-  p.i0 = p.group * kLen;
-  p.i1 = min(p.i0 + kLen, s.N);
-  p.live = p.c < s.D;
+  p.gi = threadIdx.x / s.units;
+  const int un = threadIdx.x - p.gi * s.units;
+  p.c = ((int64_t)blockIdx.y * s.units + un) * V;
+  p.i0 = (chunk * s.G + p.gi) * kLen;
+  p.live = p.gi < s.G && p.c < s.D && p.i0 < s.N;
+  p.n = p.live ? (int)min((int64_t)kLen, s.N - p.i0) : 0;
   return p;
 }
 
-// Walks the windows along ascending tokens.  b: the window of the token before (-1 before the first), next: where the
-// window after it starts.
+template <int BYTES>
+using Word = std::conditional_t<BYTES == 2, uint16_t, std::conditional_t<BYTES == 4, uint32_t, uint64_t>>;
+
+// A thread's row pieces of one (tokens, channels) array: the chunk's address, the same for all threads, and a 32-bit
+// offset, which steps from token to token (the host sees to it that a chunk spans less than 4 GB).
+template <typename T>
+struct Rows {
+  T* base;
+  uint32_t off, step;                 // in bytes
+  __device__ __forceinline__ Rows(const ScanGeo& s, const Place& p, T* array, int64_t stride, int64_t chunk) {
+    base = array + chunk * s.G * kLen * stride;
+    step = (uint32_t)stride * (uint32_t)sizeof(T);
+    off = (uint32_t)(p.gi * kLen) * step + (uint32_t)p.c * (uint32_t)sizeof(T);
+  }
+  // Token t's piece (PLAIN: the address steps with the base, which all threads share).
+  template <bool PLAIN>
+  __device__ __forceinline__ T* at(uint32_t t) const {
+    return PLAIN ? (T*)((uintptr_t)base + (uint64_t)t * step + off) : (T*)((uintptr_t)base + (uint32_t)(off + t * step));
+  }
+};
+
+// The first token of the wave's first group.
+__device__ __forceinline__ int64_t wave_first_token(const ScanGeo& s, int64_t chunk) {
+  return (chunk * s.G + (threadIdx.x & ~(kWave - 1)) / s.units) * kLen;
+}
+
+// Walks the windows along a group's ascending tokens.  b: the window of the token before (-1 before the first), next:
+// how far from the group's first token the window after it starts.
 struct Ascend {
-  int b;
-  int64_t next;
+  int b, next;
+  __device__ __forceinline__ void look(const int64_t* __restrict__ start, int64_t i0) {
+    next = (int)min(start[b + 1] - i0, (int64_t)1 << 30);
+  }
   __device__ __forceinline__ Ascend(const int64_t* __restrict__ start, int B, int64_t wave_first, int64_t i0) {
     b = count_below(start, B, wave_first) - 1;
     while (b + 1 < B && start[b + 1] < i0) ++b;
-    next = start[b + 1];
+    look(start, i0);
   }
-  // Whether token i is the first of a window, which b is then.
-  __device__ __forceinline__ bool starts(const int64_t* __restrict__ start, int B, int64_t i) {
-    if (i != next || b + 1 >= B) return false;
-    do { ++b; next = start[b + 1]; } while (next <= i && b + 1 < B);
+  // Whether token i0 + t is the first of a window, which b is then.
+  __device__ __forceinline__ bool starts(const int64_t* __restrict__ start, int B, int64_t i0, int t) {
+    if (t != next || b + 1 >= B) return false;
+    do { ++b; look(start, i0); } while (next <= t && b + 1 < B);
     return true;
   }
 };
 
-__device__ __forceinline__ int64_t wave_first_token(const ScanGeo& s) {
-  const int G = kBlock >> s.cl2;
-  return ((int64_t)blockIdx.x * G + ((threadIdx.x & ~(kWave - 1)) >> s.cl2)) * kLen;
-}
-
-// The groups' (Z, U) of a chunk through LDS: each group's exclusive prefix (in the order of the recurrence, from
-// group 0 up or, REV, from the last down) into pZ, pU, the chunk's total into cZ, cU.  Called by all threads.
-template <int V, bool REV>
-__device__ __forceinline__ void chunk_prefix(const ScanGeo& s, const Place& p, float (&Z)[V], float (&U)[V],
-                                             float* lds, float* __restrict__ pZ, float* __restrict__ pU,
-                                             float* __restrict__ cZ, float* __restrict__ cU) {
-  float* lZ = lds;
-  float* lU = lds + kBlock * V;
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    lZ[threadIdx.x * V + k] = Z[k];
-    lU[threadIdx.x * V + k] = U[k];
-  }
-  __syncthreads();
-  const int width = V << s.cl2;                  // channels of the block
-  for (int ch = threadIdx.x; ch < width; ch += kBlock) {
-    float z = 0.f, u = 0.f;
-    for (int j = 0; j < p.G; ++j) {
-      const int at = (REV ? p.G - 1 - j : j) * width + ch;
-      const float gz = lZ[at], gu = lU[at];
-      lZ[at] = z;
-      lU[at] = u;
-      u = past(gz, gu, u);
-      z = joined(z, gz);
-    }
-    const int64_t c = (int64_t)blockIdx.y * width + ch;
-    if (c < s.D) {
-      cZ[blockIdx.x * s.D + c] = z;
-      cU[blockIdx.x * s.D + c] = u;
-    }
-  }
-  __syncthreads();
-  if (p.live && p.i0 < s.N) {
-    const int64_t at = p.group * s.D + p.c;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      pZ[at + k] = lZ[threadIdx.x * V + k];
-      pU[at + k] = lU[threadIdx.x * V + k];
-    }
-  }
-}
-
-template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kBlock) k_scan_local(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
-                                                       const int64_t* __restrict__ start, const float* __restrict__ dt,
-                                                       const float* __restrict__ h0, float* __restrict__ pZ,
-                                                       float* __restrict__ pU, float* __restrict__ cZ,
-                                                       float* __restrict__ cU) {
-  __shared__ float lds[2 * kBlock * V];
-  const Place p = place_of<V>(s);
-  Ascend win(start, s.B, wave_first_token(s), p.i0);
-  float Z[V], U[V], P[V];           // Z: the sum of rates, or without gaps 1 - the decay, and P the decay
-#pragma unroll
-  for (int k = 0; k < V; ++k) Z[k] = U[k] = 0.f, P[k] = 1.f;
-  bool reset = false;
-  if (p.live)
-    for (int64_t i = p.i0; i < p.i1; ++i) {
-      float xv[V], gv[V];
-      load_f<V>(x + i * s.sx + p.c, xv);
-      load_f<V>(g + i * s.sg + p.c, gv);
-      const float d = DT ? dt[i] : 1.f;
-      if (win.starts(start, s.B, i)) {
-        reset = true;
-#pragma unroll
-        for (int k = 0; k < V; ++k) U[k] = h0 ? h0[win.b * s.D + p.c + k] : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const Gate q = gate_of<T, DT>(gv[k]);
-        const float z = q.rate2 * d;
-        const float a = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
-        U[k] = fmaf(a, U[k], q.w * xv[k]);
-        Z[k] = DT ? Z[k] + z : fmaf(q.w, 1.f - Z[k], Z[k]);
-        if (!DT) P[k] *= a;
-      }
-    }
-#pragma unroll
-  for (int k = 0; k < V; ++k) Z[k] = reset ? kAnew : DT ? Z[k] : rate_of(Z[k], P[k]);
-  chunk_prefix<V, false>(s, p, Z, U, lds, pZ, pU, cZ, cU);
-}
-
-// The state before each chunk (REV: after it, from the last chunk down), and the empty windows' last states (the
-// backward: their gradients): out[b] = in[b] or zero.
-constexpr int kCarryChannels = 16, kCarrySegments = 64, kCarryBlock = kCarryChannels * kCarrySegments;
-template <bool REV>
-__global__ void __launch_bounds__(kCarryBlock) k_scan_carry(int64_t nchunk, int64_t D, const float* __restrict__ cZ,
-                                                            const float* __restrict__ cU, float* __restrict__ carry,
-                                                            const int64_t* __restrict__ start, int B,
-                                                            const float* __restrict__ in, float* __restrict__ out,
-                                                            unsigned carry_blocks) {
-  if (blockIdx.x >= carry_blocks) {
-    const int64_t stride = (int64_t)(gridDim.x - carry_blocks) * kCarryBlock;
-    for (int64_t e = (int64_t)(blockIdx.x - carry_blocks) * kCarryBlock + threadIdx.x; e < (int64_t)B * D; e += stride) {
-      const int64_t b = e / D;
-      if (start[b + 1] <= start[b]) out[e] = in ? in[e] : 0.f;
-    }
-    return;
-  }
-  __shared__ float sZ[kCarryBlock], sU[kCarryBlock];
-  const int ch = threadIdx.x % kCarryChannels, seg = threadIdx.x / kCarryChannels;
-  const int64_t c = (int64_t)blockIdx.x * kCarryChannels + ch;
-  const int64_t per = (nchunk + kCarrySegments - 1) / kCarrySegments;
-  const int64_t j0 = min(seg * per, nchunk), j1 = min(j0 + per, nchunk);
-  const bool live = c < D;
-  float z = 0.f, u = 0.f;
-  if (live)
-    for (int64_t j = j0; j < j1; ++j) {
-      const int64_t at = (REV ? nchunk - 1 - j : j) * D + c;
-      const float gz = cZ[at];
-      u = past(gz, cU[at], u);
-      z = joined(z, gz);
-    }
-  sZ[threadIdx.x] = z;
-  sU[threadIdx.x] = u;
-  __syncthreads();
-  if (seg == 0) {
-    float h = 0.f;
-    for (int k = 0; k < kCarrySegments; ++k) {
-      const int at = k * kCarryChannels + ch;
-      const float gz = sZ[at], gu = sU[at];
-      sU[at] = h;
-      h = past(gz, gu, h);
-    }
-  }
-  __syncthreads();
-  float h = sU[threadIdx.x];
-  if (live)
-    for (int64_t j = j0; j < j1; ++j) {
-      const int64_t at = (REV ? nchunk - 1 - j : j) * D + c;
-      carry[at] = h;
-      h = past(cZ[at], cU[at], h);
-    }
-}
-
-// pU: the groups' prefixes in, their start states out (read by the backward).
-template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kBlock) k_scan_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
-                                                       const int64_t* __restrict__ start, const float* __restrict__ dt,
-                                                       const float* __restrict__ h0, const float* __restrict__ pZ,
-                                                       float* __restrict__ pU, const float* __restrict__ carry,
-                                                       T* __restrict__ y, float* __restrict__ last, bool save) {
-  const Place p = place_of<V>(s);
-  Ascend win(start, s.B, wave_first_token(s), p.i0);
-  if (!p.live || p.i0 >= s.N) return;
-  float h[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int64_t at = p.group * s.D + p.c + k;
-    h[k] = past(pZ[at], pU[at], carry[blockIdx.x * s.D + p.c + k]);
-    if (save) pU[at] = h[k];
-  }
-  for (int64_t i = p.i0; i < p.i1; ++i) {
-    float xv[V], gv[V];
-    load_f<V>(x + i * s.sx + p.c, xv);
-    load_f<V>(g + i * s.sg + p.c, gv);
-    const float d = DT ? dt[i] : 1.f;
-    if (win.starts(start, s.B, i))
-#pragma unroll
-      for (int k = 0; k < V; ++k) h[k] = h0 ? h0[win.b * s.D + p.c + k] : 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const Gate q = gate_of<T, DT>(gv[k]);
-      h[k] = fmaf(DT ? __builtin_amdgcn_exp2f(-q.rate2 * d) : q.wc, h[k], q.w * xv[k]);
-    }
-    store_f<V>(y + i * s.D + p.c, h);
-    if (i + 1 == win.next && win.b >= 0)
-#pragma unroll
-      for (int k = 0; k < V; ++k) last[win.b * s.D + p.c + k] = h[k];
-  }
-}
-
-// Walks the windows along descending tokens.  b: the window of the present token, first: where it starts.
+// Walks the windows along descending tokens.  b: the window of the present token, first: how far from the group's
+// first token it starts, last: whether the present token is its window's last.
 struct Descend {
-  int b;
-  int64_t first;
-  bool last;                          // the present token is its window's last
-  __device__ __forceinline__ Descend(const int64_t* __restrict__ start, int B, int64_t wave_first, int64_t i) {
+  int b, first;
+  bool last;
+  __device__ __forceinline__ void look(const int64_t* __restrict__ start, int64_t i0) {
+    first = (int)max(start[b] - i0, -((int64_t)1 << 30));
+  }
+  __device__ __forceinline__ Descend(const int64_t* __restrict__ start, int B, int64_t wave_first, int64_t i0, int n) {
+    const int64_t i = i0 + n - 1;
     b = count_below(start, B, wave_first + 1) - 1;                 // the last window that starts at or before it
     while (b + 1 < B && start[b + 1] <= i) ++b;
     b = max(b, 0);
-    first = start[b];
+    look(start, i0);
     last = i + 1 == start[b + 1];
   }
-  __device__ __forceinline__ void step(const int64_t* __restrict__ start, int64_t i) {      // to token i
+  __device__ __forceinline__ void step(const int64_t* __restrict__ start, int64_t i0, int t) {      // to token i0 + t
     last = false;
-    if (i < first && b > 0) {
-      do { --b; } while (b > 0 && start[b] > i);
-      first = start[b];
+    if (t < first && b > 0) {
+      do { --b; } while (b > 0 && start[b] > i0 + t);
+      look(start, i0);
       last = true;
     }
   }
 };
 
+// Whether all of the wave's groups are whole and touch no window's edge, which spares the tests for every token.
+__device__ __forceinline__ bool plain_wave(const Place& p, const Ascend& win) {
+  return __all(!p.live || (p.n == kLen && win.next > kLen));
+}
+__device__ __forceinline__ bool plain_wave(const Place& p, const Descend& win) {
+  return __all(!p.live || (p.n == kLen && win.first < 0 && !win.last));
+}
+
+// f(true_type) or f(false_type), by a flag that is the same for the whole wave.
+template <typename F>
+__device__ __forceinline__ void by_flag(bool flag, F&& f) {
+  if (flag) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+// ------------------------------------------------------------------------------------------- joining a chunk's groups
+// In LDS: each group's (Z, U), then, per segment of about sqrt(G) groups, their exclusive prefixes and the segment's total.
+template <int V>
+struct JoinLds {
+  float z[kScanBlock * V], u[kScanBlock * V];
+  float sz[kScanBlock * V], su[kScanBlock * V];       // (segments, channels)
+};
+
+// Called by all threads with their group's (Z, U) (dead ones: an identity).  On return z, u hold what lies before the
+// group in the chunk (REV: behind it); the chunk's total goes to its record in cz, cu where given.
+template <int V, bool REV>
+__device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<V>& l, float (&z)[V], float (&u)[V], int64_t record,
+                                            float* __restrict__ cz, float* __restrict__ cu) {
+  const int width = s.units * V;
+  const int at0 = threadIdx.x * V;               // (group, channel): the groups' rows are width apart
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    l.z[at0 + k] = z[k];
+    l.u[at0 + k] = u[k];
+  }
+  __syncthreads();
+  const int segs = (s.G + s.seg - 1) / s.seg;
+  for (int e = threadIdx.x; e < segs * width; e += kScanBlock) {
+    const int seg = e / width, ch = e - seg * width;
+    float pz = 0.f, pu = 0.f;
+    for (int j = seg * s.seg; j < min((seg + 1) * s.seg, s.G); ++j) {
+      const int at = (REV ? s.G - 1 - j : j) * width + ch;
+      const float gz = l.z[at], gu = l.u[at];
+      l.z[at] = pz;
+      l.u[at] = pu;
+      pu = past(gz, gu, pu);
+      pz = joined(pz, gz);
+    }
+    l.sz[e] = pz;
+    l.su[e] = pu;
+  }
+  __syncthreads();
+  if (segs > 1 || cz) {
+    for (int ch = threadIdx.x; ch < width; ch += kScanBlock) {
+      float pz = 0.f, pu = 0.f;
+      for (int seg = 0; seg < segs; ++seg) {
+        const int at = seg * width + ch;
+        const float gz = l.sz[at], gu = l.su[at];
+        l.sz[at] = pz;
+        l.su[at] = pu;
+        pu = past(gz, gu, pu);
+        pz = joined(pz, gz);
+      }
+      const int64_t c = (int64_t)blockIdx.y * width + ch;
+      if (cz && c < s.D) {
+        cz[c * s.cstride + record] = pz;
+        cu[c * s.cstride + record] = pu;
+      }
+    }
+    if (cz) return;
+    __syncthreads();
+  }
+  const int gi = threadIdx.x / s.units;
+  if (gi >= s.G) return;
+  const int seg = (REV ? s.G - 1 - gi : gi) / s.seg, ch0 = at0 - gi * width;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    z[k] = l.z[at0 + k];
+    u[k] = l.u[at0 + k];
+    if (segs > 1) {
+      u[k] = past(z[k], u[k], l.su[seg * width + ch0 + k]);
+      z[k] = joined(l.sz[seg * width + ch0 + k], z[k]);
+    }
+  }
+}
+
+// A group's decay so far, from its tokens' rates, or without gaps from their decays: one minus the product and the product.
+template <int V, bool DT>
+struct Decay {
+  float z[V], p[V];
+  __device__ __forceinline__ Decay() {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = 0.f, p[k] = 1.f;
+  }
+  __device__ __forceinline__ void add(int k, const Gate& q, float rate, float a) {
+    if (DT) {
+      z[k] += rate;
+    } else {
+      z[k] = fmaf(q.w, 1.f - z[k], z[k]);
+      p[k] *= a;
+    }
+  }
+  __device__ __forceinline__ float rate(int k, bool reset) const {
+    return reset ? kAnew : DT ? z[k] : rate_of(z[k], p[k]);
+  }
+};
+
+template <int V>
+__device__ __forceinline__ void load_or_zero(const float* __restrict__ p, int64_t at, float (&v)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = p ? p[at + k] : 0.f;
+}
+
+// ------------------------------------------------------------------------------------------- forward
+constexpr int kAhead = 8;             // tokens whose loads are in flight together
+
 template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kBlock) k_scan_bwd_local(ScanGeo s, const T* __restrict__ g,
+__global__ void __launch_bounds__(kScanBlock) k_scan_local(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
                                                            const int64_t* __restrict__ start,
-                                                           const float* __restrict__ dt, const T* __restrict__ gy,
-                                                           const float* __restrict__ glast, float* __restrict__ pZ,
-                                                           float* __restrict__ pU, float* __restrict__ cZ,
-                                                           float* __restrict__ cU) {
-  __shared__ float lds[2 * kBlock * V];
-  const Place p = place_of<V>(s);
-  Descend win(start, s.B, wave_first_token(s), p.i1 - 1);
-  float Z[V], U[V], P[V];           // Z: the sum of rates, or without gaps 1 - the decay, and P the decay
+                                                           const float* __restrict__ dt, const float* __restrict__ h0,
+                                                           float* __restrict__ cz, float* __restrict__ cu) {
+  __shared__ JoinLds<V> lds;
+  const Place p = place_of<V>(s, blockIdx.x);
+  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
+  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kLen * 4;
+  Ascend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0);
+  Decay<V, DT> decay;
+  float U[V], Z[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) Z[k] = U[k] = 0.f, P[k] = 1.f;
+  for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
-  if (p.live)
-    for (int64_t i = p.i1 - 1; i >= p.i0; --i) {
-      float gv[V], yv[V];
-      load_f<V>(g + i * s.sg + p.c, gv);
-      if (gy)
-        load_f<V>(gy + i * s.sgy + p.c, yv);
-      else
+  if (p.live) by_flag(plain_wave(p, win), [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-        for (int k = 0; k < V; ++k) yv[k] = 0.f;
-      const float d = DT ? dt[i] : 1.f;
-      if (i < p.i1 - 1) win.step(start, i);
-      if (win.last) {
+    for (int q0 = 0; q0 < kLen; q0 += kAhead) {
+      if (!PLAIN && q0 >= p.n) continue;
+      Pack<T, V> xr[kAhead], gr[kAhead];
+      float d[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t i = PLAIN ? q0 + j : min(q0 + j, p.n - 1);
+        xr[j] = load_pack<T, V>(rx.template at<PLAIN>(i));
+        gr[j] = load_pack<T, V>(rg.template at<PLAIN>(i));
+        d[j] = DT ? *rd.template at<PLAIN>(i) : 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int t = q0 + j;
+        if (!PLAIN && t >= p.n) continue;
+        if (!PLAIN && win.starts(start, s.B, p.i0, t)) {
+          reset = true;
+          load_or_zero<V>(h0, win.b * s.D + p.c, U);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const Gate q = gate_of<T, DT>((float)gr[j].e[k]);
+          const float z = q.rate2 * d[j];
+          const float a = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
+          U[k] = fmaf(a, U[k], q.w * (float)xr[j].e[k]);
+          decay.add(k, q, z, a);
+        }
+      }
+    }
+  });
+#pragma unroll
+  for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
+  join_groups<V, false>(s, lds, Z, U, blockIdx.x, cz, cu);
+}
+
+// The state before each chunk of one channel per workgroup: a scan over the chunk records in the order of the
+// recurrence, eight to a thread, joined across the wave and then across the waves.
+constexpr int kCarryBlock = 1024, kCarryPer = 8, kCarryTile = kCarryBlock * kCarryPer;
+__global__ void __launch_bounds__(kCarryBlock) k_scan_carry(int64_t nchunk, int64_t cstride, const float* __restrict__ cz,
+                                                            const float* __restrict__ cu, float* __restrict__ carry) {
+  __shared__ float wz[kCarryBlock / kWave], wu[kCarryBlock / kWave];
+  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+  cz += blockIdx.x * cstride;
+  cu += blockIdx.x * cstride;
+  carry += blockIdx.x * cstride;
+  float h = 0.f;                                  // the state before the tile
+  for (int64_t j0 = 0; j0 < nchunk; j0 += kCarryTile) {
+    const int64_t j = j0 + threadIdx.x * kCarryPer;
+    float z[kCarryPer], u[kCarryPer], tz = 0.f, tu = 0.f;
+#pragma unroll
+    for (int k = 0; k < kCarryPer; ++k) z[k] = u[k] = 0.f;
+    if (j < nchunk) {                             // records past the last one lie within the stride and are not used
+      load_f<kCarryPer>(cz + j, z);
+      load_f<kCarryPer>(cu + j, u);
+    }
+#pragma unroll
+    for (int k = 0; k < kCarryPer; ++k) {
+      if (j + k >= nchunk) z[k] = u[k] = 0.f;
+      tu = past(z[k], u[k], tu);
+      tz = joined(tz, z[k]);
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {         // inclusive over the lanes
+      const float oz = __shfl_up(tz, d, kWave), ou = __shfl_up(tu, d, kWave);
+      if (lane >= d) {
+        tu = past(tz, tu, ou);
+        tz = joined(oz, tz);
+      }
+    }
+    __syncthreads();
+    if (lane == kWave - 1) wz[wid] = tz, wu[wid] = tu;
+    __syncthreads();
+    float mine = h;                               // the state before the wave, and the tile's end
+#pragma unroll
+    for (int w = 0; w < kCarryBlock / kWave; ++w) {
+      if (w == wid) mine = h;
+      h = past(wz[w], wu[w], h);
+    }
+    const float pz = __shfl_up(tz, 1, kWave), pu = __shfl_up(tu, 1, kWave);
+    float at[kCarryPer];
+    at[0] = lane ? past(pz, pu, mine) : mine;
+#pragma unroll
+    for (int k = 1; k < kCarryPer; ++k) at[k] = past(z[k - 1], u[k - 1], at[k - 1]);
+    if (j < nchunk) store_f<kCarryPer>(carry + j, at);
+  }
+}
+
+// The empty windows' last states (the backward: the gradients of their first): out[b] = in[b] or zero.
+__device__ __forceinline__ void fill_empty(const int64_t* __restrict__ start, int B, int64_t D, const float* __restrict__ in,
+                                           float* __restrict__ out, int64_t block, int64_t blocks) {
+  for (int64_t e = block * kScanBlock + threadIdx.x; e < (int64_t)B * D; e += blocks * kScanBlock) {
+    const int64_t b = e / D;
+    if (start[b + 1] <= start[b]) out[e] = in ? in[e] : 0.f;
+  }
+}
+
+// The workgroups past the chunks fill the empty windows' states.
+template <typename T, int V, bool DT>
+__global__ void __launch_bounds__(kScanBlock) k_scan_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
+                                                           const int64_t* __restrict__ start,
+                                                           const float* __restrict__ dt, const float* __restrict__ h0,
+                                                           const float* __restrict__ carry, T* __restrict__ y,
+                                                           float* __restrict__ last, float* __restrict__ states) {
+  __shared__ JoinLds<V> lds;
+  if (blockIdx.x >= s.nchunk) {
+    if (blockIdx.y == 0) fill_empty(start, s.B, s.D, h0, last, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
+    return;
+  }
+  const Place p = place_of<V>(s, blockIdx.x);
+  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
+  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kLen * 4;
+  const Rows<T> ro(s, p, y, s.D, blockIdx.x);
+  Ascend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0);
+  const Ascend begin = win;
+  float a[kLen][V], u[kLen][V];
+  Decay<V, DT> decay;
+  float U[V], Z[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) U[k] = 0.f;
+  bool reset = false;
+  const bool plain = plain_wave(p, win);
+  if (p.live) by_flag(plain, [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
+    Pack<T, V> xr[kLen], gr[kLen];
+    float d[kLen];
+#pragma unroll
+    for (int t = 0; t < kLen; ++t) {
+      const uint32_t i = PLAIN ? t : min(t, p.n - 1);
+      xr[t] = load_pack<T, V>(rx.template at<PLAIN>(i));
+      gr[t] = load_pack<T, V>(rg.template at<PLAIN>(i));
+      d[t] = DT ? *rd.template at<PLAIN>(i) : 1.f;
+    }
+#pragma unroll
+    for (int t = 0; t < kLen; ++t) {
+      if (!PLAIN && win.starts(start, s.B, p.i0, t)) {
         reset = true;
-#pragma unroll
-        for (int k = 0; k < V; ++k) U[k] = glast ? glast[win.b * s.D + p.c + k] : 0.f;
+        load_or_zero<V>(h0, win.b * s.D + p.c, U);
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const Gate q = gate_of<T, DT>(gv[k]);
-        const float z = q.rate2 * d;
-        const float a = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
-        U[k] = a * (yv[k] + U[k]);
-        Z[k] = DT ? Z[k] + z : fmaf(q.w, 1.f - Z[k], Z[k]);
-        if (!DT) P[k] *= a;
+        const Gate q = gate_of<T, DT>((float)gr[t].e[k]);
+        const float z = q.rate2 * d[t];
+        a[t][k] = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
+        u[t][k] = q.w * (float)xr[t].e[k];
+        U[k] = fmaf(a[t][k], U[k], u[t][k]);
+        decay.add(k, q, z, a[t][k]);
       }
     }
+  });
 #pragma unroll
-  for (int k = 0; k < V; ++k) Z[k] = reset ? kAnew : DT ? Z[k] : rate_of(Z[k], P[k]);
-  chunk_prefix<V, true>(s, p, Z, U, lds, pZ, pU, cZ, cU);
+  for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
+  join_groups<V, false>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  if (!p.live) return;
+  win = begin;
+  float h[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    h[k] = past(Z[k], U[k], carry ? carry[(p.c + k) * s.cstride + blockIdx.x] : 0.f);
+    if (states) states[p.i0 / kLen * s.D + p.c + k] = h[k];
+  }
+  by_flag(plain, [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
+#pragma unroll
+    for (int t = 0; t < kLen; ++t) {
+      if (!PLAIN && t >= p.n) continue;
+      if (!PLAIN && win.starts(start, s.B, p.i0, t)) load_or_zero<V>(h0, win.b * s.D + p.c, h);
+#pragma unroll
+      for (int k = 0; k < V; ++k) h[k] = fmaf(a[t][k], h[k], u[t][k]);
+      store_f<V>(ro.template at<PLAIN>(t), h);
+      if (!PLAIN && t + 1 == win.next && win.b >= 0)
+#pragma unroll
+        for (int k = 0; k < V; ++k) last[win.b * s.D + p.c + k] = h[k];
+    }
+  });
+}
+
+// ------------------------------------------------------------------------------------------- backward
+template <typename T, int V, bool DT, bool GY>
+__global__ void __launch_bounds__(kScanBlock) k_scan_bwd_local(ScanGeo s, const T* __restrict__ g,
+                                                               const int64_t* __restrict__ start,
+                                                               const float* __restrict__ dt, const T* __restrict__ gy,
+                                                               const float* __restrict__ glast, float* __restrict__ cz,
+                                                               float* __restrict__ cu) {
+  __shared__ JoinLds<V> lds;
+  const Place p = place_of<V>(s, blockIdx.x);
+  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
+  const Rows<const T> ry(s, p, gy, s.sgy, blockIdx.x);
+  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kLen * 4;
+  Descend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0, p.n);
+  Decay<V, DT> decay;
+  float U[V], Z[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) U[k] = 0.f;
+  bool reset = false;
+  if (p.live) by_flag(plain_wave(p, win), [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
+#pragma unroll
+    for (int q0 = kLen - kAhead; q0 >= 0; q0 -= kAhead) {
+      if (!PLAIN && q0 >= p.n) continue;
+      Pack<T, V> gr[kAhead], yr[kAhead];
+      float d[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t i = PLAIN ? q0 + j : min(q0 + j, p.n - 1);
+        gr[j] = load_pack<T, V>(rg.template at<PLAIN>(i));
+        if (GY) yr[j] = load_pack<T, V>(ry.template at<PLAIN>(i));
+        d[j] = DT ? *rd.template at<PLAIN>(i) : 1.f;
+      }
+#pragma unroll
+      for (int j = kAhead - 1; j >= 0; --j) {
+        const int t = q0 + j;
+        if (!PLAIN && t >= p.n) continue;
+        if (!PLAIN && t < p.n - 1) win.step(start, p.i0, t);
+        if (!PLAIN && win.last) {
+          reset = true;
+          load_or_zero<V>(glast, win.b * s.D + p.c, U);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const Gate q = gate_of<T, DT>((float)gr[j].e[k]);
+          const float z = q.rate2 * d[j];
+          const float a = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
+          U[k] = a * ((GY ? (float)yr[j].e[k] : 0.f) + U[k]);
+          decay.add(k, q, z, a);
+        }
+      }
+    }
+  });
+#pragma unroll
+  for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
+  join_groups<V, true>(s, lds, Z, U, s.nchunk - 1 - blockIdx.x, cz, cu);
 }
 
 // gx = H w, gg = H w (x (1 - w) - dt a h_{i-1}) with H_i = gy_i + C_{i+1}; gh0 = C at a window's first token.
-template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kBlock) k_scan_bwd_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
-                                                           const int64_t* __restrict__ start,
-                                                           const float* __restrict__ dt, const float* __restrict__ h0,
-                                                           const float* __restrict__ hs, const T* __restrict__ gy,
-                                                           const float* __restrict__ glast,
-                                                           const float* __restrict__ pZ, const float* __restrict__ pU,
-                                                           const float* __restrict__ carry, T* __restrict__ gx,
-                                                           T* __restrict__ gg, float* __restrict__ gh0) {
-  const Place p = place_of<V>(s);
-  const int64_t wf = wave_first_token(s);
-  Ascend up(start, s.B, wf, p.i0);
-  Descend win(start, s.B, wf, p.i1 - 1);
-  if (!p.live || p.i0 >= s.N) return;
-  const int64_t at = p.group * s.D + p.c;
-  const int n = (int)(p.i1 - p.i0);
-  float hp[kLen][V];                             // h_{i-1}
-  Pack<T, V> xr[kLen], gr[kLen];
-  {
-    float h[V];
+template <typename T, int V, bool DT, bool GY>
+__global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
+                                                               const int64_t* __restrict__ start,
+                                                               const float* __restrict__ dt, const float* __restrict__ h0,
+                                                               const float* __restrict__ states,
+                                                               const T* __restrict__ gy, const float* __restrict__ glast,
+                                                               const float* __restrict__ carry, T* __restrict__ gx,
+                                                               T* __restrict__ gg, float* __restrict__ gh0) {
+  __shared__ JoinLds<V> lds;
+  if (blockIdx.x >= s.nchunk) {
+    if (blockIdx.y == 0) fill_empty(start, s.B, s.D, glast, gh0, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
+    return;
+  }
+  const Place p = place_of<V>(s, blockIdx.x);
+  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
+  const Rows<const T> ry(s, p, gy, s.sgy, blockIdx.x);
+  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kLen * 4;
+  const Rows<T> rox(s, p, gx, s.D, blockIdx.x), rog(s, p, gg, s.D, blockIdx.x);
+  const int64_t wf = wave_first_token(s, blockIdx.x);
+  Descend win(start, s.B, wf, p.i0, p.n);
+  const Descend begin = win;
+  float a[kLen][V], w[kLen][V], f[kLen][V];      // f: gg = H f
+  Pack<T, V> yr[kLen];
+  Decay<V, DT> decay;
+  float U[V], Z[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) h[k] = hs[at + k];
+  for (int k = 0; k < V; ++k) U[k] = 0.f;
+  bool reset = false;
+  const bool plain = plain_wave(p, win);
+  Ascend up(start, s.B, wf, p.i0);
+  if (p.live) by_flag(plain, [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
+    Pack<T, V> xr[kLen], gr[kLen];
+    float d[kLen], h[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) h[k] = states[p.i0 / kLen * s.D + p.c + k];
 #pragma unroll
     for (int t = 0; t < kLen; ++t) {
-      if (t >= n) continue;
-      const int64_t i = p.i0 + t;
-      xr[t] = load_pack<T, V>(x + i * s.sx + p.c);
-      gr[t] = load_pack<T, V>(g + i * s.sg + p.c);
-      const float d = DT ? dt[i] : 1.f;
-      if (up.starts(start, s.B, i))
+      const uint32_t i = PLAIN ? t : min(t, p.n - 1);
+      xr[t] = load_pack<T, V>(rx.template at<PLAIN>(i));
+      gr[t] = load_pack<T, V>(rg.template at<PLAIN>(i));
+      if (GY) yr[t] = load_pack<T, V>(ry.template at<PLAIN>(i));
+      d[t] = DT ? *rd.template at<PLAIN>(i) : 1.f;
+    }
 #pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = h0 ? h0[up.b * s.D + p.c + k] : 0.f;
+    for (int t = 0; t < kLen; ++t) {
+      if (!PLAIN && up.starts(start, s.B, p.i0, t)) load_or_zero<V>(h0, up.b * s.D + p.c, h);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        hp[t][k] = h[k];
         const Gate q = gate_of<T, DT>((float)gr[t].e[k]);
-        h[k] = fmaf(DT ? __builtin_amdgcn_exp2f(-q.rate2 * d) : q.wc, h[k], q.w * (float)xr[t].e[k]);
+        const float z = q.rate2 * d[t], xv = (float)xr[t].e[k];
+        a[t][k] = DT ? __builtin_amdgcn_exp2f(-z) : q.wc;
+        w[t][k] = q.w;
+        f[t][k] = q.w * fmaf(xv, q.wc, -(d[t] * a[t][k]) * h[k]);
+        h[k] = fmaf(a[t][k], h[k], q.w * xv);
+        asm volatile("" : "+v"(a[t][k]), "+v"(w[t][k]), "+v"(f[t][k]));      // kept: not what they are made of
+        if (PLAIN || t < p.n) decay.add(k, q, z, a[t][k]);
       }
     }
-  }
+#pragma unroll
+    for (int t = kLen - 1; t >= 0; --t) {
+      if (!PLAIN && t >= p.n) continue;
+      if (!PLAIN && t < p.n - 1) win.step(start, p.i0, t);
+      if (!PLAIN && win.last) {
+        reset = true;
+        load_or_zero<V>(glast, win.b * s.D + p.c, U);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) U[k] = a[t][k] * ((GY ? (float)yr[t].e[k] : 0.f) + U[k]);
+    }
+  });
+#pragma unroll
+  for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
+  join_groups<V, true>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  if (!p.live) return;
+  win = begin;
+#pragma unroll
+  for (int t = 0; t < kLen; ++t)
+    if (GY) asm volatile("" : "+v"(*(Word<sizeof(T) * V>*)&yr[t]));      // as loaded, not widened
   float C[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) C[k] = past(pZ[at + k], pU[at + k], carry[blockIdx.x * s.D + p.c + k]);
+  for (int k = 0; k < V; ++k) C[k] = past(Z[k], U[k], carry ? carry[(p.c + k) * s.cstride + s.nchunk - 1 - blockIdx.x] : 0.f);
+  by_flag(plain, [&](auto flag) {
+    constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-  for (int t = kLen - 1; t >= 0; --t) {
-    if (t >= n) continue;
-    const int64_t i = p.i0 + t;
-    float yv[V], ox[V], og[V];
-    if (gy)
-      load_f<V>(gy + i * s.sgy + p.c, yv);
-    else
+    for (int t = kLen - 1; t >= 0; --t) {
+      if (!PLAIN && t >= p.n) continue;
+      if (!PLAIN && t < p.n - 1) win.step(start, p.i0, t);
+      if (!PLAIN && win.last) load_or_zero<V>(glast, win.b * s.D + p.c, C);
+      float ox[V], og[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) yv[k] = 0.f;
-    const float d = DT ? dt[i] : 1.f;
-    if (t < n - 1) win.step(start, i);
-    if (win.last)
+      for (int k = 0; k < V; ++k) {
+        const float H = (GY ? (float)yr[t].e[k] : 0.f) + C[k];
+        C[k] = a[t][k] * H;
+        ox[k] = H * w[t][k];
+        og[k] = H * f[t][k];
+      }
+      store_f<V>(rox.template at<PLAIN>(t), ox);
+      store_f<V>(rog.template at<PLAIN>(t), og);
+      if (!PLAIN && gh0 && t == win.first)
 #pragma unroll
-      for (int k = 0; k < V; ++k) C[k] = glast ? glast[win.b * s.D + p.c + k] : 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const Gate q = gate_of<T, DT>((float)gr[t].e[k]);
-      const float a = DT ? __builtin_amdgcn_exp2f(-q.rate2 * d) : q.wc;
-      const float H = yv[k] + C[k];
-      const float Hw = H * q.w;
-      C[k] = a * H;
-      ox[k] = Hw;
-      og[k] = Hw * fmaf((float)xr[t].e[k], q.wc, -(d * a) * hp[t][k]);
+        for (int k = 0; k < V; ++k) gh0[win.b * s.D + p.c + k] = C[k];
     }
-    store_f<V>(gx + i * s.D + p.c, ox);
-    store_f<V>(gg + i * s.D + p.c, og);
-    if (gh0 && i == win.first)
-#pragma unroll
-      for (int k = 0; k < V; ++k) gh0[win.b * s.D + p.c + k] = C[k];
-  }
+  });
 }
 
 // One token of every stream: 4 bytes of state in and out per channel, bound by the launch.
@@ -477,42 +692,38 @@ __global__ void __launch_bounds__(kBlock) k_scan_step(int64_t N, int64_t D, int6
 struct ScanPlan {
   ScanGeo s;
   int V;
-  int64_t groups;
-  unsigned gx, gy;
-  int64_t pZ, pU, cZ, cU, carry, bytes;          // workspace offsets in floats, and its size
+  unsigned tiles;
+  int64_t cz, cu, carry, bytes;                  // workspace offsets in floats, and its size in bytes
 };
 
-// 8 bytes a lane where widths, strides and addresses allow it, else single elements: a lane's 16 tokens of 8 bytes are
-// what the backward keeps in registers.
+// Two channels a thread where widths, strides and addresses allow it, else one: a thread keeps the decays, weights and
+// factors of a group's tokens of its channels in registers.
 int scan_vector(int dtype, int64_t D, int64_t strides, const void* const* ptrs, int n) {
-  const int v = 8 / dtype_size(dtype);
-  if (D % v || strides % v) return 1;
+  if (D % 2 || strides % 2) return 1;
   for (int k = 0; k < n; ++k)
-    if (!aligned_to(ptrs[k], 8)) return 1;
-  return v;
+    if (!aligned_to(ptrs[k], 2 * dtype_size(dtype))) return 1;
+  return 2;
 }
 
-// A group is kLen tokens whatever V and the lanes are: the backward reads the forward's start states per group.
+// A row's threads: its channels over V, in equal parts of at most half a workgroup.  A group is kLen tokens whatever V
+// is: the backward reads the forward's start states per group.
 ScanPlan scan_plan(int64_t N, int64_t D, int V) {
   ScanPlan q;
   q.V = V;
   q.s.N = N;
   q.s.D = D;
-  int cl2 = 0;
-  while ((1 << cl2) < kWave && ((int64_t)V << cl2) < D) ++cl2;
-  q.s.cl2 = cl2;
-  const int G = kBlock >> cl2;
-  q.groups = (N + kLen - 1) / kLen;
-  q.s.nchunk = (q.groups + G - 1) / G;
-  q.gx = (unsigned)q.s.nchunk;
-  q.gy = (unsigned)((D + ((int64_t)V << cl2) - 1) / ((int64_t)V << cl2));
-  const int64_t ng = (q.groups * D + 3) / 4 * 4, nc = (q.s.nchunk * D + 3) / 4 * 4;
-  q.pZ = 0;
-  q.pU = ng;
-  q.cZ = 2 * ng;
-  q.cU = q.cZ + nc;
-  q.carry = q.cU + nc;
-  q.bytes = (q.carry + nc) * 4;
+  const int64_t all = (D + V - 1) / V;
+  q.tiles = (unsigned)((all + kScanBlock / 2 - 1) / (kScanBlock / 2));
+  q.s.units = (int)((all + q.tiles - 1) / q.tiles);
+  q.s.G = kScanBlock / q.s.units;
+  q.s.seg = q.s.G <= 4 ? q.s.G : q.s.G <= 16 ? 4 : q.s.G <= 64 ? 8 : 16;
+  const int64_t chunk = (int64_t)q.s.G * kLen;
+  q.s.nchunk = (N + chunk - 1) / chunk;
+  q.s.cstride = (q.s.nchunk + 15) / 16 * 16;
+  q.cz = 0;
+  q.cu = q.s.cstride * D;
+  q.carry = 2 * q.cu;
+  q.bytes = q.s.nchunk > 1 ? 3 * q.cu * 4 : 0;
   return q;
 }
 
@@ -521,15 +732,13 @@ bool scan_sizes_ok(int64_t N, int64_t D, int64_t B, int dtype) {
          dtype_ok(dtype);
 }
 
-template <bool REV>
-void launch_carry(const ScanPlan& q, float* ws, const int64_t* start, int64_t B, const float* in, float* out,
-                  hipStream_t stream) {
-  const unsigned cb = q.s.nchunk ? (unsigned)((q.s.D + kCarryChannels - 1) / kCarryChannels) : 0;
-  const unsigned eb = out ? (unsigned)std::min<int64_t>(256, (B * q.s.D + kCarryBlock - 1) / kCarryBlock) : 0;
-  if (cb + eb == 0) return;
-  hipLaunchKernelGGL((k_scan_carry<REV>), dim3(cb + eb), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.D, ws + q.cZ,
-                     ws + q.cU, ws + q.carry, start, (int)B, in, out, cb);
+// Whether a chunk's rows at this stride lie within a 32-bit offset.
+bool scan_span_ok(const ScanPlan& q, int64_t stride, int dtype) {
+  return stride < ((int64_t)1 << 32) / dtype_size(dtype) / kLen / q.s.G - q.s.D;
 }
+
+// Workgroups that fill the empty windows' states.
+unsigned scan_fill_blocks(int64_t B, int64_t D) { return (unsigned)std::min<int64_t>(256, (B * D + kScanBlock - 1) / kScanBlock); }
 
 template <typename F>
 void by_type(int dtype, bool vec, bool dt, F&& f) {
@@ -541,10 +750,10 @@ void by_type(int dtype, bool vec, bool dt, F&& f) {
     if (vec) inner(float{}, std::integral_constant<int, 2>{});
     else inner(float{}, std::integral_constant<int, 1>{});
   } else if (dtype == kBF16) {
-    if (vec) inner(bf16_t{}, std::integral_constant<int, 4>{});
+    if (vec) inner(bf16_t{}, std::integral_constant<int, 2>{});
     else inner(bf16_t{}, std::integral_constant<int, 1>{});
   } else {
-    if (vec) inner(f16_t{}, std::integral_constant<int, 4>{});
+    if (vec) inner(f16_t{}, std::integral_constant<int, 2>{});
     else inner(f16_t{}, std::integral_constant<int, 1>{});
   }
 }
@@ -560,7 +769,7 @@ int64_t atl_gated_scan_groups(int64_t N) { return N < 0 ? -1 : (N + kLen - 1) / 
 
 int64_t atl_gated_scan_ws_bytes(int64_t N, int64_t D, int dtype) {
   if (!scan_sizes_ok(N, D, 1, dtype)) return -1;
-  return std::max(scan_plan(N, D, 8 / dtype_size(dtype)).bytes, scan_plan(N, D, 1).bytes);
+  return std::max(scan_plan(N, D, 2).bytes, scan_plan(N, D, 1).bytes);
 }
 
 int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
@@ -568,27 +777,29 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
                        float* states, void* ws, int64_t ws_bytes, hipStream_t stream) {
   if (!scan_sizes_ok(N, D, B, dtype) || (N > 0 && (sx < 0 || sg < 0))) { set_error("gated_scan_fwd: bad sizes N=%lld D=%lld B=%lld type %d", (long long)N, (long long)D, (long long)B, dtype); return 1; }
   if (B == 0) return 0;
-  if (!start || !last || (N > 0 && (!x || !gate || !y || !ws))) { set_error("gated_scan_fwd: null argument"); return 1; }
-  if (N > 0 && ws_bytes < atl_gated_scan_ws_bytes(N, D, dtype)) { set_error("gated_scan_fwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_gated_scan_ws_bytes(N, D, dtype)); return 1; }
+  const int64_t need = atl_gated_scan_ws_bytes(N, D, dtype);
+  if (!start || !last || (N > 0 && (!x || !gate || !y)) || (need > 0 && !ws)) { set_error("gated_scan_fwd: null argument"); return 1; }
+  if (ws_bytes < need) { set_error("gated_scan_fwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const void* ptrs[] = {x, gate, y};
   ScanPlan q = scan_plan(N, D, scan_vector(dtype, D, sx | sg, ptrs, 3));
+  if (!scan_span_ok(q, std::max(sx, sg), dtype)) { set_error("gated_scan_fwd: row strides %lld, %lld too large", (long long)sx, (long long)sg); return 1; }
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = 0; q.s.B = (int)B;
   float* w = (float*)ws;
-  float* pU = states ? states : w + q.pU;
-  if (N > 0)
-    by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
-      using T = decltype(t);
-      hipLaunchKernelGGL((k_scan_local<T, decltype(v)::value, decltype(d)::value>), dim3(q.gx, q.gy), dim3(kBlock), 0, stream,
-                         q.s, (const T*)x, (const T*)gate, start, dt, h0, w + q.pZ, pU, w + q.cZ, w + q.cU);
-    });
-  launch_carry<false>(q, w, start, B, h0, last, stream);
-  if (N > 0)
-    by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
-      using T = decltype(t);
-      hipLaunchKernelGGL((k_scan_apply<T, decltype(v)::value, decltype(d)::value>), dim3(q.gx, q.gy), dim3(kBlock), 0, stream,
-                         q.s, (const T*)x, (const T*)gate, start, dt, h0, (const float*)(w + q.pZ), pU,
-                         (const float*)(w + q.carry), (T*)y, last, states != nullptr);
-    });
+  const bool many = q.s.nchunk > 1;
+  by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
+    using T = decltype(t);
+    constexpr int V = decltype(v)::value;
+    constexpr bool DT = decltype(d)::value;
+    if (many) {
+      hipLaunchKernelGGL((k_scan_local<T, V, DT>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+                         (const T*)x, (const T*)gate, start, dt, h0, w + q.cz, w + q.cu);
+      hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
+                         (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
+    }
+    hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + scan_fill_blocks(B, D), q.tiles), dim3(kScanBlock), 0,
+                       stream, q.s, (const T*)x, (const T*)gate, start, dt, h0, (const float*)(many ? w + q.carry : nullptr),
+                       (T*)y, last, states);
+  });
   return check_launch("gated_scan_fwd");
 }
 
@@ -598,27 +809,35 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
                        int64_t ws_bytes, hipStream_t stream) {
   if (!scan_sizes_ok(N, D, B, dtype) || (N > 0 && (sx < 0 || sg < 0 || sgy < 0))) { set_error("gated_scan_bwd: bad sizes N=%lld D=%lld B=%lld type %d", (long long)N, (long long)D, (long long)B, dtype); return 1; }
   if (B == 0) return 0;
-  if (!start || (N > 0 && (!x || !gate || !states || !gx || !ggate || !ws))) { set_error("gated_scan_bwd: null argument"); return 1; }
-  if (N > 0 && ws_bytes < atl_gated_scan_ws_bytes(N, D, dtype)) { set_error("gated_scan_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_gated_scan_ws_bytes(N, D, dtype)); return 1; }
+  const int64_t need = atl_gated_scan_ws_bytes(N, D, dtype);
+  if (!start || (N > 0 && (!x || !gate || !states || !gx || !ggate)) || (need > 0 && !ws)) { set_error("gated_scan_bwd: null argument"); return 1; }
+  if (ws_bytes < need) { set_error("gated_scan_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const void* ptrs[] = {x, gate, gx, ggate, gy};
   ScanPlan q = scan_plan(N, D, scan_vector(dtype, D, sx | sg | (gy ? sgy : 0), ptrs, 5));
+  if (!scan_span_ok(q, std::max(sx, std::max(sg, gy ? sgy : 0)), dtype)) { set_error("gated_scan_bwd: row strides too large"); return 1; }
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = sgy; q.s.B = (int)B;
   float* w = (float*)ws;
-  if (N > 0)
-    by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
-      using T = decltype(t);
-      hipLaunchKernelGGL((k_scan_bwd_local<T, decltype(v)::value, decltype(d)::value>), dim3(q.gx, q.gy), dim3(kBlock), 0, stream,
-                         q.s, (const T*)gate, start, dt, (const T*)gy, glast, w + q.pZ, w + q.pU, w + q.cZ, w + q.cU);
-    });
-  launch_carry<true>(q, w, start, B, glast, gh0, stream);
-  if (N > 0)
-    by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
-      using T = decltype(t);
-      hipLaunchKernelGGL((k_scan_bwd_apply<T, decltype(v)::value, decltype(d)::value>), dim3(q.gx, q.gy), dim3(kBlock), 0, stream,
-                         q.s, (const T*)x, (const T*)gate, start, dt, h0, states, (const T*)gy, glast,
-                         (const float*)(w + q.pZ), (const float*)(w + q.pU), (const float*)(w + q.carry), (T*)gx,
-                         (T*)ggate, gh0);
-    });
+  const bool many = q.s.nchunk > 1;
+  const unsigned fill = gh0 ? scan_fill_blocks(B, D) : 0;
+  if (q.s.nchunk + fill == 0) return 0;
+  auto go = [&](auto t, auto v, auto d, auto y) {
+    using T = decltype(t);
+    constexpr int V = decltype(v)::value;
+    constexpr bool DT = decltype(d)::value, GY = decltype(y)::value;
+    if (many) {
+      hipLaunchKernelGGL((k_scan_bwd_local<T, V, DT, GY>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+                         (const T*)gate, start, dt, (const T*)gy, glast, w + q.cz, w + q.cu);
+      hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
+                         (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
+    }
+    hipLaunchKernelGGL((k_scan_bwd_apply<T, V, DT, GY>), dim3((unsigned)q.s.nchunk + fill, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+                       (const T*)x, (const T*)gate, start, dt, h0, states, (const T*)gy, glast,
+                       (const float*)(many ? w + q.carry : nullptr), (T*)gx, (T*)ggate, gh0);
+  };
+  by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
+    if (gy) go(t, v, d, std::true_type{});
+    else go(t, v, d, std::false_type{});
+  });
   return check_launch("gated_scan_bwd");
 }
 

@@ -20,6 +20,7 @@ from ._ext import F32, I64, call, ext_supports, load_library, on_device, ptr, st
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_NORM_WIDTH = 8192
+MAX_ROW_STRIDE = 65536
 _U64 = 2 ** 64 - 1
 
 
@@ -40,10 +41,11 @@ def _on(t, name: str, dev):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as (rows, D) with contiguous rows: a view where its strides allow it, else a copy."""
+    """``t`` as (rows, D) with contiguous rows: a view where its strides allow it (rows less than MAX_ROW_STRIDE elements
+    apart), else a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) <= MAX_ROW_STRIDE else t.contiguous()
 
 
 def _grads_wanted(*ts) -> bool:
