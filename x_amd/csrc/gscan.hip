@@ -5,7 +5,7 @@
 // from h0 (or zero) at each window's first token.  z is the gate's rate times the time gap to the token before (1
 // where no gaps are given: then a = 1 - w and h is a running average); tokens of one time stamp (dt = 0) add up.
 //
-// The recurrence is associative in (Z, U): h_out = exp(-Z) h_in + U.  Tokens are cut into groups of kLen, one thread
+// The recurrence is associative in (Z, U): h_out = exp(-Z) h_in + U.  Tokens are cut into groups of 16 or 8, one thread
 // per group and V channels; a workgroup holds as many groups side by side as its threads allow (a chunk).  Forward:
 //   1. k_scan_local: every chunk's (Z, U), its groups joined in LDS;
 //   2. k_scan_carry: the state before every chunk;
@@ -24,31 +24,36 @@
 namespace atlhip {
 namespace {
 
-constexpr int kLen = 8;               // tokens of a group
+// Tokens of a group, and threads of a workgroup.  The forward keeps a decay and an input a token and channel in
+// registers, the backward a decay, a weight, a factor and the gradient: it takes half the tokens a thread, so that four
+// waves fit a SIMD (1M x 64 bfloat16: 196 us against 297 with 16 tokens and two waves).
+constexpr int kFwdLen = 16, kFwdBlock = 256, kBwdLen = 8, kBwdBlock = 512;
 constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.925962991e-8f, kLn2 = 0.69314718055994530942f;
 
 // The gate's weight w, 1 - w and its rate softplus(g) in units of log 2, from one exp2, one reciprocal and one log2:
-// with e = exp(-|g|), p = 1 + e: w or 1 - w is 1 / p, the other e / p, and softplus = max(g, 0) + log p.  What p
-// rounded off e enters as (e - (p - 1)) / p, so that small rates keep their relative precision (they are multiplied
-// by gaps and summed over up to a million tokens).  exp2's argument rounds off up to |g| 2^-24 of e; for single
-// precision tokens that is put back.
+// with E = exp(g) and p = 1 + E, w = E / p, 1 - w = 1 / p and softplus = log p, or g itself where E would overflow.
+// These kernels are bound by the number of vector instructions next to memory (a transcendental one costs as much as
+// two others), hence the form with the fewest.  What p rounds off E is put back into the logarithm: a small rate would
+// lose it, and gaps of many time constants multiply it.  What exp2's argument rounds off (up to |g| 2^-24 of E) is put
+// back for single precision; a 16-bit gate's own last bit moves E by more.
 struct Gate { float w, wc, rate2; };
 template <typename T, bool RATE>
 __device__ __forceinline__ Gate gate_of(float g) {
-  const float arg = -fabsf(g) * kLog2e;
-  float e = __builtin_amdgcn_exp2f(arg);
+  const float arg = g * kLog2e;
+  float E = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(arg, 120.f));      // a NaN stays one
   if (sizeof(T) == 4) {
-    const float off = fmaf(-fabsf(g), kLog2e, -arg) - fabsf(g) * kLog2eLow;
-    e = fmaf(e, fmaxf(off, -1.f) * kLn2, e);       // the maximum: an infinite gate's off is not a number
+    const float off = fmaf(g, kLog2e, -arg) + g * kLog2eLow;
+    E = fmaf(E, fminf(fmaxf(off, -1e-5f), 1e-5f) * kLn2, E);      // the bounds: an infinite gate's off is not a number
   }
-  const float p = 1.f + e;
-  const float rp = __builtin_amdgcn_rcpf(p);
-  const float ep = e * rp;
-  const bool pos = g >= 0.f;
+  const float p = 1.f + E;
   Gate q;
-  q.w = pos ? rp : ep;
-  q.wc = pos ? ep : rp;
-  q.rate2 = RATE ? fmaf(fmaxf(g, 0.f) + (e - (p - 1.f)) * rp, kLog2e, __builtin_amdgcn_logf(p)) : 0.f;
+  q.wc = __builtin_amdgcn_rcpf(p);
+  q.w = E * q.wc;
+  q.rate2 = 0.f;
+  if (RATE) {
+    const float l = fmaf((E - (p - 1.f)) * q.wc, kLog2e, __builtin_amdgcn_logf(p));
+    q.rate2 = __builtin_elementwise_maximum(l, arg);
+  }
   return q;
 }
 
@@ -76,8 +81,6 @@ __device__ __forceinline__ float joined(float Za, float Zb) { return anew(Za) ||
 __device__ __forceinline__ float rate_of(float M, float P) {
   return M < 0.5f ? -log1pf(-M) * kLog2e : -__builtin_amdgcn_logf(P);
 }
-
-constexpr int kScanBlock = 512;
 
 struct ScanGeo {
   int64_t N, D, sx, sg, sgy;          // tokens, channels, row strides in elements
@@ -107,15 +110,15 @@ struct Place {
   int gi, n;
   bool live;                          // has channels and tokens
 };
-template <int V>
+template <int LEN, int V>
 __device__ __forceinline__ Place place_of(const ScanGeo& s, int64_t chunk) {
   Place p;
   p.gi = threadIdx.x / s.units;
   const int un = threadIdx.x - p.gi * s.units;
   p.c = ((int64_t)blockIdx.y * s.units + un) * V;
-  p.i0 = (chunk * s.G + p.gi) * kLen;
+  p.i0 = (chunk * s.G + p.gi) * LEN;
   p.live = p.gi < s.G && p.c < s.D && p.i0 < s.N;
-  p.n = p.live ? (int)min((int64_t)kLen, s.N - p.i0) : 0;
+  p.n = p.live ? (int)min((int64_t)LEN, s.N - p.i0) : 0;
   return p;
 }
 
@@ -124,14 +127,14 @@ using Word = std::conditional_t<BYTES == 2, uint16_t, std::conditional_t<BYTES =
 
 // A thread's row pieces of one (tokens, channels) array: the chunk's address, the same for all threads, and a 32-bit
 // offset, which steps from token to token (the host sees to it that a chunk spans less than 4 GB).
-template <typename T>
+template <typename T, int LEN>
 struct Rows {
   T* base;
   uint32_t off, step;                 // in bytes
   __device__ __forceinline__ Rows(const ScanGeo& s, const Place& p, T* array, int64_t stride, int64_t chunk) {
-    base = array + chunk * s.G * kLen * stride;
+    base = array + chunk * s.G * LEN * stride;
     step = (uint32_t)stride * (uint32_t)sizeof(T);
-    off = (uint32_t)(p.gi * kLen) * step + (uint32_t)p.c * (uint32_t)sizeof(T);
+    off = (uint32_t)(p.gi * LEN) * step + (uint32_t)p.c * (uint32_t)sizeof(T);
   }
   // Token t's piece (PLAIN: the address steps with the base, which all threads share).
   template <bool PLAIN>
@@ -141,8 +144,9 @@ struct Rows {
 };
 
 // The first token of the wave's first group.
+template <int LEN>
 __device__ __forceinline__ int64_t wave_first_token(const ScanGeo& s, int64_t chunk) {
-  return (chunk * s.G + (threadIdx.x & ~(kWave - 1)) / s.units) * kLen;
+  return (chunk * s.G + (threadIdx.x & ~(kWave - 1)) / s.units) * LEN;
 }
 
 // Walks the windows along a group's ascending tokens.  b: the window of the token before (-1 before the first), next:
@@ -192,11 +196,13 @@ struct Descend {
 };
 
 // Whether all of the wave's groups are whole and touch no window's edge, which spares the tests for every token.
+template <int LEN>
 __device__ __forceinline__ bool plain_wave(const Place& p, const Ascend& win) {
-  return __all(!p.live || (p.n == kLen && win.next > kLen));
+  return __all(!p.live || (p.n == LEN && win.next > LEN));
 }
+template <int LEN>
 __device__ __forceinline__ bool plain_wave(const Place& p, const Descend& win) {
-  return __all(!p.live || (p.n == kLen && win.first < 0 && !win.last));
+  return __all(!p.live || (p.n == LEN && win.first < 0 && !win.last));
 }
 
 // f(true_type) or f(false_type), by a flag that is the same for the whole wave.
@@ -208,16 +214,16 @@ __device__ __forceinline__ void by_flag(bool flag, F&& f) {
 
 // ------------------------------------------------------------------------------------------- joining a chunk's groups
 // In LDS: each group's (Z, U), then, per segment of about sqrt(G) groups, their exclusive prefixes and the segment's total.
-template <int V>
+template <int BLOCK, int V>
 struct JoinLds {
-  float z[kScanBlock * V], u[kScanBlock * V];
-  float sz[kScanBlock * V], su[kScanBlock * V];       // (segments, channels)
+  float z[BLOCK * V], u[BLOCK * V];
+  float sz[BLOCK * V], su[BLOCK * V];       // (segments, channels)
 };
 
 // Called by all threads with their group's (Z, U) (dead ones: an identity).  On return z, u hold what lies before the
 // group in the chunk (REV: behind it); the chunk's total goes to its record in cz, cu where given.
-template <int V, bool REV>
-__device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<V>& l, float (&z)[V], float (&u)[V], int64_t record,
+template <int BLOCK, int V, bool REV>
+__device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<BLOCK, V>& l, float (&z)[V], float (&u)[V], int64_t record,
                                             float* __restrict__ cz, float* __restrict__ cu) {
   const int width = s.units * V;
   const int at0 = threadIdx.x * V;               // (group, channel): the groups' rows are width apart
@@ -228,7 +234,7 @@ __device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<V>& l, flo
   }
   __syncthreads();
   const int segs = (s.G + s.seg - 1) / s.seg;
-  for (int e = threadIdx.x; e < segs * width; e += kScanBlock) {
+  for (int e = threadIdx.x; e < segs * width; e += BLOCK) {
     const int seg = e / width, ch = e - seg * width;
     float pz = 0.f, pu = 0.f;
     for (int j = seg * s.seg; j < min((seg + 1) * s.seg, s.G); ++j) {
@@ -244,7 +250,7 @@ __device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<V>& l, flo
   }
   __syncthreads();
   if (segs > 1 || cz) {
-    for (int ch = threadIdx.x; ch < width; ch += kScanBlock) {
+    for (int ch = threadIdx.x; ch < width; ch += BLOCK) {
       float pz = 0.f, pu = 0.f;
       for (int seg = 0; seg < segs; ++seg) {
         const int at = seg * width + ch;
@@ -308,26 +314,26 @@ __device__ __forceinline__ void load_or_zero(const float* __restrict__ p, int64_
 constexpr int kAhead = 8;             // tokens whose loads are in flight together
 
 template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kScanBlock) k_scan_local(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
+__global__ void __launch_bounds__(kFwdBlock) k_scan_local(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
                                                            const int64_t* __restrict__ start,
                                                            const float* __restrict__ dt, const float* __restrict__ h0,
                                                            float* __restrict__ cz, float* __restrict__ cu) {
-  __shared__ JoinLds<V> lds;
-  const Place p = place_of<V>(s, blockIdx.x);
-  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
-  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
-  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
-  rd.off = p.gi * kLen * 4;
-  Ascend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0);
+  __shared__ JoinLds<kFwdBlock, V> lds;
+  const Place p = place_of<kFwdLen, V>(s, blockIdx.x);
+  const Rows<const T, kFwdLen> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T, kFwdLen> rg(s, p, g, s.sg, blockIdx.x);
+  Rows<const float, kFwdLen> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kFwdLen * 4;
+  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, blockIdx.x), p.i0);
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
-  if (p.live) by_flag(plain_wave(p, win), [&](auto flag) {
+  if (p.live) by_flag(plain_wave<kFwdLen>(p, win), [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-    for (int q0 = 0; q0 < kLen; q0 += kAhead) {
+    for (int q0 = 0; q0 < kFwdLen; q0 += kAhead) {
       if (!PLAIN && q0 >= p.n) continue;
       Pack<T, V> xr[kAhead], gr[kAhead];
       float d[kAhead];
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_local(ScanGeo s, const T* _
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<V, false>(s, lds, Z, U, blockIdx.x, cz, cu);
+  join_groups<kFwdBlock, V, false>(s, lds, Z, U, blockIdx.x, cz, cu);
 }
 
 // The state before each chunk of one channel per workgroup: a scan over the chunk records in the order of the
@@ -415,9 +421,10 @@ __global__ void __launch_bounds__(kCarryBlock) k_scan_carry(int64_t nchunk, int6
 }
 
 // The empty windows' last states (the backward: the gradients of their first): out[b] = in[b] or zero.
+template <int BLOCK>
 __device__ __forceinline__ void fill_empty(const int64_t* __restrict__ start, int B, int64_t D, const float* __restrict__ in,
                                            float* __restrict__ out, int64_t block, int64_t blocks) {
-  for (int64_t e = block * kScanBlock + threadIdx.x; e < (int64_t)B * D; e += blocks * kScanBlock) {
+  for (int64_t e = block * BLOCK + threadIdx.x; e < (int64_t)B * D; e += blocks * BLOCK) {
     const int64_t b = e / D;
     if (start[b + 1] <= start[b]) out[e] = in ? in[e] : 0.f;
   }
@@ -425,44 +432,44 @@ __device__ __forceinline__ void fill_empty(const int64_t* __restrict__ start, in
 
 // The workgroups past the chunks fill the empty windows' states.
 template <typename T, int V, bool DT>
-__global__ void __launch_bounds__(kScanBlock) k_scan_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
+__global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
                                                            const int64_t* __restrict__ start,
                                                            const float* __restrict__ dt, const float* __restrict__ h0,
                                                            const float* __restrict__ carry, T* __restrict__ y,
                                                            float* __restrict__ last, float* __restrict__ states) {
-  __shared__ JoinLds<V> lds;
+  __shared__ JoinLds<kFwdBlock, V> lds;
   if (blockIdx.x >= s.nchunk) {
-    if (blockIdx.y == 0) fill_empty(start, s.B, s.D, h0, last, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
+    if (blockIdx.y == 0) fill_empty<kFwdBlock>(start, s.B, s.D, h0, last, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
     return;
   }
-  const Place p = place_of<V>(s, blockIdx.x);
-  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
-  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
-  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
-  rd.off = p.gi * kLen * 4;
-  const Rows<T> ro(s, p, y, s.D, blockIdx.x);
-  Ascend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0);
+  const Place p = place_of<kFwdLen, V>(s, blockIdx.x);
+  const Rows<const T, kFwdLen> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T, kFwdLen> rg(s, p, g, s.sg, blockIdx.x);
+  Rows<const float, kFwdLen> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kFwdLen * 4;
+  const Rows<T, kFwdLen> ro(s, p, y, s.D, blockIdx.x);
+  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, blockIdx.x), p.i0);
   const Ascend begin = win;
-  float a[kLen][V], u[kLen][V];
+  float a[kFwdLen][V], u[kFwdLen][V];
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
-  const bool plain = plain_wave(p, win);
+  const bool plain = plain_wave<kFwdLen>(p, win);
   if (p.live) by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
-    Pack<T, V> xr[kLen], gr[kLen];
-    float d[kLen];
+    Pack<T, V> xr[kFwdLen], gr[kFwdLen];
+    float d[kFwdLen];
 #pragma unroll
-    for (int t = 0; t < kLen; ++t) {
+    for (int t = 0; t < kFwdLen; ++t) {
       const uint32_t i = PLAIN ? t : min(t, p.n - 1);
       xr[t] = load_pack<T, V>(rx.template at<PLAIN>(i));
       gr[t] = load_pack<T, V>(rg.template at<PLAIN>(i));
       d[t] = DT ? *rd.template at<PLAIN>(i) : 1.f;
     }
 #pragma unroll
-    for (int t = 0; t < kLen; ++t) {
+    for (int t = 0; t < kFwdLen; ++t) {
       if (!PLAIN && win.starts(start, s.B, p.i0, t)) {
         reset = true;
         load_or_zero<V>(h0, win.b * s.D + p.c, U);
@@ -480,20 +487,22 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_apply(ScanGeo s, const T* _
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<V, false>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  join_groups<kFwdBlock, V, false>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
   if (!p.live) return;
   win = begin;
   float h[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     h[k] = past(Z[k], U[k], carry ? carry[(p.c + k) * s.cstride + blockIdx.x] : 0.f);
-    if (states) states[p.i0 / kLen * s.D + p.c + k] = h[k];
   }
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-    for (int t = 0; t < kLen; ++t) {
+    for (int t = 0; t < kFwdLen; ++t) {
       if (!PLAIN && t >= p.n) continue;
+      if (t % kBwdLen == 0 && states)
+#pragma unroll
+        for (int k = 0; k < V; ++k) states[(p.i0 + t) / kBwdLen * s.D + p.c + k] = h[k];
       if (!PLAIN && win.starts(start, s.B, p.i0, t)) load_or_zero<V>(h0, win.b * s.D + p.c, h);
 #pragma unroll
       for (int k = 0; k < V; ++k) h[k] = fmaf(a[t][k], h[k], u[t][k]);
@@ -507,27 +516,27 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_apply(ScanGeo s, const T* _
 
 // ------------------------------------------------------------------------------------------- backward
 template <typename T, int V, bool DT, bool GY>
-__global__ void __launch_bounds__(kScanBlock) k_scan_bwd_local(ScanGeo s, const T* __restrict__ g,
+__global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_local(ScanGeo s, const T* __restrict__ g,
                                                                const int64_t* __restrict__ start,
                                                                const float* __restrict__ dt, const T* __restrict__ gy,
                                                                const float* __restrict__ glast, float* __restrict__ cz,
                                                                float* __restrict__ cu) {
-  __shared__ JoinLds<V> lds;
-  const Place p = place_of<V>(s, blockIdx.x);
-  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
-  const Rows<const T> ry(s, p, gy, s.sgy, blockIdx.x);
-  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
-  rd.off = p.gi * kLen * 4;
-  Descend win(start, s.B, wave_first_token(s, blockIdx.x), p.i0, p.n);
+  __shared__ JoinLds<kBwdBlock, V> lds;
+  const Place p = place_of<kBwdLen, V>(s, blockIdx.x);
+  const Rows<const T, kBwdLen> rg(s, p, g, s.sg, blockIdx.x);
+  const Rows<const T, kBwdLen> ry(s, p, gy, s.sgy, blockIdx.x);
+  Rows<const float, kBwdLen> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kBwdLen * 4;
+  Descend win(start, s.B, wave_first_token<kBwdLen>(s, blockIdx.x), p.i0, p.n);
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
-  if (p.live) by_flag(plain_wave(p, win), [&](auto flag) {
+  if (p.live) by_flag(plain_wave<kBwdLen>(p, win), [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-    for (int q0 = kLen - kAhead; q0 >= 0; q0 -= kAhead) {
+    for (int q0 = kBwdLen - kAhead; q0 >= 0; q0 -= kAhead) {
       if (!PLAIN && q0 >= p.n) continue;
       Pack<T, V> gr[kAhead], yr[kAhead];
       float d[kAhead];
@@ -560,50 +569,50 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_bwd_local(ScanGeo s, const 
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<V, true>(s, lds, Z, U, s.nchunk - 1 - blockIdx.x, cz, cu);
+  join_groups<kBwdBlock, V, true>(s, lds, Z, U, s.nchunk - 1 - blockIdx.x, cz, cu);
 }
 
 // gx = H w, gg = H w (x (1 - w) - dt a h_{i-1}) with H_i = gy_i + C_{i+1}; gh0 = C at a window's first token.
 template <typename T, int V, bool DT, bool GY>
-__global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
+__global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
                                                                const int64_t* __restrict__ start,
                                                                const float* __restrict__ dt, const float* __restrict__ h0,
                                                                const float* __restrict__ states,
                                                                const T* __restrict__ gy, const float* __restrict__ glast,
                                                                const float* __restrict__ carry, T* __restrict__ gx,
                                                                T* __restrict__ gg, float* __restrict__ gh0) {
-  __shared__ JoinLds<V> lds;
+  __shared__ JoinLds<kBwdBlock, V> lds;
   if (blockIdx.x >= s.nchunk) {
-    if (blockIdx.y == 0) fill_empty(start, s.B, s.D, glast, gh0, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
+    if (blockIdx.y == 0) fill_empty<kBwdBlock>(start, s.B, s.D, glast, gh0, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
     return;
   }
-  const Place p = place_of<V>(s, blockIdx.x);
-  const Rows<const T> rx(s, p, x, s.sx, blockIdx.x);
-  const Rows<const T> rg(s, p, g, s.sg, blockIdx.x);
-  const Rows<const T> ry(s, p, gy, s.sgy, blockIdx.x);
-  Rows<const float> rd(s, p, dt, 1, blockIdx.x);
-  rd.off = p.gi * kLen * 4;
-  const Rows<T> rox(s, p, gx, s.D, blockIdx.x), rog(s, p, gg, s.D, blockIdx.x);
-  const int64_t wf = wave_first_token(s, blockIdx.x);
+  const Place p = place_of<kBwdLen, V>(s, blockIdx.x);
+  const Rows<const T, kBwdLen> rx(s, p, x, s.sx, blockIdx.x);
+  const Rows<const T, kBwdLen> rg(s, p, g, s.sg, blockIdx.x);
+  const Rows<const T, kBwdLen> ry(s, p, gy, s.sgy, blockIdx.x);
+  Rows<const float, kBwdLen> rd(s, p, dt, 1, blockIdx.x);
+  rd.off = p.gi * kBwdLen * 4;
+  const Rows<T, kBwdLen> rox(s, p, gx, s.D, blockIdx.x), rog(s, p, gg, s.D, blockIdx.x);
+  const int64_t wf = wave_first_token<kBwdLen>(s, blockIdx.x);
   Descend win(start, s.B, wf, p.i0, p.n);
   const Descend begin = win;
-  float a[kLen][V], w[kLen][V], f[kLen][V];      // f: gg = H f
-  Pack<T, V> yr[kLen];
+  float a[kBwdLen][V], w[kBwdLen][V], f[kBwdLen][V];      // f: gg = H f
+  Pack<T, V> yr[kBwdLen];
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
-  const bool plain = plain_wave(p, win);
+  const bool plain = plain_wave<kBwdLen>(p, win);
   Ascend up(start, s.B, wf, p.i0);
   if (p.live) by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
-    Pack<T, V> xr[kLen], gr[kLen];
-    float d[kLen], h[V];
+    Pack<T, V> xr[kBwdLen], gr[kBwdLen];
+    float d[kBwdLen], h[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) h[k] = states[p.i0 / kLen * s.D + p.c + k];
+    for (int k = 0; k < V; ++k) h[k] = states[p.i0 / kBwdLen * s.D + p.c + k];
 #pragma unroll
-    for (int t = 0; t < kLen; ++t) {
+    for (int t = 0; t < kBwdLen; ++t) {
       const uint32_t i = PLAIN ? t : min(t, p.n - 1);
       xr[t] = load_pack<T, V>(rx.template at<PLAIN>(i));
       gr[t] = load_pack<T, V>(rg.template at<PLAIN>(i));
@@ -611,7 +620,7 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const 
       d[t] = DT ? *rd.template at<PLAIN>(i) : 1.f;
     }
 #pragma unroll
-    for (int t = 0; t < kLen; ++t) {
+    for (int t = 0; t < kBwdLen; ++t) {
       if (!PLAIN && up.starts(start, s.B, p.i0, t)) load_or_zero<V>(h0, up.b * s.D + p.c, h);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const 
       }
     }
 #pragma unroll
-    for (int t = kLen - 1; t >= 0; --t) {
+    for (int t = kBwdLen - 1; t >= 0; --t) {
       if (!PLAIN && t >= p.n) continue;
       if (!PLAIN && t < p.n - 1) win.step(start, p.i0, t);
       if (!PLAIN && win.last) {
@@ -639,11 +648,11 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const 
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<V, true>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  join_groups<kBwdBlock, V, true>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
   if (!p.live) return;
   win = begin;
 #pragma unroll
-  for (int t = 0; t < kLen; ++t)
+  for (int t = 0; t < kBwdLen; ++t)
     if (GY) asm volatile("" : "+v"(*(Word<sizeof(T) * V>*)&yr[t]));      // as loaded, not widened
   float C[V];
 #pragma unroll
@@ -651,7 +660,7 @@ __global__ void __launch_bounds__(kScanBlock) k_scan_bwd_apply(ScanGeo s, const 
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
-    for (int t = kLen - 1; t >= 0; --t) {
+    for (int t = kBwdLen - 1; t >= 0; --t) {
       if (!PLAIN && t >= p.n) continue;
       if (!PLAIN && t < p.n - 1) win.step(start, p.i0, t);
       if (!PLAIN && win.last) load_or_zero<V>(glast, win.b * s.D + p.c, C);
@@ -705,19 +714,20 @@ int scan_vector(int dtype, int64_t D, int64_t strides, const void* const* ptrs, 
   return 2;
 }
 
-// A row's threads: its channels over V, in equal parts of at most half a workgroup.  A group is kLen tokens whatever V
-// is: the backward reads the forward's start states per group.
+// A row's threads: its channels over V, in equal parts of at most half a workgroup.  The states the
+// backward starts from lie kBwdLen tokens apart whatever V is.
+template <int LEN, int BLOCK>
 ScanPlan scan_plan(int64_t N, int64_t D, int V) {
   ScanPlan q;
   q.V = V;
   q.s.N = N;
   q.s.D = D;
   const int64_t all = (D + V - 1) / V;
-  q.tiles = (unsigned)((all + kScanBlock / 2 - 1) / (kScanBlock / 2));
+  q.tiles = (unsigned)((all + BLOCK / 2 - 1) / (BLOCK / 2));
   q.s.units = (int)((all + q.tiles - 1) / q.tiles);
-  q.s.G = kScanBlock / q.s.units;
+  q.s.G = BLOCK / q.s.units;
   q.s.seg = q.s.G <= 4 ? q.s.G : q.s.G <= 16 ? 4 : q.s.G <= 64 ? 8 : 16;
-  const int64_t chunk = (int64_t)q.s.G * kLen;
+  const int64_t chunk = (int64_t)q.s.G * LEN;
   q.s.nchunk = (N + chunk - 1) / chunk;
   q.s.cstride = (q.s.nchunk + 15) / 16 * 16;
   q.cz = 0;
@@ -733,12 +743,12 @@ bool scan_sizes_ok(int64_t N, int64_t D, int64_t B, int dtype) {
 }
 
 // Whether a chunk's rows at this stride lie within a 32-bit offset.
-bool scan_span_ok(const ScanPlan& q, int64_t stride, int dtype) {
-  return stride < ((int64_t)1 << 32) / dtype_size(dtype) / kLen / q.s.G - q.s.D;
+bool scan_span_ok(const ScanPlan& q, int len, int64_t stride, int dtype) {
+  return stride < ((int64_t)1 << 32) / dtype_size(dtype) / len / q.s.G - q.s.D;
 }
 
 // Workgroups that fill the empty windows' states.
-unsigned scan_fill_blocks(int64_t B, int64_t D) { return (unsigned)std::min<int64_t>(256, (B * D + kScanBlock - 1) / kScanBlock); }
+unsigned scan_fill_blocks(int64_t B, int64_t D) { return (unsigned)std::min<int64_t>(256, (B * D + 511) / 512); }
 
 template <typename F>
 void by_type(int dtype, bool vec, bool dt, F&& f) {
@@ -765,11 +775,14 @@ using namespace atlhip;
 
 extern "C" {
 
-int64_t atl_gated_scan_groups(int64_t N) { return N < 0 ? -1 : (N + kLen - 1) / kLen; }
+int64_t atl_gated_scan_groups(int64_t N) { return N < 0 ? -1 : (N + kBwdLen - 1) / kBwdLen; }
 
 int64_t atl_gated_scan_ws_bytes(int64_t N, int64_t D, int dtype) {
   if (!scan_sizes_ok(N, D, 1, dtype)) return -1;
-  return std::max(scan_plan(N, D, 2).bytes, scan_plan(N, D, 1).bytes);
+  int64_t bytes = 0;
+  for (int V = 1; V <= 2; ++V)
+    bytes = std::max(bytes, std::max(scan_plan<kFwdLen, kFwdBlock>(N, D, V).bytes, scan_plan<kBwdLen, kBwdBlock>(N, D, V).bytes));
+  return bytes;
 }
 
 int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
@@ -781,8 +794,8 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   if (!start || !last || (N > 0 && (!x || !gate || !y)) || (need > 0 && !ws)) { set_error("gated_scan_fwd: null argument"); return 1; }
   if (ws_bytes < need) { set_error("gated_scan_fwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const void* ptrs[] = {x, gate, y};
-  ScanPlan q = scan_plan(N, D, scan_vector(dtype, D, sx | sg, ptrs, 3));
-  if (!scan_span_ok(q, std::max(sx, sg), dtype)) { set_error("gated_scan_fwd: row strides %lld, %lld too large", (long long)sx, (long long)sg); return 1; }
+  ScanPlan q = scan_plan<kFwdLen, kFwdBlock>(N, D, scan_vector(dtype, D, sx | sg, ptrs, 3));
+  if (!scan_span_ok(q, kFwdLen, std::max(sx, sg), dtype)) { set_error("gated_scan_fwd: row strides %lld, %lld too large", (long long)sx, (long long)sg); return 1; }
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = 0; q.s.B = (int)B;
   float* w = (float*)ws;
   const bool many = q.s.nchunk > 1;
@@ -791,12 +804,12 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
     constexpr int V = decltype(v)::value;
     constexpr bool DT = decltype(d)::value;
     if (many) {
-      hipLaunchKernelGGL((k_scan_local<T, V, DT>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+      hipLaunchKernelGGL((k_scan_local<T, V, DT>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kFwdBlock), 0, stream, q.s,
                          (const T*)x, (const T*)gate, start, dt, h0, w + q.cz, w + q.cu);
       hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
                          (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
     }
-    hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + scan_fill_blocks(B, D), q.tiles), dim3(kScanBlock), 0,
+    hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + scan_fill_blocks(B, D), q.tiles), dim3(kFwdBlock), 0,
                        stream, q.s, (const T*)x, (const T*)gate, start, dt, h0, (const float*)(many ? w + q.carry : nullptr),
                        (T*)y, last, states);
   });
@@ -813,8 +826,8 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   if (!start || (N > 0 && (!x || !gate || !states || !gx || !ggate)) || (need > 0 && !ws)) { set_error("gated_scan_bwd: null argument"); return 1; }
   if (ws_bytes < need) { set_error("gated_scan_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const void* ptrs[] = {x, gate, gx, ggate, gy};
-  ScanPlan q = scan_plan(N, D, scan_vector(dtype, D, sx | sg | (gy ? sgy : 0), ptrs, 5));
-  if (!scan_span_ok(q, std::max(sx, std::max(sg, gy ? sgy : 0)), dtype)) { set_error("gated_scan_bwd: row strides too large"); return 1; }
+  ScanPlan q = scan_plan<kBwdLen, kBwdBlock>(N, D, scan_vector(dtype, D, sx | sg | (gy ? sgy : 0), ptrs, 5));
+  if (!scan_span_ok(q, kBwdLen, std::max(sx, std::max(sg, gy ? sgy : 0)), dtype)) { set_error("gated_scan_bwd: row strides too large"); return 1; }
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = sgy; q.s.B = (int)B;
   float* w = (float*)ws;
   const bool many = q.s.nchunk > 1;
@@ -825,12 +838,12 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
     constexpr int V = decltype(v)::value;
     constexpr bool DT = decltype(d)::value, GY = decltype(y)::value;
     if (many) {
-      hipLaunchKernelGGL((k_scan_bwd_local<T, V, DT, GY>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+      hipLaunchKernelGGL((k_scan_bwd_local<T, V, DT, GY>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kBwdBlock), 0, stream, q.s,
                          (const T*)gate, start, dt, (const T*)gy, glast, w + q.cz, w + q.cu);
       hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
                          (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
     }
-    hipLaunchKernelGGL((k_scan_bwd_apply<T, V, DT, GY>), dim3((unsigned)q.s.nchunk + fill, q.tiles), dim3(kScanBlock), 0, stream, q.s,
+    hipLaunchKernelGGL((k_scan_bwd_apply<T, V, DT, GY>), dim3((unsigned)q.s.nchunk + fill, q.tiles), dim3(kBwdBlock), 0, stream, q.s,
                        (const T*)x, (const T*)gate, start, dt, h0, states, (const T*)gy, glast,
                        (const float*)(many ? w + q.carry : nullptr), (T*)gx, (T*)ggate, gh0);
   };
