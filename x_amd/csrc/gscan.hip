@@ -8,7 +8,7 @@
 // The recurrence is associative in (Z, U): h_out = exp(-Z) h_in + U.  Tokens are cut into groups of 16 or 8, one thread
 // per group and V channels; a workgroup holds as many groups side by side as its threads allow (a chunk).  Forward:
 //   1. k_scan_local: every chunk's (Z, U), its groups joined in LDS;
-//   2. k_scan_carry: the state before every chunk;
+//   2. k_scan_block, k_scan_carry: the states before blocks of chunks, and the chunks' ranges within their block;
 //   3. k_scan_apply: decays and inputs once into registers, the groups joined in LDS again, then every group from its
 //      own start state: y, the last states, and (for the backward) the start states.
 // A call of one chunk needs the third alone.  The backward is the same recurrence from the end, C_i = a_i (gy_i +
@@ -84,10 +84,17 @@ __device__ __forceinline__ float rate_of(float M, float P) {
 
 struct ScanGeo {
   int64_t N, D, sx, sg, sgy;          // tokens, channels, row strides in elements
-  int64_t nchunk, cstride;            // chunks, and the distance of two channels' chunk records
+  int64_t nchunk;
   int B;
   int units, G, seg;                  // threads of a row, groups of a workgroup and of a segment of them
+  int segs;                           // segments
+  uint32_t unit_m, seg_m;             // multipliers of divisions by units and by seg (see over())
 };
+
+// n / d for n < 1024 and d < 1024 by the multiplier ceil(2^20 / d): what the multiplier is too large by, n times, stays
+// below 2^20.
+__device__ __forceinline__ int over(int n, uint32_t m) { return (int)((uint32_t)n * m >> 20); }
+inline uint32_t over_multiplier(int d) { return ((1u << 20) + d - 1) / d; }
 
 // Number of entries of start[0, B) below i (start ascends), by the whole wave: 64 probes a step.
 __device__ __forceinline__ int count_below(const int64_t* __restrict__ start, int B, int64_t i) {
@@ -113,7 +120,7 @@ struct Place {
 template <int LEN, int V>
 __device__ __forceinline__ Place place_of(const ScanGeo& s, int64_t chunk) {
   Place p;
-  p.gi = threadIdx.x / s.units;
+  p.gi = over(threadIdx.x, s.unit_m);
   const int un = threadIdx.x - p.gi * s.units;
   p.c = ((int64_t)blockIdx.y * s.units + un) * V;
   p.i0 = (chunk * s.G + p.gi) * LEN;
@@ -146,7 +153,7 @@ struct Rows {
 // The first token of the wave's first group.
 template <int LEN>
 __device__ __forceinline__ int64_t wave_first_token(const ScanGeo& s, int64_t chunk) {
-  return (chunk * s.G + (threadIdx.x & ~(kWave - 1)) / s.units) * LEN;
+  return (chunk * s.G + over(threadIdx.x & ~(kWave - 1), s.unit_m)) * LEN;
 }
 
 // Walks the windows along a group's ascending tokens.  b: the window of the token before (-1 before the first), next:
@@ -233,9 +240,8 @@ __device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<BLOCK, V>&
     l.u[at0 + k] = u[k];
   }
   __syncthreads();
-  const int segs = (s.G + s.seg - 1) / s.seg;
-  for (int e = threadIdx.x; e < segs * width; e += BLOCK) {
-    const int seg = e / width, ch = e - seg * width;
+  for (int e = threadIdx.x; e < s.segs * width; e += BLOCK) {
+    const int seg = over(e / V, s.unit_m), ch = e - seg * width;
     float pz = 0.f, pu = 0.f;
     for (int j = seg * s.seg; j < min((seg + 1) * s.seg, s.G); ++j) {
       const int at = (REV ? s.G - 1 - j : j) * width + ch;
@@ -249,10 +255,10 @@ __device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<BLOCK, V>&
     l.su[e] = pu;
   }
   __syncthreads();
-  if (segs > 1 || cz) {
+  if (s.segs > 1 || cz) {
     for (int ch = threadIdx.x; ch < width; ch += BLOCK) {
       float pz = 0.f, pu = 0.f;
-      for (int seg = 0; seg < segs; ++seg) {
+      for (int seg = 0; seg < s.segs; ++seg) {
         const int at = seg * width + ch;
         const float gz = l.sz[at], gu = l.su[at];
         l.sz[at] = pz;
@@ -262,21 +268,21 @@ __device__ __forceinline__ void join_groups(const ScanGeo& s, JoinLds<BLOCK, V>&
       }
       const int64_t c = (int64_t)blockIdx.y * width + ch;
       if (cz && c < s.D) {
-        cz[c * s.cstride + record] = pz;
-        cu[c * s.cstride + record] = pu;
+        cz[record * s.D + c] = pz;
+        cu[record * s.D + c] = pu;
       }
     }
     if (cz) return;
     __syncthreads();
   }
-  const int gi = threadIdx.x / s.units;
+  const int gi = over(threadIdx.x, s.unit_m);
   if (gi >= s.G) return;
-  const int seg = (REV ? s.G - 1 - gi : gi) / s.seg, ch0 = at0 - gi * width;
+  const int seg = over(REV ? s.G - 1 - gi : gi, s.seg_m), ch0 = at0 - gi * width;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     z[k] = l.z[at0 + k];
     u[k] = l.u[at0 + k];
-    if (segs > 1) {
+    if (s.segs > 1) {
       u[k] = past(z[k], u[k], l.su[seg * width + ch0 + k]);
       z[k] = joined(l.sz[seg * width + ch0 + k], z[k]);
     }
@@ -368,57 +374,105 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_local(ScanGeo s, const T* __
   join_groups<kFwdBlock, V, false>(s, lds, Z, U, blockIdx.x, cz, cu);
 }
 
-// The state before each chunk of one channel per workgroup: a scan over the chunk records in the order of the
-// recurrence, eight to a thread, joined across the wave and then across the waves.
-constexpr int kCarryBlock = 1024, kCarryPer = 8, kCarryTile = kCarryBlock * kCarryPer;
-__global__ void __launch_bounds__(kCarryBlock) k_scan_carry(int64_t nchunk, int64_t cstride, const float* __restrict__ cz,
-                                                            const float* __restrict__ cu, float* __restrict__ carry) {
-  __shared__ float wz[kCarryBlock / kWave], wu[kCarryBlock / kWave];
-  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
-  cz += blockIdx.x * cstride;
-  cu += blockIdx.x * cstride;
-  carry += blockIdx.x * cstride;
-  float h = 0.f;                                  // the state before the tile
-  for (int64_t j0 = 0; j0 < nchunk; j0 += kCarryTile) {
-    const int64_t j = j0 + threadIdx.x * kCarryPer;
-    float z[kCarryPer], u[kCarryPer], tz = 0.f, tu = 0.f;
+// Joins the records of up to kBlockChunks chunks (in the order of the recurrence) per channel: each becomes what lies
+// before its chunk in the block, the block's total goes to bz, bu.  Records lie chunk by chunk, as their workgroups write
+// them: written channel by channel, a line per value, they cost the local kernels a third of their time.
+constexpr int kBlockChunks = 32, kBlockSubs = 4;
+__global__ void __launch_bounds__(kWave* kBlockSubs) k_scan_block(int64_t nchunk, int64_t D, float* __restrict__ cz,
+                                                                  float* __restrict__ cu, float* __restrict__ bz,
+                                                                  float* __restrict__ bu) {
+  constexpr int kPer = kBlockChunks / kBlockSubs;
+  __shared__ float lz[kBlockSubs][kWave], lu[kBlockSubs][kWave];
+  const int lane = threadIdx.x & (kWave - 1), sub = threadIdx.x / kWave;
+  const int64_t c = min((int64_t)blockIdx.y * kWave + lane, D - 1);              // spare lanes repeat the last channel
+  const int64_t j0 = (int64_t)blockIdx.x * kBlockChunks + sub * kPer;
+  float z[kPer], u[kPer];
 #pragma unroll
-    for (int k = 0; k < kCarryPer; ++k) z[k] = u[k] = 0.f;
-    if (j < nchunk) {                             // records past the last one lie within the stride and are not used
-      load_f<kCarryPer>(cz + j, z);
-      load_f<kCarryPer>(cu + j, u);
-    }
+  for (int k = 0; k < kPer; ++k) {
+    const int64_t at = min(j0 + k, nchunk - 1) * D + c;
+    z[k] = cz[at];
+    u[k] = cu[at];
+  }
+  float tz = 0.f, tu = 0.f;
 #pragma unroll
-    for (int k = 0; k < kCarryPer; ++k) {
-      if (j + k >= nchunk) z[k] = u[k] = 0.f;
-      tu = past(z[k], u[k], tu);
-      tz = joined(tz, z[k]);
-    }
+  for (int k = 0; k < kPer; ++k) {
+    const float gz = j0 + k < nchunk ? z[k] : 0.f, gu = j0 + k < nchunk ? u[k] : 0.f;
+    z[k] = tz;
+    u[k] = tu;
+    tu = past(gz, gu, tu);
+    tz = joined(tz, gz);
+  }
+  lz[sub][lane] = tz;
+  lu[sub][lane] = tu;
+  __syncthreads();
+  float pz = 0.f, pu = 0.f;                       // before the sub
+  for (int k = 0; k < sub; ++k) {
+    pu = past(lz[k][lane], lu[k][lane], pu);
+    pz = joined(pz, lz[k][lane]);
+  }
+  if ((int64_t)blockIdx.y * kWave + lane >= D) return;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {         // inclusive over the lanes
-      const float oz = __shfl_up(tz, d, kWave), ou = __shfl_up(tu, d, kWave);
-      if (lane >= d) {
-        tu = past(tz, tu, ou);
-        tz = joined(oz, tz);
-      }
-    }
-    __syncthreads();
-    if (lane == kWave - 1) wz[wid] = tz, wu[wid] = tu;
-    __syncthreads();
-    float mine = h;                               // the state before the wave, and the tile's end
-#pragma unroll
-    for (int w = 0; w < kCarryBlock / kWave; ++w) {
-      if (w == wid) mine = h;
-      h = past(wz[w], wu[w], h);
-    }
-    const float pz = __shfl_up(tz, 1, kWave), pu = __shfl_up(tu, 1, kWave);
-    float at[kCarryPer];
-    at[0] = lane ? past(pz, pu, mine) : mine;
-#pragma unroll
-    for (int k = 1; k < kCarryPer; ++k) at[k] = past(z[k - 1], u[k - 1], at[k - 1]);
-    if (j < nchunk) store_f<kCarryPer>(carry + j, at);
+  for (int k = 0; k < kPer; ++k) {
+    if (j0 + k >= nchunk) break;
+    cz[(j0 + k) * D + c] = joined(pz, z[k]);
+    cu[(j0 + k) * D + c] = past(z[k], u[k], pu);
+  }
+  if (sub == kBlockSubs - 1) {
+    bz[blockIdx.x * D + c] = joined(pz, tz);
+    bu[blockIdx.x * D + c] = past(tz, tu, pu);
   }
 }
+
+// The state before each block of chunks: 16 channels a workgroup, a stretch of the blocks' records per thread, joined
+// across the wave and then across the waves.
+constexpr int kCarryBlock = 1024, kCarryChannels = 16, kCarrySegs = kCarryBlock / kCarryChannels;
+__global__ void __launch_bounds__(kCarryBlock) k_scan_carry(int64_t n, int64_t D, const float* __restrict__ bz,
+                                                            const float* __restrict__ bu, float* __restrict__ carry) {
+  __shared__ float wz[kCarryBlock / kWave][kCarryChannels], wu[kCarryBlock / kWave][kCarryChannels];
+  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+  const int ch = threadIdx.x % kCarryChannels, seg = threadIdx.x / kCarryChannels;
+  const int64_t c = min((int64_t)blockIdx.x * kCarryChannels + ch, D - 1);       // spare threads repeat the last channel
+  const int64_t per = (n + kCarrySegs - 1) / kCarrySegs;
+  const int64_t j0 = min(seg * per, n), j1 = min(j0 + per, n);
+  float tz = 0.f, tu = 0.f;
+#pragma unroll 4
+  for (int64_t j = j0; j < j1; ++j) {
+    const float z = bz[j * D + c], u = bu[j * D + c];
+    tu = past(z, u, tu);
+    tz = joined(tz, z);
+  }
+#pragma unroll
+  for (int d = kCarryChannels; d < kWave; d <<= 1) {      // inclusive over the wave's stretches
+    const float oz = __shfl_up(tz, d, kWave), ou = __shfl_up(tu, d, kWave);
+    if (lane >= d) {
+      tu = past(tz, tu, ou);
+      tz = joined(oz, tz);
+    }
+  }
+  if (lane >= kWave - kCarryChannels) wz[wid][ch] = tz, wu[wid][ch] = tu;
+  __syncthreads();
+  float h = 0.f;                                  // the state before the wave's, then the thread's stretch
+  for (int w = 0; w < wid; ++w) h = past(wz[w][ch], wu[w][ch], h);
+  const float pz = __shfl_up(tz, kCarryChannels, kWave), pu = __shfl_up(tu, kCarryChannels, kWave);
+  if (lane >= kCarryChannels) h = past(pz, pu, h);
+#pragma unroll 4
+  for (int64_t j = j0; j < j1; ++j) {
+    carry[j * D + c] = h;
+    h = past(bz[j * D + c], bu[j * D + c], h);
+  }
+}
+
+// The chunk records of a call, as the apply kernels read them: what lies before a chunk in its block of chunks, and the
+// state before the block (null: one block, from nothing).
+struct Carry {
+  const float *z, *u, *block;
+  // The state before the chunk at the given place in the order; null z: a single chunk.
+  __device__ __forceinline__ float before(int64_t record, int64_t D, int64_t c) const {
+    if (!z) return 0.f;
+    const int64_t at = record * D + c;
+    return past(z[at], u[at], block ? block[record / kBlockChunks * D + c] : 0.f);
+  }
+};
 
 // The empty windows' last states (the backward: the gradients of their first): out[b] = in[b] or zero.
 template <int BLOCK>
@@ -435,7 +489,7 @@ template <typename T, int V, bool DT>
 __global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __restrict__ x, const T* __restrict__ g,
                                                            const int64_t* __restrict__ start,
                                                            const float* __restrict__ dt, const float* __restrict__ h0,
-                                                           const float* __restrict__ carry, T* __restrict__ y,
+                                                           Carry carry, T* __restrict__ y,
                                                            float* __restrict__ last, float* __restrict__ states) {
   __shared__ JoinLds<kFwdBlock, V> lds;
   if (blockIdx.x >= s.nchunk) {
@@ -493,7 +547,7 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __
   float h[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    h[k] = past(Z[k], U[k], carry ? carry[(p.c + k) * s.cstride + blockIdx.x] : 0.f);
+    h[k] = past(Z[k], U[k], carry.before(blockIdx.x, s.D, p.c + k));
   }
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
@@ -579,7 +633,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
                                                                const float* __restrict__ dt, const float* __restrict__ h0,
                                                                const float* __restrict__ states,
                                                                const T* __restrict__ gy, const float* __restrict__ glast,
-                                                               const float* __restrict__ carry, T* __restrict__ gx,
+                                                               Carry carry, T* __restrict__ gx,
                                                                T* __restrict__ gg, float* __restrict__ gh0) {
   __shared__ JoinLds<kBwdBlock, V> lds;
   if (blockIdx.x >= s.nchunk) {
@@ -656,7 +710,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
     if (GY) asm volatile("" : "+v"(*(Word<sizeof(T) * V>*)&yr[t]));      // as loaded, not widened
   float C[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) C[k] = past(Z[k], U[k], carry ? carry[(p.c + k) * s.cstride + s.nchunk - 1 - blockIdx.x] : 0.f);
+  for (int k = 0; k < V; ++k) C[k] = past(Z[k], U[k], carry.before(s.nchunk - 1 - blockIdx.x, s.D, p.c + k));
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
@@ -702,7 +756,8 @@ struct ScanPlan {
   ScanGeo s;
   int V;
   unsigned tiles;
-  int64_t cz, cu, carry, bytes;                  // workspace offsets in floats, and its size in bytes
+  int64_t blocks;                                // of chunks
+  int64_t cz, cu, bz, bu, carry, bytes;          // workspace offsets in floats, and its size in bytes
 };
 
 // Two channels a thread where widths, strides and addresses allow it, else one: a thread keeps the decays, weights and
@@ -727,13 +782,18 @@ ScanPlan scan_plan(int64_t N, int64_t D, int V) {
   q.s.units = (int)((all + q.tiles - 1) / q.tiles);
   q.s.G = BLOCK / q.s.units;
   q.s.seg = q.s.G <= 4 ? q.s.G : q.s.G <= 16 ? 4 : q.s.G <= 64 ? 8 : 16;
+  q.s.segs = (q.s.G + q.s.seg - 1) / q.s.seg;
+  q.s.unit_m = over_multiplier(q.s.units);
+  q.s.seg_m = over_multiplier(q.s.seg);
   const int64_t chunk = (int64_t)q.s.G * LEN;
   q.s.nchunk = (N + chunk - 1) / chunk;
-  q.s.cstride = (q.s.nchunk + 15) / 16 * 16;
+  q.blocks = (q.s.nchunk + kBlockChunks - 1) / kBlockChunks;
   q.cz = 0;
-  q.cu = q.s.cstride * D;
-  q.carry = 2 * q.cu;
-  q.bytes = q.s.nchunk > 1 ? 3 * q.cu * 4 : 0;
+  q.cu = q.s.nchunk * D;
+  q.bz = 2 * q.cu;
+  q.bu = q.bz + q.blocks * D;
+  q.carry = q.bu + q.blocks * D;
+  q.bytes = q.s.nchunk > 1 ? (q.carry + q.blocks * D) * 4 : 0;
   return q;
 }
 
@@ -745,6 +805,17 @@ bool scan_sizes_ok(int64_t N, int64_t D, int64_t B, int dtype) {
 // Whether a chunk's rows at this stride lie within a 32-bit offset.
 bool scan_span_ok(const ScanPlan& q, int len, int64_t stride, int dtype) {
   return stride < ((int64_t)1 << 32) / dtype_size(dtype) / len / q.s.G - q.s.D;
+}
+
+// Joins the chunk records that the local kernels wrote.
+Carry scan_join(const ScanPlan& q, float* w, hipStream_t stream) {
+  const int64_t D = q.s.D;
+  hipLaunchKernelGGL(k_scan_block, dim3((unsigned)q.blocks, grid_for(D, kWave)), dim3(kWave * kBlockSubs), 0, stream,
+                     q.s.nchunk, D, w + q.cz, w + q.cu, w + q.bz, w + q.bu);
+  if (q.blocks > 1)
+    hipLaunchKernelGGL(k_scan_carry, dim3(grid_for(D, kCarryChannels)), dim3(kCarryBlock), 0, stream, q.blocks, D,
+                       (const float*)(w + q.bz), (const float*)(w + q.bu), w + q.carry);
+  return Carry{w + q.cz, w + q.cu, q.blocks > 1 ? w + q.carry : nullptr};
 }
 
 // Workgroups that fill the empty windows' states.
@@ -799,6 +870,7 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = 0; q.s.B = (int)B;
   float* w = (float*)ws;
   const bool many = q.s.nchunk > 1;
+  Carry carry{};
   by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
@@ -806,11 +878,10 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
     if (many) {
       hipLaunchKernelGGL((k_scan_local<T, V, DT>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kFwdBlock), 0, stream, q.s,
                          (const T*)x, (const T*)gate, start, dt, h0, w + q.cz, w + q.cu);
-      hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
-                         (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
+      carry = scan_join(q, w, stream);
     }
     hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + scan_fill_blocks(B, D), q.tiles), dim3(kFwdBlock), 0,
-                       stream, q.s, (const T*)x, (const T*)gate, start, dt, h0, (const float*)(many ? w + q.carry : nullptr),
+                       stream, q.s, (const T*)x, (const T*)gate, start, dt, h0, carry,
                        (T*)y, last, states);
   });
   return check_launch("gated_scan_fwd");
@@ -831,6 +902,7 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = sgy; q.s.B = (int)B;
   float* w = (float*)ws;
   const bool many = q.s.nchunk > 1;
+  Carry carry{};
   const unsigned fill = gh0 ? scan_fill_blocks(B, D) : 0;
   if (q.s.nchunk + fill == 0) return 0;
   auto go = [&](auto t, auto v, auto d, auto y) {
@@ -840,12 +912,11 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
     if (many) {
       hipLaunchKernelGGL((k_scan_bwd_local<T, V, DT, GY>), dim3((unsigned)q.s.nchunk, q.tiles), dim3(kBwdBlock), 0, stream, q.s,
                          (const T*)gate, start, dt, (const T*)gy, glast, w + q.cz, w + q.cu);
-      hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)D), dim3(kCarryBlock), 0, stream, q.s.nchunk, q.s.cstride,
-                         (const float*)(w + q.cz), (const float*)(w + q.cu), w + q.carry);
+      carry = scan_join(q, w, stream);
     }
     hipLaunchKernelGGL((k_scan_bwd_apply<T, V, DT, GY>), dim3((unsigned)q.s.nchunk + fill, q.tiles), dim3(kBwdBlock), 0, stream, q.s,
                        (const T*)x, (const T*)gate, start, dt, h0, states, (const T*)gy, glast,
-                       (const float*)(many ? w + q.carry : nullptr), (T*)gx, (T*)ggate, gh0);
+                       carry, (T*)gx, (T*)ggate, gh0);
   };
   by_type(dtype, q.V > 1, dt != nullptr, [&](auto t, auto v, auto d) {
     if (gy) go(t, v, d, std::true_type{});
