@@ -11,7 +11,7 @@
 //   gw = sum over the rows of gy shat.
 //
 // A row lies in the registers of a power of two of lanes (a wave at most, or a workgroup for the widest), which read
-// 16 bytes each where widths and addresses allow: one pass over memory.  Sums are fp32.
+// 16 bytes each, aligned to them where widths, strides and addresses are: one pass over memory.  Sums are fp32.
 #include "philox.h"
 #include "typed.h"
 #include "../../include/atl_hip.h"
@@ -38,15 +38,13 @@ struct NormGeo {
 template <int V>
 __device__ __forceinline__ void dropout(const NormGeo& n, int64_t row, int64_t c, float (&v)[V]) {
   const U4 r = philox4x32_10(U4{(uint32_t)row, 0x80000000u | (uint32_t)(c >> 3), n.o0, n.o1}, n.k0, n.k1);
-  uint32_t w[(V + 1) / 2];
+  uint32_t w[V / 2];
   if constexpr (V == 8) {
     w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
-  } else if constexpr (V == 4) {
+  } else {
+    static_assert(V == 4, "pieces of four or eight elements");
     const bool hi = c & 4;
     w[0] = hi ? r.z : r.x, w[1] = hi ? r.w : r.y;
-  } else {
-    const uint32_t word = (c & 4) ? ((c & 2) ? r.w : r.z) : ((c & 2) ? r.y : r.x);
-    w[0] = (c & 1) ? word >> 16 : word;
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) v[k] = ((w[k >> 1] >> ((k & 1) * 16)) & 0xFFFFu) >= n.t ? v[k] * n.keep : 0.f;
@@ -82,22 +80,36 @@ __device__ __forceinline__ float row_top(float v, int cl2, float* lds) {
 }
 
 template <int V>
-__device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V]) {
-  if constexpr (V >= 4) {
-    int w[V / 4];
+__device__ __forceinline__ void store_fp8(uint8_t* p, int64_t n, bool whole, const float (&v)[V]) {
+  int w[V / 4];
 #pragma unroll
-    for (int k = 0; k < V / 4; ++k) {
-      w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
-      w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], w[k], true);
-    }
+  for (int k = 0; k < V / 4; ++k) {
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+    w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], w[k], true);
+  }
+  if (whole) {
     *reinterpret_cast<Pack<int, V / 4>*>(p) = *reinterpret_cast<const Pack<int, V / 4>*>(w);
   } else {
-    *p = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xFF);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < n) p[k] = (uint8_t)(w[k / 4] >> (k % 4 * 8));
   }
 }
 
+// A piece from column c on of a row of D: aligned and whole, or neither.
+template <bool WHOLE, int V, typename T>
+__device__ __forceinline__ void load_piece(const T* row, int64_t c, int64_t D, float (&v)[V]) {
+  if constexpr (WHOLE) load_f<V>(row + c, v);
+  else load_loose<V>(row + c, D - c, v);
+}
+template <bool WHOLE, int V, typename T>
+__device__ __forceinline__ void store_piece(T* row, int64_t c, int64_t D, const float (&v)[V]) {
+  if constexpr (WHOLE) store_f<V>(row + c, v);
+  else store_loose<V>(row + c, D - c, v);
+}
+
 // Q8: y in e4m3 with a scale per row, a / 448 with a = max |y|.
-template <typename T, typename R, int V, int NV, bool WIDE, bool Q8>
+template <typename T, typename R, int V, int NV, bool WIDE, bool WHOLE, bool Q8>
 __global__ void __launch_bounds__(kBlock) k_norm_fwd(NormGeo n, const T* __restrict__ x, const R* __restrict__ res,
                                                      const float* __restrict__ w, void* __restrict__ y,
                                                      R* __restrict__ s, float* __restrict__ scale) {
@@ -116,15 +128,15 @@ __global__ void __launch_bounds__(kBlock) k_norm_fwd(NormGeo n, const T* __restr
       for (int k = 0; k < V; ++k) v[j][k] = 0.f;
       continue;
     }
-    load_f<V>(x + row * n.sx + c, v[j]);
+    load_piece<WHOLE, V>(x + row * n.sx, c, n.D, v[j]);
     if (n.t) dropout<V>(n, row, c, v[j]);
     if (res) {
       float rv[V];
-      load_f<V>(res + row * n.sr + c, rv);
+      load_piece<WHOLE, V>(res + row * n.sr, c, n.D, rv);
 #pragma unroll
       for (int k = 0; k < V; ++k) v[j][k] = rv[k] + v[j][k];
     }
-    if (s) store_f<V>(s + row * n.D + c, v[j]);
+    if (s) store_piece<WHOLE, V>(s + row * n.D, c, n.D, v[j]);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       v[j][k] = (float)(R)v[j][k];
@@ -138,13 +150,13 @@ __global__ void __launch_bounds__(kBlock) k_norm_fwd(NormGeo n, const T* __restr
     const int64_t c = ((int64_t)j * lanes + lane) * V;
     if (c >= n.D) continue;
     float wv[V];
-    load_f<V>(w + c, wv);
+    load_piece<WHOLE, V>(w, c, n.D, wv);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       v[j][k] = v[j][k] * inv * wv[k];
       if (Q8) top = top_of(top, fabsf(v[j][k]));
     }
-    if (!Q8) store_f<V>((T*)y + row * n.D + c, v[j]);
+    if (!Q8) store_piece<WHOLE, V>((T*)y + row * n.D, c, n.D, v[j]);
   }
   if constexpr (Q8) {
     top = top_of(row_top<WIDE>(top, n.cl2, lds), kFp8Least);
@@ -155,14 +167,14 @@ __global__ void __launch_bounds__(kBlock) k_norm_fwd(NormGeo n, const T* __restr
       if (c >= n.D) continue;
 #pragma unroll
       for (int k = 0; k < V; ++k) v[j][k] *= to8;
-      store_fp8<V>((uint8_t*)y + row * n.D + c, v[j]);
+      store_fp8<V>((uint8_t*)y + row * n.D + c, n.D - c, WHOLE, v[j]);
     }
     if (lane == 0) scale[row] = top * (1.f / kFp8Max);
   }
 }
 
 // part (gridDim.x, D): the workgroup's share of gw, its rows added in a fixed order.
-template <typename T, typename R, int V, int NV, bool WIDE>
+template <typename T, typename R, int V, int NV, bool WIDE, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restrict__ s, const float* __restrict__ w,
                                                      const T* __restrict__ gy, const R* __restrict__ gs,
                                                      T* __restrict__ gx, R* __restrict__ gres,
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
     const int64_t c = ((int64_t)j * lanes + lane) * V;
 #pragma unroll
     for (int k = 0; k < V; ++k) wv[j][k] = gw[j][k] = 0.f;
-    if (c < n.D) load_f<V>(w + c, wv[j]);
+    if (c < n.D) load_piece<WHOLE, V>(w, c, n.D, wv[j]);
   }
   for (int64_t row = (int64_t)blockIdx.x * rows + gi; row < n.N; row += (int64_t)gridDim.x * rows) {
     float sv[NV][V], yv[NV][V];
@@ -188,8 +200,8 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
 #pragma unroll
       for (int k = 0; k < V; ++k) sv[j][k] = yv[j][k] = 0.f;
       if (c >= n.D) continue;
-      load_f<V>(s + row * n.sr + c, sv[j]);
-      if (gy) load_f<V>(gy + row * n.sgy + c, yv[j]);
+      load_piece<WHOLE, V>(s + row * n.sr, c, n.D, sv[j]);
+      if (gy) load_piece<WHOLE, V>(gy + row * n.sgy, c, n.D, yv[j]);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         ss = fmaf(sv[j][k], sv[j][k], ss);
@@ -204,7 +216,7 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
       if (c >= n.D) continue;
       float d[V];
       if (gs)
-        load_f<V>(gs + row * n.sgs + c, d);
+        load_piece<WHOLE, V>(gs + row * n.sgs, c, n.D, d);
       else
 #pragma unroll
         for (int k = 0; k < V; ++k) d[k] = 0.f;
@@ -214,10 +226,10 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
         gw[j][k] = fmaf(yv[j][k], hat, gw[j][k]);
         d[k] = fmaf(inv, fmaf(wv[j][k], yv[j][k], -hat * mean), d[k]);
       }
-      if (gres) store_f<V>(gres + row * n.D + c, d);
+      if (gres) store_piece<WHOLE, V>(gres + row * n.D, c, n.D, d);
       if (gx) {
         if (n.t) dropout<V>(n, row, c, d);
-        store_f<V>(gx + row * n.D + c, d);
+        store_piece<WHOLE, V>(gx + row * n.D, c, n.D, d);
       }
     }
   }
@@ -236,40 +248,44 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
   }
 }
 
-// gw[c] = sum over the workgroups' shares, 16 interleaved runs of them side by side.
-constexpr int kSumRuns = 16;
-__global__ void __launch_bounds__(kWave* kSumRuns) k_norm_gw(const float* __restrict__ part, int nblk, int64_t D,
-                                                             float* __restrict__ gw) {
-  __shared__ float lds[kSumRuns][kWave];
-  const int lane = threadIdx.x & (kWave - 1), run = threadIdx.x / kWave;
-  const int64_t c = (int64_t)blockIdx.x * kWave + lane;
+// gw[c] = sum over the workgroups' shares: 16 channels a workgroup, 64 interleaved runs of the shares side by side.
+constexpr int kSumChannels = 16, kSumRuns = 64;
+__global__ void __launch_bounds__(kSumChannels* kSumRuns) k_norm_gw(const float* __restrict__ part, int nblk, int64_t D,
+                                                                    float* __restrict__ gw) {
+  __shared__ float lds[kSumRuns][kSumChannels];
+  const int ch = threadIdx.x % kSumChannels, run = threadIdx.x / kSumChannels;
+  const int64_t c = (int64_t)blockIdx.x * kSumChannels + ch;
   float sum = 0.f;
   if (c < D)
+#pragma unroll 4
     for (int b = run; b < nblk; b += kSumRuns) sum += part[b * D + c];
-  lds[run][lane] = sum;
+  lds[run][ch] = sum;
   __syncthreads();
-  if (run == 0 && c < D) {
-    for (int k = 1; k < kSumRuns; ++k) sum += lds[k][lane];
-    gw[c] = sum;
+  for (int half = kSumRuns / 2; half >= 1; half /= 2) {
+    if (run < half) lds[run][ch] += lds[run + half][ch];
+    __syncthreads();
   }
+  if (run == 0 && c < D) gw[c] = lds[0][ch];
 }
 
 // ------------------------------------------------------------------------------------------- host
 struct NormPlan {
   int V, NV, cl2;
-  bool wide;
+  bool wide, whole;
 };
 
-// V: 16 bytes of x where the width, strides and addresses are multiples of it, else one element.  A row takes as few
-// lanes as hold it with one vector each, then up to four vectors (16 elements) a lane, then a workgroup.
-NormPlan norm_plan(int dtype, int64_t D, bool vec) {
+// V: 16 bytes of x; whole: the width, strides and addresses are multiples of it (else pieces are read as they lie, and a
+// row's last one in part: 60007 x 345 single precision forward and backward runs 230 us with single elements instead).
+// A row takes as few lanes as hold it with one piece each, then up to four pieces a lane, then a workgroup.
+NormPlan norm_plan(int dtype, int64_t D, bool whole) {
   NormPlan q;
-  q.V = vec ? 16 / dtype_size(dtype) : 1;
+  q.V = 16 / dtype_size(dtype);
+  q.whole = whole;
   const int64_t units = (D + q.V - 1) / q.V;
   q.cl2 = 0;
   while ((1 << q.cl2) < kWave && (1 << q.cl2) < units) ++q.cl2;
   const int64_t per = (units + (1 << q.cl2) - 1) >> q.cl2;
-  q.wide = per > (q.V == 1 ? 16 : 4);
+  q.wide = per > 4;
   q.NV = q.wide ? 32 / q.V : ceil_pow2(per);
   return q;
 }
@@ -292,22 +308,14 @@ template <typename T, typename F>
 void by_shape(const NormPlan& q, F&& f) {
   constexpr int VM = 16 / sizeof(T);
   using std::integral_constant;
-  auto go = [&](auto v, auto nv, auto wide) { f(v, nv, wide); };
-#define ATL_NORM_CASE(v, nv, wide) go(integral_constant<int, v>{}, integral_constant<int, nv>{}, integral_constant<bool, wide>{})
-  if (q.V == 1) {
-    if (q.wide) ATL_NORM_CASE(1, 32, true);
-    else if (q.NV == 1) ATL_NORM_CASE(1, 1, false);
-    else if (q.NV == 2) ATL_NORM_CASE(1, 2, false);
-    else if (q.NV == 4) ATL_NORM_CASE(1, 4, false);
-    else if (q.NV == 8) ATL_NORM_CASE(1, 8, false);
-    else ATL_NORM_CASE(1, 16, false);
-  } else {
-    if (q.wide) ATL_NORM_CASE(VM, 32 / VM, true);
-    else if (q.NV == 1) ATL_NORM_CASE(VM, 1, false);
-    else if (q.NV == 2) ATL_NORM_CASE(VM, 2, false);
-    else ATL_NORM_CASE(VM, 4, false);
-  }
-#undef ATL_NORM_CASE
+  auto go = [&](auto nv, auto wide) {
+    if (q.whole) f(integral_constant<int, VM>{}, nv, wide, std::true_type{});
+    else f(integral_constant<int, VM>{}, nv, wide, std::false_type{});
+  };
+  if (q.wide) go(integral_constant<int, 32 / VM>{}, std::true_type{});
+  else if (q.NV == 1) go(integral_constant<int, 1>{}, std::false_type{});
+  else if (q.NV == 2) go(integral_constant<int, 2>{}, std::false_type{});
+  else go(integral_constant<int, 4>{}, std::false_type{});
 }
 
 bool norm_ok(int dtype, int rtype, int64_t N, int64_t D, double eps, double p) {
@@ -327,7 +335,7 @@ NormGeo norm_geo(int64_t N, int64_t D, double eps, double p, uint64_t seed, uint
   return n;
 }
 
-bool norm_vec(int dtype, int64_t D, int64_t strides, const void* const* ptrs, int n) {
+bool norm_whole(int dtype, int64_t D, int64_t strides, const void* const* ptrs, int n) {
   const int v = 16 / dtype_size(dtype);
   if (D % v || strides % v) return false;
   for (int k = 0; k < n; ++k)
@@ -351,20 +359,20 @@ int atl_rms_norm_fwd(const void* x, int64_t sx, int dtype, const void* res, int6
   NormGeo n = norm_geo(N, D, eps, p, seed, offset);
   n.sx = sx; n.sr = sr;
   const void* ptrs[] = {x, res, w, y, s};
-  const NormPlan q = norm_plan(dtype, D, norm_vec(dtype, D, sx | (res ? sr : 0), ptrs, 5));
+  const NormPlan q = norm_plan(dtype, D, norm_whole(dtype, D, sx | (res ? sr : 0), ptrs, 5));
   n.cl2 = q.cl2;
   const dim3 grid(q.wide ? (unsigned)N : grid_for(N, kBlock >> q.cl2));
   by_types(dtype, rtype, [&](auto t, auto r) {
     using T = decltype(t);
     using R = decltype(r);
-    by_shape<T>(q, [&](auto v, auto nv, auto wide) {
+    by_shape<T>(q, [&](auto v, auto nv, auto wide, auto whole) {
       constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-      constexpr bool W = decltype(wide)::value;
+      constexpr bool W = decltype(wide)::value, H = decltype(whole)::value;
       if (scale)
-        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, true>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
+        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, true>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
                            (const R*)res, w, y, (R*)s, scale);
       else
-        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, false>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
+        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, false>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
                            (const R*)res, w, y, (R*)s, scale);
     });
   });
@@ -386,22 +394,22 @@ int atl_rms_norm_bwd(const void* s, int64_t ss, int rtype, const float* w, const
   NormGeo n = norm_geo(N, D, eps, p, seed, offset);
   n.sr = ss; n.sgy = sgy; n.sgs = sgs;
   const void* ptrs[] = {s, w, gy, gs, gx, gres};
-  const NormPlan q = norm_plan(dtype, D, norm_vec(dtype, D, ss | (gy ? sgy : 0) | (gs ? sgs : 0), ptrs, 6));
+  const NormPlan q = norm_plan(dtype, D, norm_whole(dtype, D, ss | (gy ? sgy : 0) | (gs ? sgs : 0), ptrs, 6));
   n.cl2 = q.cl2;
   const int nblk = norm_blocks(N, q);
   if (nblk > 0)
     by_types(dtype, rtype, [&](auto t, auto r) {
       using T = decltype(t);
       using R = decltype(r);
-      by_shape<T>(q, [&](auto v, auto nv, auto wide) {
+      by_shape<T>(q, [&](auto v, auto nv, auto wide, auto whole) {
         constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-        hipLaunchKernelGGL((k_norm_bwd<T, R, V, NV, decltype(wide)::value>), dim3(nblk), dim3(kBlock),
+        hipLaunchKernelGGL((k_norm_bwd<T, R, V, NV, decltype(wide)::value, decltype(whole)::value>), dim3(nblk), dim3(kBlock),
                            kBlock * NV * V * 4, stream, n, (const R*)s, w, (const T*)gy, (const R*)gs, (T*)gx,
                            (R*)gres, gw ? (float*)ws : nullptr);
       });
     });
   if (gw)
-    hipLaunchKernelGGL(k_norm_gw, dim3(grid_for(D, kWave)), dim3(kWave * kSumRuns), 0, stream, (const float*)ws, nblk,
+    hipLaunchKernelGGL(k_norm_gw, dim3(grid_for(D, kSumChannels)), dim3(kSumChannels * kSumRuns), 0, stream, (const float*)ws, nblk,
                        D, gw);
   return check_launch("rms_norm_bwd");
 }

@@ -23,6 +23,37 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
+// The same where a piece is aligned to its elements only (global memory takes that), of its first n elements; the others
+// read as zero and are not written.
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {
+  T e[V];
+};
+template <int V, typename T>
+__device__ __forceinline__ void load_loose(const T* p, int64_t n, float (&v)[V]) {
+  if (n >= V) {
+    const LoosePack<T, V> r = *reinterpret_cast<const LoosePack<T, V>*>(p);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = (float)r.e[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = k < n ? (float)p[k] : 0.f;
+  }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_loose(T* p, int64_t n, const float (&v)[V]) {
+  if (n >= V) {
+    LoosePack<T, V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.e[k] = (T)v[k];
+    *reinterpret_cast<LoosePack<T, V>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < n) p[k] = (T)v[k];
+  }
+}
+
 template <int V, typename T>
 __device__ __forceinline__ void load_f(const T* p, float (&v)[V]) {
   const Pack<T, V> r = load_pack<T, V>(p);
