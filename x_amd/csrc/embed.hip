@@ -7,7 +7,6 @@
 // call however often an id occurs (a hot pixel may own a tenth of a million events).  The sorted positions are cut into
 // equal chunks, so a long run is shared by many lanes: a run inside a chunk is written at once, the partial sums of runs
 // that cross chunks are joined afterwards, in order.  Sums are fp32, each row is rounded once.
-#include "scan.h"
 #include "typed.h"
 #include "../../include/atl_hip.h"
 
@@ -27,26 +26,38 @@ template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kBlock) k_embed_fwd(const void* __restrict__ ids, bool wide, int64_t N, int64_t vocab,
                                                       const T* __restrict__ table, int64_t st, uint32_t units,
                                                       float scale, O* __restrict__ out, int rows) {
+  constexpr int kAhead = 4;                       // pieces in flight: ids, then rows, then stores
   const int64_t r0 = (int64_t)blockIdx.x * rows;
   const uint32_t items = (uint32_t)min((int64_t)rows, N - r0) * units;
-  for (uint32_t e = threadIdx.x; e < items; e += kBlock) {
-    const uint32_t r = e / units, c = (e - r * units) * V;
-    const int64_t id = id_at(ids, wide, r0 + r);
-    float v[V];
-    if (id >= 0 && id < vocab) {
-      load_f<V>(table + id * st + c, v);
+  for (uint32_t e0 = threadIdx.x; e0 < items; e0 += kBlock * kAhead) {
+    int64_t id[kAhead];
+    uint32_t row[kAhead], c[kAhead];
+    Pack<T, V> v[kAhead];
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] *= scale;
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = 0.f;
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t e = min(e0 + k * kBlock, items - 1);
+      row[k] = e / units;
+      c[k] = (e - row[k] * units) * V;
+      id[k] = id_at(ids, wide, r0 + row[k]);
     }
-    store_f<V>(out + (r0 + r) * (int64_t)units * V + c, v);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      v[k] = load_pack<T, V>(table + (id[k] >= 0 && id[k] < vocab ? id[k] : 0) * st + c[k]);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (e0 + k * kBlock >= items) break;
+      float f[V];
+      const bool token = id[k] >= 0 && id[k] < vocab;
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = token ? (float)v[k].e[j] * scale : 0.f;
+      store_f<V>(out + (r0 + row[k]) * (int64_t)units * V + c[k], f);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------- stable radix sort
-constexpr int kSortItems = 16, kSortTile = kBlock * kSortItems, kMaxDigitBits = 10;
+constexpr int kSortBlock = 1024, kSortItems = 4, kSortTile = kSortBlock * kSortItems, kMaxDigitBits = 10;
+constexpr int kSortWaves = kSortBlock / kWave;
 
 // The record at position i: of the first pass from the ids (an id that is no token sorts behind all others).
 template <bool FIRST>
@@ -59,86 +70,180 @@ __device__ __forceinline__ Rec rec_at(const void* __restrict__ src, bool wide, i
   }
 }
 
-// cnt (blocks, digits): how often each digit occurs in the block's tile.
+// Zeros, by 16 bytes, of the given piece of pieces; p is aligned to them.
+__device__ __forceinline__ void clear_piece(uint16_t* __restrict__ p, int64_t halves, int64_t piece, int64_t pieces) {
+  for (int64_t i = (piece * kSortBlock + threadIdx.x) * 8; i < halves; i += pieces * kSortBlock * 8) {
+    if (i + 8 <= halves) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+    else
+      for (int64_t k = i; k < halves; ++k) p[k] = 0;
+  }
+}
+
+// cnt (blocks, digits): how often each digit occurs in the block's tile.  The workgroups past the tiles clear the
+// gradient's rows (of the first pass; most ids may have no token).
 template <bool FIRST>
-__global__ void __launch_bounds__(kBlock) k_sort_count(const void* __restrict__ src, bool wide, int64_t vocab,
-                                                       int64_t N, int shift, int bits, int* __restrict__ cnt) {
+__global__ void __launch_bounds__(kSortBlock) k_sort_count(const void* __restrict__ src, bool wide, int64_t vocab,
+                                                           int64_t N, int shift, int bits, int nblk, int* __restrict__ cnt,
+                                                           uint16_t* __restrict__ gt, int64_t halves) {
   __shared__ int hist[1 << kMaxDigitBits];
+  if ((int)blockIdx.x >= nblk) {
+    clear_piece(gt, halves, blockIdx.x - nblk, gridDim.x - nblk);
+    return;
+  }
   const int nd = 1 << bits;
-  for (int d = threadIdx.x; d < nd; d += kBlock) hist[d] = 0;
+  for (int d = threadIdx.x; d < nd; d += kSortBlock) hist[d] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
-    const int64_t i = base + k * kBlock + threadIdx.x;
+    const int64_t i = base + k * kSortBlock + threadIdx.x;
     if (i < N) atomicAdd(&hist[(rec_at<FIRST>(src, wide, vocab, i).key >> shift) & (nd - 1)], 1);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < nd; d += kBlock) cnt[(int64_t)blockIdx.x * nd + d] = hist[d];
+  for (int d = threadIdx.x; d < nd; d += kSortBlock) cnt[(int64_t)blockIdx.x * nd + d] = hist[d];
 }
 
-// off (digits, blocks): where the block's records of a digit go.  Each wave takes a quarter of the tile in rounds of
-// 64; a record's rank among its wave's records of the same digit is that of its lane among the lanes found equal by a
-// ballot per bit, so equal digits keep their order.
-template <bool FIRST>
-__global__ void __launch_bounds__(kBlock) k_sort_scatter(const void* __restrict__ src, bool wide, int64_t vocab,
-                                                         int64_t N, int shift, int bits, const int* __restrict__ off,
-                                                         int nblk, Rec* __restrict__ dst) {
-  constexpr int W = kBlock / kWave;
-  __shared__ int at[W][1 << kMaxDigitBits];
-  const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  for (int d = lane; d < nd; d += kWave) at[w][d] = 0;
+// In place, per digit: the count of a block becomes that of the blocks before it; tot (digits): of all.  64 digits a
+// workgroup, a stretch of the blocks per wave.
+__global__ void __launch_bounds__(kSortBlock) k_sort_offsets(int* __restrict__ cnt, int nblk, int nd, int* __restrict__ tot) {
+  __shared__ int part[kSortWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int d = min((int)blockIdx.x * kWave + lane, nd - 1);          // spare lanes repeat the last digit
+  const int per = (nblk + kSortWaves - 1) / kSortWaves, b0 = min(w * per, nblk), b1 = min(b0 + per, nblk);
+  int sum = 0;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) sum += cnt[(int64_t)b * nd + d];
+  part[w][lane] = sum;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortTile + w * (kSortTile / W);
-  Rec rec[kSortItems];
-  int rank[kSortItems];
+  int run = 0;
+  for (int k = 0; k < w; ++k) run += part[k][lane];
+  if (w == kSortWaves - 1) tot[d] = run + sum;
+  if ((int)blockIdx.x * kWave + lane >= nd) return;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) {
+    const int n = cnt[(int64_t)b * nd + d];
+    cnt[(int64_t)b * nd + d] = run;
+    run += n;
+  }
+}
+
+struct SortLds {
+  uint16_t at[kSortWaves][1 << kMaxDigitBits];    // a wave's records of a digit so far, then those of the waves before it
+  int base[1 << kMaxDigitBits];                   // where the tile's records of a digit go
+  int wsum[kSortWaves + 1];
+};
+
+// A wave's ranks of its kSortItems x 64 records by digit, in their order: among its lanes of the same digit (found equal
+// by a ballot per bit), behind the digit's records of the rounds before.  Leaves the waves' counts in l.at.
+__device__ __forceinline__ void rank_records(SortLds& l, const Rec (&rec)[kSortItems], const bool (&live)[kSortItems],
+                                             int shift, int bits, int (&rank)[kSortItems]) {
+  const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  for (int d = lane; d < nd; d += kWave) l.at[w][d] = 0;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
-    const int64_t i = base + k * kWave + lane;
-    const bool live = i < N;
-    rec[k] = live ? rec_at<FIRST>(src, wide, vocab, i) : Rec{0, 0};
     const int d = (rec[k].key >> shift) & (nd - 1);
-    uint64_t same = __ballot(live);
+    uint64_t same = __ballot(live[k]);
     for (int b = 0; b < bits; ++b) {
       const uint64_t one = __ballot((d >> b) & 1);
       same &= (d >> b) & 1 ? one : ~one;
     }
-    const int before = live ? at[w][d] : 0;
-    rank[k] = before + __popcll(same & below);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");        // LDS accesses of one wave take effect in order
-    if (live && (same & below) == 0) at[w][d] = before + __popcll(same);
+    const int before = live[k] ? l.at[w][d] : 0;
+    rank[k] = before + __popcll(same & below);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (live[k] && (same & below) == 0) l.at[w][d] = (uint16_t)(before + __popcll(same));
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < nd; d += kBlock) {
-    int run = off[(int64_t)d * nblk + blockIdx.x];
+  for (int d = threadIdx.x; d < nd; d += kSortBlock) {            // the waves' counts into those before each
+    int run = 0;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const int n = at[j][d];
-      at[j][d] = run;
+    for (int j = 0; j < kSortWaves; ++j) {
+      const int n = l.at[j][d];
+      l.at[j][d] = (uint16_t)run;
       run += n;
     }
+    l.base[d] = run;
   }
   __syncthreads();
+}
+
+// off (blocks, digits), tot (digits): as k_sort_offsets leaves them.
+template <bool FIRST>
+__global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const void* __restrict__ src, bool wide, int64_t vocab,
+                                                             int64_t N, int shift, int bits, const int* __restrict__ off,
+                                                             const int* __restrict__ tot, Rec* __restrict__ dst) {
+  __shared__ SortLds l;
+  const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int64_t i0 = (int64_t)blockIdx.x * kSortTile + w * (kWave * kSortItems) + lane;
+  Rec rec[kSortItems];
+  bool live[kSortItems];
+  int rank[kSortItems];
 #pragma unroll
-  for (int k = 0; k < kSortItems; ++k)
-    if (base + k * kWave + lane < N) dst[at[w][(rec[k].key >> shift) & (nd - 1)] + rank[k]] = rec[k];
+  for (int k = 0; k < kSortItems; ++k) {
+    live[k] = i0 + k * kWave < N;
+    rec[k] = live[k] ? rec_at<FIRST>(src, wide, vocab, i0 + k * kWave) : Rec{0, 0};
+  }
+  const int t = (int)threadIdx.x < nd ? tot[threadIdx.x] : 0;
+  rank_records(l, rec, live, shift, bits, rank);
+  int total;
+  const int before = block_exclusive_scan<kSortBlock>(t, l.wsum, total);        // records of smaller digits
+  if ((int)threadIdx.x < nd) l.base[threadIdx.x] = before + off[(int64_t)blockIdx.x * nd + threadIdx.x];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int d = (rec[k].key >> shift) & (nd - 1);
+    if (live[k]) dst[l.base[d] + l.at[w][d] + rank[k]] = rec[k];
+  }
+}
+
+// All passes of up to a tile's tokens in one workgroup; the other workgroups clear the gradient's rows.
+__global__ void __launch_bounds__(kSortBlock) k_sort_small(const void* __restrict__ ids, bool wide, int64_t vocab, int64_t N,
+                                                           int passes, int bits, Rec* __restrict__ dst,
+                                                           uint16_t* __restrict__ gt, int64_t halves) {
+  __shared__ SortLds l;
+  if (blockIdx.x > 0) {
+    clear_piece(gt, halves, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
+  const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int i0 = w * (kWave * kSortItems) + lane;
+  Rec rec[kSortItems];
+  bool live[kSortItems];
+  int rank[kSortItems];
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    live[k] = i0 + k * kWave < N;
+    rec[k] = live[k] ? rec_at<true>(ids, wide, vocab, i0 + k * kWave) : Rec{0, 0};
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    rank_records(l, rec, live, shift, bits, rank);
+    int total;
+    const int n = (int)threadIdx.x < nd ? l.base[threadIdx.x] : 0;
+    const int before = block_exclusive_scan<kSortBlock>(n, l.wsum, total);
+    if ((int)threadIdx.x < nd) l.base[threadIdx.x] = before;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+      const int d = (rec[k].key >> shift) & (nd - 1);
+      if (live[k]) dst[l.base[d] + l.at[w][d] + rank[k]] = rec[k];
+    }
+    __syncthreads();                              // the workgroup's own stores are seen past this
+    if (pass + 1 < passes)
+#pragma unroll
+      for (int k = 0; k < kSortItems; ++k)
+        if (live[k]) rec[k] = dst[i0 + k * kWave];
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------------------------------- sums of the runs
-constexpr int kChunk = 64;            // sorted positions of a group of lanes
 constexpr int kAhead = 8;             // rows in flight
-
-// Zeros, by 16 bytes; p is aligned to them.
-__global__ void __launch_bounds__(kBlock) k_clear(uint16_t* __restrict__ p, int64_t halves) {
-  const int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
-  if (i + 8 <= halves) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
-  else
-    for (int64_t k = i; k < halves; ++k) p[k] = 0;
-}
 
 struct RunGeo {
   int64_t N, D, sgo, nchunk;
+  int chunk;                          // sorted positions of a group of lanes
   uint32_t vocab;
   int cl2;
   float scale;
@@ -150,7 +255,7 @@ __global__ void __launch_bounds__(kBlock) k_embed_runs(RunGeo g, const Rec* __re
                                                        O* __restrict__ gt, float* __restrict__ part) {
   const int64_t chunk = (int64_t)blockIdx.x * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
   const int64_t c = (((int64_t)blockIdx.y << g.cl2) + (threadIdx.x & ((1 << g.cl2) - 1))) * V;
-  const int64_t p0 = chunk * kChunk, p1 = min(p0 + kChunk, g.N);
+  const int64_t p0 = chunk * g.chunk, p1 = min(p0 + g.chunk, g.N);
   if (p0 >= g.N || c >= g.D) return;
   float acc[V];
 #pragma unroll
@@ -206,15 +311,22 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
   const bool live = c < g.D;
   int64_t after = 0;                              // chunks behind this one that share its last run
   uint32_t key = 0;
-  const int64_t p0 = chunk * kChunk, p1 = p0 + kChunk;
+  const int64_t p0 = chunk * g.chunk, p1 = p0 + g.chunk;
   if (p1 < g.N) {
     key = rec[p1 - 1].key;
     const bool begins = !(p0 > 0 && rec[p0].key == key && rec[p0 - 1].key == key);
     if (key < g.vocab && rec[p1].key == key && begins) {
-      int64_t lo = chunk + 1, hi = g.nchunk;      // the first chunk in (lo, hi) that begins with another key
+      int64_t lo = chunk + 1, hi = g.nchunk;      // the first chunk in (lo, hi) that begins with another key: most runs
+      for (int64_t far = 1; lo + far < hi; far *= 2) {             // end soon, so look near first
+        if (rec[(lo + far) * g.chunk].key != key) {
+          hi = lo + far;
+          break;
+        }
+        lo += far;
+      }
       while (hi - lo > 1) {
         const int64_t mid = (lo + hi) / 2;
-        if (rec[mid * kChunk].key == key) lo = mid;
+        if (rec[mid * g.chunk].key == key) lo = mid;
         else hi = mid;
       }
       after = hi - chunk - 1;
@@ -265,7 +377,7 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
         for (int k = 0; k < V; ++k) acc[k] += lds[(o * lanes + threadIdx.x) * V + k];
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] *= g.scale;
-      store_f<V>(gt + (int64_t)rec[first * kChunk + kChunk - 1].key * g.D + c, acc);
+      store_f<V>(gt + (int64_t)rec[first * g.chunk + g.chunk - 1].key * g.D + c, acc);
     }
     __syncthreads();
   }
@@ -273,8 +385,9 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
 
 // ------------------------------------------------------------------------------------------- host
 struct SortPlan {
-  int passes, bits, nblk;
-  int64_t rec_a, rec_b, cnt, off, scan, part, bytes;      // workspace offsets in bytes
+  int passes, bits, nblk, chunk;
+  int64_t nchunk;
+  int64_t rec_a, rec_b, cnt, tot, part, bytes;      // workspace offsets in bytes
 };
 
 SortPlan sort_plan(int64_t N, int64_t D, int64_t vocab) {
@@ -284,15 +397,17 @@ SortPlan sort_plan(int64_t N, int64_t D, int64_t vocab) {
   q.passes = (total + kMaxDigitBits - 1) / kMaxDigitBits;
   q.bits = (total + q.passes - 1) / q.passes;
   q.nblk = (int)((N + kSortTile - 1) / kSortTile);
-  const int64_t n = (int64_t)q.nblk << q.bits;
+  // A chunk is worked off row by row: short ones where there are few tokens, so that more lanes share them (3000 tokens:
+  // 22 us with 64 rows a chunk), long ones where partial sums would cost traffic.
+  q.chunk = N <= 16 * kSortTile ? 16 : 64;
+  q.nchunk = (N + q.chunk - 1) / q.chunk;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   q.rec_a = take(N * 8);
   q.rec_b = take(N * 8);
-  q.cnt = take(n * 4);
-  q.off = take((n + 1) * 4);
-  q.scan = take((scan_tiles(n) + 1) * 4);
-  q.part = take((N + kChunk - 1) / kChunk * 2 * D * 4);
+  q.cnt = take(((int64_t)q.nblk << q.bits) * 4);
+  q.tot = take(((int64_t)1 << q.bits) * 4);
+  q.part = take(q.nchunk * 2 * D * 4);
   q.bytes = at;
   return q;
 }
@@ -361,31 +476,42 @@ int atl_embed_bwd(const void* ids, int wide_ids, int64_t N, const void* gout, in
   const SortPlan q = sort_plan(N, D, vocab);
   if (N > 0 && ws_bytes < q.bytes) { set_error("embed_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)q.bytes); return 1; }
   const int64_t halves = vocab * D * dtype_size(ttype) / 2;
-  if ((halves + kBlock * 8 - 1) / (kBlock * 8) >= ((int64_t)1 << 31)) { set_error("embed_bwd: table too large"); return 1; }
-  hipLaunchKernelGGL(k_clear, dim3(grid_for(halves, kBlock * 8)), dim3(kBlock), 0, stream, (uint16_t*)gtable, halves);
-  if (N == 0) return check_launch("embed_bwd");
+  const unsigned clear = (unsigned)std::max<int64_t>(1, std::min<int64_t>(2048, (halves + kSortBlock * 8 - 1) / (kSortBlock * 8)));
   char* w = (char*)ws;
+  Rec* const rec_a = (Rec*)(w + q.rec_a);
+  Rec* const rec_b = (Rec*)(w + q.rec_b);
+  int* const cnt = (int*)(w + q.cnt);
+  int* const tot = (int*)(w + q.tot);
   const void* src = ids;
-  Rec* dst = (Rec*)(w + q.rec_a);
-  for (int pass = 0; pass < q.passes; ++pass) {
-    const int shift = pass * q.bits;
-    int* cnt = (int*)(w + q.cnt);
-    int* off = (int*)(w + q.off);
-    if (pass == 0)
-      hipLaunchKernelGGL((k_sort_count<true>), dim3(q.nblk), dim3(kBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits, cnt);
-    else
-      hipLaunchKernelGGL((k_sort_count<false>), dim3(q.nblk), dim3(kBlock), 0, stream, src, false, vocab, N, shift, q.bits, cnt);
-    scan32t(cnt, 1 << q.bits, q.nblk, (int*)(w + q.scan), off, stream);
-    if (pass == 0)
-      hipLaunchKernelGGL((k_sort_scatter<true>), dim3(q.nblk), dim3(kBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits, (const int*)off, q.nblk, dst);
-    else
-      hipLaunchKernelGGL((k_sort_scatter<false>), dim3(q.nblk), dim3(kBlock), 0, stream, src, false, vocab, N, shift, q.bits, (const int*)off, q.nblk, dst);
-    src = dst;
-    dst = dst == (Rec*)(w + q.rec_a) ? (Rec*)(w + q.rec_b) : (Rec*)(w + q.rec_a);
+  if (q.nblk <= 1) {
+    hipLaunchKernelGGL(k_sort_small, dim3(1 + clear), dim3(kSortBlock), 0, stream, ids, wide_ids != 0, vocab, N, q.passes, q.bits,
+                       rec_a, (uint16_t*)gtable, halves);
+    src = rec_a;
+  } else {
+    for (int pass = 0; pass < q.passes; ++pass) {
+      const int shift = pass * q.bits, nd = 1 << q.bits;
+      Rec* const dst = src == rec_a ? rec_b : rec_a;
+      if (pass == 0)
+        hipLaunchKernelGGL((k_sort_count<true>), dim3(q.nblk + clear), dim3(kSortBlock), 0, stream, src, wide_ids != 0, vocab, N, shift,
+                           q.bits, q.nblk, cnt, (uint16_t*)gtable, halves);
+      else
+        hipLaunchKernelGGL((k_sort_count<false>), dim3(q.nblk), dim3(kSortBlock), 0, stream, src, false, vocab, N, shift, q.bits, q.nblk,
+                           cnt, (uint16_t*)gtable, halves);
+      hipLaunchKernelGGL(k_sort_offsets, dim3(grid_for(nd, kWave)), dim3(kSortBlock), 0, stream, cnt, q.nblk, nd, tot);
+      if (pass == 0)
+        hipLaunchKernelGGL((k_sort_scatter<true>), dim3(q.nblk), dim3(kSortBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits,
+                           (const int*)cnt, (const int*)tot, dst);
+      else
+        hipLaunchKernelGGL((k_sort_scatter<false>), dim3(q.nblk), dim3(kSortBlock), 0, stream, src, false, vocab, N, shift, q.bits,
+                           (const int*)cnt, (const int*)tot, dst);
+      src = dst;
+    }
   }
+  if (N == 0) return check_launch("embed_bwd");
   RunGeo g{};
   g.N = N; g.D = D; g.sgo = sgo; g.vocab = (uint32_t)vocab; g.scale = (float)scale;
-  g.nchunk = (N + kChunk - 1) / kChunk;
+  g.nchunk = q.nchunk;
+  g.chunk = q.chunk;
   const bool vec = D % 8 == 0 && sgo % 8 == 0 && aligned_to(gout, 16);
   const int V = vec ? 16 / dtype_size(otype) : 1;
   while ((1 << g.cl2) < kWave && ((int64_t)V << g.cl2) < D) ++g.cl2;
