@@ -25,7 +25,7 @@ __device__ __forceinline__ int64_t id_at(const void* __restrict__ ids, bool wide
 template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kBlock) k_embed_fwd(const void* __restrict__ ids, bool wide, int64_t N, int64_t vocab,
                                                       const T* __restrict__ table, int64_t st, uint32_t units,
-                                                      float scale, O* __restrict__ out, int rows) {
+                                                      uint32_t unit_m, float scale, O* __restrict__ out, int rows) {
   constexpr int kAhead = 4;                       // pieces in flight: ids, then rows, then stores
   const int64_t r0 = (int64_t)blockIdx.x * rows;
   const uint32_t items = (uint32_t)min((int64_t)rows, N - r0) * units;
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kBlock) k_embed_fwd(const void* __restrict__ i
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const uint32_t e = min(e0 + k * kBlock, items - 1);
-      row[k] = e / units;
+      row[k] = units == 1 ? e : __umulhi(e, unit_m);       // e / units: e and units are below 2^16 + 1
       c[k] = (e - row[k] * units) * V;
       id[k] = id_at(ids, wide, r0 + row[k]);
     }
@@ -249,55 +249,90 @@ struct RunGeo {
   float scale;
 };
 
-// part (chunks, 2, D): the chunk's sum of a run that began before it, and of one that goes on after it.
+// A workgroup's groups first join the runs that pass from one to the next, in LDS and in order.
+// part (workgroups, 2, D): the workgroup's sum of a run that began before it, and of one that goes on after it.
 template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kBlock) k_embed_runs(RunGeo g, const Rec* __restrict__ rec, const T* __restrict__ go,
                                                        O* __restrict__ gt, float* __restrict__ part) {
-  const int64_t chunk = (int64_t)blockIdx.x * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
-  const int64_t c = (((int64_t)blockIdx.y << g.cl2) + (threadIdx.x & ((1 << g.cl2) - 1))) * V;
-  const int64_t p0 = chunk * g.chunk, p1 = min(p0 + g.chunk, g.N);
-  if (p0 >= g.N || c >= g.D) return;
+  enum { kNone = 0, kEnds = 1, kPasses = 2 };     // a group's run that began before it
+  __shared__ float heads[kBlock * V];
+  __shared__ uint8_t head_of[kBlock];
+  const int lanes = 1 << g.cl2, G = kBlock >> g.cl2, gi = threadIdx.x >> g.cl2;
+  const int64_t c = (((int64_t)blockIdx.y << g.cl2) + (threadIdx.x & (lanes - 1))) * V;
+  const int64_t p0 = ((int64_t)blockIdx.x * G + gi) * g.chunk, p1 = min(p0 + g.chunk, g.N);
+  const bool live = p0 < g.N && c < g.D;
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.f;
-  uint32_t cur = rec[p0].key;
-  bool head = p0 > 0 && rec[p0 - 1].key == cur;
-  auto flush = [&](int slot) {
-    if (slot >= 0) {
-      store_f<V>(part + (chunk * 2 + slot) * g.D + c, acc);
-    } else {
+  uint32_t cur = g.vocab;
+  bool head = false, goes_on = false;
+  int state = kNone;
+  auto to_row = [&]() {
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] *= g.scale;
-      store_f<V>(gt + cur * g.D + c, acc);
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    for (int k = 0; k < V; ++k) acc[k] *= g.scale;
+    store_f<V>(gt + cur * g.D + c, acc);
   };
-  for (int64_t q = p0; q < p1 && cur < g.vocab; q += kAhead) {
-    Rec r[kAhead];
-    Pack<T, V> v[kAhead];
+  auto to_heads = [&](int how) {
+    state = how;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) r[k] = rec[min(q + k, p1 - 1)];
+    for (int k = 0; k < V; ++k) heads[threadIdx.x * V + k] = acc[k];
+  };
+  if (live) {
+    cur = rec[p0].key;
+    head = p0 > 0 && cur < g.vocab && rec[p0 - 1].key == cur;
+    for (int64_t q = p0; q < p1 && cur < g.vocab; q += kAhead) {
+      Rec r[kAhead];
+      Pack<T, V> v[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) v[k] = load_pack<T, V>(go + (int64_t)r[k].idx * g.sgo + c);
+      for (int k = 0; k < kAhead; ++k) r[k] = rec[min(q + k, p1 - 1)];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (q + k >= p1 || cur >= g.vocab) break;
-      if (r[k].key != cur) {
-        flush(head ? 0 : -1);
-        head = false;
-        cur = r[k].key;
-        if (cur >= g.vocab) break;
+      for (int k = 0; k < kAhead; ++k) v[k] = load_pack<T, V>(go + (int64_t)r[k].idx * g.sgo + c);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (q + k >= p1 || cur >= g.vocab) continue;
+        if (r[k].key != cur) {
+          if (head) to_heads(kEnds);
+          else to_row();
+          head = false;
+          cur = r[k].key;
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] = 0.f;
+          if (cur >= g.vocab) continue;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += (float)v[k].e[j];
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += (float)v[k].e[j];
+    }
+    if (cur < g.vocab) {
+      goes_on = p1 < g.N && rec[p1].key == cur;
+      if (head) to_heads(goes_on ? kPasses : kEnds);
+      else if (!goes_on) to_row();
     }
   }
-  if (cur < g.vocab) flush(head ? 0 : p1 < g.N && rec[p1].key == cur ? 1 : -1);
+  if ((threadIdx.x & (lanes - 1)) == 0) head_of[gi] = (uint8_t)state;
+  __syncthreads();
+  const bool first = gi == 0 && state != kNone;   // leads the run that began before the workgroup
+  const bool own = goes_on && !head;              // leads its last run on
+  auto follow = [&](int how, int slot, bool ends_in_row) {
+    int j = gi + 1;
+    while (how != kEnds && j < G) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += heads[(j * lanes + (threadIdx.x & (lanes - 1))) * V + k];
+      how = head_of[j++];
+    }
+    if (how == kEnds && ends_in_row) to_row();
+    else store_f<V>(part + ((int64_t)blockIdx.x * 2 + slot) * g.D + c, acc);
+  };
+  if (live && own) follow(kPasses, 1, true);
+  if (live && first) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = heads[threadIdx.x * V + k];
+    follow(state, 0, false);
+  }
 }
 
-// Joins the partial sums of the runs that cross chunks, each by the group of the chunk where the run begins: its own
-// share, then those of the chunks after it.  Runs of more than kSerial chunks are added up by the whole workgroup, a
+// Joins the partial sums of the runs that cross workgroups (chunks here), each by the group of the chunk where the run
+// begins: its own share, then those of the chunks after it.  Runs of more than kSerial chunks are added up by the whole workgroup, a
 // stretch per group, the stretches joined in order.
 constexpr int kSerial = 16;
 template <typename O, int V>
@@ -349,7 +384,7 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
     long_n[gi] = after > kSerial ? after : 0;
     long_chunk[gi] = chunk;
   }
-  __syncthreads();
+  if (!__syncthreads_or(after > kSerial)) return;
   for (int run = 0; run < G; ++run) {             // every thread takes the same turns
     const int64_t n = long_n[run];
     if (n == 0) continue;
@@ -360,12 +395,14 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
     for (int k = 0; k < V; ++k) acc[k] = 0.f;
     if (live) {
       if (gi == 0) load_f<V>(part + (first * 2 + 1) * g.D + c, acc);
-#pragma unroll 8
-      for (int64_t j = j0; j < j1; ++j) {
-        float v[V];
-        load_f<V>(part + j * 2 * g.D + c, v);
+      for (int64_t j = j0; j < j1; j += kAhead) {
+        Pack<float, V> v[kAhead];
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += v[k];
+        for (int q = 0; q < kAhead; ++q) v[q] = load_pack<float, V>(part + min(j + q, j1 - 1) * 2 * g.D + c);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] += j + q < j1 ? v[q].e[k] : 0.f;
       }
     }
 #pragma unroll
@@ -386,7 +423,6 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
 // ------------------------------------------------------------------------------------------- host
 struct SortPlan {
   int passes, bits, nblk, chunk;
-  int64_t nchunk;
   int64_t rec_a, rec_b, cnt, tot, part, bytes;      // workspace offsets in bytes
 };
 
@@ -399,15 +435,15 @@ SortPlan sort_plan(int64_t N, int64_t D, int64_t vocab) {
   q.nblk = (int)((N + kSortTile - 1) / kSortTile);
   // A chunk is worked off row by row: short ones where there are few tokens, so that more lanes share them (3000 tokens:
   // 22 us with 64 rows a chunk), long ones where partial sums would cost traffic.
-  q.chunk = N <= 16 * kSortTile ? 16 : 64;
-  q.nchunk = (N + q.chunk - 1) / q.chunk;
+  q.chunk = N <= 16 * kSortTile ? 8 : 32;
+  const int64_t groups = (N + q.chunk - 1) / q.chunk;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   q.rec_a = take(N * 8);
   q.rec_b = take(N * 8);
   q.cnt = take(((int64_t)q.nblk << q.bits) * 4);
   q.tot = take(((int64_t)1 << q.bits) * 4);
-  q.part = take(q.nchunk * 2 * D * 4);
+  q.part = take((groups + 3) / 4 * 2 * D * 4);            // a workgroup holds at least four groups
   q.bytes = at;
   return q;
 }
@@ -457,7 +493,8 @@ int atl_embed_fwd(const void* ids, int wide_ids, int64_t N, const void* table, i
     using T = decltype(t);
     using O = decltype(o);
     hipLaunchKernelGGL((k_embed_fwd<T, O, decltype(v)::value>), dim3((unsigned)((N + rows - 1) / rows)), dim3(kBlock), 0, stream, ids,
-                       wide_ids != 0, N, vocab, (const T*)table, st, (uint32_t)units, (float)scale, (O*)out, (int)rows);
+                       wide_ids != 0, N, vocab, (const T*)table, st, (uint32_t)units,
+                       (uint32_t)((((int64_t)1 << 32) + units - 1) / units), (float)scale, (O*)out, (int)rows);
   };
   if (vec) by_pair<8>(ttype, otype, go);
   else by_pair<1>(ttype, otype, go);
@@ -510,18 +547,22 @@ int atl_embed_bwd(const void* ids, int wide_ids, int64_t N, const void* gout, in
   if (N == 0) return check_launch("embed_bwd");
   RunGeo g{};
   g.N = N; g.D = D; g.sgo = sgo; g.vocab = (uint32_t)vocab; g.scale = (float)scale;
-  g.nchunk = q.nchunk;
   g.chunk = q.chunk;
   const bool vec = D % 8 == 0 && sgo % 8 == 0 && aligned_to(gout, 16);
   const int V = vec ? 16 / dtype_size(otype) : 1;
   while ((1 << g.cl2) < kWave && ((int64_t)V << g.cl2) < D) ++g.cl2;
-  const dim3 grid((unsigned)((g.nchunk + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2)), (unsigned)((D + ((int64_t)V << g.cl2) - 1) / ((int64_t)V << g.cl2)));
+  const int G = kBlock >> g.cl2;
+  RunGeo j = g;                                   // the workgroups' sums are the joining kernel's chunks
+  j.chunk = q.chunk * G;
+  j.nchunk = (N + j.chunk - 1) / j.chunk;
+  const unsigned tiles = (unsigned)((D + ((int64_t)V << g.cl2) - 1) / ((int64_t)V << g.cl2));
   auto go = [&](auto o, auto t, auto v) {
     using T = decltype(o);
     using O = decltype(t);
     constexpr int VV = decltype(v)::value;
-    hipLaunchKernelGGL((k_embed_runs<T, O, VV>), grid, dim3(kBlock), 0, stream, g, (const Rec*)src, (const T*)gout, (O*)gtable, (float*)(w + q.part));
-    hipLaunchKernelGGL((k_embed_join<O, VV>), grid, dim3(kBlock), 0, stream, g, (const Rec*)src, (O*)gtable, (const float*)(w + q.part));
+    hipLaunchKernelGGL((k_embed_runs<T, O, VV>), dim3((unsigned)j.nchunk, tiles), dim3(kBlock), 0, stream, g, (const Rec*)src, (const T*)gout, (O*)gtable, (float*)(w + q.part));
+    if (j.nchunk > 1)
+      hipLaunchKernelGGL((k_embed_join<O, VV>), dim3(grid_for(j.nchunk, G), tiles), dim3(kBlock), 0, stream, j, (const Rec*)src, (O*)gtable, (const float*)(w + q.part));
   };
   if (vec) by_pair_vec(otype, ttype, go);
   else by_pair<1>(otype, ttype, go);
