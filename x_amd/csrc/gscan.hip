@@ -496,13 +496,14 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __
     if (blockIdx.y == 0) fill_empty<kFwdBlock>(start, s.B, s.D, h0, last, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
     return;
   }
-  const Place p = place_of<kFwdLen, V>(s, blockIdx.x);
-  const Rows<const T, kFwdLen> rx(s, p, x, s.sx, blockIdx.x);
-  const Rows<const T, kFwdLen> rg(s, p, g, s.sg, blockIdx.x);
-  Rows<const float, kFwdLen> rd(s, p, dt, 1, blockIdx.x);
+  const int64_t chunk = s.nchunk - 1 - blockIdx.x;         // from the end: what the local kernel read last is still cached
+  const Place p = place_of<kFwdLen, V>(s, chunk);
+  const Rows<const T, kFwdLen> rx(s, p, x, s.sx, chunk);
+  const Rows<const T, kFwdLen> rg(s, p, g, s.sg, chunk);
+  Rows<const float, kFwdLen> rd(s, p, dt, 1, chunk);
   rd.off = p.gi * kFwdLen * 4;
-  const Rows<T, kFwdLen> ro(s, p, y, s.D, blockIdx.x);
-  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, blockIdx.x), p.i0);
+  const Rows<T, kFwdLen> ro(s, p, y, s.D, chunk);
+  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, chunk), p.i0);
   const Ascend begin = win;
   float a[kFwdLen][V], u[kFwdLen][V];
   Decay<V, DT> decay;
@@ -541,13 +542,13 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<kFwdBlock, V, false>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  join_groups<kFwdBlock, V, false>(s, lds, Z, U, chunk, nullptr, nullptr);
   if (!p.live) return;
   win = begin;
   float h[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    h[k] = past(Z[k], U[k], carry.before(blockIdx.x, s.D, p.c + k));
+    h[k] = past(Z[k], U[k], carry.before(chunk, s.D, p.c + k));
   }
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
@@ -640,14 +641,15 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
     if (blockIdx.y == 0) fill_empty<kBwdBlock>(start, s.B, s.D, glast, gh0, blockIdx.x - s.nchunk, gridDim.x - s.nchunk);
     return;
   }
-  const Place p = place_of<kBwdLen, V>(s, blockIdx.x);
-  const Rows<const T, kBwdLen> rx(s, p, x, s.sx, blockIdx.x);
-  const Rows<const T, kBwdLen> rg(s, p, g, s.sg, blockIdx.x);
-  const Rows<const T, kBwdLen> ry(s, p, gy, s.sgy, blockIdx.x);
-  Rows<const float, kBwdLen> rd(s, p, dt, 1, blockIdx.x);
+  const int64_t chunk = s.nchunk - 1 - blockIdx.x;         // from the end: what the local kernel read last is still cached
+  const Place p = place_of<kBwdLen, V>(s, chunk);
+  const Rows<const T, kBwdLen> rx(s, p, x, s.sx, chunk);
+  const Rows<const T, kBwdLen> rg(s, p, g, s.sg, chunk);
+  const Rows<const T, kBwdLen> ry(s, p, gy, s.sgy, chunk);
+  Rows<const float, kBwdLen> rd(s, p, dt, 1, chunk);
   rd.off = p.gi * kBwdLen * 4;
-  const Rows<T, kBwdLen> rox(s, p, gx, s.D, blockIdx.x), rog(s, p, gg, s.D, blockIdx.x);
-  const int64_t wf = wave_first_token<kBwdLen>(s, blockIdx.x);
+  const Rows<T, kBwdLen> rox(s, p, gx, s.D, chunk), rog(s, p, gg, s.D, chunk);
+  const int64_t wf = wave_first_token<kBwdLen>(s, chunk);
   Descend win(start, s.B, wf, p.i0, p.n);
   const Descend begin = win;
   float a[kBwdLen][V], w[kBwdLen][V], f[kBwdLen][V];      // f: gg = H f
@@ -702,7 +704,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
   });
 #pragma unroll
   for (int k = 0; k < V; ++k) Z[k] = decay.rate(k, reset);
-  join_groups<kBwdBlock, V, true>(s, lds, Z, U, blockIdx.x, nullptr, nullptr);
+  join_groups<kBwdBlock, V, true>(s, lds, Z, U, chunk, nullptr, nullptr);
   if (!p.live) return;
   win = begin;
 #pragma unroll
@@ -710,7 +712,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
     if (GY) asm volatile("" : "+v"(*(Word<sizeof(T) * V>*)&yr[t]));      // as loaded, not widened
   float C[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) C[k] = past(Z[k], U[k], carry.before(s.nchunk - 1 - blockIdx.x, s.D, p.c + k));
+  for (int k = 0; k < V; ++k) C[k] = past(Z[k], U[k], carry.before(s.nchunk - 1 - chunk, s.D, p.c + k));
   by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
