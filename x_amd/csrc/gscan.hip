@@ -77,9 +77,11 @@ __device__ __forceinline__ bool anew(float Z) { return Z < 0.f; }
 __device__ __forceinline__ float past(float Z, float U, float h) { return anew(Z) ? U : fmaf(decay_of(Z), h, U); }
 __device__ __forceinline__ float joined(float Za, float Zb) { return anew(Za) || anew(Zb) ? kAnew : Za + Zb; }
 
-// The rates behind a decay P = 1 - M, from whichever holds more of it.
+// The rates behind a decay P = 1 - M, from whichever holds more of it (what 1 - M rounds off is put back).
 __device__ __forceinline__ float rate_of(float M, float P) {
-  return M < 0.5f ? -log1pf(-M) * kLog2e : -__builtin_amdgcn_logf(P);
+  if (M >= 0.5f) return -__builtin_amdgcn_logf(P);
+  const float p = 1.f - M;
+  return -fmaf(((1.f - p) - M) * __builtin_amdgcn_rcpf(p), kLog2e, __builtin_amdgcn_logf(p));
 }
 
 struct ScanGeo {
