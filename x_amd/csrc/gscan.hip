@@ -854,7 +854,7 @@ int64_t atl_gated_scan_groups(int64_t N) { return N < 0 ? -1 : (N + kBwdLen - 1)
 
 int64_t atl_gated_scan_ws_bytes(int64_t N, int64_t D, int dtype) {
   if (!scan_sizes_ok(N, D, 1, dtype)) return -1;
-  int64_t bytes = 0;
+  int64_t bytes = 256;
   for (int V = 1; V <= 2; ++V)
     bytes = std::max(bytes, std::max(scan_plan<kFwdLen, kFwdBlock>(N, D, V).bytes, scan_plan<kBwdLen, kBwdBlock>(N, D, V).bytes));
   return bytes;

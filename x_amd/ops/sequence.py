@@ -16,12 +16,17 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import reference as ref
-from ._ext import F32, I64, call, ext_supports, load_library, on_device, ptr, stream_of
+from ._ext import F32, I64, call, ext_supports, load_library, on_device, raw_stream
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_NORM_WIDTH = 8192
 MAX_ROW_STRIDE = 65536
 _U64 = 2 ** 64 - 1
+
+
+def _at(t: torch.Tensor | None) -> int:
+    """A tensor's address as the entry points take it (an integer converts faster than a pointer object)."""
+    return 0 if t is None else t.data_ptr()
 
 
 def _float_type(t, name: str) -> int:
@@ -63,8 +68,8 @@ def _embed_fwd(ids, table, scale, dtype):
     N, (V, D) = ids.numel(), table.shape
     out = torch.empty(*ids.shape, D, dtype=dtype, device=table.device)
     with on_device(table.device):
-        call("atl_embed_fwd", ptr(ids), int(ids.dtype == I64), N, ptr(table), table.stride(0), _CODE[table.dtype], V, D,
-             scale, ptr(out), _CODE[dtype], stream_of(table))
+        call("atl_embed_fwd", _at(ids), int(ids.dtype == I64), N, _at(table), table.stride(0), _CODE[table.dtype], V, D,
+             scale, _at(out), _CODE[dtype], raw_stream(table.device))
     return out
 
 
@@ -86,8 +91,8 @@ class _Embed(torch.autograd.Function):
         nbytes = int(load_library().atl_embed_bwd_ws_bytes(N, V, D))
         ws = _ws(nbytes, g.device, "embed_tokens")
         with on_device(g.device):
-            call("atl_embed_bwd", ptr(ids), int(ids.dtype == I64), N, ptr(g), g.stride(0), _CODE[g.dtype], V, D, scale,
-                 ptr(gt), _CODE[ttype], ptr(ws), nbytes, stream_of(g))
+            call("atl_embed_bwd", _at(ids), int(ids.dtype == I64), N, _at(g), g.stride(0), _CODE[g.dtype], V, D, scale,
+                 _at(gt), _CODE[ttype], _at(ws), nbytes, raw_stream(g.device))
         return None, gt, None, None
 
 
@@ -114,16 +119,16 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dty
 
 
 # ------------------------------------------------------------------------------------------- residual norm
-def _norm_fwd(x, res, w, eps, p, seed, offset, fp8=False):
-    """(y, s, scale) for rows x (N, D) and res (N, D) or None; s None where it would be x itself."""
+def _norm_fwd(x, res, w, shape, eps, p, seed, offset, fp8=False):
+    """(y, s, scale) in the given shape for rows x (N, D) and res (N, D) or None; s None where it would be x itself."""
     N, D = x.shape
     dev, rtype = x.device, (x if res is None else res).dtype
-    y = torch.empty(N, D, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
-    s = None if res is None and p == 0 else torch.empty(N, D, dtype=rtype, device=dev)
-    scale = torch.empty(N, 1, dtype=F32, device=dev) if fp8 else None
+    y = torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
+    s = None if res is None and p == 0 else torch.empty(shape, dtype=rtype, device=dev)
+    scale = torch.empty(*shape[:-1], 1, dtype=F32, device=dev) if fp8 else None
     with on_device(dev):
-        call("atl_rms_norm_fwd", ptr(x), x.stride(0), _CODE[x.dtype], ptr(res), 0 if res is None else res.stride(0),
-             _CODE[rtype], ptr(w), N, D, eps, p, seed, offset, ptr(y), ptr(s), ptr(scale), stream_of(x))
+        call("atl_rms_norm_fwd", _at(x), x.stride(0), _CODE[x.dtype], _at(res), 0 if res is None else res.stride(0),
+             _CODE[rtype], _at(w), N, D, eps, p, seed, offset, _at(y), _at(s), _at(scale), raw_stream(x.device))
     return y, s, scale
 
 
@@ -131,35 +136,36 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, w, eps, p, seed, offset):
         rx, rr = _rows(x), None if res is None else _rows(res)
-        y, s, _ = _norm_fwd(rx, rr, w, eps, p, seed, offset)
+        y, s, _ = _norm_fwd(rx, rr, w, x.shape, eps, p, seed, offset)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(rx if s is None else s, w)
-        ctx.meta = (x.shape, x.dtype, None if res is None else res.shape, eps, p, seed, offset)
-        return y.view(x.shape), (None if s is None else s.view(x.shape))
+        ctx.meta = (x.shape, x.dtype, eps, p, seed, offset)
+        return y, s
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy, gs=None):
         s, w = ctx.saved_tensors
-        shape, xtype, rshape, eps, p, seed, offset = ctx.meta
+        shape, xtype, eps, p, seed, offset = ctx.meta
         want_x, want_r, want_w = ctx.needs_input_grad[:3]
         if gy is None and gs is None:
             return (None,) * 7
+        s = _rows(s)
         N, D = s.shape
         dev = s.device
         gy, gs = None if gy is None else _rows(gy), None if gs is None else _rows(gs)
         same = p == 0 and xtype == s.dtype                 # then both gradients are one tensor
-        gr = torch.empty(N, D, dtype=s.dtype, device=dev) if (want_r or same) and (want_r or want_x) else None
-        gx = torch.empty(N, D, dtype=xtype, device=dev) if want_x and not same else None
+        gr = torch.empty(shape, dtype=s.dtype, device=dev) if want_r or (same and want_x) else None
+        gx = torch.empty(shape, dtype=xtype, device=dev) if want_x and not same else None
         gw = torch.empty(D, dtype=F32, device=dev) if want_w else None
         nbytes = int(load_library().atl_rms_norm_bwd_ws_bytes(N, D)) if want_w else 0
         ws = _ws(nbytes, dev, "residual_rms_norm") if want_w else None
         with on_device(dev):
-            call("atl_rms_norm_bwd", ptr(s), s.stride(0), _CODE[s.dtype], ptr(w), ptr(gy),
-                 0 if gy is None else gy.stride(0), _CODE[xtype], ptr(gs), 0 if gs is None else gs.stride(0), N, D, eps,
-                 p, seed, offset, ptr(gx), ptr(gr), ptr(gw), ptr(ws), nbytes, stream_of(s))
+            call("atl_rms_norm_bwd", _at(s), s.stride(0), _CODE[s.dtype], _at(w), _at(gy),
+                 0 if gy is None else gy.stride(0), _CODE[xtype], _at(gs), 0 if gs is None else gs.stride(0), N, D, eps,
+                 p, seed, offset, _at(gx), _at(gr), _at(gw), _at(ws), nbytes, raw_stream(s.device))
         gx = gr if same else gx
-        return (gx.view(shape) if want_x else None, gr.view(rshape) if want_r else None, gw, None, None, None, None)
+        return gx if want_x else None, gr if want_r else None, gw, None, None, None, None
 
 
 def _norm_args(x, residual, weight, eps, p=0.0):
@@ -204,8 +210,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     if _grads_wanted(x, residual, w):
         y, s = _Norm.apply(x, residual, w, eps, p, seed, offset)
     else:
-        y, s, _ = _norm_fwd(_rows(x), None if residual is None else _rows(residual), w, eps, p, seed, offset)
-        y, s = y.view(x.shape), None if s is None else s.view(x.shape)
+        y, s, _ = _norm_fwd(_rows(x), None if residual is None else _rows(residual), w, x.shape, eps, p, seed, offset)
     return y, x if s is None else s
 
 
@@ -214,12 +219,12 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight
     scale (..., 1) = max(max |y|, 1e-30) / 448, q = 448 y / max |y| rounded to nearest.  For inference (no gradient): q
     and scale are what a row-scaled 8-bit product takes."""
     eps, _ = _norm_args(x, residual, weight, eps)
-    with torch.no_grad():
-        if not ext_supports(x):
+    if not ext_supports(x):
+        with torch.no_grad():
             return ref.residual_rms_norm_fp8(x, residual, weight, eps)
-        y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.to(F32).contiguous(),
-                                eps, 0.0, 0, 0, fp8=True)
-        return y.view(x.shape), scale.view(*x.shape[:-1], 1), x if s is None else s.view(x.shape)
+    y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.detach().to(F32).contiguous(),
+                            x.shape, eps, 0.0, 0, 0, fp8=True)
+    return y, scale, x.detach() if s is None else s
 
 
 # ------------------------------------------------------------------------------------------- recurrence
@@ -233,8 +238,8 @@ def _scan_fwd(x, gate, start, dt, h0, save):
     ws = _ws(nbytes, dev, "gated_scan")
     states = torch.empty(int(lib.atl_gated_scan_groups(N)), D, dtype=F32, device=dev) if save else None
     with on_device(dev):
-        call("atl_gated_scan_fwd", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], N, D, ptr(start), B,
-             ptr(dt), ptr(h0), ptr(y), ptr(last), ptr(states), ptr(ws), nbytes, stream_of(x))
+        call("atl_gated_scan_fwd", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(start), B,
+             _at(dt), _at(h0), _at(y), _at(last), _at(states), _at(ws), nbytes, raw_stream(x.device))
     return y, last, states
 
 
@@ -262,9 +267,9 @@ class _Scan(torch.autograd.Function):
         nbytes = int(load_library().atl_gated_scan_ws_bytes(N, D, _CODE[x.dtype]))
         ws = _ws(nbytes, dev, "gated_scan")
         with on_device(dev):
-            call("atl_gated_scan_bwd", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], N, D, ptr(start),
-                 B, ptr(dt), ptr(h0), ptr(states), ptr(gy), 0 if gy is None else gy.stride(0), ptr(glast), ptr(gx),
-                 ptr(gg), ptr(gh0), ptr(ws), nbytes, stream_of(x))
+            call("atl_gated_scan_bwd", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(start),
+                 B, _at(dt), _at(h0), _at(states), _at(gy), 0 if gy is None else gy.stride(0), _at(glast), _at(gx),
+                 _at(gg), _at(gh0), _at(ws), nbytes, raw_stream(x.device))
         return gx, gg, None, None, gh0
 
 
@@ -327,12 +332,13 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
         raise ValueError(f"state must be a contiguous float32 tensor of {tuple(x.shape)} without gradient, got "
                          f"{tuple(state.shape)}, {state.dtype}")
-    with torch.no_grad():
-        if not ext_supports(x):
+    if not ext_supports(x):
+        with torch.no_grad():
             return ref.gated_scan_step(x, gate, state, dt)
-        x, gate = _rows(x), _rows(gate)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with on_device(x.device):
-            call("atl_gated_scan_step", ptr(x), x.stride(0), ptr(gate), gate.stride(0), _CODE[x.dtype], x.shape[0],
-                 x.shape[1], ptr(dt), ptr(state), ptr(y), stream_of(x))
-        return y
+    x, gate = _rows(x), _rows(gate)
+    N, D = x.shape
+    y = torch.empty(N, D, dtype=x.dtype, device=x.device)
+    with on_device(x.device):
+        call("atl_gated_scan_step", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(dt),
+             _at(state), _at(y), raw_stream(x.device))
+    return y
