@@ -512,3 +512,74 @@ def test_offsets_past_32_bits():
         y, s = ops.residual_rms_norm(x, g, w)
         y1, s1 = ops.residual_rms_norm(small[0], small[1], w)
     assert torch.equal(y[-tail:], y1) and torch.equal(s[-tail:], s1)
+
+
+def test_scan_of_very_many_windows():
+    """More windows than two steps of the 64-way search cover, empty ones among them."""
+    rng = np.random.default_rng(15)
+    sizes = rng.integers(0, 6, 9000)
+    start = [0, *np.cumsum(sizes).tolist()]
+    N, D = start[-1], 4
+    x, g, gy = (_t(rng.normal(size=(N, D))) for _ in range(3))
+    gl = _t(rng.normal(size=(9000, D)))
+    ins = [a.requires_grad_() for a in (x, g)]
+    y, last = ops.gated_scan(*ins, torch.tensor(start, device=DEV))
+    wy, wl, E = O.scan(_np(x), _np(g), start)
+    _close(y, wy, E)
+    some = sizes > 0
+    _close(last, wl, np.where(some[:, None], E[np.array(start[1:]) - 1], 0))
+    got = torch.autograd.grad((y, last), ins, (gy, gl))
+    want, bound = O.scan_bwd(_np(x), _np(g), start, _np(gy), _np(gl))
+    for a, b, c in zip(got, want, bound):
+        _close(a, b, c)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_nan_gate_shows(dtype):
+    """A gate that is not a number makes its token and the window's later states so, in its channel only."""
+    N, D = 100, 8
+    x, g = torch.randn(N, D, device=DEV).to(dtype), torch.randn(N, D, device=DEV).to(dtype)
+    g[20, 2] = float("nan")
+    for dt in (None, torch.rand(N, device=DEV)):
+        y, last = ops.gated_scan(x, g, torch.tensor([0, 50, N], device=DEV), dt=dt)
+        hit = torch.zeros(N, D, dtype=torch.bool, device=DEV)
+        hit[20:50, 2] = True
+        assert torch.equal(y.isnan(), hit) and last[0, 2].isnan() and last.isnan().sum() == 1
+        state = torch.zeros(N, D, device=DEV)
+        ops.gated_scan_step(x, g, state, dt=dt)
+        assert state.isnan().sum() == 1
+
+
+def test_second_derivatives_are_refused():
+    x, g = (torch.randn(10, 8, device=DEV, requires_grad=True) for _ in range(2))
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    table = torch.randn(5, 8, device=DEV, requires_grad=True)
+    start, ids = torch.tensor([0, 10], device=DEV), torch.arange(5, device=DEV)
+    for out, wrt in ((ops.gated_scan(x, g, start)[0], x), (ops.residual_rms_norm(x, g, w)[0], x),
+                     (ops.embed_tokens(ids, table), table)):
+        first, = torch.autograd.grad(out.square().sum(), wrt, create_graph=True)
+        with pytest.raises(RuntimeError):
+            first.sum().backward()
+
+
+def test_gradients_of_some_inputs():
+    """Each input's gradient alone is the one it has beside the others."""
+    x, res, gy = torch.randn(3, 40, 24, device=DEV)
+    w = torch.randn(24, device=DEV)
+    for p in (0.0, 0.4):
+        full = [t.clone().requires_grad_() for t in (x, res, w)]
+        want = torch.autograd.grad(ops.residual_rms_norm(*full, p=p, seed=2)[0], full, gy)
+        for k in range(3):
+            part = [t.clone().requires_grad_(j == k) for j, t in enumerate((x, res, w))]
+            got, = torch.autograd.grad(ops.residual_rms_norm(*part, p=p, seed=2)[0], part[k], gy)
+            assert torch.equal(got, want[k]), (p, k)
+        sums = [t.clone().requires_grad_() for t in (x, res, w)]
+        gx, gr, gw = torch.autograd.grad(ops.residual_rms_norm(*sums, p=p, seed=2)[1], sums, gy, allow_unused=True)
+        assert torch.equal(gr, gy) and (gw is None or not gw.any()) and (p > 0 or torch.equal(gx, gy))
+    start = torch.tensor([0, 40], device=DEV)
+    full = [t.clone().requires_grad_() for t in (x, res)]
+    want = torch.autograd.grad(ops.gated_scan(*full, start)[0], full, gy)
+    for k in range(2):
+        part = [t.clone().requires_grad_(j == k) for j, t in enumerate((x, res))]
+        got, = torch.autograd.grad(ops.gated_scan(*part, start)[0], part[k], gy)
+        assert torch.equal(got, want[k])
