@@ -43,7 +43,7 @@ def scan(x, g, start, dt=None, h0=None):
         m, e = np.abs(h), np.zeros(D)
         for i in range(start[b], start[b + 1]):
             u = w[i] * x[i]
-            e = a[i] * (e + (4 + 4 * z[i]) * m)
+            e = a[i] * (e + (4 + 4 * np.abs(z[i])) * m)
             m = a[i] * m + np.abs(u)
             e = e + 8 * np.abs(u) + m
             h = a[i] * h + u
@@ -78,11 +78,11 @@ def scan_bwd(x, g, start, gy, glast, dt=None, h0=None):
             Bx[i] = (eH + 6 * U * mH) * w[i]
             da = step[i] * a[i]
             t = x[i] * wc[i] - da * hp
-            mt = np.abs(x[i]) * wc[i] + da * mp
+            mt = np.abs(x[i]) * wc[i] + np.abs(da) * mp
             gg[i] = H * w[i] * t
-            Bg[i] = w[i] * (eH * mt + mH * (U * (16 + 4 * z[i]) * mt + da * ep))
+            Bg[i] = w[i] * (eH * mt + mH * (U * (16 + 4 * np.abs(z[i])) * mt + np.abs(da) * ep))
             C = a[i] * H
-            eC = a[i] * (eH + (5 + 4 * z[i]) * mH * U)
+            eC = a[i] * (eH + (5 + 4 * np.abs(z[i])) * mH * U)
             mC = a[i] * mH
         gh0[b], B0[b] = C, eC
     return (gx, gg, gh0), (Bx, Bg, B0)

@@ -131,6 +131,33 @@ def test_scan_gaps(gap):
     _scan_case(5000, 8, F32, "one", True, False, None, seed=14, gap=gap)
 
 
+def test_scan_gaps_back_in_time():
+    """Events out of order: negative gaps grow the state as the formula has it, within a group of tokens, over whole
+    groups and over workgroups, forward and backward."""
+    N, D = 3000, 8
+    rng = np.random.default_rng(21)
+    gap = rng.exponential(size=N) * 0.05
+    gap[rng.random(N) < 0.3] *= -1
+    gap[1000:1100] = -np.abs(gap[1000:1100])
+    x, g, gy = (rng.normal(size=(N, D)) for _ in range(3))
+    start = [0, 2000, N]
+    ins = [_t(a).requires_grad_() for a in (x, g)]
+    dt = _t(gap)
+    y, last = ops.gated_scan(*ins, torch.tensor(start, device=DEV), dt=dt)
+    args = (_np(ins[0]), _np(ins[1]), start)
+    wy, wl, E = O.scan(*args, _np(dt))
+    _close(y, wy, E, "y")
+    _close(last, wl, E[np.array(start[1:]) - 1], "last")
+    got = torch.autograd.grad(y, ins, _t(gy))
+    want, bound = O.scan_bwd(*args, _np(_t(gy)), np.zeros((2, D)), _np(dt))
+    for name, a, b, c in zip(("gx", "gg"), got, want, bound):
+        _close(a, b, c, name)
+    state = torch.ones(D, D, device=DEV)
+    one = O.scan(_np(ins[0][:D]), _np(ins[1][:D]), list(range(D + 1)), _np(-dt[:D].abs()), np.ones((D, D)))
+    ops.gated_scan_step(ins[0][:D].detach(), ins[1][:D].detach(), state, dt=-dt[:D].abs())
+    _close(state, one[1], one[2], "state")
+
+
 def test_scan_equal_times_add_up():
     x, g = torch.ones(40, 8, device=DEV), torch.zeros(40, 8, device=DEV)
     y, last = ops.gated_scan(x, g, torch.tensor([0, 40], device=DEV), dt=torch.zeros(40, device=DEV))

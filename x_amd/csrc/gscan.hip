@@ -12,8 +12,10 @@
 //   3. k_scan_apply: decays and inputs once into registers, the groups joined in LDS again, then every group from its
 //      own start state: y, the last states, and (for the backward) the start states.
 // A call of one chunk needs the third alone.  The backward is the same recurrence from the end, C_i = a_i (gy_i +
-// C_{i+1}), in the same three steps, with the group's states recomputed from its saved start state.  A range that holds a window's start is marked: its U alone is its outcome, whatever came
-// before it (an infinity or NaN of one window stays there), so chunks need not know about windows.
+// C_{i+1}), in the same three steps, with the group's states recomputed from its saved start state.
+//
+// A range that holds a window's start is marked: its U alone is its outcome, whatever came before it (an infinity or NaN
+// of one window stays there), so chunks need not know about windows.
 // States, decays and sums are fp32 whatever the tokens' type; y is rounded once.
 #include "typed.h"
 #include "../../include/atl_hip.h"
@@ -67,13 +69,14 @@ __device__ __forceinline__ float decay_of(float Z) {
   q = fmaf(x, -q, 1.f / 6);
   q = fmaf(x, -q, 0.5f);
   q = fmaf(x, -q, 1.f);
-  return Z < 0.25f ? fmaf(-x, q, 1.f) : __builtin_amdgcn_exp2f(-Z);
+  return fabsf(Z) < 0.25f ? fmaf(-x, q, 1.f) : __builtin_amdgcn_exp2f(-Z);
 }
 
 // A range of tokens as (Z, U): h_out = decay(Z) h_in + U.  Ranges are joined by adding their Z, so that a decay is
-// rounded once however long its range.  Z = kAnew marks a range that holds a window's start.
-constexpr float kAnew = -1.f;
-__device__ __forceinline__ bool anew(float Z) { return Z < 0.f; }
+// rounded once however long its range.  Z = kAnew marks a range that holds a window's start: no sum of finite
+// rates, whatever the signs of the gaps.
+constexpr float kAnew = -__builtin_inff();
+__device__ __forceinline__ bool anew(float Z) { return Z == kAnew; }
 __device__ __forceinline__ float past(float Z, float U, float h) { return anew(Z) ? U : fmaf(decay_of(Z), h, U); }
 __device__ __forceinline__ float joined(float Za, float Zb) { return anew(Za) || anew(Zb) ? kAnew : Za + Zb; }
 

@@ -301,7 +301,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: tor
 
     ``start`` (B + 1) holds the windows' first tokens and N (``EventPacket.offsets``); it must ascend from 0 to N, which
     is not checked on the device.  ``dt`` (N,) is the gap to the token before, in units of a time constant (the first
-    token's: since h0), not negative; None stands for ones: then h is a running average.  No gradient flows to dt."""
+    token's: since h0); None stands for ones: then h is a running average.  A negative gap (events out of order) grows the
+    state as the formula has it.  No gradient flows to dt."""
     dt = _scan_args(x, gate, dt)
     N, D = x.shape
     _on(start, "start", x.device)
