@@ -541,6 +541,37 @@ def test_offsets_past_32_bits():
     assert torch.equal(y[-tail:], y1) and torch.equal(s[-tail:], s1)
 
 
+def test_calls_of_several_launches():
+    """More workgroups than a launch takes: the last rows and streams against a call on them alone, the first of the
+    second launch among them."""
+    tail, D = 300, 64
+    N = 2 ** 31 // D + tail - 7
+    print(f"several launches: step N={N}", flush=True)
+    few = torch.randn(tail, D, device=DEV)
+    state, x = torch.ones(N, D, device=DEV), torch.ones(1, D, dtype=BF16, device=DEV).expand(N, D)
+    state[-tail:] = few
+    y = ops.gated_scan_step(x, x, state)
+    y1 = ops.gated_scan_step(x[-tail:], x[-tail:], few)
+    assert torch.equal(y[-tail:], y1) and torch.equal(state[-tail:], few)
+    assert torch.equal(y[:-tail:4096], y[:1].expand(y[:-tail:4096].shape))
+    del state, y
+    N, D = 2 ** 25 + tail - 7, 260
+    print(f"several launches: norm N={N}", flush=True)
+    x, w = torch.ones(N, D, dtype=BF16, device=DEV), torch.ones(D, device=DEV)
+    x[-tail:] = torch.randn(tail, D, device=DEV)
+    with torch.no_grad():
+        y, _ = ops.residual_rms_norm(x, None, w)
+        assert torch.equal(y[-tail:], ops.residual_rms_norm(x[-tail:], None, w)[0])
+    assert torch.equal(y[:-tail:4096], torch.ones_like(y[:-tail:4096]))
+    del x, y
+    N, D = 2 ** 23 + tail - 7, 1031
+    print(f"several launches: embedding N={N}", flush=True)
+    ids = torch.randint(0, 5, (N,), device=DEV)
+    table = torch.randn(5, D, device=DEV)
+    y = ops.embed_tokens(ids, table, dtype=BF16)
+    assert torch.equal(y[-tail:], table[ids[-tail:]].to(BF16)) and torch.equal(y[::4096], table[ids[::4096]].to(BF16))
+
+
 def test_scan_of_very_many_windows():
     """More windows than two steps of the 64-way search cover, empty ones among them."""
     rng = np.random.default_rng(15)

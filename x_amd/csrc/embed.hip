@@ -26,9 +26,10 @@ __device__ __forceinline__ int64_t id_at(const void* __restrict__ ids, bool wide
 template <typename T, typename O, int V>
 __global__ void __launch_bounds__(kBlock) k_embed_fwd(const void* __restrict__ ids, bool wide, int64_t N, int64_t vocab,
                                                       const T* __restrict__ table, int64_t st, uint32_t units,
-                                                      uint32_t unit_m, float scale, O* __restrict__ out, int rows) {
+                                                      uint32_t unit_m, float scale, O* __restrict__ out, int rows,
+                                                      int64_t first) {
   constexpr int kAhead = 4;                       // pieces in flight: ids, then rows, then stores
-  const int64_t r0 = (int64_t)blockIdx.x * rows;
+  const int64_t r0 = (first + blockIdx.x) * rows;
   const uint32_t items = (uint32_t)min((int64_t)rows, N - r0) * units;
   for (uint32_t e0 = threadIdx.x; e0 < items; e0 += kBlock * kAhead) {
     int64_t id[kAhead];
@@ -493,9 +494,11 @@ int atl_embed_fwd(const void* ids, int wide_ids, int64_t N, const void* table, i
   auto go = [&](auto t, auto o, auto v) {
     using T = decltype(t);
     using O = decltype(o);
-    hipLaunchKernelGGL((k_embed_fwd<T, O, decltype(v)::value>), dim3((unsigned)((N + rows - 1) / rows)), dim3(kBlock), 0, stream, ids,
-                       wide_ids != 0, N, vocab, (const T*)table, st, (uint32_t)units,
-                       (uint32_t)((((int64_t)1 << 32) + units - 1) / units), (float)scale, (O*)out, (int)rows);
+    in_launches((N + rows - 1) / rows, [&](int64_t first, unsigned n) {
+      hipLaunchKernelGGL((k_embed_fwd<T, O, decltype(v)::value>), dim3(n), dim3(kBlock), 0, stream, ids, wide_ids != 0, N, vocab,
+                         (const T*)table, st, (uint32_t)units, (uint32_t)((((int64_t)1 << 32) + units - 1) / units), (float)scale,
+                         (O*)out, (int)rows, first);
+    });
   };
   if (vec) by_pair<8>(ttype, otype, go);
   else by_pair<1>(ttype, otype, go);

@@ -744,11 +744,11 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
 
 // One token of every stream: 4 bytes of state in and out per channel, bound by the launch.
 template <typename T, bool DT>
-__global__ void __launch_bounds__(kBlock) k_scan_step(int64_t N, int64_t D, int64_t sx, int64_t sg,
+__global__ void __launch_bounds__(kBlock) k_scan_step(int64_t first, int64_t N, int64_t D, int64_t sx, int64_t sg,
                                                       const T* __restrict__ x, const T* __restrict__ g,
                                                       const float* __restrict__ dt, float* __restrict__ h,
                                                       T* __restrict__ y) {
-  const int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t e = (first + blockIdx.x) * kBlock + threadIdx.x;
   if (e >= N * D) return;
   const int64_t i = e / D, c = e - i * D;
   const Gate q = gate_of<T, DT>((float)g[i * sg + c]);
@@ -828,6 +828,10 @@ Carry scan_join(const ScanPlan& q, float* w, hipStream_t stream) {
 // Workgroups that fill the empty windows' states.
 unsigned scan_fill_blocks(int64_t B, int64_t D) { return (unsigned)std::min<int64_t>(256, (B * D + 511) / 512); }
 
+// Whether the workgroups fit a launch (fewer than 2^32 threads; calls of more do not fit the memory but for rows that
+// repeat).
+bool scan_grid_ok(const ScanPlan& q, unsigned fill, int block) { return (q.s.nchunk + fill) * block < (int64_t)1 << 32; }
+
 template <typename F>
 void by_type(int dtype, bool vec, bool dt, F&& f) {
   auto inner = [&](auto t, auto v) {
@@ -875,6 +879,8 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   ScanPlan q = scan_plan<kFwdLen, kFwdBlock>(N, D, scan_vector(dtype, D, sx | sg, ptrs, 3));
   if (!scan_span_ok(q, kFwdLen, std::max(sx, sg), dtype)) { set_error("gated_scan_fwd: row strides %lld, %lld too large", (long long)sx, (long long)sg); return 1; }
   q.s.sx = sx; q.s.sg = sg; q.s.sgy = 0; q.s.B = (int)B;
+  const unsigned fill = scan_fill_blocks(B, D);
+  if (!scan_grid_ok(q, fill, kFwdBlock)) { set_error("gated_scan_fwd: too many tokens, N=%lld D=%lld", (long long)N, (long long)D); return 1; }
   float* w = (float*)ws;
   const bool many = q.s.nchunk > 1;
   Carry carry{};
@@ -887,7 +893,7 @@ int atl_gated_scan_fwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
                          (const T*)x, (const T*)gate, start, dt, h0, w + q.cz, w + q.cu);
       carry = scan_join(q, w, stream);
     }
-    hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + scan_fill_blocks(B, D), q.tiles), dim3(kFwdBlock), 0,
+    hipLaunchKernelGGL((k_scan_apply<T, V, DT>), dim3((unsigned)q.s.nchunk + fill, q.tiles), dim3(kFwdBlock), 0,
                        stream, q.s, (const T*)x, (const T*)gate, start, dt, h0, carry,
                        (T*)y, last, states);
   });
@@ -911,6 +917,7 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
   const bool many = q.s.nchunk > 1;
   Carry carry{};
   const unsigned fill = gh0 ? scan_fill_blocks(B, D) : 0;
+  if (!scan_grid_ok(q, fill, kBwdBlock)) { set_error("gated_scan_bwd: too many tokens, N=%lld D=%lld", (long long)N, (long long)D); return 1; }
   if (q.s.nchunk + fill == 0) return 0;
   auto go = [&](auto t, auto v, auto d, auto y) {
     using T = decltype(t);
@@ -937,11 +944,12 @@ int atl_gated_scan_step(const void* x, int64_t sx, const void* gate, int64_t sg,
   if (!scan_sizes_ok(N, D, 1, dtype) || sx < 0 || sg < 0) { set_error("gated_scan_step: bad sizes N=%lld D=%lld type %d", (long long)N, (long long)D, dtype); return 1; }
   if (N == 0) return 0;
   if (!x || !gate || !state || !y) { set_error("gated_scan_step: null argument"); return 1; }
-  if ((N * D + kBlock - 1) / kBlock >= ((int64_t)1 << 31)) { set_error("gated_scan_step: too large"); return 1; }
   by_type(dtype, false, dt != nullptr, [&](auto t, auto, auto d) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_scan_step<T, decltype(d)::value>), dim3(grid_for(N * D)), dim3(kBlock), 0, stream, N, D, sx, sg,
-                       (const T*)x, (const T*)gate, dt, state, (T*)y);
+    in_launches((N * D + kBlock - 1) / kBlock, [&](int64_t first, unsigned n) {
+      hipLaunchKernelGGL((k_scan_step<T, decltype(d)::value>), dim3(n), dim3(kBlock), 0, stream, first, N, D, sx, sg, (const T*)x,
+                         (const T*)gate, dt, state, (T*)y);
+    });
   });
   return check_launch("gated_scan_step");
 }

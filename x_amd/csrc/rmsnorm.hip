@@ -112,11 +112,12 @@ __device__ __forceinline__ void store_piece(T* row, int64_t c, int64_t D, const 
 template <typename T, typename R, int V, int NV, bool WIDE, bool WHOLE, bool Q8>
 __global__ void __launch_bounds__(kBlock) k_norm_fwd(NormGeo n, const T* __restrict__ x, const R* __restrict__ res,
                                                      const float* __restrict__ w, void* __restrict__ y,
-                                                     R* __restrict__ s, float* __restrict__ scale) {
+                                                     R* __restrict__ s, float* __restrict__ scale, int64_t first) {
   __shared__ float lds[kBlock / kWave];
   const int lanes = WIDE ? kBlock : 1 << n.cl2;
   const int lane = threadIdx.x & (lanes - 1);
-  const int64_t row = WIDE ? blockIdx.x : (int64_t)blockIdx.x * (kBlock >> n.cl2) + (threadIdx.x >> n.cl2);
+  const int64_t block = first + blockIdx.x;
+  const int64_t row = WIDE ? block : block * (kBlock >> n.cl2) + (threadIdx.x >> n.cl2);
   if (!WIDE && row >= n.N) return;
   float v[NV][V];
   float ss = 0.f;
@@ -361,19 +362,21 @@ int atl_rms_norm_fwd(const void* x, int64_t sx, int dtype, const void* res, int6
   const void* ptrs[] = {x, res, w, y, s};
   const NormPlan q = norm_plan(dtype, D, norm_whole(dtype, D, sx | (res ? sr : 0), ptrs, 5));
   n.cl2 = q.cl2;
-  const dim3 grid(q.wide ? (unsigned)N : grid_for(N, kBlock >> q.cl2));
+  const int64_t blocks = q.wide ? N : grid_for(N, kBlock >> q.cl2);
   by_types(dtype, rtype, [&](auto t, auto r) {
     using T = decltype(t);
     using R = decltype(r);
     by_shape<T>(q, [&](auto v, auto nv, auto wide, auto whole) {
       constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
       constexpr bool W = decltype(wide)::value, H = decltype(whole)::value;
-      if (scale)
-        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, true>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
-                           (const R*)res, w, y, (R*)s, scale);
-      else
-        hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, false>), grid, dim3(kBlock), 0, stream, n, (const T*)x,
-                           (const R*)res, w, y, (R*)s, scale);
+      in_launches(blocks, [&](int64_t first, unsigned count) {
+        if (scale)
+          hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, true>), dim3(count), dim3(kBlock), 0, stream, n, (const T*)x,
+                             (const R*)res, w, y, (R*)s, scale, first);
+        else
+          hipLaunchKernelGGL((k_norm_fwd<T, R, V, NV, W, H, false>), dim3(count), dim3(kBlock), 0, stream, n, (const T*)x,
+                             (const R*)res, w, y, (R*)s, scale, first);
+      });
     });
   });
   return check_launch("rms_norm_fwd");

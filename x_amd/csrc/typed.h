@@ -70,6 +70,14 @@ __device__ __forceinline__ void store_f(T* p, const float (&v)[V]) {
   *reinterpret_cast<Pack<T, V>*>(p) = r;
 }
 
+// f(first, n): n of a call's workgroups (of at most 256 threads) from the first on.  A launch takes fewer than 2^32
+// threads in a direction, so a call of more is several launches.
+template <typename F>
+void in_launches(int64_t blocks, F&& f) {
+  constexpr int64_t most = (int64_t)1 << 23;
+  for (int64_t first = 0; first < blocks; first += most) f(first, (unsigned)(blocks - first < most ? blocks - first : most));
+}
+
 // Smallest power of two >= n (n >= 1).
 inline int ceil_pow2(int64_t n) {
   int p = 1;
