@@ -105,22 +105,28 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_count(const void* __restric
   for (int d = threadIdx.x; d < nd; d += kSortBlock) cnt[(int64_t)blockIdx.x * nd + d] = hist[d];
 }
 
-// In place, per digit: the count of a block becomes that of the blocks before it; tot (digits): of all.  64 digits a
-// workgroup, a stretch of the blocks per wave.
+// In place, per digit: the count of a block becomes that of the blocks before it; tot (digits): of all.  16 digits a
+// workgroup, a stretch of the blocks per 16 threads.
+constexpr int kOffDigits = 16, kOffRuns = kSortBlock / kOffDigits;
 __global__ void __launch_bounds__(kSortBlock) k_sort_offsets(int* __restrict__ cnt, int nblk, int nd, int* __restrict__ tot) {
-  __shared__ int part[kSortWaves][kWave];
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const int d = min((int)blockIdx.x * kWave + lane, nd - 1);          // spare lanes repeat the last digit
-  const int per = (nblk + kSortWaves - 1) / kSortWaves, b0 = min(w * per, nblk), b1 = min(b0 + per, nblk);
+  __shared__ int part[kOffRuns][kOffDigits];
+  const int ch = threadIdx.x % kOffDigits, r = threadIdx.x / kOffDigits;
+  const int d = min((int)blockIdx.x * kOffDigits + ch, nd - 1);       // spare threads repeat the last digit
+  const int per = (nblk + kOffRuns - 1) / kOffRuns, b0 = min(r * per, nblk), b1 = min(b0 + per, nblk);
   int sum = 0;
 #pragma unroll 8
   for (int b = b0; b < b1; ++b) sum += cnt[(int64_t)b * nd + d];
-  part[w][lane] = sum;
+  part[r][ch] = sum;
   __syncthreads();
-  int run = 0;
-  for (int k = 0; k < w; ++k) run += part[k][lane];
-  if (w == kSortWaves - 1) tot[d] = run + sum;
-  if ((int)blockIdx.x * kWave + lane >= nd) return;
+  for (int k = 1; k < kOffRuns; k <<= 1) {        // inclusive over the stretches
+    const int v = r >= k ? part[r - k][ch] : 0;
+    __syncthreads();
+    part[r][ch] += v;
+    __syncthreads();
+  }
+  int run = part[r][ch] - sum;
+  if ((int)blockIdx.x * kOffDigits + ch >= nd) return;
+  if (r == kOffRuns - 1) tot[d] = run + sum;
 #pragma unroll 8
   for (int b = b0; b < b1; ++b) {
     const int n = cnt[(int64_t)b * nd + d];
@@ -170,12 +176,15 @@ __device__ __forceinline__ void rank_records(SortLds& l, const Rec (&rec)[kSortI
   __syncthreads();
 }
 
-// off (blocks, digits), tot (digits): as k_sort_offsets leaves them.
+// off (blocks, digits), tot (digits): as k_sort_offsets leaves them.  The tile's records are put in order in LDS first and
+// leave in runs of equal digits: 1M records over 128 digits 9.4 us, 11.4 us each to its place.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const void* __restrict__ src, bool wide, int64_t vocab,
                                                              int64_t N, int shift, int bits, const int* __restrict__ off,
                                                              const int* __restrict__ tot, Rec* __restrict__ dst) {
   __shared__ SortLds l;
+  __shared__ Rec sorted[kSortTile];
+  __shared__ int tile_at[1 << kMaxDigitBits];
   const int nd = 1 << bits, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int64_t i0 = (int64_t)blockIdx.x * kSortTile + w * (kWave * kSortItems) + lane;
   Rec rec[kSortItems];
@@ -187,15 +196,30 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_scatter(const void* __restr
     rec[k] = live[k] ? rec_at<FIRST>(src, wide, vocab, i0 + k * kWave) : Rec{0, 0};
   }
   const int t = (int)threadIdx.x < nd ? tot[threadIdx.x] : 0;
+  const int o = (int)threadIdx.x < nd ? off[(int64_t)blockIdx.x * nd + threadIdx.x] : 0;
   rank_records(l, rec, live, shift, bits, rank);
   int total;
   const int before = block_exclusive_scan<kSortBlock>(t, l.wsum, total);        // records of smaller digits
-  if ((int)threadIdx.x < nd) l.base[threadIdx.x] = before + off[(int64_t)blockIdx.x * nd + threadIdx.x];
+  const int c = (int)threadIdx.x < nd ? l.base[threadIdx.x] : 0;
+  const int here = block_exclusive_scan<kSortBlock>(c, l.wsum, total);          // those of the tile
+  if ((int)threadIdx.x < nd) {
+    tile_at[threadIdx.x] = here;
+    l.base[threadIdx.x] = before + o - here;
+  }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int d = (rec[k].key >> shift) & (nd - 1);
-    if (live[k]) dst[l.base[d] + l.at[w][d] + rank[k]] = rec[k];
+    if (live[k]) sorted[tile_at[d] + l.at[w][d] + rank[k]] = rec[k];
+  }
+  __syncthreads();
+  const int n = (int)min((int64_t)kSortTile, N - (int64_t)blockIdx.x * kSortTile);
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int at = k * kSortBlock + threadIdx.x;
+    if (at >= n) break;
+    const Rec r = sorted[at];
+    dst[l.base[(r.key >> shift) & (nd - 1)] + at] = r;
   }
 }
 
@@ -538,7 +562,7 @@ int atl_embed_bwd(const void* ids, int wide_ids, int64_t N, const void* gout, in
       else
         hipLaunchKernelGGL((k_sort_count<false>), dim3(q.nblk), dim3(kSortBlock), 0, stream, src, false, vocab, N, shift, q.bits, q.nblk,
                            cnt, (uint16_t*)gtable, halves);
-      hipLaunchKernelGGL(k_sort_offsets, dim3(grid_for(nd, kWave)), dim3(kSortBlock), 0, stream, cnt, q.nblk, nd, tot);
+      hipLaunchKernelGGL(k_sort_offsets, dim3(grid_for(nd, kOffDigits)), dim3(kSortBlock), 0, stream, cnt, q.nblk, nd, tot);
       if (pass == 0)
         hipLaunchKernelGGL((k_sort_scatter<true>), dim3(q.nblk), dim3(kSortBlock), 0, stream, src, wide_ids != 0, vocab, N, shift, q.bits,
                            (const int*)cnt, (const int*)tot, dst);
