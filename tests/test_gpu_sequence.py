@@ -420,7 +420,7 @@ def test_embed_layouts(layout, ttype, otype):
 
 
 def test_embed_hot_token_of_many_chunks():
-    """A run of 300,000 tokens (4700 chunks, added up by a workgroup) between others."""
+    """A run of 300,000 tokens (over 73 workgroups, whose shares one workgroup adds up) between others."""
     rng = np.random.default_rng(1)
     N, V, D = 400_000, 1000, 8
     ids = rng.integers(0, V, N)
@@ -430,9 +430,28 @@ def test_embed_hot_token_of_many_chunks():
     y = ops.embed_tokens(torch.as_tensor(ids, device=DEV), table)
     got = torch.autograd.grad(y, table, _t(g))[0]
     want, bound = O.embed_bwd(ids, V, 1.0, g.astype(float))
-    # chunks of 64, their sums in 32 stretches of some 150: 64 + 150 + 32 roundings of the magnitudes, not 300,000
+    # 32 rows a group, 128 groups a workgroup, 128 stretches of a share: 32 + 128 + 1 + 128 roundings of the magnitudes,
+    # not 300,000
     mag = O.embed_bwd(ids, V, 1.0, np.abs(g).astype(float))[0]
     _close(got, want, np.minimum(bound, 400 * O.U * mag))
+
+
+@pytest.mark.parametrize("D", [1, 2, 8, 64, 260, 520])
+def test_embed_runs_of_all_lengths(D):
+    """Tokens that occur from once to 300000 times: runs within a group of lanes, over groups, over up to 16 workgroups
+    and over many.  Whole numbers, so every sum is exact."""
+    rng = np.random.default_rng(D)
+    often = np.array([1, 2, 31, 32, 33, 300_000, 0, 255, 256, 257, 1023, 1024, 1025, 2047, 4099, 1, 17_000, 9_000, 33_000, 0, 40_001, 1])
+    if D > 64:
+        often = often // 4
+    ids = rng.permutation(np.repeat(np.arange(len(often)), often))
+    g = rng.integers(-4, 5, size=(len(ids), D)).astype(np.float32)
+    print(f"embed runs N={len(ids)} D={D}", flush=True)
+    table = torch.zeros(len(often), D, device=DEV, requires_grad=True)
+    out = ops.embed_tokens(torch.as_tensor(ids, device=DEV), table)
+    got, = torch.autograd.grad(out, table, torch.as_tensor(g, device=DEV))
+    want = torch.zeros(len(often), D, dtype=torch.float64).index_add_(0, torch.as_tensor(ids), torch.as_tensor(g).double())
+    assert torch.equal(got.double().cpu(), want)
 
 
 def test_embed_odd_half_precision_table():

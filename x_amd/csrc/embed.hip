@@ -375,20 +375,20 @@ __global__ void __launch_bounds__(kBlock) k_embed_join(RunGeo g, const Rec* __re
   const int64_t p0 = chunk * g.chunk, p1 = p0 + g.chunk;
   if (p1 < g.N) {
     key = rec[p1 - 1].key;
+    const uint32_t behind = rec[p1].key, after_next = rec[min(p1 + g.chunk, g.N - 1)].key;
     const bool begins = !(p0 > 0 && rec[p0].key == key && rec[p0 - 1].key == key);
-    if (key < g.vocab && rec[p1].key == key && begins) {
-      int64_t lo = chunk + 1, hi = g.nchunk;      // the first chunk in (lo, hi) that begins with another key: most runs
-      for (int64_t far = 1; lo + far < hi; far *= 2) {             // end soon, so look near first
-        if (rec[(lo + far) * g.chunk].key != key) {
-          hi = lo + far;
-          break;
-        }
-        lo += far;
-      }
+    if (key < g.vocab && behind == key && begins) {
+      // The first chunk in (lo, hi] that begins with another key: most often the next, else a search by the group's
+      // lanes (one probe at a time, a hot token's run of a hundred chunks took 2 us more).
+      int lo = (int)chunk + 1, hi = (int)g.nchunk;
+      if (lo + 1 < hi && after_next != key) hi = lo + 1;
+      const int lane = threadIdx.x & (lanes - 1);
       while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        if (rec[mid * g.chunk].key == key) lo = mid;
-        else hi = mid;
+        const int step = (hi - lo + lanes) / (lanes + 1), at = lo + step * (lane + 1);
+        const uint64_t same = __ballot(at < hi && rec[(int64_t)min(at, hi - 1) * g.chunk].key == key);
+        const int n = __popcll(same >> (threadIdx.x & (kWave - 1) & ~(lanes - 1)) & (~(uint64_t)0 >> (kWave - lanes)));
+        hi = min(hi, lo + step * (n + 1));
+        lo += step * n;
       }
       after = hi - chunk - 1;
     }
