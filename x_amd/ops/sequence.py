@@ -197,7 +197,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: to
                       p: float = 0.0, seed: int = 0, offset: int = 0):
     """(y, s): the sum s = residual + dropout(x) and its root-mean-square norm y = s / sqrt(mean(s^2) + eps) * weight
     over the last axis (of up to 8192 channels).  s has the residual's type (x's or float32) and is the next residual;
-    y has x's, and is the norm of s as it is returned.  Without a residual s is dropout(x).
+    y has x's, and is the norm of s as it is returned.  Without a residual s is dropout(x) (x itself where p is 0).
 
     Dropout zeroes an element with probability p (to the nearest 1 / 65536) and scales the others by 1 / (1 - p).  Its
     bits come from Philox4x32-10 at counter (row, 2^31 + column // 8, ``offset``) under the key ``seed``, so equal
