@@ -660,3 +660,27 @@ def test_gradients_of_some_inputs():
         part = [t.clone().requires_grad_(j == k) for j, t in enumerate((x, res))]
         got, = torch.autograd.grad(ops.gated_scan(*part, start)[0], part[k], gy)
         assert torch.equal(got, want[k])
+
+
+# ------------------------------------------------------------------------------------------- beside autograd
+def test_step_after_a_use_of_its_state_is_noticed():
+    """A state that a later backward needs and a step has overwritten: that backward raises, as after any operation in
+    place, and a scan from the state as it is works."""
+    x, g = torch.randn(2, 6, 16, device=DEV)
+    state = torch.randn(6, 16, device=DEV)
+    w = torch.randn(16, 16, device=DEV, requires_grad=True)
+    start = torch.arange(7, device=DEV)
+    gate = g.clone().requires_grad_()
+    product = torch.nn.functional.linear(state, w)
+    y, _ = ops.gated_scan(x, gate, start, h0=state)
+    before = state._version
+    ops.gated_scan_step(x, g, state)
+    assert state._version > before
+    for out, wrt in ((product, w), (y, gate)):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), wrt)
+    y, _ = ops.gated_scan(x, gate, start, h0=state)
+    assert torch.autograd.grad(y.sum(), gate)[0].isfinite().all()
+    with torch.inference_mode():
+        inner = torch.zeros(6, 16, device=DEV)
+        assert torch.equal(ops.gated_scan_step(x, g, inner), inner)

@@ -327,7 +327,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: tor
 
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt: torch.Tensor | None = None):
     """One token of each of N streams: ``state`` (N, D) float32 becomes exp(-dt softplus(gate)) state + sigmoid(gate) x in
-    place; returns it in x's type.  For inference (no gradient)."""
+    place; returns it in x's type.  For inference (no gradient): a backward that needs the state as it was raises."""
     dt = _scan_args(x, gate, dt)
     _on(state, "state", x.device)
     if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
@@ -342,4 +342,6 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     with on_device(x.device):
         call("atl_gated_scan_step", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(dt),
              _at(state), _at(y), raw_stream(x.device))
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)      # written by address: whoever saved it has to know
     return y
