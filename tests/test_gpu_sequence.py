@@ -684,3 +684,67 @@ def test_step_after_a_use_of_its_state_is_noticed():
     with torch.inference_mode():
         inner = torch.zeros(6, 16, device=DEV)
         assert torch.equal(ops.gated_scan_step(x, g, inner), inner)
+
+
+def _calls():
+    """The operators as functions of one float tensor, and such a tensor."""
+    ids, start = torch.tensor([0, 3, -1, 5, 2], device=DEV), torch.tensor([0, 2, 6], device=DEV)
+    w = torch.rand(8, device=DEV) + 0.5
+    other = torch.randn(6, 8, device=DEV)
+    return torch.randn(6, 8, device=DEV), {
+        "embed": lambda t: ops.embed_tokens(ids, t, scale=2.0),
+        "norm": lambda t: torch.stack(ops.residual_rms_norm(t, other, w, p=0.25, seed=3)),
+        "scan": lambda t: ops.gated_scan(t, other, start)[0],
+        "gate": lambda t: torch.cat(ops.gated_scan(other, t, start)),
+        "h0": lambda t: torch.cat(ops.gated_scan(other, other, start, h0=t[:2])),
+        "fp8": lambda t: ops.residual_rms_norm_fp8(t, other, w)[1],
+        "step": lambda t: ops.gated_scan_step(t, other, torch.ones(6, 8, device=DEV)),
+    }
+
+
+@pytest.mark.parametrize("which", ["embed", "norm", "scan", "gate", "h0"])
+def test_forward_mode_derivatives_are_refused(which):
+    """A tangent is refused, not dropped; without one a call at a forward-mode level is a call as any other."""
+    t, calls = _calls()
+    want = calls[which](t)
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.equal(calls[which](t), want)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            calls[which](torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("which", ["embed", "norm", "scan", "gate", "h0", "fp8", "step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_recorded_calls_compute_or_are_refused(which, grad):
+    """A recording that would replay the outputs' memory alone is refused; torch.jit.trace keeps the differentiable
+    operators as calls, which compute on the new input."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t, calls = _calls()
+    fn = calls[which]
+    t.requires_grad_(grad)
+    for how in ({}, {"pre_dispatch": True}, {"tracing_mode": "fake"}):
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(fn, **how)(t)
+    if which in ("fp8", "step"):
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(fn, (t,), check_trace=False)
+        return
+    traced = torch.jit.trace(fn, (t,), check_trace=False)
+    for _ in range(3):
+        new = torch.randn_like(t)
+        assert torch.equal(traced(new), fn(new))
+
+
+@pytest.mark.parametrize("which", ["embed", "norm", "scan", "h0", "fp8", "step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_compiled_calls_compute(which, grad):
+    """torch.compile breaks its graph at the operators and calls them."""
+    t, calls = _calls()
+    torch._dynamo.reset()
+    fn = torch.compile(lambda a: calls[which](a * 2) + 1, backend="eager")
+    for _ in range(2):
+        t = torch.randn_like(t).requires_grad_(grad)
+        got, want = fn(t), calls[which](t * 2) + 1
+        assert torch.equal(got, want)
+        if grad and want.requires_grad:
+            assert torch.equal(torch.autograd.grad(got.sum(), t)[0], torch.autograd.grad(want.sum(), t)[0])

@@ -12,7 +12,10 @@ layouts are copied first.  Device tensors run on the HIP kernels, CPU tensors on
 """
 from __future__ import annotations
 
+import sys
+
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import reference as ref
@@ -54,7 +57,30 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grads_wanted(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    """Whether a call goes through its autograd function: for a gradient, and wherever a derivative or a recording would
+    take the kernel's output for memory that nothing was computed into.  The function refuses tangents, and
+    torch.jit.trace keeps it as a call."""
+    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts))
+            or (not torch.compiler.is_compiling()
+                and (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)))
+
+
+def _on_kernels(t: torch.Tensor, what: str, function: bool = True) -> bool:
+    """Whether the operator runs on the HIP kernels; raises where the call is being recorded in a way that would not hold
+    it: operation by operation (make_fx, the kernels are none), or by torch.jit.trace without an autograd function.
+    torch.compile leaves the calls outside of its graphs."""
+    if not ext_supports(t):
+        return False
+    if torch.compiler.is_compiling():
+        return True
+    C = torch._C
+    if C._len_torch_dispatch_stack() or C._dispatch_tls_is_dispatch_key_included(C.DispatchKey.PreDispatch):
+        proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+        if proxies is not None and proxies.get_proxy_mode() is not None:
+            raise RuntimeError(f"{what} cannot be recorded operation by operation: call it outside of the recorded program")
+    if not function and C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what} cannot be recorded: it has no gradient and no autograd function to keep")
+    return True
 
 
 def _ws(nbytes: int, dev, what: str) -> torch.Tensor:
@@ -110,7 +136,7 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dty
     if dtype not in _CODE:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     scale = float(scale)
-    if not ext_supports(table):
+    if not _on_kernels(table, "embed_tokens"):
         return ref.embed_tokens(ids, table, scale, dtype)
     ids, rows = ids.contiguous(), _rows(table)
     if _grads_wanted(table):
@@ -204,7 +230,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     (seed, offset) give equal masks whatever the launch, the backward draws them again, and no mask is stored."""
     eps, p = _norm_args(x, residual, weight, eps, p)
     seed, offset = int(seed) & _U64, int(offset) & _U64
-    if not ext_supports(x):
+    if not _on_kernels(x, "residual_rms_norm"):
         return ref.residual_rms_norm(x, residual, weight, eps, p, seed, offset)
     w = weight.to(F32).contiguous()
     if _grads_wanted(x, residual, w):
@@ -219,7 +245,7 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight
     scale (..., 1) = max(max |y|, 1e-30) / 448, q = 448 y / max |y| rounded to nearest.  For inference (no gradient): q
     and scale are what a row-scaled 8-bit product takes."""
     eps, _ = _norm_args(x, residual, weight, eps)
-    if not ext_supports(x):
+    if not _on_kernels(x, "residual_rms_norm_fp8", function=False):
         with torch.no_grad():
             return ref.residual_rms_norm_fp8(x, residual, weight, eps)
     y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.detach().to(F32).contiguous(),
@@ -317,7 +343,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: tor
             raise ValueError(f"h0 must be ({B}, {D}), got {tuple(h0.shape)}")
         h0 = h0.to(F32).contiguous()
     start = start.to(I64).contiguous()
-    if not ext_supports(x):
+    if not _on_kernels(x, "gated_scan"):
         return ref.gated_scan(x, gate, start, dt, h0)
     rx, rg = _rows(x), _rows(gate)
     if _grads_wanted(x, gate, h0):
@@ -333,7 +359,7 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
         raise ValueError(f"state must be a contiguous float32 tensor of {tuple(x.shape)} without gradient, got "
                          f"{tuple(state.shape)}, {state.dtype}")
-    if not ext_supports(x):
+    if not _on_kernels(x, "gated_scan_step", function=False):
         with torch.no_grad():
             return ref.gated_scan_step(x, gate, state, dt)
     x, gate = _rows(x), _rows(gate)
