@@ -124,3 +124,76 @@ def test_refuses_bad_sizes():
             EventRecurrence(40, 48, **kw)
     with pytest.raises(ValueError):
         EventRecurrence(40, 48, dim=40).fp8_weights()
+
+
+def _two_windows(dev, B=3, seed=6):
+    """Consecutive windows of B streams, each with times of its own in [0, 1], and idle time on both sides of the
+    boundary; the last stream's middle window is empty.  Returns the three windows and all events as one scan's rows
+    (xy, p, gaps in windows, start)."""
+    gen = torch.Generator().manual_seed(seed)
+    windows, events = [], [[] for _ in range(B)]
+    for k, sizes in enumerate(([9, 7, 8], [6, 9, 0], [5, 4, 7])):
+        parts = []
+        for b in range(B):
+            n = sizes[b]
+            t = torch.sort(torch.rand(n, generator=gen)).values * 0.4 + 0.3
+            xy = torch.rand(n, 2, generator=gen) * torch.tensor([47.0, 39.0])
+            p = torch.where(torch.rand(n, generator=gen) < 0.5, 1.0, -1.0)
+            parts.append((xy, t, p, torch.full((n,), b)))
+            events[b].append((xy, t.double() + k, p))
+        windows.append(EventPacket(*(torch.cat(v) for v in zip(*parts)), B, 40, 48).to(dev))
+    rows = [[torch.cat(v) for v in zip(*e)] for e in events]
+    gaps = torch.cat([torch.diff(t, prepend=torch.zeros(1, dtype=t.dtype)) for _, t, _ in rows]).float()
+    start = torch.tensor([0, *torch.cumsum(torch.tensor([len(t) for _, t, _ in rows]), 0).tolist()])
+    return windows, torch.cat([r[0] for r in rows]).to(dev), torch.cat([r[2] for r in rows]).to(dev), gaps.to(dev), start.to(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_streams_window_by_window(dev):
+    """States handed on over windows, with the time since each stream's last event, are those of all events in one
+    scan, event by event too: also over an empty window."""
+    net = _net(dev, torch.float32, tau=0.5)
+    windows, xy, p, gaps, start = _two_windows(dev)
+    want = net.fresh_states(3)
+    for k in range(int((start[1:] - start[:-1]).max())):
+        on = (start[:-1] + k < start[1:]).nonzero()[:, 0]
+        at = start[:-1][on] + k
+        part = net.step(xy[at], p[at], gaps[at] / net.tau, [s[on] for s in want])
+        for s, q in zip(want, part):
+            s[on] = q
+    h0 = since = None
+    for ev in windows:
+        h0, since = net.states(ev, h0=h0, since=since), net.idle(ev, since)
+    for a, b in zip(h0, want):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)
+    last = torch.stack([(1 - windows[2].t[windows[2].b == b][-1]) for b in range(3)])
+    assert torch.allclose(since, last)
+    # an event at 0.1 of the next window: 0.1 and the idle time after the last one
+    late = EventPacket(torch.zeros(1, 2, device=dev), torch.full((1,), 0.1, device=dev), torch.ones(1, device=dev),
+                       torch.ones(1, dtype=torch.int64, device=dev), 3, 40, 48)
+    assert torch.allclose(net.gaps(late, since) * net.tau, since[1:2] + 0.1)
+    assert torch.allclose(net.idle(late, since), torch.stack([since[0] + 1, 1 - late.t[0], since[2] + 1]))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_time_since_reaches_the_motion(dev):
+    net, ev = _net(dev, torch.float32), _packet(dev, n=100, B=2)
+    h0 = [torch.ones(2, net.dim, device=dev) for _ in net.norm]
+    since = torch.tensor([0.0, 30.0], device=dev)
+    near = net.motion(ev, h0=h0).coeff_grid
+    far = net.motion(ev, h0=h0, since=since).coeff_grid
+    fresh = net.motion(ev).coeff_grid
+    assert torch.equal(near[0], far[0]) and not torch.equal(near[1], far[1])
+    assert torch.allclose(far[1], fresh[1], atol=1e-6)             # 480 time constants forget everything
+
+
+def test_time_since_is_checked():
+    net, ev = _net("cpu", torch.float32), _packet("cpu", n=20, B=2)
+    h0 = net.fresh_states(2)
+    for bad in (torch.zeros(3), torch.zeros(2, 1)):
+        with pytest.raises(ValueError):
+            net.states(ev, h0=h0, since=bad)
+        with pytest.raises(ValueError):
+            net.idle(ev, bad)
+    with pytest.raises(ValueError):
+        net.states(ev, since=torch.zeros(2))

@@ -11,7 +11,10 @@ states give the coefficients of a grid of trajectories, upsampled to the sensor:
     loss = AnchoredExact(h=1.0, tau=0.2)(ev, motion)["loss"]
     loss.backward()
 
-A stream is followed event by event with :meth:`step`, or window by window by handing the states on.
+A stream is followed event by event with :meth:`step`, or window by window by handing on the states and the time since
+the last events, which the first gap of the next window adds to its own:
+
+    states, since = net.states(ev, h0=states, since=since), net.idle(ev, since)      # (None, None before the first)
 """
 from __future__ import annotations
 
@@ -56,17 +59,39 @@ class EventRecurrence(nn.Module):
                torch.div(col, self.cell, rounding_mode="floor")) * 2 + (p > 0).long()
         return torch.where(inside, ids, -1)
 
-    def gaps(self, ev: EventPacket) -> torch.Tensor:
-        """Time since the event before in units of tau; the first of a window since the window's start."""
+    def gaps(self, ev: EventPacket, since=None) -> torch.Tensor:
+        """Time since the event before in units of tau; the first of a window since the window's start, and with ``since``
+        (B,) since the stream's last event, so long (in windows) before the window's start."""
         before = torch.cat([ev.t.new_zeros(1), ev.t[:-1]])[:ev.n]
         fresh = torch.cat([ev.b.new_full((1,), -1), ev.b[:-1]])[:ev.n] != ev.b
-        return (ev.t - torch.where(fresh, 0.0, before)) / self.tau
+        first = 0.0 if since is None else -self._since(ev, since)[ev.b]
+        return (ev.t - torch.where(fresh, first, before)) / self.tau
+
+    def idle(self, ev: EventPacket, since=None) -> torch.Tensor:
+        """Time (B,) from every window's last event to the window's end, in windows: ``since`` for the windows after these.
+        A window without events adds its whole length to its own ``since`` (None: zeros)."""
+        since = ev.t.new_zeros(ev.batch_size) if since is None else self._since(ev, since)
+        start = ev.offsets
+        if ev.n == 0:
+            return since + 1
+        last = ev.t[(start[1:] - 1).clamp(min=0)]
+        return torch.where(start[1:] > start[:-1], 1 - last, since + 1)
+
+    @staticmethod
+    def _since(ev: EventPacket, since: torch.Tensor) -> torch.Tensor:
+        if since.shape != (ev.batch_size,):
+            raise ValueError(f"since must be ({ev.batch_size},), got {tuple(since.shape)}")
+        return since.to(ev.t.dtype)
 
     # ------------------------------------------------------------------------------------------ windows
-    def states(self, ev: EventPacket, h0=None, p: float = 0.0, seed: int = 0) -> list:
+    def states(self, ev: EventPacket, h0=None, p: float = 0.0, seed: int = 0, since=None) -> list:
         """The layers' last states (B, dim) of every window, from ``h0`` (as returned for the window before) or zero; p
-        drops the layers' outputs (masks by (seed, layer))."""
-        start, dt = ev.offsets, self.gaps(ev)
+        drops the layers' outputs (masks by (seed, layer)).  ``since`` (B,), with ``h0``: the time from each stream's last
+        event to the window's start, in windows (:meth:`idle` of the window before); without it the windows start at
+        those events."""
+        if since is not None and h0 is None:
+            raise ValueError("since says how old the states in h0 are, and h0 is None")
+        start, dt = ev.offsets, self.gaps(ev, since)
         s = embed_tokens(self.tokens(ev.xy, ev.p), self.table, scale=math.sqrt(self.dim), dtype=self.dtype)
         x, last = None, []
         for k, (w, into) in enumerate(zip(self.norm, self.into)):
@@ -86,9 +111,9 @@ class EventRecurrence(nn.Module):
         c = nn.functional.linear(torch.cat(states, 1), self.head).view(-1, 2 * self.K, *self.grid)
         return nn.functional.interpolate(c, size=(self.H, self.W), mode="bilinear", align_corners=False)
 
-    def motion(self, ev: EventPacket, h0=None, p: float = 0.0, seed: int = 0, **kw) -> PixelTrajectories:
-        """The windows' motion; keywords go to :class:`PixelTrajectories`."""
-        return PixelTrajectories(self.coefficients(self.states(ev, h0, p, seed)), self.K, **kw)
+    def motion(self, ev: EventPacket, h0=None, p: float = 0.0, seed: int = 0, since=None, **kw) -> PixelTrajectories:
+        """The windows' motion (:meth:`states`' arguments); keywords go to :class:`PixelTrajectories`."""
+        return PixelTrajectories(self.coefficients(self.states(ev, h0, p, seed, since)), self.K, **kw)
 
     # ------------------------------------------------------------------------------------------ streams
     def fresh_states(self, streams: int) -> list:
