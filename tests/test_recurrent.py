@@ -197,3 +197,12 @@ def test_time_since_is_checked():
             net.idle(ev, bad)
     with pytest.raises(ValueError):
         net.states(ev, since=torch.zeros(2))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_positions_that_are_not_numbers_are_no_tokens(dev):
+    net = _net(dev, torch.float32)
+    bad = [float("nan"), float("inf"), -float("inf"), 1e30, -1e30]
+    xy = torch.tensor([[v, 3.0] for v in bad] + [[3.0, v] for v in bad] + [[3.0, 3.0]], device=dev)
+    ids = net.tokens(xy, torch.ones(11, device=dev))
+    assert ids.tolist() == [-1] * 10 + [1]

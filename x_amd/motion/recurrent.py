@@ -52,9 +52,11 @@ class EventRecurrence(nn.Module):
 
     # ------------------------------------------------------------------------------------------ tokens
     def tokens(self, xy: torch.Tensor, p: torch.Tensor) -> torch.Tensor:
-        """Ids of events: (row of cells, column of cells, polarity); -1 (no token) outside the sensor."""
-        col, row = torch.floor(xy[:, 0] + 0.5).long(), torch.floor(xy[:, 1] + 0.5).long()
+        """Ids of events: (row of cells, column of cells, polarity); -1 (no token) outside the sensor or where a position
+        is not a number (told before the conversion to integers, which makes a zero of it on the device)."""
+        col, row = torch.floor(xy[:, 0] + 0.5), torch.floor(xy[:, 1] + 0.5)
         inside = (col >= 0) & (col < self.W) & (row >= 0) & (row < self.H)
+        col, row = torch.where(inside, col, 0.0).long(), torch.where(inside, row, 0.0).long()
         ids = (torch.div(row, self.cell, rounding_mode="floor") * self.columns +
                torch.div(col, self.cell, rounding_mode="floor")) * 2 + (p > 0).long()
         return torch.where(inside, ids, -1)
