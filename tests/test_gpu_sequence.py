@@ -748,3 +748,28 @@ def test_compiled_calls_compute(which, grad):
         assert torch.equal(got, want)
         if grad and want.requires_grad:
             assert torch.equal(torch.autograd.grad(got.sum(), t)[0], torch.autograd.grad(want.sum(), t)[0])
+
+
+@pytest.mark.parametrize("dtype,D", [(F32, 24), (BF16, 64), (F16, 64), (F32, 5000)])
+@pytest.mark.parametrize("p", [0.0, 0.4])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_which_the_sum_alone_is_used(dtype, D, p, residual):
+    """The gradient of s alone is gs (through the dropout for x) also in rows whose norm is not finite: a row of zeros
+    with eps = 0 and a row with an infinity.  The weight has no part in it."""
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    x, res, gs = (torch.randn(50, D, device=DEV, generator=gen).to(dtype) for _ in range(3))
+    x[3], res[3] = 0, 0
+    res[7, 2], x[7, 2] = float("inf"), 1
+    if not residual:
+        x[7, 2] = float("inf")
+    w = torch.ones(D, device=DEV, requires_grad=True)
+    ins = [x.requires_grad_(), *([res.requires_grad_()] if residual else [])]
+    y, s = ops.residual_rms_norm(x, res if residual else None, w, eps=0.0, p=p, seed=4)
+    got = torch.autograd.grad(s, [*ins, w], gs, allow_unused=True)
+    keep = torch.as_tensor(O.keeps(50, D, p, 4, 0), device=DEV)
+    factor = 65536 / (65536 - round(65536 * p))
+    # one product in single precision, rounded to the type
+    assert torch.equal(got[0], torch.where(keep, gs.float() * torch.tensor(factor, device=DEV), 0.0).to(dtype))
+    if residual:
+        assert torch.equal(got[1], gs)
+    assert got[-1] is None or not got[-1].any()

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
       for (int k = 0; k < V; ++k) sv[j][k] = yv[j][k] = 0.f;
       if (c >= n.D) continue;
       load_piece<WHOLE, V>(s + row * n.sr, c, n.D, sv[j]);
-      if (gy) load_piece<WHOLE, V>(gy + row * n.sgy, c, n.D, yv[j]);
+      load_piece<WHOLE, V>(gy + row * n.sgy, c, n.D, yv[j]);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         ss = fmaf(sv[j][k], sv[j][k], ss);
@@ -247,6 +247,26 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd(NormGeo n, const R* __restr
     for (int g = 0; g < rows; ++g) sum += dyn[g * width + c];
     part[blockIdx.x * n.D + c] = sum;
   }
+}
+
+// The same where the sum alone was used (no gy): ds = gs, and the norm has no part, nor has a root of a row that is not
+// finite (zero times it would be no number).  gs null: zeros.
+template <typename T, typename R, int V, bool WHOLE>
+__global__ void __launch_bounds__(kBlock) k_norm_bwd_sum(NormGeo n, const R* __restrict__ gs, T* __restrict__ gx,
+                                                         R* __restrict__ gres) {
+  const int rows = kBlock >> n.cl2, lane = threadIdx.x & ((1 << n.cl2) - 1);
+  for (int64_t row = (int64_t)blockIdx.x * rows + (threadIdx.x >> n.cl2); row < n.N; row += (int64_t)gridDim.x * rows)
+    for (int64_t c = lane * V; c < n.D; c += V << n.cl2) {
+      float d[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) d[k] = 0.f;
+      if (gs) load_piece<WHOLE, V>(gs + row * n.sgs, c, n.D, d);
+      if (gres) store_piece<WHOLE, V>(gres + row * n.D, c, n.D, d);
+      if (gx) {
+        if (n.t) dropout<V>(n, row, c, d);
+        store_piece<WHOLE, V>(gx + row * n.D, c, n.D, d);
+      }
+    }
 }
 
 // gw[c] = sum over the workgroups' shares: 16 channels a workgroup, 64 interleaved runs of the shares side by side.
@@ -399,7 +419,18 @@ int atl_rms_norm_bwd(const void* s, int64_t ss, int rtype, const float* w, const
   const void* ptrs[] = {s, w, gy, gs, gx, gres};
   const NormPlan q = norm_plan(dtype, D, norm_whole(dtype, D, ss | (gy ? sgy : 0) | (gs ? sgs : 0), ptrs, 6));
   n.cl2 = q.cl2;
-  const int nblk = norm_blocks(N, q);
+  const int nblk = gy ? norm_blocks(N, q) : 0;    // shares of gw
+  if (!gy && N > 0)
+    by_types(dtype, rtype, [&](auto t, auto r) {
+      using T = decltype(t);
+      using R = decltype(r);
+      constexpr int V = 16 / sizeof(T);
+      const dim3 grid((unsigned)std::min<int64_t>(grid_for(N, kBlock >> q.cl2), 2048));
+      if (q.whole)
+        hipLaunchKernelGGL((k_norm_bwd_sum<T, R, V, true>), grid, dim3(kBlock), 0, stream, n, (const R*)gs, (T*)gx, (R*)gres);
+      else
+        hipLaunchKernelGGL((k_norm_bwd_sum<T, R, V, false>), grid, dim3(kBlock), 0, stream, n, (const R*)gs, (T*)gx, (R*)gres);
+    });
   if (nblk > 0)
     by_types(dtype, rtype, [&](auto t, auto r) {
       using T = decltype(t);

@@ -176,6 +176,7 @@ class _Norm(torch.autograd.Function):
         want_x, want_r, want_w = ctx.needs_input_grad[:3]
         if gy is None and gs is None:
             return (None,) * 7
+        want_w = want_w and gy is not None                 # the weight has no part in the sum
         s = _rows(s)
         N, D = s.shape
         dev = s.device
