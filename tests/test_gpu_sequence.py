@@ -773,3 +773,23 @@ def test_norm_of_which_the_sum_alone_is_used(dtype, D, p, residual):
     if residual:
         assert torch.equal(got[1], gs)
     assert got[-1] is None or not got[-1].any()
+
+
+@pytest.mark.parametrize("D", [1, 3, 64])
+def test_one_row_of_a_very_wide_tensor(D):
+    """A single token cut from a row of four million: the stride of one row means nothing."""
+    wide = torch.randn(1, 2 ** 22, device=DEV)
+    a, b = wide[:, 5:5 + D], wide[:, 900_001:900_001 + D]
+    print(f"one row D={D} stride {a.stride(0)}", flush=True)
+    few = [t.clone() for t in (a, b)]
+    start, w, ids = torch.tensor([0, 1], device=DEV), torch.ones(D, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    grads = [[] for _ in range(2)]
+    for k, (x, g) in enumerate(((a, b), few)):
+        x, g = x.detach().requires_grad_(), g.detach().requires_grad_()
+        y, last = ops.gated_scan(x, g, start)
+        n, s = ops.residual_rms_norm(x, g, w)
+        e = ops.embed_tokens(ids, x)
+        state = torch.ones(1, D, device=DEV)
+        ops.gated_scan_step(x.detach(), g.detach(), state)
+        grads[k] = [y, last, n, s, e, state, *torch.autograd.grad((y, n, e), (x, g), (b, b, b.expand(3, D)))]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))

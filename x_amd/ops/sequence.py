@@ -53,6 +53,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     apart), else a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] < 2 and t.stride(0) > MAX_ROW_STRIDE:
+        t = t.reshape(-1).view(t.shape)                # a single row's stride says nothing
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) <= MAX_ROW_STRIDE else t.contiguous()
 
 
