@@ -793,3 +793,58 @@ def test_one_row_of_a_very_wide_tensor(D):
         ops.gated_scan_step(x.detach(), g.detach(), state)
         grads[k] = [y, last, n, s, e, state, *torch.autograd.grad((y, n, e), (x, g), (b, b, b.expand(3, D)))]
     assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+def _mostly_empty(empty, dtype, seed):
+    """Tokens in few windows among ``empty`` windows without any: between the tokens, before them and behind them."""
+    rng = np.random.default_rng(seed)
+    sizes = np.zeros(empty + 40, np.int64)
+    at = np.sort(rng.choice(empty // 8, 20, replace=False)) + empty // 16       # some far apart, and 20 side by side
+    at = np.concatenate([at, np.arange(20) + empty // 4 * 3])
+    sizes[at] = rng.integers(1, 90, 40)
+    start = np.concatenate([[0], np.cumsum(sizes)])
+    N, D = int(start[-1]), 8
+    x, g, gy = (_t(rng.normal(size=(N, D)), dtype) for _ in range(3))
+    dt = _t(rng.exponential(size=N) * 0.1)
+    h0, gl = (torch.randn(len(sizes), D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(k)) for k in (1, 2))
+    return start, at, x, g, gy, dt, h0, gl
+
+
+@pytest.mark.parametrize("empty,dtype", [(3000, F32), (1_000_000, F32), (1_000_000, BF16)])
+def test_scan_among_very_many_empty_windows(empty, dtype):
+    """The windows with tokens against the oracle on them alone; the empty ones hand on h0 and the last state's
+    gradient."""
+    start, at, x, g, gy, dt, h0, gl = _mostly_empty(empty, dtype, seed=empty)
+    print(f"scan among {empty} empty windows, N={x.shape[0]}", flush=True)
+    ins = [a.requires_grad_() for a in (x, g, h0)]
+    y, last = ops.gated_scan(x, g, torch.as_tensor(start, device=DEV), dt=dt, h0=h0)
+    got = torch.autograd.grad((y, last), ins, (gy, gl))
+    few = [0, *start[at + 1].tolist()]
+    args = (_np(x), _np(g), few)
+    wy, wl, E = O.scan(*args, _np(dt), _np(h0[at]))
+    _close(y, wy, E, "y")
+    _close(last[at], wl, E[np.array(few[1:]) - 1], "last")
+    want, bound = O.scan_bwd(*args, _np(gy), _np(gl[at]), _np(dt), _np(h0[at]))
+    for name, a, b, c in zip(("gx", "gg", "gh0"), (got[0], got[1], got[2][at]), want, bound):
+        _close(a, b, c, name)
+    none = torch.ones(len(start) - 1, dtype=torch.bool, device=DEV)
+    none[at] = False
+    assert torch.equal(last[none], h0[none]) and torch.equal(got[2][none], gl[none])
+
+
+def test_scan_time_does_not_follow_the_empty_windows():
+    """A million empty windows cost a search, not a walk: forward and backward of a few tokens stay within 20 ms (a
+    dependent read for each would be a second, writing the windows' states takes under one millisecond)."""
+    start, _, x, g, gy, dt, _, _ = _mostly_empty(1_000_000, F32, seed=5)
+    start = torch.as_tensor(start, device=DEV)
+    ins = [a.requires_grad_() for a in (x, g)]
+    best = 1e9
+    for _ in range(4):
+        e0, e1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        e0.record()
+        torch.autograd.grad(ops.gated_scan(x, g, start, dt=dt)[0], ins, gy)
+        e1.record()
+        e1.synchronize()
+        best = min(best, e0.elapsed_time(e1))
+    print(f"{best:.2f} ms", flush=True)
+    assert best < 20

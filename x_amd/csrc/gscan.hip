@@ -116,6 +116,24 @@ __device__ __forceinline__ int count_below(const int64_t* __restrict__ start, in
   return lo + __popcll(__ballot(lane < n && start[lo + (lane < n ? lane : 0)] < i));
 }
 
+// The last window from b on that starts before token i (those up to b do).  Steps double until they pass the place and
+// halve back to it: windows without tokens may stand there by the million, a window with some is the next one.
+__device__ __forceinline__ int last_before(const int64_t* __restrict__ start, int B, int b, int64_t i) {
+  uint32_t step = 1;
+  for (; step < (uint32_t)B - (uint32_t)b && start[b + (int)step] < i; step <<= 1) b += (int)step;
+  for (step >>= 1; step > 0; step >>= 1)
+    if (step < (uint32_t)B - (uint32_t)b && start[b + (int)step] < i) b += (int)step;
+  return b;
+}
+// The last window below b that starts at or before token i (b and those behind it start after it), or window 0.
+__device__ __forceinline__ int last_upto(const int64_t* __restrict__ start, int b, int64_t i) {
+  uint32_t step = 1;
+  for (; step < (uint32_t)b && start[b - (int)step] > i; step <<= 1) b -= (int)step;
+  for (step >>= 1; step > 0; step >>= 1)
+    if (step < (uint32_t)b && start[b - (int)step] > i) b -= (int)step;
+  return b - 1;
+}
+
 // Where a thread works: its channels, its group and the group's n tokens from i0 on.
 struct Place {
   int64_t c, i0;
@@ -168,15 +186,20 @@ struct Ascend {
   __device__ __forceinline__ void look(const int64_t* __restrict__ start, int64_t i0) {
     next = (int)min(start[b + 1] - i0, (int64_t)1 << 30);
   }
-  __device__ __forceinline__ Ascend(const int64_t* __restrict__ start, int B, int64_t wave_first, int64_t i0) {
+  __device__ __forceinline__ Ascend(const int64_t* __restrict__ start, int B, int64_t wave_first, const Place& p) {
     b = count_below(start, B, wave_first) - 1;
-    while (b + 1 < B && start[b + 1] < i0) ++b;
-    look(start, i0);
+    if (p.live) b = last_before(start, B, b, p.i0);
+    look(start, p.i0);
   }
   // Whether token i0 + t is the first of a window, which b is then.
   __device__ __forceinline__ bool starts(const int64_t* __restrict__ start, int B, int64_t i0, int t) {
     if (t != next || b + 1 >= B) return false;
-    do { ++b; look(start, i0); } while (next <= t && b + 1 < B);
+    ++b;
+    look(start, i0);
+    if (next <= t && b + 1 < B) {                 // windows without tokens
+      b = last_before(start, B, b, i0 + t + 1);
+      look(start, i0);
+    }
     return true;
   }
 };
@@ -189,18 +212,18 @@ struct Descend {
   __device__ __forceinline__ void look(const int64_t* __restrict__ start, int64_t i0) {
     first = (int)max(start[b] - i0, -((int64_t)1 << 30));
   }
-  __device__ __forceinline__ Descend(const int64_t* __restrict__ start, int B, int64_t wave_first, int64_t i0, int n) {
-    const int64_t i = i0 + n - 1;
+  __device__ __forceinline__ Descend(const int64_t* __restrict__ start, int B, int64_t wave_first, const Place& p) {
+    const int64_t behind = p.i0 + p.n;
     b = count_below(start, B, wave_first + 1) - 1;                 // the last window that starts at or before it
-    while (b + 1 < B && start[b + 1] <= i) ++b;
+    if (p.live) b = last_before(start, B, b, behind);
     b = max(b, 0);
-    look(start, i0);
-    last = i + 1 == start[b + 1];
+    look(start, p.i0);
+    last = behind == start[b + 1];
   }
   __device__ __forceinline__ void step(const int64_t* __restrict__ start, int64_t i0, int t) {      // to token i0 + t
     last = false;
     if (t < first && b > 0) {
-      do { --b; } while (b > 0 && start[b] > i0 + t);
+      b = last_upto(start, b, i0 + t);
       look(start, i0);
       last = true;
     }
@@ -335,7 +358,7 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_local(ScanGeo s, const T* __
   const Rows<const T, kFwdLen> rg(s, p, g, s.sg, blockIdx.x);
   Rows<const float, kFwdLen> rd(s, p, dt, 1, blockIdx.x);
   rd.off = p.gi * kFwdLen * 4;
-  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, blockIdx.x), p.i0);
+  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, blockIdx.x), p);
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(kFwdBlock) k_scan_apply(ScanGeo s, const T* __
   Rows<const float, kFwdLen> rd(s, p, dt, 1, chunk);
   rd.off = p.gi * kFwdLen * 4;
   const Rows<T, kFwdLen> ro(s, p, y, s.D, chunk);
-  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, chunk), p.i0);
+  Ascend win(start, s.B, wave_first_token<kFwdLen>(s, chunk), p);
   const Ascend begin = win;
   float a[kFwdLen][V], u[kFwdLen][V];
   Decay<V, DT> decay;
@@ -587,7 +610,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_local(ScanGeo s, const T
   const Rows<const T, kBwdLen> ry(s, p, gy, s.sgy, blockIdx.x);
   Rows<const float, kBwdLen> rd(s, p, dt, 1, blockIdx.x);
   rd.off = p.gi * kBwdLen * 4;
-  Descend win(start, s.B, wave_first_token<kBwdLen>(s, blockIdx.x), p.i0, p.n);
+  Descend win(start, s.B, wave_first_token<kBwdLen>(s, blockIdx.x), p);
   Decay<V, DT> decay;
   float U[V], Z[V];
 #pragma unroll
@@ -655,7 +678,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
   rd.off = p.gi * kBwdLen * 4;
   const Rows<T, kBwdLen> rox(s, p, gx, s.D, chunk), rog(s, p, gg, s.D, chunk);
   const int64_t wf = wave_first_token<kBwdLen>(s, chunk);
-  Descend win(start, s.B, wf, p.i0, p.n);
+  Descend win(start, s.B, wf, p);
   const Descend begin = win;
   float a[kBwdLen][V], w[kBwdLen][V], f[kBwdLen][V];      // f: gg = H f
   Pack<T, V> yr[kBwdLen];
@@ -665,7 +688,7 @@ __global__ void __launch_bounds__(kBwdBlock) k_scan_bwd_apply(ScanGeo s, const T
   for (int k = 0; k < V; ++k) U[k] = 0.f;
   bool reset = false;
   const bool plain = plain_wave<kBwdLen>(p, win);
-  Ascend up(start, s.B, wf, p.i0);
+  Ascend up(start, s.B, wf, p);
   if (p.live) by_flag(plain, [&](auto flag) {
     constexpr bool PLAIN = decltype(flag)::value;
     Pack<T, V> xr[kBwdLen], gr[kBwdLen];
