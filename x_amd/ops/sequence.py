@@ -59,30 +59,34 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grads_wanted(*ts) -> bool:
-    """Whether a call goes through its autograd function: for a gradient, and wherever a derivative or a recording would
-    take the kernel's output for memory that nothing was computed into.  The function refuses tangents, and
-    torch.jit.trace keeps it as a call."""
-    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts))
-            or (not torch.compiler.is_compiling()
-                and (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)))
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-def _on_kernels(t: torch.Tensor, what: str, function: bool = True) -> bool:
-    """Whether the operator runs on the HIP kernels; raises where the call is being recorded in a way that would not hold
-    it: operation by operation (make_fx, the kernels are none), or by torch.jit.trace without an autograd function.
-    torch.compile leaves the calls outside of its graphs."""
+# Looked up once: every call asks them.
+_compiling, _tracing, _modes = torch.compiler.is_dynamo_compiling, torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
+_key_set, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+
+
+def _route(t: torch.Tensor, what: str, function: bool = True) -> bool | None:
+    """None where the operator runs as torch operations (CPU tensors), else whether the kernels have to be called through
+    the operator's autograd function whether a gradient is wanted or not: at a forward-mode level, where the function
+    refuses tangents, and under torch.jit.trace, which keeps it as a call.  (Past the function either would take the
+    output for memory that nothing was computed into.)  Raises where a recording could not hold the call: operation by
+    operation (make_fx; the kernels are none), or by torch.jit.trace without an autograd function.  torch.compile leaves
+    the calls outside of its graphs."""
     if not ext_supports(t):
+        return None
+    if _compiling():
         return False
-    if torch.compiler.is_compiling():
-        return True
-    C = torch._C
-    if C._len_torch_dispatch_stack() or C._dispatch_tls_is_dispatch_key_included(C.DispatchKey.PreDispatch):
+    if _modes() or _key_set(_PRE_DISPATCH):
         proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
         if proxies is not None and proxies.get_proxy_mode() is not None:
             raise RuntimeError(f"{what} cannot be recorded operation by operation: call it outside of the recorded program")
-    if not function and C._get_tracing_state() is not None:
-        raise RuntimeError(f"{what} cannot be recorded: it has no gradient and no autograd function to keep")
-    return True
+    if _tracing() is not None:
+        if not function:
+            raise RuntimeError(f"{what} cannot be recorded: it has no gradient and no autograd function to keep")
+        return True
+    return forward_ad._current_level >= 0
 
 
 def _ws(nbytes: int, dev, what: str) -> torch.Tensor:
@@ -138,10 +142,11 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dty
     if dtype not in _CODE:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     scale = float(scale)
-    if not _on_kernels(table, "embed_tokens"):
+    through = _route(table, "embed_tokens")
+    if through is None:
         return ref.embed_tokens(ids, table, scale, dtype)
     ids, rows = ids.contiguous(), _rows(table)
-    if _grads_wanted(table):
+    if through or _grads_wanted(table):
         return _Embed.apply(ids, rows, scale, dtype)
     return _embed_fwd(ids, rows, scale, dtype)
 
@@ -233,10 +238,11 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     (seed, offset) give equal masks whatever the launch, the backward draws them again, and no mask is stored."""
     eps, p = _norm_args(x, residual, weight, eps, p)
     seed, offset = int(seed) & _U64, int(offset) & _U64
-    if not _on_kernels(x, "residual_rms_norm"):
+    through = _route(x, "residual_rms_norm")
+    if through is None:
         return ref.residual_rms_norm(x, residual, weight, eps, p, seed, offset)
     w = weight.to(F32).contiguous()
-    if _grads_wanted(x, residual, w):
+    if through or _grads_wanted(x, residual, w):
         y, s = _Norm.apply(x, residual, w, eps, p, seed, offset)
     else:
         y, s, _ = _norm_fwd(_rows(x), None if residual is None else _rows(residual), w, x.shape, eps, p, seed, offset)
@@ -248,7 +254,7 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight
     scale (..., 1) = max(max |y|, 1e-30) / 448, q = 448 y / max |y| rounded to nearest.  For inference (no gradient): q
     and scale are what a row-scaled 8-bit product takes."""
     eps, _ = _norm_args(x, residual, weight, eps)
-    if not _on_kernels(x, "residual_rms_norm_fp8", function=False):
+    if _route(x, "residual_rms_norm_fp8", function=False) is None:
         with torch.no_grad():
             return ref.residual_rms_norm_fp8(x, residual, weight, eps)
     y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.detach().to(F32).contiguous(),
@@ -346,10 +352,11 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: tor
             raise ValueError(f"h0 must be ({B}, {D}), got {tuple(h0.shape)}")
         h0 = h0.to(F32).contiguous()
     start = start.to(I64).contiguous()
-    if not _on_kernels(x, "gated_scan"):
+    through = _route(x, "gated_scan")
+    if through is None:
         return ref.gated_scan(x, gate, start, dt, h0)
     rx, rg = _rows(x), _rows(gate)
-    if _grads_wanted(x, gate, h0):
+    if through or _grads_wanted(x, gate, h0):
         return _Scan.apply(rx, rg, start, dt, h0)
     return _scan_fwd(rx, rg, start, dt, h0, False)[:2]
 
@@ -362,7 +369,7 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
         raise ValueError(f"state must be a contiguous float32 tensor of {tuple(x.shape)} without gradient, got "
                          f"{tuple(state.shape)}, {state.dtype}")
-    if not _on_kernels(x, "gated_scan_step", function=False):
+    if _route(x, "gated_scan_step", function=False) is None:
         with torch.no_grad():
             return ref.gated_scan_step(x, gate, state, dt)
     x, gate = _rows(x), _rows(gate)
@@ -371,6 +378,5 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     with on_device(x.device):
         call("atl_gated_scan_step", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(dt),
              _at(state), _at(y), raw_stream(x.device))
-    if not state.is_inference():
-        torch.autograd.graph.increment_version(state)      # written by address: whoever saved it has to know
+    torch.autograd.graph.increment_version(state)          # written by address: whoever saved it has to know
     return y
