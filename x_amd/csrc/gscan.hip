@@ -188,8 +188,11 @@ struct Ascend {
   }
   __device__ __forceinline__ Ascend(const int64_t* __restrict__ start, int B, int64_t wave_first, const Place& p) {
     b = count_below(start, B, wave_first) - 1;
-    if (p.live) b = last_before(start, B, b, p.i0);
     look(start, p.i0);
+    if (p.live && next < 0 && b + 1 < B) {
+      b = last_before(start, B, b, p.i0);
+      look(start, p.i0);
+    }
   }
   // Whether token i0 + t is the first of a window, which b is then.
   __device__ __forceinline__ bool starts(const int64_t* __restrict__ start, int B, int64_t i0, int t) {
@@ -214,17 +217,24 @@ struct Descend {
   }
   __device__ __forceinline__ Descend(const int64_t* __restrict__ start, int B, int64_t wave_first, const Place& p) {
     const int64_t behind = p.i0 + p.n;
-    b = count_below(start, B, wave_first + 1) - 1;                 // the last window that starts at or before it
-    if (p.live) b = last_before(start, B, b, behind);
-    b = max(b, 0);
+    b = max(count_below(start, B, wave_first + 1) - 1, 0);         // the last window that starts at or before it
+    int64_t end = start[b + 1];
+    if (p.live && end < behind && b + 1 < B) {
+      b = last_before(start, B, b, behind);
+      end = start[b + 1];
+    }
     look(start, p.i0);
-    last = behind == start[b + 1];
+    last = behind == end;
   }
   __device__ __forceinline__ void step(const int64_t* __restrict__ start, int64_t i0, int t) {      // to token i0 + t
     last = false;
     if (t < first && b > 0) {
-      b = last_upto(start, b, i0 + t);
+      --b;
       look(start, i0);
+      if (t < first && b > 0) {                   // windows without tokens
+        b = last_upto(start, b, i0 + t);
+        look(start, i0);
+      }
       last = true;
     }
   }
