@@ -848,3 +848,115 @@ def test_scan_time_does_not_follow_the_empty_windows():
         best = min(best, e0.elapsed_time(e1))
     print(f"{best:.2f} ms", flush=True)
     assert best < 20
+
+
+# ------------------------------------------------------------------------------------------- long windows
+def _recur(a, u):
+    """h_i = a_i h_{i-1} + u_i along the rows in float64, from zero: blocks of about sqrt(N) rows side by side, then
+    through their ends one by one."""
+    N, D = u.shape
+    m = max(1, int(N ** 0.5))
+    n = -(-N // m)
+    pad = torch.zeros(n * m - N, D, dtype=u.dtype, device=u.device)
+    a, u = torch.cat([a, pad]).view(n, m, D), torch.cat([u, pad]).view(n, m, D)
+    h, prod = u.clone(), a.clone()
+    for j in range(1, m):
+        h[:, j] += a[:, j] * h[:, j - 1]
+        prod[:, j] *= prod[:, j - 1]
+    before = torch.zeros_like(h[:, 0])
+    for k in range(1, n):
+        before[k] = h[k - 1, -1] + prod[k - 1, -1] * before[k - 1]
+    return (h + prod * before[:, None]).view(-1, D)[:N]
+
+
+def _states(a, z, u, edges, begin):
+    """States, their magnitudes M (of |u|) and P = sum of |u_j| decay Z, with Z the rates between j and i; at the rows
+    ``edges`` the recurrence begins anew from ``begin``.  A decay counts where the row before hands on."""
+    inner = a.clone()
+    inner[edges] = 0
+
+    def run(add, first):
+        add = add.clone()
+        add[edges] += a[edges] * first
+        return _recur(inner, add)
+
+    h, M = run(u, begin), run(u.abs(), begin.abs())
+    prev = torch.cat([torch.zeros_like(M[:1]), M[:-1]])
+    prev[edges] = begin.abs()
+    return h, M, _recur(inner, a * z * prev)
+
+
+def _long_case(N, D, dtype, with_dt, cuts, seed):
+    """Against float64 on the device, token by token in blocks.  Bounds: a state's way from its tokens holds at most 16
+    steps in a group (4 units of a decay and a sum each), 80 joins of ranges (3 each) and the token's own 8 + |gate|
+    (<= 32): 400 units of the magnitudes M.  A rate is off by 8 + |gate| units, one without gaps comes from a product of 16
+    decays (50), and sums of rates round at most 90 times: 200 units of each Z, hence of P."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+    start = torch.tensor([0, *cuts, N], device=DEV)
+    B = len(start) - 1
+    x, gy = (rand(N, D) + 1).to(dtype), (rand(N, D) + 0.5).to(dtype)
+    g = (rand(N, D) * 1.5 - 1 if with_dt else rand(N, D) - 11).to(dtype)
+    dt = torch.rand(N, device=DEV, generator=gen) * 4e-5 if with_dt else None
+    h0, gl = rand(B, D), rand(B, D) * 100
+    print(f"scan N={N} D={D} {dtype} dt={with_dt} B={B}", flush=True)
+    ins = [t.requires_grad_() for t in (x, g, h0)]
+    y, last = ops.gated_scan(x, g, start, dt=dt, h0=h0)
+    got = torch.autograd.grad((y, last), ins, (gy, gl))
+    with torch.no_grad():
+        y2, last2 = ops.gated_scan(x, g, start, dt=dt, h0=h0)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+
+    gd, xd = g.detach().double(), x.detach().double()
+    step = torch.ones(N, 1, dtype=torch.float64, device=DEV) if dt is None else dt.double()[:, None]
+    z = torch.logaddexp(gd, torch.zeros_like(gd)) * step
+    a, w, wc = torch.exp(-z), torch.sigmoid(gd), torch.sigmoid(-gd)
+    some = start[1:] > start[:-1]
+    head, tail = start[:-1][some], start[1:][some] - 1
+    begin = h0.detach().double()[some]
+    h, M, P = _states(a, z, w * xd, head, begin)
+    E = O.U * (400 * M + 200 * P)
+    _close(y, _np(h), _np(E), "y")
+    _close(last[some], _np(h[tail]), _np(E[tail]), "last")
+    assert torch.equal(last[~some], h0[~some])
+    # C_i = a_i (gy_i + C_{i+1}) from the end, H_i = gy_i + C_{i+1}
+    back = lambda t: t.flip(0)
+    ends = N - 1 - tail
+    C, MC, PC = _states(back(a), back(z), back(a * gy.double()), ends, gl.double()[some])
+    C, EC, MC = back(C), back(O.U * (400 * MC + 200 * PC)), back(MC)
+
+    def behind(t, edge):
+        t = torch.cat([t[1:], torch.zeros_like(t[:1])])
+        t[tail] = edge
+        return t
+
+    H, mH = gy.double() + behind(C, gl.double()[some]), gy.double().abs() + behind(MC, gl.double()[some].abs())
+    eH = behind(EC, 0.0) + O.U * mH
+    before = lambda t, first: torch.cat([torch.zeros_like(t[:1]), t[:-1]]).index_put((head,), first)
+    hp, ep = before(h, begin), before(E, torch.zeros_like(begin))
+    t = xd * wc - step * a * hp
+    mt = xd.abs() * wc + step * a * (hp.abs() + ep)
+    _close(got[0], _np(H * w), _np((eH + 32 * O.U * mH) * w), "gx")
+    _close(got[1], _np(H * w * t), _np(w * (eH * mt + mH * (O.U * (40 + 4 * z) * mt + step * a * ep))), "gg")
+    _close(got[2][some], _np(C[head]), _np(EC[head]), "gh0")
+    assert torch.equal(got[2][~some], gl[~some])
+    return float((last[-1].detach().double() - h[-1]).abs().max() / h[-1].abs().max())
+
+
+@pytest.mark.parametrize("N,D,dtype", [(40_003, 64, F32), (40_003, 64, BF16), (300_001, 64, F32), (300_001, 64, F16),
+                                       (251_117, 65, F32), (300_001, 6, BF16)])
+@pytest.mark.parametrize("with_dt", [False, True])
+@pytest.mark.parametrize("windows", [1, 4])
+def test_scan_of_long_windows(N, D, dtype, with_dt, windows):
+    """States that live over many chunks, blocks of chunks and stretches of blocks, forward and backward, from given states,
+    also over windows that begin inside them and one without tokens."""
+    cuts = [] if windows == 1 else [N // 3, N // 3, N // 2 + 7]
+    _long_case(N, D, dtype, with_dt, cuts, seed=N + D)
+
+
+def test_scan_of_a_million_tokens():
+    """The last state after 1M tokens with decays next to one: as near as its ranges' joins allow, not as a product of a
+    million factors would be (4e-4)."""
+    off = _long_case(1_000_000, 8, F32, True, [], seed=9)
+    print(f"last state off by {off:.2g} of its size", flush=True)
+    assert off < 5e-6
