@@ -19,7 +19,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import reference as ref
-from ._ext import F32, I64, call, ext_supports, load_library, on_device, raw_stream
+from ._ext import F32, I64, call, load_library, on_device, raw_stream
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_NORM_WIDTH = 8192
@@ -33,7 +33,7 @@ def _at(t: torch.Tensor | None) -> int:
 
 
 def _float_type(t, name: str) -> int:
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     code = _CODE.get(t.dtype)
     if code is None:
@@ -42,10 +42,15 @@ def _float_type(t, name: str) -> int:
 
 
 def _on(t, name: str, dev):
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.device != dev:
         raise ValueError(f"{name} must be on {dev}, got {t.device}")
+
+
+def _plain(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``t`` contiguous in ``dtype``: itself where it is (told in less time than two conversions to nothing)."""
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -53,7 +58,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     apart), else a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] < 2 and t.stride(0) > MAX_ROW_STRIDE:
+    if t.stride(0) > MAX_ROW_STRIDE and t.shape[0] < 2:
         t = t.reshape(-1).view(t.shape)                # a single row's stride says nothing
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) <= MAX_ROW_STRIDE else t.contiguous()
 
@@ -74,7 +79,7 @@ def _route(t: torch.Tensor, what: str, function: bool = True) -> bool | None:
     output for memory that nothing was computed into.)  Raises where a recording could not hold the call: operation by
     operation (make_fx; the kernels are none), or by torch.jit.trace without an autograd function.  torch.compile leaves
     the calls outside of its graphs."""
-    if not ext_supports(t):
+    if not t.is_cuda:
         return None
     if _compiling():
         return False
@@ -97,11 +102,11 @@ def _ws(nbytes: int, dev, what: str) -> torch.Tensor:
 
 # ------------------------------------------------------------------------------------------- embedding
 def _embed_fwd(ids, table, scale, dtype):
-    N, (V, D) = ids.numel(), table.shape
-    out = torch.empty(*ids.shape, D, dtype=dtype, device=table.device)
-    with on_device(table.device):
+    N, (V, D), dev = ids.numel(), table.shape, table.device
+    out = torch.empty(*ids.shape, D, dtype=dtype, device=dev)
+    with on_device(dev):
         call("atl_embed_fwd", _at(ids), int(ids.dtype == I64), N, _at(table), table.stride(0), _CODE[table.dtype], V, D,
-             scale, _at(out), _CODE[dtype], raw_stream(table.device))
+             scale, _at(out), _CODE[dtype], raw_stream(dev))
     return out
 
 
@@ -161,7 +166,7 @@ def _norm_fwd(x, res, w, shape, eps, p, seed, offset, fp8=False):
     scale = torch.empty(*shape[:-1], 1, dtype=F32, device=dev) if fp8 else None
     with on_device(dev):
         call("atl_rms_norm_fwd", _at(x), x.stride(0), _CODE[x.dtype], _at(res), 0 if res is None else res.stride(0),
-             _CODE[rtype], _at(w), N, D, eps, p, seed, offset, _at(y), _at(s), _at(scale), raw_stream(x.device))
+             _CODE[rtype], _at(w), N, D, eps, p, seed, offset, _at(y), _at(s), _at(scale), raw_stream(dev))
     return y, s, scale
 
 
@@ -241,7 +246,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     through = _route(x, "residual_rms_norm")
     if through is None:
         return ref.residual_rms_norm(x, residual, weight, eps, p, seed, offset)
-    w = weight.to(F32).contiguous()
+    w = _plain(weight, F32)
     if through or _grads_wanted(x, residual, w):
         y, s = _Norm.apply(x, residual, w, eps, p, seed, offset)
     else:
@@ -257,7 +262,7 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight
     if _route(x, "residual_rms_norm_fp8", function=False) is None:
         with torch.no_grad():
             return ref.residual_rms_norm_fp8(x, residual, weight, eps)
-    y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), weight.detach().to(F32).contiguous(),
+    y, s, scale = _norm_fwd(_rows(x), None if residual is None else _rows(residual), _plain(weight.detach(), F32),
                             x.shape, eps, 0.0, 0, 0, fp8=True)
     return y, scale, x.detach() if s is None else s
 
@@ -310,19 +315,20 @@ class _Scan(torch.autograd.Function):
 
 def _scan_args(x, gate, dt):
     _float_type(x, "x")
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"x must be (N, D), got {tuple(x.shape)}")
-    _on(gate, "gate", x.device)
-    if gate.dtype != x.dtype or gate.shape != x.shape:
-        raise ValueError(f"gate must be like x ({tuple(x.shape)}, {x.dtype}), got {tuple(gate.shape)}, {gate.dtype}")
+    dev, shape = x.device, x.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"x must be (N, D), got {tuple(shape)}")
+    _on(gate, "gate", dev)
+    if gate.dtype != x.dtype or gate.shape != shape:
+        raise ValueError(f"gate must be like x ({tuple(shape)}, {x.dtype}), got {tuple(gate.shape)}, {gate.dtype}")
     if dt is None:
         return None
-    _on(dt, "dt", x.device)
-    if dt.shape != (x.shape[0],):
-        raise ValueError(f"dt must be ({x.shape[0]},), got {tuple(dt.shape)}")
+    _on(dt, "dt", dev)
+    if dt.shape != shape[:1]:
+        raise ValueError(f"dt must be ({shape[0]},), got {tuple(dt.shape)}")
     if dt.requires_grad:
         raise ValueError("no gradient flows to dt: detach it")
-    return dt.to(F32).contiguous()
+    return _plain(dt, F32)
 
 
 def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: torch.Tensor | None = None,
@@ -350,8 +356,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, start: torch.Tensor, dt: tor
         _on(h0, "h0", x.device)
         if h0.shape != (B, D):
             raise ValueError(f"h0 must be ({B}, {D}), got {tuple(h0.shape)}")
-        h0 = h0.to(F32).contiguous()
-    start = start.to(I64).contiguous()
+        h0 = _plain(h0, F32)
+    start = _plain(start, I64)
     through = _route(x, "gated_scan")
     if through is None:
         return ref.gated_scan(x, gate, start, dt, h0)
@@ -365,18 +371,19 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, dt
     """One token of each of N streams: ``state`` (N, D) float32 becomes exp(-dt softplus(gate)) state + sigmoid(gate) x in
     place; returns it in x's type.  For inference (no gradient): a backward that needs the state as it was raises."""
     dt = _scan_args(x, gate, dt)
-    _on(state, "state", x.device)
-    if state.dtype != F32 or state.shape != x.shape or not state.is_contiguous() or state.requires_grad:
-        raise ValueError(f"state must be a contiguous float32 tensor of {tuple(x.shape)} without gradient, got "
+    dev, shape = x.device, x.shape
+    _on(state, "state", dev)
+    if state.dtype != F32 or state.shape != shape or not state.is_contiguous() or state.requires_grad:
+        raise ValueError(f"state must be a contiguous float32 tensor of {tuple(shape)} without gradient, got "
                          f"{tuple(state.shape)}, {state.dtype}")
     if _route(x, "gated_scan_step", function=False) is None:
         with torch.no_grad():
             return ref.gated_scan_step(x, gate, state, dt)
     x, gate = _rows(x), _rows(gate)
-    N, D = x.shape
-    y = torch.empty(N, D, dtype=x.dtype, device=x.device)
-    with on_device(x.device):
+    N, D = shape
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    with on_device(dev):
         call("atl_gated_scan_step", _at(x), x.stride(0), _at(gate), gate.stride(0), _CODE[x.dtype], N, D, _at(dt),
-             _at(state), _at(y), raw_stream(x.device))
+             _at(state), _at(y), raw_stream(dev))
     torch.autograd.graph.increment_version(state)          # written by address: whoever saved it has to know
     return y
