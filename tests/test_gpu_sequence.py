@@ -960,3 +960,19 @@ def test_scan_of_a_million_tokens():
     off = _long_case(1_000_000, 8, F32, True, [], seed=9)
     print(f"last state off by {off:.2g} of its size", flush=True)
     assert off < 5e-6
+
+
+@pytest.mark.parametrize("which", ["embed", "norm", "scan", "gate", "h0", "fp8", "step"])
+def test_transforms_raise(which):
+    """torch.func's transforms and batched gradients are refused, whatever the operator has of a gradient."""
+    t, calls = _calls()
+    fn = calls[which]
+    for call in (lambda: torch.func.vmap(fn)(torch.stack([t, t])), lambda: torch.func.grad(lambda a: fn(a).sum())(t),
+                 lambda: torch.func.jvp(fn, (t,), (t,)), lambda: torch.func.functionalize(fn)(t)):
+        with pytest.raises(RuntimeError):
+            call()
+    if which not in ("fp8", "step"):
+        x = t.clone().requires_grad_()
+        y = fn(x)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, x, torch.stack([torch.ones_like(y)] * 2), is_grads_batched=True)
