@@ -516,7 +516,8 @@ int atl_rms_norm_fwd(const void* x, int64_t sx, int dtype, const void* res, int6
                      int64_t N, int64_t D, double eps, double p, uint64_t seed, uint64_t offset, void* y, void* s,
                      float* scale, hipStream_t stream);
 /* Its backward from s (row stride ss), gy (dtype; may be null) and gs (rtype; may be null): gx (N,D) dtype, gres (N,D)
- * rtype and gw (D) written, each unless null.  ws (for gw): atl_rms_norm_bwd_ws_bytes bytes (-1: sizes unsupported). */
+ * rtype and gw (D) written, each unless null; without gy they are gs, gs through the dropout, and zeros, whatever the
+ * rows' norms.  ws (for gw): atl_rms_norm_bwd_ws_bytes bytes (-1: sizes unsupported). */
 int64_t atl_rms_norm_bwd_ws_bytes(int64_t N, int64_t D);
 int atl_rms_norm_bwd(const void* s, int64_t ss, int rtype, const float* w, const void* gy, int64_t sgy, int dtype,
                      const void* gs, int64_t sgs, int64_t N, int64_t D, double eps, double p, uint64_t seed,

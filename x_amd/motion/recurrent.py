@@ -135,7 +135,8 @@ class EventRecurrence(nn.Module):
     @torch.no_grad()
     def step(self, xy: torch.Tensor, p: torch.Tensor, dt: torch.Tensor, states: list, fp8=None) -> list:
         """One event of each of n streams (xy (n, 2), p (n,), dt (n,) gaps in units of tau): the layers' states, updated
-        in place.  ``fp8`` (:meth:`fp8_weights`): the input projections in 8 bits (on the GPU)."""
+        in place.  ``fp8`` (:meth:`fp8_weights`): the input projections in 8 bits (on the GPU), for half the bytes of weights:
+        up to widths of 1024 and 4096 streams the step is bound by the host, 305-310 us in 16 bits and 314-339 in 8."""
         s = embed_tokens(self.tokens(xy, p), self.table, scale=math.sqrt(self.dim), dtype=self.dtype)
         x = None
         for k, (w, into) in enumerate(zip(self.norm, self.into)):
