@@ -544,6 +544,50 @@ int atl_gated_scan_bwd(const void* x, int64_t sx, const void* gate, int64_t sg, 
 int atl_gated_scan_step(const void* x, int64_t sx, const void* gate, int64_t sg, int dtype, int64_t N, int64_t D,
                         const float* dt, float* state, void* y, hipStream_t stream);
 
+/* ---------------------------------------------------------------- attention with a state of fixed size (no counterpart in
+ * the reference's extension).  Queries, keys and values are (N, H, D) with contiguous heads of D channels, token and head
+ * strides (s*n, s*h) in elements (a head stride of 0 shares one head); outputs are contiguous. */
+
+/* x / sqrt(mean_D(x^2) + eps) * w of every head of q (N,H,D) and k (N,Hk,D) (wq, wk (D) single precision; null: no norm),
+ * then channel pairs (2p, 2p+1) turned by pos[n, a] * freqs[p], a the axis of p: sections (A, host memory) holds the pairs
+ * of each axis, in order; channels past them are not turned.  pos (N,A) in double precision if pos64, else single.  yq
+ * (N,H,D), yk (N,Hk,D) written.  D <= 256, A <= 4. */
+int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
+                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, void* yq,
+                             void* yk, hipStream_t stream);
+/* Its backward from gyq, gyk (either may be null: zeros): gq, gk and gw (2,D: the weights' gradients, queries' first)
+ * written, each unless null.  q, k may be null without norms.  ws (for gw): atl_head_norm_rotary_bwd_ws_bytes bytes (-1:
+ * width unsupported). */
+int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t D);
+int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
+                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, const void* gyq,
+                             int64_t sgqn, int64_t sgqh, const void* gyk, int64_t sgkn, int64_t sgkh, void* gq, void* gk,
+                             float* gw, void* ws, int64_t ws_bytes, hipStream_t stream);
+
+/* S_i = exp(-rate dt_i) S_{i-1} + k_i v_i^T, y_i = scale q_i S_i per head (dt null: ones; rate (H)) within each window of
+ * tokens [start[b], start[b+1]) (start (B+1) ascends within [0, N]; empty windows allowed; tokens outside are in no window:
+ * zeros), from h0 (B,H,D,D) or zero.  y (N,H,D) and last (B,H,D,D) = every window's last state (an empty window's: h0 or
+ * zero) written.  states: atl_decay_attn_states floats (null where that is 0), kept for the backward.  ws:
+ * atl_decay_attn_ws_bytes bytes (-1: sizes unsupported).  D <= 128. */
+int64_t atl_decay_attn_states(int64_t N, int64_t H, int64_t D);
+int64_t atl_decay_attn_ws_bytes(int64_t N, int64_t H, int64_t D, int backward);
+int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
+                       int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate,
+                       const int64_t* start, int64_t B, const float* dt, const float* h0, double scale, void* y, float* last,
+                       float* states, void* ws, int64_t ws_bytes, hipStream_t stream);
+/* Its backward from gy and glast (may be null): gq, gk, gv (N,H,D) and gh0 (B,H,D,D; may be null) written. */
+int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
+                       int64_t svn, int64_t svh, const void* gy, int64_t sgn, int64_t sgh, int dtype, int64_t N, int64_t H,
+                       int64_t D, const float* rate, const int64_t* start, int64_t B, const float* dt, const float* h0,
+                       const float* glast, double scale, const float* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
+                       int64_t ws_bytes, hipStream_t stream);
+/* One token of each of N streams: state (N,H,D,D) updated in place, y (N,H,D) = scale q state. */
+int atl_decay_attn_step(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
+                        int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate, const float* dt,
+                        double scale, float* state, void* y, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

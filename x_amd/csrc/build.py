@@ -14,7 +14,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parents[1]
-SOURCES = ["abi.hip", "events.hip", "tiles.hip", "pairs.hip", "fastpair.hip", "knn.hip", "embed.hip", "rmsnorm.hip", "gscan.hip"]
+SOURCES = ["abi.hip", "events.hip", "tiles.hip", "pairs.hip", "fastpair.hip", "knn.hip", "embed.hip", "rmsnorm.hip", "gscan.hip", "headrot.hip", "decay.hip"]
 OUT = HERE / "libatl_hip.so"
 ARCH = os.environ.get("ATL_HIP_ARCH", "gfx950")
 

@@ -1,0 +1,306 @@
+// Root-mean-square norm of every head's queries and keys, and the rotation of their channel pairs by the token's position,
+// in one pass:
+//
+//   xh = x r w,  r = 1 / sqrt(mean(x^2) + eps)      (no norm: xh = x)
+//   (y_2p, y_2p+1) = (xh_2p cos t - xh_2p+1 sin t, xh_2p sin t + xh_2p+1 cos t),  t = pos[axis(p)] freq_p,  p < pairs
+//
+// the channels past the pairs unturned.  Backward, with g = the output's gradient turned back by t:
+//
+//   gw = sum over tokens and heads of g x r,   gx = r (w g - x r mean(w g x r)).
+//
+// Angles are taken in turns in 64 bits and reduced to half a turn before they become single precision: a position of a
+// million with a frequency near one keeps its angle.  They are those of all the token's heads, so a group of lanes that
+// holds a row (16 bytes a lane) goes through several heads with them.  Bound by memory: a read and a write of the rows
+// forward, two reads and a write backward.
+#include "shares.h"
+#include "typed.h"
+#include "../../include/atl_hip.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace atlhip {
+namespace {
+
+constexpr int kMaxHeadWidth = 256, kMaxAxes = 4;
+
+struct HeadRows {
+  const void* p;
+  int64_t sn, sh;                     // token and head strides in elements
+};
+
+struct RotGeo {
+  int64_t N;
+  int H, Hk, D, A, pairs;             // heads of the queries and keys, channels, axes, turned pairs
+  int bound[kMaxAxes];                // first pair behind each axis
+  const void* pos;                    // (N, A)
+  int pos64;                          // in double precision
+  const float* freq;
+  float eps, inv_d;
+  int cl2, per, blocks_of;            // log2 of a row's lanes, heads of an item, items of a token
+};
+
+// Cosine and sine of the lane's pairs from column c on.
+template <int V>
+__device__ __forceinline__ void angles(const RotGeo& g, int64_t n, int c, float (&co)[V / 2], float (&si)[V / 2]) {
+#pragma unroll
+  for (int m = 0; m < V / 2; ++m) {
+    const int p = c / 2 + m;
+    co[m] = 1.f, si[m] = 0.f;
+    if (p >= g.pairs) continue;
+    int a = 0;
+#pragma unroll
+    for (int k = 0; k < kMaxAxes - 1; ++k) a += k < g.A - 1 && p >= g.bound[k];
+    const int64_t at = n * g.A + a;
+    const double x = g.pos64 ? ((const double*)g.pos)[at] : (double)((const float*)g.pos)[at];
+    const double turns = x * ((double)g.freq[p] * 0.15915494309189535);
+    sincospif(2.f * (float)(turns - rint(turns)), &si[m], &co[m]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void turn(float (&v)[V], const float (&co)[V / 2], const float (&si)[V / 2], float sign) {
+#pragma unroll
+  for (int m = 0; m < V / 2; ++m) {
+    const float a = v[2 * m], b = v[2 * m + 1], s = sign * si[m];
+    v[2 * m] = fmaf(a, co[m], -b * s);
+    v[2 * m + 1] = fmaf(a, s, b * co[m]);
+  }
+}
+
+// Sum over a row's lanes, returned to each.
+__device__ __forceinline__ float lanes_sum(float v, int cl2) {
+  for (int d = 1 << cl2 >> 1; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
+  return v;
+}
+
+// A piece of a row of D channels, from column c < D on; zeros past it.
+template <bool WHOLE, int V, typename T>
+__device__ __forceinline__ void load_part(const T* row, int c, int D, float (&v)[V]) {
+  if constexpr (WHOLE) load_f<V>(row + c, v);
+  else load_loose<V>(row + c, D - c, v);
+}
+template <bool WHOLE, int V, typename T>
+__device__ __forceinline__ void store_part(T* row, int c, int D, const float (&v)[V]) {
+  if constexpr (WHOLE) store_f<V>(row + c, v);
+  else store_loose<V>(row + c, D - c, v);
+}
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kBlock) k_headrot_fwd(RotGeo g, HeadRows q, HeadRows k, const float* __restrict__ wq,
+                                                        const float* __restrict__ wk, T* __restrict__ yq, T* __restrict__ yk,
+                                                        int64_t first) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & ((1 << g.cl2) - 1), c = lane * V;
+  const int64_t item = (first + blockIdx.x) * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
+  const int64_t n = item / g.blocks_of;
+  if (n >= g.N) return;                                   // a whole row's lanes
+  const int h0 = (int)(item - n * g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
+  const bool in = c < g.D;
+  float co[V / 2], si[V / 2];
+  angles<V>(g, n, c, co, si);
+  for (int h = h0; h < h1; ++h) {
+    const bool key = h >= g.H;
+    const HeadRows& r = key ? k : q;
+    const int head = key ? h - g.H : h;
+    const float* w = key ? wk : wq;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.f;
+    if (in) load_part<WHOLE, V>((const T*)r.p + n * r.sn + head * r.sh, c, g.D, v);
+    if (w) {
+      float ss = 0.f, wv[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss), wv[e] = 0.f;
+      if (in) load_part<WHOLE, V>(w, c, g.D, wv);
+      const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = v[e] * inv * wv[e];
+    }
+    turn<V>(v, co, si, 1.f);
+    if (in) store_part<WHOLE, V>((key ? yk + (n * g.Hk + head) * g.D : yq + (n * g.H + head) * g.D), c, g.D, v);
+  }
+}
+
+// part (gridDim.x, 2, D): the workgroup's share of the weights' gradients, its rows added in a fixed order.  A null gradient
+// stands for zeros.
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, HeadRows k, const float* __restrict__ wq,
+                                                        const float* __restrict__ wk, HeadRows gq, HeadRows gk,
+                                                        T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ part) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float lds[kBlock * V];
+  const int lanes = 1 << g.cl2, lane = threadIdx.x & (lanes - 1), c = lane * V, group = threadIdx.x >> g.cl2;
+  const bool in = c < g.D;
+  float wv[2][V], gw[2][V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) wv[0][e] = wv[1][e] = gw[0][e] = gw[1][e] = 0.f;
+  if (in && wq) load_part<WHOLE, V>(wq, c, g.D, wv[0]);
+  if (in && wk) load_part<WHOLE, V>(wk, c, g.D, wv[1]);
+  const int64_t items = g.N * g.blocks_of, step = (int64_t)gridDim.x * (kBlock >> g.cl2);
+  for (int64_t item = (int64_t)blockIdx.x * (kBlock >> g.cl2) + group; item < items; item += step) {
+    const int64_t n = item / g.blocks_of;
+    const int h0 = (int)(item - n * g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
+    float co[V / 2], si[V / 2];
+    angles<V>(g, n, c, co, si);
+    auto row = [&](int h, auto which) {
+      constexpr int K = decltype(which)::value;
+      const HeadRows &r = K ? k : q, &gr = K ? gk : gq;
+      const int head = K ? h - g.H : h;
+      const float* w = K ? wk : wq;
+      T* out = K ? dk : dq;
+      float y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = 0.f;
+      if (in && gr.p) load_part<WHOLE, V>((const T*)gr.p + n * gr.sn + head * gr.sh, c, g.D, y);
+      if (w) {
+        float x[V], ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = 0.f;
+        if (in) load_part<WHOLE, V>((const T*)r.p + n * r.sn + head * r.sh, c, g.D, x);
+        turn<V>(y, co, si, -1.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          ss = fmaf(x[e], x[e], ss);
+          dot = fmaf(wv[K][e] * y[e], x[e], dot);
+        }
+        const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
+        const float mean = lanes_sum(dot, g.cl2) * inv * g.inv_d;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float hat = x[e] * inv;
+          gw[K][e] = fmaf(y[e], hat, gw[K][e]);
+          y[e] = inv * fmaf(wv[K][e], y[e], -hat * mean);
+        }
+      } else {
+        turn<V>(y, co, si, -1.f);
+      }
+      if (in && out) store_part<WHOLE, V>(out + (n * (K ? g.Hk : g.H) + head) * g.D, c, g.D, y);
+    };
+    for (int h = h0; h < min(h1, g.H); ++h) row(h, std::integral_constant<int, 0>{});
+    for (int h = max(h0, g.H); h < h1; ++h) row(h, std::integral_constant<int, 1>{});
+  }
+  if (!part) return;
+#pragma unroll
+  for (int K = 0; K < 2; ++K) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) lds[group * lanes * V + c + e] = gw[K][e];
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < g.D; ch += kBlock) {
+      float sum = 0.f;
+      for (int r = 0; r < kBlock >> g.cl2; ++r) sum += lds[r * lanes * V + ch];
+      part[((int64_t)blockIdx.x * 2 + K) * g.D + ch] = sum;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------- host
+constexpr int64_t kRotBlocks = 2048;
+
+bool rot_ok(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t A, const int64_t* sections, double eps) {
+  if (!dtype_ok(dtype) || N < 0 || N >= ((int64_t)1 << 40) || H < 1 || Hk < 1 || H > 65536 || Hk > 65536 || D < 1 ||
+      D > kMaxHeadWidth || A < 1 || A > kMaxAxes || !sections || !(eps >= 0 && eps < 1e30))
+    return false;
+  int64_t pairs = 0;
+  for (int64_t a = 0; a < A; ++a) {
+    if (sections[a] < 0 || sections[a] > D) return false;
+    pairs += sections[a];
+  }
+  return 2 * pairs <= D;
+}
+
+RotGeo rot_geo(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, const void* pos, int pos64, const float* freq, int64_t A,
+               const int64_t* sections, double eps) {
+  RotGeo g{};
+  g.N = N; g.H = (int)H; g.Hk = (int)Hk; g.D = (int)D; g.A = (int)A;
+  g.pos = pos; g.pos64 = pos64; g.freq = freq;
+  g.eps = (float)eps;
+  g.inv_d = 1.f / (float)D;
+  for (int a = 0; a < (int)A; ++a) g.bound[a] = g.pairs += (int)sections[a];
+  const int64_t units = (D * dtype_size(dtype) + 15) / 16;
+  while ((1 << g.cl2) < units) ++g.cl2;
+  // Heads that share a token's angles: all up to eight, fewer where that leaves the card without work.
+  g.per = (int)std::min<int64_t>(H + Hk, 8);
+  while (g.per > 1 && N * ((H + Hk + g.per - 1) / g.per) << g.cl2 < 256 * 1024) g.per = (g.per + 1) / 2;
+  g.blocks_of = (int)((H + Hk + g.per - 1) / g.per);
+  return g;
+}
+
+bool rot_whole(int dtype, int64_t D, int64_t strides, std::initializer_list<const void*> ptrs) {
+  const int v = 16 / dtype_size(dtype);
+  if (D % v || strides % v) return false;
+  for (const void* p : ptrs)
+    if (!aligned_to(p, 16)) return false;
+  return true;
+}
+
+template <typename F>
+void by_type(int dtype, F&& f) {
+  if (dtype == kF32) f(float{});
+  else if (dtype == kBF16) f(bf16_t{});
+  else f(f16_t{});
+}
+
+}  // namespace
+}  // namespace atlhip
+
+using namespace atlhip;
+
+extern "C" {
+
+int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
+                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, void* yq,
+                             void* yk, hipStream_t stream) {
+  if (!rot_ok(dtype, N, H, Hk, D, A, sections, eps) || (N > 0 && (sqn < 0 || sqh < 0 || skn < 0 || skh < 0))) { set_error("head_norm_rotary_fwd: bad sizes or settings N=%lld H=%lld, %lld D=%lld axes=%lld type %d eps=%g", (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)A, dtype, eps); return 1; }
+  if (N == 0) return 0;
+  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, pos64, freqs, A, sections, eps);
+  if (!q || !k || !yq || !yk || (g.pairs && (!pos || !freqs))) { set_error("head_norm_rotary_fwd: null argument"); return 1; }
+  const bool whole = rot_whole(dtype, D, sqn | sqh | skn | skh, {q, k, wq, wk, yq, yk});
+  const HeadRows rq{q, sqn, sqh}, rk{k, skn, skh};
+  const int64_t blocks = (N * g.blocks_of + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2);
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    in_launches(blocks, [&](int64_t first, unsigned count) {
+      if (whole)
+        hipLaunchKernelGGL((k_headrot_fwd<T, true>), dim3(count), dim3(kBlock), 0, stream, g, rq, rk, wq, wk, (T*)yq, (T*)yk, first);
+      else
+        hipLaunchKernelGGL((k_headrot_fwd<T, false>), dim3(count), dim3(kBlock), 0, stream, g, rq, rk, wq, wk, (T*)yq, (T*)yk, first);
+    });
+  });
+  return check_launch("head_norm_rotary_fwd");
+}
+
+int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t D) { return D < 1 || D > kMaxHeadWidth ? -1 : kRotBlocks * 2 * D * 4; }
+
+int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
+                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, const void* gyq,
+                             int64_t sgqn, int64_t sgqh, const void* gyk, int64_t sgkn, int64_t sgkh, void* gq, void* gk,
+                             float* gw, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  if (!rot_ok(dtype, N, H, Hk, D, A, sections, eps) || (N > 0 && (sqn < 0 || sqh < 0 || skn < 0 || skh < 0 || sgqn < 0 || sgqh < 0 || sgkn < 0 || sgkh < 0))) { set_error("head_norm_rotary_bwd: bad sizes or settings N=%lld H=%lld, %lld D=%lld axes=%lld type %d eps=%g", (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)A, dtype, eps); return 1; }
+  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, pos64, freqs, A, sections, eps);
+  if ((N > 0 && ((wq && !q) || (wk && !k) || (g.pairs && (!pos || !freqs)))) || (gw && !ws)) { set_error("head_norm_rotary_bwd: null argument"); return 1; }
+  if (gw && ws_bytes < atl_head_norm_rotary_bwd_ws_bytes(D)) { set_error("head_norm_rotary_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_head_norm_rotary_bwd_ws_bytes(D)); return 1; }
+  const bool whole = rot_whole(dtype, D, (wq ? sqn | sqh : 0) | (wk ? skn | skh : 0) | (gyq ? sgqn | sgqh : 0) | (gyk ? sgkn | sgkh : 0),
+                               {wq ? q : nullptr, wk ? k : nullptr, wq, wk, gyq, gyk, gq, gk});
+  const HeadRows rq{q, sqn, sqh}, rk{k, skn, skh}, rgq{gyq, sgqn, sgqh}, rgk{gyk, sgkn, sgkh};
+  const int nblk = (int)std::min<int64_t>((N * g.blocks_of + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2), kRotBlocks);
+  if (nblk > 0)
+    by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      if (whole)
+        hipLaunchKernelGGL((k_headrot_bwd<T, true>), dim3(nblk), dim3(kBlock), 0, stream, g, rq, rk, wq, wk, rgq, rgk, (T*)gq,
+                           (T*)gk, gw ? (float*)ws : nullptr);
+      else
+        hipLaunchKernelGGL((k_headrot_bwd<T, false>), dim3(nblk), dim3(kBlock), 0, stream, g, rq, rk, wq, wk, rgq, rgk, (T*)gq,
+                           (T*)gk, gw ? (float*)ws : nullptr);
+    });
+  if (gw)
+    hipLaunchKernelGGL(k_sum_shares, dim3(grid_for(2 * D, kSumChannels)), dim3(kSumChannels * kSumRuns), 0, stream, (const float*)ws,
+                       nblk, 2 * D, gw);
+  return check_launch("head_norm_rotary_bwd");
+}
+
+}  // extern "C"

@@ -13,6 +13,7 @@
 // A row lies in the registers of a power of two of lanes (a wave at most, or a workgroup for the widest), which read
 // 16 bytes each, aligned to them where widths, strides and addresses are: one pass over memory.  Sums are fp32.
 #include "philox.h"
+#include "shares.h"
 #include "typed.h"
 #include "../../include/atl_hip.h"
 
@@ -269,26 +270,6 @@ __global__ void __launch_bounds__(kBlock) k_norm_bwd_sum(NormGeo n, const R* __r
     }
 }
 
-// gw[c] = sum over the workgroups' shares: 16 channels a workgroup, 64 interleaved runs of the shares side by side.
-constexpr int kSumChannels = 16, kSumRuns = 64;
-__global__ void __launch_bounds__(kSumChannels* kSumRuns) k_norm_gw(const float* __restrict__ part, int nblk, int64_t D,
-                                                                    float* __restrict__ gw) {
-  __shared__ float lds[kSumRuns][kSumChannels];
-  const int ch = threadIdx.x % kSumChannels, run = threadIdx.x / kSumChannels;
-  const int64_t c = (int64_t)blockIdx.x * kSumChannels + ch;
-  float sum = 0.f;
-  if (c < D)
-#pragma unroll 4
-    for (int b = run; b < nblk; b += kSumRuns) sum += part[b * D + c];
-  lds[run][ch] = sum;
-  __syncthreads();
-  for (int half = kSumRuns / 2; half >= 1; half /= 2) {
-    if (run < half) lds[run][ch] += lds[run + half][ch];
-    __syncthreads();
-  }
-  if (run == 0 && c < D) gw[c] = lds[0][ch];
-}
-
 // ------------------------------------------------------------------------------------------- host
 struct NormPlan {
   int V, NV, cl2;
@@ -443,7 +424,7 @@ int atl_rms_norm_bwd(const void* s, int64_t ss, int rtype, const float* w, const
       });
     });
   if (gw)
-    hipLaunchKernelGGL(k_norm_gw, dim3(grid_for(D, kSumChannels)), dim3(kSumChannels * kSumRuns), 0, stream, (const float*)ws, nblk,
+    hipLaunchKernelGGL(k_sum_shares, dim3(grid_for(D, kSumChannels)), dim3(kSumChannels * kSumRuns), 0, stream, (const float*)ws, nblk,
                        D, gw);
   return check_launch("rms_norm_bwd");
 }

@@ -218,3 +218,46 @@ def gated_scan_step(x, gate, state, dt):
     rate = torch.logaddexp(g, torch.zeros_like(g))
     state.copy_(torch.exp(-rate if dt is None else -rate * dt[:, None]) * state + torch.sigmoid(g) * v)
     return state.to(x.dtype)
+
+
+def head_norm_rotary(q, k, q_weight, k_weight, pos, freqs, sections, eps):
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections)).to(pos.device)
+    angle = (pos.double()[:, axis] * freqs.double())[:, None]
+
+    def one(x, w):
+        f = _wide(x)
+        if w is not None:
+            f = f * torch.rsqrt(f.square().mean(-1, keepdim=True) + eps) * _wide(w)
+        cos, sin, turned = torch.cos(angle).to(f.dtype), torch.sin(angle).to(f.dtype), 2 * angle.shape[-1]
+        a, b = f[..., 0:turned:2], f[..., 1:turned:2]
+        pairs = torch.stack([a * cos - b * sin, a * sin + b * cos], -1).flatten(-2)
+        return torch.cat([pairs, f[..., turned:]], -1).to(x.dtype)
+
+    return one(q, q_weight), one(k, k_weight)
+
+
+def decay_attention(q, k, v, rate, start, dt, h0, scale):
+    """Token by token from the definition, the windows side by side: step n takes the n-th token of every window."""
+    a, b, c = _wide(q), _wide(k), _wide(v)
+    N, H, D = q.shape
+    z = rate if dt is None else rate * dt[:, None]
+    decay = torch.exp(-z).to(a.dtype).expand(N, H)[..., None, None]
+    sizes = (start[1:] - start[:-1]).clamp(min=0)
+    S = a.new_zeros(sizes.shape[0], H, D, D) if h0 is None else _wide(h0)
+    parts, where = [], []
+    for n in range(int(sizes.max()) if sizes.numel() else 0):
+        on = sizes > n
+        at = (start[:-1] + n)[on]
+        new = decay[at] * S[on] + b[at][..., :, None] * c[at][..., None, :]
+        S = S.index_put((on.nonzero()[:, 0],), new)
+        parts.append((a[at][..., None, :] @ new)[..., 0, :] * scale)
+        where.append(at)
+    y = torch.zeros_like(a).index_put((torch.cat(where),), torch.cat(parts)) if parts else torch.zeros_like(a)
+    return y.to(q.dtype), S
+
+
+def decay_attention_step(q, k, v, rate, state, dt, scale):
+    z = rate if dt is None else rate * dt[:, None]
+    a, b, c = _wide(q), _wide(k), _wide(v)
+    state.copy_(torch.exp(-z).expand(q.shape[:2])[..., None, None] * state + b[..., :, None] * c[..., None, :])
+    return ((a[..., None, :] @ state.to(a.dtype))[..., 0, :] * scale).to(q.dtype)
