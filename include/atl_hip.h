@@ -570,9 +570,10 @@ int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void
  * tokens [start[b], start[b+1]) (start (B+1) ascends within [0, N]; empty windows allowed; tokens outside are in no window:
  * zeros), from h0 (B,H,D,D) or zero.  y (N,H,D) and last (B,H,D,D) = every window's last state (an empty window's: h0 or
  * zero) written.  states: atl_decay_attn_states floats (null where that is 0), kept for the backward.  ws:
- * atl_decay_attn_ws_bytes bytes (-1: sizes unsupported).  D <= 128. */
-int64_t atl_decay_attn_states(int64_t N, int64_t H, int64_t D);
-int64_t atl_decay_attn_ws_bytes(int64_t N, int64_t H, int64_t D, int backward);
+ * atl_decay_attn_ws_bytes bytes (-1: sizes unsupported).  D <= 128, H D < 2^22; token strides (of two tokens or more) from
+ * D to below 2^22. */
+int64_t atl_decay_attn_states(int64_t N, int64_t B, int64_t H, int64_t D);
+int64_t atl_decay_attn_ws_bytes(int64_t N, int64_t B, int64_t H, int64_t D, int backward);
 int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate,
                        const int64_t* start, int64_t B, const float* dt, const float* h0, double scale, void* y, float* last,

@@ -217,10 +217,10 @@ def test_entries_reject_before_launch():
                                                                   8, 1e-6, *rows, *rows, fake, fake, fake, ws, bytes, n)
     refused(back(bytes=need - 1), b"workspace")
     refused(back(ws=n), b"null")
-    states = L.atl_decay_attn_states(100_000, 2, 8)
-    assert states > 0 and L.atl_decay_attn_states(5, 2, 8) == 0 and L.atl_decay_attn_states(5, 2, 129) == -1
-    need, need2 = (L.atl_decay_attn_ws_bytes(100_000, 2, 8, back) for back in (0, 1))
-    assert need2 >= need + 4 * states and L.atl_decay_attn_ws_bytes(-1, 2, 8, 0) == -1
+    states = L.atl_decay_attn_states(100_000, 1, 2, 8)
+    assert states > 0 and L.atl_decay_attn_states(5, 1, 2, 8) == 0 and L.atl_decay_attn_states(5, 1, 2, 129) == -1
+    need, need2 = (L.atl_decay_attn_ws_bytes(100_000, 1, 2, 8, back) for back in (0, 1))
+    assert need2 >= need + 4 * states and L.atl_decay_attn_ws_bytes(-1, 1, 2, 8, 0) == -1
     fwd = lambda N=100_000, D=8, dtype=0, B=1, held=fake, bytes=need, sn=16, start=fake: L.atl_decay_attn_fwd(
         fake, sn, 8, *rows, *rows, dtype, N, 2, D, fake, start, B, n, n, 1.0, fake, fake, held, fake, bytes, n)
     refused(fwd(N=-1), b"bad sizes")

@@ -14,7 +14,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parents[1]
-SOURCES = ["abi.hip", "events.hip", "tiles.hip", "pairs.hip", "fastpair.hip", "knn.hip", "embed.hip", "rmsnorm.hip", "gscan.hip", "headrot.hip", "decay.hip"]
+SOURCES = ["abi.hip", "events.hip", "tiles.hip", "pairs.hip", "fastpair.hip", "knn.hip", "embed.hip", "rmsnorm.hip", "gscan.hip", "headrot.hip", "decay.hip", "decay_f32.hip",
+           "decay_bf16.hip", "decay_f16.hip"]
 OUT = HERE / "libatl_hip.so"
 ARCH = os.environ.get("ATL_HIP_ARCH", "gfx950")
 

@@ -1,0 +1,974 @@
+// Linear attention with a decay for each head, over windows of tokens.  With a_i = exp(-rate dt_i) and per head
+//
+//   S_i = a_i S_{i-1} + k_i v_i^T,   y_i = scale q_i S_i                                      (S is D x D)
+//
+// the gradients have the same form: dq_i = scale S_i gy_i is the recurrence over (gy, v, k) instead of (q, k, v), and with
+// G_i = scale q_i gy_i^T + a_{i+1} G_{i+1}, dv_j = k_j G_j and dk_j = G_j v_j are recurrences from the end over (k, q, gy) and
+// (v, gy, q).  So there is one sweep, over rows X, Y, W in either direction, with a state M of Y by W channels:
+//
+//   out_i = ps sum_{j <= i} e^{-(E_i - E_j)} (X_i Y_j) W_j + xs e^{-E_i} X_i M,   M' = e^{-E} M + us sum_j e^{-(E - E_j)} Y_j W_j^T
+//
+// for a chunk of 32 rows, with E_i the decay from the chunk's begin to row i: up to the row's own gap forward, up to the gap
+// before it from the end (a token's gap lies before it).  The products run on the matrix cores.  Decays stay exponents, in
+// 64 bits within a chunk, and a factor of the state near one is applied as M + M expm1(-E): a product of many factors just
+// below one would lose what each rounds off.  Exponents past 400 (in powers of two: the factor is zero in 32 bits) count as 400,
+// so an endless gap forgets what was before it and no difference of infinities appears.
+//
+// A window is cut into stretches of L tokens; a workgroup follows one stretch of one head.  The state before a stretch comes
+// from a pass that sums every stretch but the last on its own (k_decay_local) and one that joins them (k_decay_join); windows
+// of one stretch need neither, and both return at once there.
+#pragma once
+#include "decay.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace atlhip {
+namespace {
+
+constexpr int kChunk = 32;                 // rows of a chunk: what one step of a matrix instruction sums
+
+constexpr double kForgotten = 400.0;       // exponents (of two) from which a factor is zero
+
+using F4 = float __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------------------------------- fragments
+// Eight elements a lane of a 16 x 32 operand of a matrix product: lane l holds index l % 16 of the operand's outer axis, and a
+// fourth of the axis that is summed over, in any order that both operands have.  A product's result has its outer axes at
+// (4 (l / 16) + r, l % 16), r < 4.  Two orders make results the next product's operands as they lie in their lanes:
+//
+//   rows (tokens) are summed in the order t 16 + 4 (l / 16) + r, t < 2, of two results' blocks of 16;
+//   channels are summed in their order, 8 (l / 16) + 4 t + r, and a state's blocks hold the channels that this asks for:
+//   block 2 k + t at 32 k + 8 (m / 4) + 4 t + m % 4, m < 16.
+template <typename T>
+struct FragOf {
+  using type = T __attribute__((ext_vector_type(8)));
+};
+template <>
+struct FragOf<float> {
+  struct type {
+    float e[8];
+    __device__ __forceinline__ float& operator[](int k) { return e[k]; }
+    __device__ __forceinline__ float operator[](int k) const { return e[k]; }
+  };
+};
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ F4 mma(Frag<bf16_t> a, Frag<bf16_t> b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ F4 mma(Frag<f16_t> a, Frag<f16_t> b, F4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ F4 mma(const Frag<float>& a, const Frag<float>& b, F4 c) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], c, 0, 0, 0);
+  return c;
+}
+
+// Row `row` of a tile (the lane's own), channels 32 kb to 32 kb + 31.
+template <typename T, int LD>
+__device__ __forceinline__ Frag<T> frag_row(const T* tile, int row, int kb) {
+  const int g = (threadIdx.x & (kWave - 1)) >> 4;
+  union { Pack<T, 16 / sizeof(T)> p[sizeof(T) / 2]; Frag<T> f; } u;
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(T) / 2; ++k) u.p[k] = load_pack<T, 16 / sizeof(T)>(tile + row * LD + kb * 32 + g * 8 + k * 4);
+  return u.f;
+}
+
+// A channel of a chunk's rows: col0 + l % 16, or where STATE the l % 16-th of a state's block col0 / 16.
+template <typename T, int LD, bool STATE>
+__device__ __forceinline__ Frag<T> frag_col(const T* tile, int col0) {
+  const int l = threadIdx.x & (kWave - 1), g = l >> 4, i = l & 15;
+  const int base = STATE ? col0 / 32 * 32 + (col0 / 16 & 1) * 4 : col0, four = STATE ? 8 : 4;
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    // The transposed read: 16 lanes name four rows of four times four elements, and each gets a column of four.
+    using S4 = short __attribute__((ext_vector_type(4)));
+    using LdsS4 = __attribute__((address_space(3))) S4;
+    union { S4 s[2]; Frag<T> f; } u;
+    const T* p = tile + (g * 4 + (i >> 2)) * LD + base + (i & 3) * four;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4*)p);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4*)(p + 16 * LD));
+    f = u.f;
+  } else {
+    const T* p = tile + g * 4 * LD + base + (i >> 2) * four + (i & 3);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = p[((k >> 2) * 16 + (k & 3)) * LD];
+  }
+  return f;
+}
+
+// Values in 32 bits as the sum of NS fragments of T, so that the products' sums are those of values in 24 bits (NS = 3), or
+// within 2^-16 (bfloat16, NS = 2).  Bfloat16 pieces but the last are the value's and the remainders' upper halves, cut
+// off: a mask and a subtraction, and one instruction that packs two.  Rounded pieces would need a conversion there and back.
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+template <typename T, int NS>
+__device__ __forceinline__ void split(const float (&v)[8], Frag<T> (&f)[NS]) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[0][k] = v[k];
+  } else if constexpr (std::is_same<T, bf16_t>::value) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = v[k];
+#pragma unroll
+    for (int s = 0; s + 1 < NS; ++s) {
+      union { uint32_t w[4]; Frag<T> f; } u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u.w[k] = upper_halves(x[2 * k], x[2 * k + 1]);
+      f[s] = u.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] -= __uint_as_float(__float_as_uint(x[k]) & 0xFFFF0000u);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[NS - 1][k] = (T)x[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float x = v[k];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        f[s][k] = (T)x;
+        x -= (float)f[s][k];
+      }
+    }
+  }
+}
+// The same where some values are not finite: those are one piece.
+template <typename T, int NS>
+__device__ __forceinline__ void split_any(const float (&v)[8], Frag<T> (&f)[NS]) {
+  float x[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = fabsf(v[k]) < INFINITY ? v[k] : 0.f;
+  split<T, NS>(x, f);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (!(fabsf(v[k]) < INFINITY)) f[0][k] = (T)v[k];
+}
+template <typename T>
+constexpr int pieces(int n) {
+  return std::is_same<T, float>::value ? 1 : n;
+}
+
+// Half precision reaches from 6e-8 to 65504 only: what goes into it is brought to a largest value of 2^14 to 2^15 first, by
+// a power of two.
+struct Fit {
+  float up, down;
+};
+__device__ __forceinline__ float finite_top(float top, float v) { return fabsf(v) < INFINITY ? fmaxf(top, fabsf(v)) : top; }
+__device__ __forceinline__ Fit fit_of(float top) {
+  const uint32_t e = max(__float_as_uint(top) >> 23, 15u);
+  return Fit{__uint_as_float((268u - e) << 23), __uint_as_float((e - 14u) << 23)};
+}
+// Of the lanes l % 16 alike.
+__device__ __forceinline__ float top_of_four(float top) {
+  top = fmaxf(top, __shfl_xor(top, 16, kWave));
+  return fmaxf(top, __shfl_xor(top, 32, kWave));
+}
+
+// A state's factor e^{-z}: for small z by what it is less than one (else that would lose the factor's own bits).
+struct Fade {
+  float a;
+  int keep;
+  __device__ __forceinline__ float operator()(float m) const { return fmaf(m, a, keep ? m : 0.f); }
+};
+__device__ __forceinline__ Fade fade_of(float z) {
+  const bool keep = !(z > 0.5f);
+  return Fade{keep ? expm1f(-z) : expf(-z), keep};
+}
+
+// ------------------------------------------------------------------------------------------- windows
+// Stretch of a slot.  Windows are numbered with the tokens before the first (window -1) and behind the last (window B), which
+// are in none; window b begins at slot floor(first token / L) + b + 1, so every window has as many slots as stretches or
+// more, and no sum over the windows is needed.
+struct Stretch {
+  int64_t window, lo, hi;                  // tokens of the stretch
+  bool first, last, live;                  // of its window; live: there is one
+  int64_t entry;                           // of the states after stretches: unlike for all but windows' last stretches
+};
+
+__device__ __forceinline__ int64_t edge_of(const DecayGeo& d, int64_t e) {     // first token of window e - 1
+  if (e <= 0) return 0;
+  if (e > d.B + 1) return d.N;
+  const int64_t s = d.start[e - 1];
+  return s < 0 ? 0 : s > d.N ? d.N : s;
+}
+
+// The last of 0..n-1 that holds `at` (which holds for the first ones only, 0 among them).  Every lane of a wave calls it: 64
+// are looked at in one step.
+template <typename F>
+__device__ __forceinline__ int64_t last_of(int64_t n, F&& at) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int64_t lo = 0;
+  while (n > 1) {
+    const int64_t step = (n + kWave - 1) / kWave;
+    const int c = __popcll(__ballot(lane * step < n && at(lo + lane * step)));
+    const int64_t k = c > 0 ? c - 1 : 0;
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ Stretch stretch_of(const DecayGeo& d, int64_t slot) {
+  const int64_t lo = last_of(d.B + 2, [&](int64_t e) { return edge_of(d, e) / d.L + e <= slot; });
+  Stretch s;
+  const int64_t begin = edge_of(d, lo), end = max(begin, edge_of(d, lo + 1));
+  const int64_t k = slot - (begin / d.L + lo);
+  s.window = lo - 1;
+  s.entry = begin / d.L + k;
+  s.lo = begin + k * d.L;
+  s.hi = min(end, s.lo + d.L);
+  s.first = k == 0;
+  s.last = s.lo + d.L >= end;
+  s.live = k == 0 || (k > 0 && s.lo < end);
+  return s;
+}
+
+// Workgroups of one die (they are dealt out round robin over eight) take neighbouring slots and heads, whose rows share lines.
+__device__ __forceinline__ int64_t near_first(int64_t block, int64_t blocks) {
+  const int64_t per = (blocks + 7) / 8;
+  return (block & 7) * per + (block >> 3);
+}
+
+// ------------------------------------------------------------------------------------------- a chunk
+template <typename T, int DP>
+constexpr int tile_ld() { return DP + 16 / (int)sizeof(T); }                // rows a vector apart: no bank conflicts
+
+// The exponents E_i of a chunk (in powers of two) and the factors made of them.  A pair's factor e^{-(E_i - E_j)} is taken from
+// the exponents inside a block of 16 rows, and between the two blocks as row_i col_j, from and to the first block's last
+// row: a product instead of an exponential.
+struct Decays {
+  double e[kChunk];
+  float row[kChunk], col[kChunk];                           // ps e^{-..}, e^{-..}
+  float xe[kChunk], we[kChunk];                             // xs e^{-E_i}, us e^{-(E - E_i)}
+  Fade fade;                                                // e^{-E}
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dppd(double v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, true);
+  return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+
+// Those of two chunks, by one wave: a lane's gap is that of its row.  Returns E over both.
+template <bool REV>
+__device__ __forceinline__ double exponents(Decays (&two)[2], float gap, float rate, int len, float ps, float xs, float us) {
+  const int lane = threadIdx.x & (kWave - 1), block = lane >> 4;
+  double z = (double)rate * (double)gap * 1.4426950408889634;
+  if (z > kForgotten) z = kForgotten;                       // a NaN stays
+  if (lane >= len) z = 0;
+  double sum = z;                                           // within the block of 16, then within the chunk
+  sum += dppd<0x111>(sum);
+  sum += dppd<0x112>(sum);
+  sum += dppd<0x114>(sum);
+  sum += dppd<0x118>(sum);
+  const double a = lane_of(sum, 15), b = a + lane_of(sum, 31), c = lane_of(sum, 47), d = c + lane_of(sum, 63);
+  const double half = block < 2 ? a : c, total = block < 2 ? b : d;
+  if (block & 1) sum += half;
+  const double e = REV ? sum - z : sum;
+  Decays& s = two[block >> 1];
+  const int i = lane & (kChunk - 1);
+  s.e[i] = e;
+  s.row[i] = ps * exp2f((float)(half - e));
+  s.col[i] = exp2f((float)(e - half));
+  s.xe[i] = xs * exp2f((float)-e);
+  s.we[i] = us * exp2f((float)(e - total));
+  if (i == 0) s.fade = fade_of((float)(total * 0.6931471805599453));
+  return b + d;
+}
+
+// A chunk's rows as a buffer: its lowest token at p, row r at offset r stride (or (len - 1 - r) stride where REV), so that a row
+// that is not there, and a channel past D (kNoChannel), lie outside, where loads give zeros and stores do nothing.  Strides
+// are below 2^22 elements, so 32 rows are 2^29 bytes at most.
+constexpr uint32_t kNoChannel = 0x80000000u;
+using U4v = uint32_t __attribute__((ext_vector_type(4)));
+using U2v = uint32_t __attribute__((ext_vector_type(2)));
+template <bool REV>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_buffer(const void* row0, int64_t stride, int len, int width) {
+  const char* p = (const char*)row0 - (REV ? (len - 1) * stride : 0);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (len - 1) * (int)stride + width, 0x00020000);
+}
+template <bool REV>
+__device__ __forceinline__ uint32_t row_offset(int r, int stride, int len) {
+  return (uint32_t)((REV ? len - 1 - r : r) * stride);
+}
+
+// Pieces of 16 bytes of a chunk's rows, in registers until the chunk's turn.
+template <typename T, int DP, int THREADS>
+struct Stage {
+  static constexpr int V = 16 / (int)sizeof(T), PER = DP / V, COUNT = kChunk * PER / THREADS, STEP = THREADS / PER;
+  static_assert(COUNT * THREADS == kChunk * PER && STEP * PER == THREADS, "whole rounds of whole rows");
+  Pack<T, V> v[COUNT];
+
+  // Row r of the chunk is token at + r (or at - r where REV); len rows are there, the others zero.
+  template <bool REV, bool WHOLE>
+  __device__ __forceinline__ void load(const Rows& rows, int64_t head, int64_t at, int len, int D) {
+    const T* row0 = (const T*)rows.p + head * rows.sh + at * rows.sn;
+    const int r0 = threadIdx.x / PER, c = threadIdx.x % PER * V;
+    if constexpr (WHOLE) {
+      const int stride = (int)rows.sn * (int)sizeof(T);
+      const auto buf = chunk_buffer<REV>(row0, stride, len, D * (int)sizeof(T));
+      const uint32_t off = row_offset<REV>(r0, stride, len) + (c < D ? c * (uint32_t)sizeof(T) : kNoChannel);
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n) {
+        const U4v w = __builtin_amdgcn_raw_buffer_load_b128(buf, off + (uint32_t)((REV ? -n : n) * STEP * stride), 0, 0);
+        v[n] = *reinterpret_cast<const Pack<T, V>*>(&w);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n) {
+        const int r = r0 + n * STEP;
+        Pack<T, V> q{};
+        if (r < len && c < D) {
+          const T* from = row0 + (REV ? -r : r) * rows.sn + c;
+          if (c + V <= D) {
+            const LoosePack<T, V> z = *reinterpret_cast<const LoosePack<T, V>*>(from);
+#pragma unroll
+            for (int k = 0; k < V; ++k) q.e[k] = z.e[k];
+          } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              if (c + k < D) q.e[k] = from[k];
+          }
+        }
+        v[n] = q;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+    T* to = tile + threadIdx.x / PER * tile_ld<T, DP>() + threadIdx.x % PER * V;
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) *reinterpret_cast<Pack<T, V>*>(to + n * STEP * tile_ld<T, DP>()) = v[n];
+  }
+};
+
+// M = e^{-E} M + us sum_j e^{-(E - E_j)} Y_j W_j^T over the chunk; the wave holds the columns (W channels) of its CT tiles.  The
+// weighted W go in as three pieces, so a state is as good as one summed in single precision; the chunk's sum is taken
+// from zero and added once.  Returns whether some of the wave's W are not finite.
+template <typename T, int DP, int CT>
+__device__ __forceinline__ bool add_chunk(const Decays& s, const T* y, F4 (&M)[CT][DP / 16], const Frag<T> (&wf)[CT]) {
+  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, NS = pieces<T>(3);
+  constexpr bool HALF = std::is_same<T, f16_t>::value;
+  const int g = (threadIdx.x & (kWave - 1)) >> 4;
+  const Pack<float, 4> we[2] = {load_pack<float, 4>(s.we + g * 4), load_pack<float, 4>(s.we + 16 + g * 4)};
+  Frag<T> b[CT][NS];
+  float wv[CT][8], down[CT], odd = 0.f;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      wv[ct][k] = we[k >> 2].e[k & 3] * (float)wf[ct][k];
+      if (HALF) top = finite_top(top, wv[ct][k]);
+      odd = fmaf(wv[ct][k], 0.f, odd);
+    }
+    if (HALF) {
+      const Fit f = fit_of(top_of_four(top));
+      down[ct] = f.down;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) wv[ct][k] *= f.up;
+    }
+  }
+  const bool odds = __any(odd != 0.f);
+  if (!std::is_same<T, float>::value && odds) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) split_any<T, NS>(wv[ct], b[ct]);
+  } else {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) split<T, NS>(wv[ct], b[ct]);
+  }
+  const Fade fade = s.fade;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const Frag<T> a = frag_col<T, LD, true>(y, dt * 16);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      F4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NS; ++n) u = mma(a, b[ct][n], u);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float m = fade(M[ct][dt][r]);
+        M[ct][dt][r] = HALF ? fmaf(u[r], down[ct], m) : m + u[r];
+      }
+    }
+  }
+  return odds;
+}
+
+// The Y channel of a lane's element r of block dt of a state.
+__device__ __forceinline__ int state_row(int dt, int r) {
+  return dt / 2 * 32 + ((threadIdx.x & (kWave - 1)) >> 4) * 8 + (dt & 1) * 4 + r;
+}
+// The lane's elements of a state (D x D at p, rows Y channels, or columns where flip), zeros past D.
+template <int DP, int CT>
+__device__ __forceinline__ void load_state(const float* p, bool flip, int D, int c0, F4 (&M)[CT][DP / 16]) {
+  const int i = threadIdx.x & 15, sy = flip ? 1 : D, sw = flip ? D : 1;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int y = state_row(dt, r), w = c0 + ct * 16 + i;
+        M[ct][dt][r] = p && y < D && w < D ? p[y * sy + w * sw] : 0.f;
+      }
+}
+template <int DP, int CT>
+__device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&M)[CT][DP / 16]) {
+  const int i = threadIdx.x & 15;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int y = state_row(dt, r), w = c0 + ct * 16 + i;
+        if (y < D && w < D) p[y * D + w] = M[ct][dt][r];
+      }
+}
+
+// ------------------------------------------------------------------------------------------- the sweep
+constexpr int kLdsBytes = 160 * 1024, kSweepWaves = 2;
+
+// A workgroup of several waves has two buffers of tiles: it fills one while it works on the other, with one barrier a chunk.
+template <typename T, int DP, int NT, int THREADS>
+struct ChunkLds {
+  static constexpr int BUFS = THREADS > kWave ? 2 : 1;
+  T tile[BUFS][NT][kChunk * tile_ld<T, DP>()];
+  Decays decay[2][2];                                       // of two chunks and of the next two
+};
+// Waves to a SIMD that the shared memory leaves room for.
+template <typename LDS, int MOST>
+constexpr int waves_of(int waves) {
+  const int n = (int)(kLdsBytes / sizeof(LDS)) * waves / 4;
+  return n < 1 ? 1 : n > MOST ? MOST : n;
+}
+
+// One recurrence (JOBS = 1: X, Y, W are rows 0, 1, 2), or two that share their rows (q, k, v, gy: dv over (k, q, gy), dk over
+// (v, gy, q)), each by its own waves.
+struct Sweep {
+  Rows rows[4];
+  void* out[2];                            // (N, H, D)
+  const float *carry, *given;              // states after stretches (entries, H, D, D); before the windows (B, H, D, D) or null
+  float* end;                              // behind the windows (B, H, D, D), or null (the first job's)
+  int flip;                                // the states lie transposed (the first job's; the second's the other way)
+  float ps, xs, us;
+};
+
+constexpr int kTiles = 2;                  // blocks of 16 W channels of a wave
+
+// Goes through a stretch's chunks: chunk(done, len, tiles, decays) with its rows and exponents in shared memory.
+template <typename T, int DP, int NT, int THREADS, bool REV, bool WHOLE, typename Chunk>
+__device__ __forceinline__ double follow(ChunkLds<T, DP, NT, THREADS>& s, const DecayGeo& d, const Stretch& st, const Rows (&rows)[NT],
+                                         int head, float ps, float xs, float us, Chunk&& chunk) {
+  constexpr int BUFS = ChunkLds<T, DP, NT, THREADS>::BUFS;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const float rate = d.rate[head];
+  const int tokens = (int)(st.hi - st.lo);
+  const int64_t from = REV ? st.hi - 1 : st.lo;             // the token of the stretch's first row
+  Stage<T, DP, THREADS> stage[NT];
+  auto fetch = [&](int done) {
+    if (done >= tokens) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      stage[n].template load<REV, WHOLE>(rows[n], head, REV ? from - done : from + done, min(kChunk, tokens - done), d.D);
+  };
+  auto put = [&](int done) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) stage[n].store(s.tile[BUFS == 1 ? 0 : done / kChunk & 1][n]);
+  };
+  // The last wave makes the exponents, two chunks at a time and two ahead.
+  const bool decays = wave == THREADS / kWave - 1;
+  double sum = 0;
+  auto gap_of = [&](int done) {
+    return d.dt && done + lane < tokens ? d.dt[REV ? from - done - lane : from + done + lane] : 1.f;
+  };
+  auto make = [&](int done, float gap) {
+    sum += exponents<REV>(s.decay[done / kWave & 1], gap, rate, tokens - done, ps, xs, us);
+  };
+  float gap = 1.f;
+  if (tokens > 0) fetch(0);
+  if (decays && tokens > 0) {
+    make(0, gap_of(0));
+    gap = gap_of(kWave);
+  }
+  if (BUFS == 2 && tokens > 0) {
+    put(0);
+    fetch(kChunk);
+  }
+  for (int done = 0; done < tokens; done += kChunk) {
+    __syncthreads();
+    if (BUFS == 1) {
+      put(done);
+      __syncthreads();
+    } else if (done + kChunk < tokens) {
+      put(done + kChunk);
+    }
+    fetch(done + BUFS * kChunk);
+    if (decays && done % kWave == 0 && done + kWave < tokens) {
+      make(done + kWave, gap);
+      gap = gap_of(done + 2 * kWave);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    chunk(done, min(kChunk, tokens - done), s.tile[BUFS == 1 ? 0 : done / kChunk & 1], s.decay[done / kWave & 1][done / kChunk & 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return sum;
+}
+
+template <typename T, int DP, int JOBS>
+constexpr int sweep_threads() { return DP / 32 * JOBS * kWave; }
+
+template <typename T, int DP, int JOBS, bool REV, bool WHOLE>
+__global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<ChunkLds<T, DP, JOBS + 2, sweep_threads<T, DP, JOBS>()>, kSweepWaves>(DP / 32 * JOBS)))
+    k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
+  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, KD = DP / 32, THREADS = sweep_threads<T, DP, JOBS>();
+  constexpr int NT = JOBS + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
+  constexpr bool HALF = std::is_same<T, f16_t>::value;
+  __shared__ ChunkLds<T, DP, NT, THREADS> s;
+  const int64_t work = near_first(first + blockIdx.x, d.slots * d.H);
+  if (work >= d.slots * d.H) return;
+  const int64_t slot = work / d.H;
+  const int head = (int)(work - slot * d.H);
+  const Stretch st = stretch_of(d, slot);
+  if (!st.live) return;
+  const int every = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), job = every / NW, wave = every % NW;
+  const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i16 = lane & 15;
+  const int c0 = wave * CT * 16;
+  T* out = (T*)a.out[job];
+  if (st.window < 0 || st.window >= d.B) {                  // tokens of no window
+    for (int64_t t = st.lo + wave; t < st.hi; t += NW)
+      for (int c = lane; c < d.D; c += kWave) out[(t * d.H + head) * d.D + c] = (T)0.f;
+    return;
+  }
+  const bool begins = REV ? st.last : st.first, ends = REV ? st.first : st.last;
+  const int64_t DD = (int64_t)d.D * d.D;
+  F4 M[CT][DT];
+  load_state<DP, CT>(begins ? (a.given ? a.given + (st.window * d.H + head) * DD : nullptr)
+                            : a.carry + ((st.entry + (REV ? 1 : -1)) * d.H + head) * DD,
+                     (a.flip != 0) != (job != 0), d.D, c0, M);
+  Rows rows[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) rows[n] = a.rows[n];
+  const int out_stride = d.H * d.D * (int)sizeof(T);
+  const int64_t from = REV ? st.hi - 1 : st.lo;
+  follow<T, DP, NT, THREADS, REV, WHOLE>(s, d, st, rows, head, a.ps, a.xs, a.us, [&](int done, int len, const auto& tile, const Decays& dec) {
+    const T* X = tile[JOBS == 1 ? 0 : job ? 2 : 1];
+    const T* Y = tile[JOBS == 1 ? 1 : job ? 3 : 0];
+    const T* W = tile[JOBS == 1 ? 2 : job ? 0 : 3];
+    // What the rows take from the state before the chunk, M^T X^T: a lane holds four neighbouring channels of its row.
+    F4 far[2][CT];
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) far[it][ct] = F4{0.f, 0.f, 0.f, 0.f};
+    Fit fm{1.f, 1.f};
+    if (HALF) {
+      float top = 0.f;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = finite_top(top, M[ct][dt][r]);
+#pragma unroll
+      for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
+      fm = fit_of(top_of_four(top));
+    }
+    Frag<T> xf[2][KD];
+#pragma unroll
+    for (int k = 0; k < KD; ++k) {
+#pragma unroll
+      for (int it = 0; it < 2; ++it) xf[it][k] = frag_row<T, LD>(X, it * 16 + i16, k);
+      Frag<T> sf[CT][NS];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = HALF ? M[ct][k * 2 + (e >> 2)][e & 3] * fm.up : M[ct][k * 2 + (e >> 2)][e & 3];
+        split<T, NS>(v, sf[ct]);
+      }
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int n = 0; n < NS; ++n) far[it][ct] = mma(sf[ct][n], xf[it][k], far[it][ct]);
+    }
+    // The pairs, as Y X^T: a lane holds four neighbouring j of its i, in the order in which the next product sums them.
+    // Rounded once: as far off as the output's own rounding.
+    Frag<T> pf[2];
+    Fit fp[2] = {{1.f, 1.f}, {1.f, 1.f}};
+    F4 acc[3];                                              // blocks (0, 0), (1, 0), (1, 1)
+#pragma unroll
+    for (int n = 0; n < 3; ++n) acc[n] = F4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KD; ++k) {
+      const Frag<T> y0 = frag_row<T, LD>(Y, i16, k), y1 = frag_row<T, LD>(Y, 16 + i16, k);
+      acc[0] = mma(y0, xf[0][k], acc[0]);
+      acc[1] = mma(y0, xf[1][k], acc[1]);
+      acc[2] = mma(y1, xf[1][k], acc[2]);
+    }
+    Frag<T> wf[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(W, c0 + ct * 16);
+    {
+      float v[3][4];
+      const float row = dec.row[16 + i16];
+      const Pack<float, 4> col = load_pack<float, 4>(dec.col + g * 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[1][r] = acc[1][r] * row * col.e[r];
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const double e = dec.e[it * 16 + i16];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {                       // (taken for all lanes, without a branch; past i it may overflow)
+          const float p = acc[it * 2][r] * a.ps * __builtin_amdgcn_exp2f((float)(dec.e[it * 16 + g * 4 + r] - e));
+          v[it * 2][r] = g * 4 + r <= i16 ? p : 0.f;
+        }
+      }
+      if (HALF) {
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top[n > 0] = finite_top(top[n > 0], v[n][r]);
+#pragma unroll
+        for (int it = 0; it < 2; ++it) fp[it] = fit_of(top_of_four(top[it]));
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[n][r] *= fp[n > 0].up;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        pf[0][r] = (T)v[0][r];
+        pf[0][4 + r] = (T)0.f;
+        pf[1][r] = (T)v[1][r];
+        pf[1][4 + r] = (T)v[2][r];
+      }
+    }
+    const bool odds = add_chunk<T, DP, CT>(dec, Y, M, wf);
+    // The outputs.  Rows past i have weight zero, and zero times an infinity or NaN would be a NaN: where there are any (ODD),
+    // the product is taken without such values, and those of the rows up to i are added, their weights taken anew.
+    const auto out_buf = chunk_buffer<REV>(out + ((REV ? from - done : from + done) * d.H + head) * d.D, out_stride, len, d.D * (int)sizeof(T));
+    auto emit = [&](auto is_odd) {
+      constexpr bool ODD = decltype(is_odd)::value;
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int i = it * 16 + i16;
+        const float xe = HALF ? dec.xe[i] * fm.down : dec.xe[i];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          Frag<T> w = wf[ct];
+          if (ODD)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = fabsf((float)w[k]) < INFINITY ? w[k] : (T)0.f;
+          const F4 pv = mma(w, pf[it], F4{0.f, 0.f, 0.f, 0.f});
+          const int c = c0 + ct * 16 + g * 4;
+          float o[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
+          if (ODD)
+            for (int j = 0; j <= i; ++j)
+#pragma unroll 1
+              for (int r = 0; r < 4; ++r) {
+                const float z = (float)W[j * LD + c + r];
+                if (fabsf(z) < INFINITY) continue;
+                float dot = 0.f;
+#pragma unroll 1
+                for (int h = 0; h < DP; ++h) dot = fmaf((float)X[i * LD + h], (float)Y[j * LD + h], dot);
+                dot *= a.ps * exp2f((float)(dec.e[j] - dec.e[i]));
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (q == r) o[q] = fmaf(dot, z, o[q]);
+              }
+          if constexpr (WHOLE) {
+            const uint32_t off = row_offset<REV>(i, out_stride, len) + (c < d.D ? c * (uint32_t)sizeof(T) : kNoChannel);
+            Pack<T, 4> q;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q.e[r] = (T)o[r];
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(*reinterpret_cast<const U2v*>(&q), out_buf, off, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const U4v*>(&q), out_buf, off, 0, 0);
+          } else if (i < len && c < d.D) {
+            store_loose<4>(out + ((REV ? from - done - i : from + done + i) * d.H + head) * d.D + c, d.D - c, o);
+          }
+        }
+      }
+    };
+    if (odds) emit(std::true_type{});
+    else emit(std::false_type{});
+  });
+  if (ends && a.end && job == 0) store_state<DP, CT>(a.end + (st.window * d.H + head) * DD, d.D, c0, M);
+}
+
+// A stretch's own sum from nothing (all but the last of a window, in the sweep's direction): carry (entries, H, D, D), and
+// its exponent and factor (entries, H).
+struct Span {
+  double z;
+  Fade fade;
+};
+template <typename T, int DP, bool REV, bool WHOLE>
+__global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2, DP / 32 * kWave>, kSweepWaves>(DP / 32)))
+    k_decay_local(DecayGeo d, Rows y, Rows w, float us, float* __restrict__ carry, Span* __restrict__ spans, int64_t first) {
+  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, THREADS = NW * kWave;
+  __shared__ ChunkLds<T, DP, 2, THREADS> s;
+  const int64_t work = near_first(first + blockIdx.x, d.slots * d.H);
+  if (work >= d.slots * d.H) return;
+  const int64_t slot = work / d.H;
+  const int head = (int)(work - slot * d.H);
+  const Stretch st = stretch_of(d, slot);
+  if (!st.live || (REV ? st.first : st.last) || st.window < 0 || st.window >= d.B) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), c0 = wave * CT * 16;
+  F4 M[CT][DT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
+  const Rows rows[2] = {y, w};
+  const double sum = follow<T, DP, 2, THREADS, REV, WHOLE>(s, d, st, rows, head, 1.f, 1.f, us,
+                                                           [&](int, int, const auto& tile, const Decays& dec) {
+    Frag<T> wf[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(tile[1], c0 + ct * 16);
+    add_chunk<T, DP, CT>(dec, tile[0], M, wf);
+  });
+  store_state<DP, CT>(carry + (st.entry * d.H + head) * (int64_t)d.D * d.D, d.D, c0, M);
+  if (threadIdx.x == THREADS - kWave) spans[st.entry * d.H + head] = Span{sum, fade_of((float)(sum * 0.6931471805599453))};
+}
+
+// The states after the stretches of every window (all but its last) from the stretches' own sums, in place: a thread an
+// element, for windows of fewer than kFew stretches.
+constexpr int kFew = 64, kAhead = 8;
+struct Join {
+  float* p;                                // the element's sum of the first stretch in the sweep's direction
+  const Span* z;
+  int64_t n, step, zstep;                  // stretches but the last
+  float given;
+  bool in;
+};
+template <bool REV>
+__device__ __forceinline__ Join join_of(const DecayGeo& d, const float* given, float* carry, const Span* spans, int64_t b, int head,
+                                        int64_t el) {
+  const int64_t DD = (int64_t)d.D * d.D, lo = edge_of(d, b + 1), hi = max(lo, edge_of(d, b + 2));
+  Join j;
+  j.n = (hi - lo + d.L - 1) / d.L - 1;
+  j.in = el < DD && j.n > 0;
+  const int64_t at = lo / d.L + (REV ? j.n : 0);
+  j.p = carry + (at * d.H + head) * DD + el;
+  j.z = spans + at * d.H + head;
+  j.step = (REV ? -1 : 1) * d.H * DD;
+  j.zstep = (REV ? -1 : 1) * d.H;
+  j.given = given && j.in ? given[(b * d.H + head) * DD + el] : 0.f;
+  return j;
+}
+template <bool WRITE>
+__device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1, float state) {
+  for (int64_t k = k0; k < k1; k += kAhead) {
+    float u[kAhead];
+    Fade f[kAhead];
+#pragma unroll
+    for (int m = 0; m < kAhead; ++m) {
+      const int64_t at = min(k + m, k1 - 1);
+      u[m] = j.in ? j.p[at * j.step] : 0.f;
+      f[m] = j.z[at * j.zstep].fade;
+    }
+#pragma unroll
+    for (int m = 0; m < kAhead; ++m) {
+      if (k + m >= k1) break;
+      state = f[m](state) + u[m];
+      if (WRITE && j.in) j.p[(k + m) * j.step] = state;
+    }
+  }
+  return state;
+}
+template <bool REV>
+__global__ void __launch_bounds__(kBlock) k_decay_join(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
+                                                       const Span* __restrict__ spans, int64_t first) {
+  const int64_t per = ((int64_t)d.D * d.D + kBlock - 1) / kBlock, block = first + blockIdx.x, bh = block / per;
+  const int64_t b = bh / d.H;
+  const Join j = join_of<REV>(d, given, carry, spans, b, (int)(bh - b * d.H), (block - bh * per) * kBlock + threadIdx.x);
+  if (j.n < 1 || j.n >= kFew || !j.in) return;
+  join_run<true>(j, 0, j.n, j.given);
+}
+
+// The same for windows of kFew stretches or more: a workgroup has EL elements of the state and cuts the stretches into runs:
+// every run's own sum, those joined, every run again from its begin (which the cache still holds).  A long window is found by
+// the first multiple of kFew L in it (or, with fewer windows than multiples, by its number).
+template <bool REV, int EL>
+__global__ void __launch_bounds__(1024) k_decay_join_long(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
+                                                          const Span* __restrict__ spans, int by_place, int64_t first) {
+  constexpr int RUNS = 1024 / EL;
+  __shared__ float end[RUNS][EL];
+  __shared__ Fade fade[RUNS];
+  const int64_t per = ((int64_t)d.D * d.D + EL - 1) / EL, block = first + blockIdx.x, bh = block / per;
+  int64_t b = bh / d.H;
+  const int head = (int)(bh - b * d.H);
+  if (by_place) {
+    const int64_t place = b * kFew * d.L;
+    const int64_t e = last_of(d.B + 2, [&](int64_t e) { return edge_of(d, e) <= place; });
+    if (e < 1 || e > d.B || edge_of(d, e) + kFew * d.L <= place) return;      // in no window, or not the first multiple in it
+    b = e - 1;
+  }
+  const int e = threadIdx.x % EL, run = threadIdx.x / EL;
+  const Join j = join_of<REV>(d, given, carry, spans, b, head, (block - bh * per) * EL + e);
+  if (j.n < kFew) return;
+  const int64_t len = (j.n + RUNS - 1) / RUNS, k0 = min(run * len, j.n), k1 = min(k0 + len, j.n);
+  end[run][e] = join_run<false>(j, k0, k1, 0.f);
+  if (threadIdx.x < RUNS) {
+    double total = 0;
+    for (int64_t k = min(threadIdx.x * len, j.n); k < min((threadIdx.x + 1) * len, j.n); ++k) total += j.z[k * j.zstep].z;
+    fade[threadIdx.x] = fade_of((float)(total * 0.6931471805599453));
+  }
+  __syncthreads();
+  float state = j.given;
+  for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state) + end[r][e];
+  join_run<true>(j, k0, k1, state);
+}
+
+// One token of every stream: M = e^{-z} M + k v^T in place, y = scale q M.  A wave a stream's head: lanes side by side along
+// the rows of M, 16 bytes each where they are aligned; bound by reading and writing the states.
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock) k_decay_step(Rows q, Rows k, Rows v, const float* __restrict__ rate,
+                                                       const float* __restrict__ dt, int64_t N, int H, int D, int cl2, float scale,
+                                                       float* __restrict__ state, T* __restrict__ y, int64_t first) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t nh = (first + blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave;
+  if (nh >= N * H) return;
+  const int64_t n = nh / H;
+  const int h = (int)(nh - n * H);
+  const Fade fade = fade_of(rate[h] * (dt ? dt[n] : 1.f));
+  const T* qp = (const T*)q.p + n * q.sn + h * q.sh;
+  const T* kp = (const T*)k.p + n * k.sn + h * k.sh;
+  const T* vp = (const T*)v.p + n * v.sn + h * v.sh;
+  float* M = state + nh * D * D;
+  const int rows = kWave >> cl2, row = lane >> cl2;
+  for (int c = (lane & ((1 << cl2) - 1)) * V; c - (lane & ((1 << cl2) - 1)) * V < D; c += V << cl2) {
+    const bool in = c < D;
+    float vv[V], acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) vv[e] = in ? (float)vp[c + e] : 0.f, acc[e] = 0.f;
+#pragma unroll 8
+    for (int r = row; r < D; r += rows) {
+      if (!in) continue;
+      float m[V];
+      load_f<V>(M + r * D + c, m);
+      const float kr = (float)kp[r], qr = (float)qp[r];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        m[e] = fmaf(kr, vv[e], fade(m[e]));
+        acc[e] = fmaf(qr, m[e], acc[e]);
+      }
+      store_f<V>(M + r * D + c, m);
+    }
+    for (int s = 1 << cl2; s < kWave; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += __shfl_xor(acc[e], s, kWave);
+    if (row == 0 && in)
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[nh * D + c + e] = (T)(acc[e] * scale);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- launches
+template <typename F>
+void by_head(int64_t D, F&& f) {
+  if (D <= 32) f(std::integral_constant<int, 32>{});
+  else if (D <= 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+template <typename T>
+bool rows_whole(const Rows& r, int64_t D) {
+  const int v = 16 / (int)sizeof(T);
+  return D % v == 0 && r.sn % v == 0 && r.sh % v == 0 && aligned_to(r.p, 16);
+}
+
+template <typename T, bool REV>
+void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const float* given, void* ws, float* carry,
+                hipStream_t stream) {
+  if (d.N <= d.L) return;                                  // every window is one stretch at most
+  const bool whole = rows_whole<T>(y, d.D) && rows_whole<T>(w, d.D);
+  by_head(d.D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
+      if (whole)
+        hipLaunchKernelGGL((k_decay_local<T, DP, REV, true>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
+                           (Span*)ws, first);
+      else
+        hipLaunchKernelGGL((k_decay_local<T, DP, REV, false>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
+                           (Span*)ws, first);
+    }, DP / 32 * kWave);
+  });
+  const int64_t DD = (int64_t)d.D * d.D, entries = d.N / d.L + 1;
+  const Span* spans = (const Span*)ws;
+  if (d.B > 1 || entries <= kFew)
+    in_launches(d.B * d.H * ((DD + kBlock - 1) / kBlock), [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL((k_decay_join<REV>), dim3(count), dim3(kBlock), 0, stream, d, given, carry, spans, first);
+    });
+  if (entries > kFew) {
+    const int64_t places = d.N / (kFew * d.L) + 1;
+    const int by_place = places < d.B;
+    const int64_t of = (by_place ? places : d.B) * d.H;
+    if (DD * d.H <= 16384)                                 // few elements: more runs, for as many threads
+      in_launches(of * ((DD + 15) / 16), [&](int64_t first, unsigned count) {
+        hipLaunchKernelGGL((k_decay_join_long<REV, 16>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, first);
+      }, 1024);
+    else
+      in_launches(of * ((DD + 63) / 64), [&](int64_t first, unsigned count) {
+        hipLaunchKernelGGL((k_decay_join_long<REV, 64>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, first);
+      }, 1024);
+  }
+}
+
+template <typename T, int JOBS, bool REV>
+void run_sweep(const DecayGeo& d, const Sweep& a, hipStream_t stream) {
+  bool whole = true;
+  for (int n = 0; n < (JOBS == 1 ? 3 : 4); ++n) whole = whole && rows_whole<T>(a.rows[n], d.D);
+  for (int n = 0; n < JOBS; ++n) whole = whole && aligned_to(a.out[n], 16);
+  by_head(d.D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
+      if (whole)
+        hipLaunchKernelGGL((k_decay_sweep<T, DP, JOBS, REV, true>), dim3(count), dim3(DP / 32 * JOBS * kWave), 0, stream, d, a, first);
+      else
+        hipLaunchKernelGGL((k_decay_sweep<T, DP, JOBS, REV, false>), dim3(count), dim3(DP / 32 * JOBS * kWave), 0, stream, d, a, first);
+    }, DP / 32 * JOBS * kWave);
+  });
+}
+
+template <typename T>
+void run_fwd(const DecayGeo& d, const DecayFwd& a, hipStream_t stream) {
+  run_states<T, false>(d, a.k, a.v, 1.f, a.h0, a.ws, a.states, stream);
+  run_sweep<T, 1, false>(d, Sweep{{a.q, a.k, a.v}, {a.y}, a.states, a.h0, a.last, 0, a.scale, a.scale, 1.f}, stream);
+}
+template <typename T>
+void run_bwd(const DecayGeo& d, const DecayBwd& a, hipStream_t stream) {
+  run_states<T, true>(d, a.q, a.gy, a.scale, a.glast, a.ws, a.carry, stream);
+  run_sweep<T, 1, false>(d, Sweep{{a.gy, a.v, a.k}, {a.gq}, a.states, a.h0, nullptr, 1, a.scale, a.scale, 1.f}, stream);
+  run_sweep<T, 2, true>(d, Sweep{{a.q, a.k, a.v, a.gy}, {a.gv, a.gk}, a.carry, a.glast, a.gh0, 0, a.scale, 1.f, a.scale}, stream);
+}
+template <typename T>
+void run_step(const DecayStep& a, hipStream_t stream) {
+  const bool vec = a.D % 4 == 0 && aligned_to(a.state, 16);
+  const int64_t units = vec ? a.D / 4 : a.D;
+  int cl2 = 0;
+  while ((1 << cl2) < kWave && (1 << cl2) < units) ++cl2;
+  in_launches((a.N * a.H + kBlock / kWave - 1) / (kBlock / kWave), [&](int64_t first, unsigned count) {
+    if (vec)
+      hipLaunchKernelGGL((k_decay_step<T, 4>), dim3(count), dim3(kBlock), 0, stream, a.q, a.k, a.v, a.rate, a.dt, a.N, a.H, a.D, cl2,
+                         a.scale, a.state, (T*)a.y, first);
+    else
+      hipLaunchKernelGGL((k_decay_step<T, 1>), dim3(count), dim3(kBlock), 0, stream, a.q, a.k, a.v, a.rate, a.dt, a.N, a.H, a.D, cl2,
+                         a.scale, a.state, (T*)a.y, first);
+  });
+}
+
+}  // namespace
+}  // namespace atlhip

@@ -141,8 +141,8 @@ _SIGS = {
     "atl_head_norm_rotary_bwd": [_P, _I, _I, _P, _I, _I, _C, _P, _P, _P, _C, _P, _I, _P, _I, _I, _I, _I, _D, _P, _I, _I, _P, _I, _I,
                                  _P, _P, _P, _P, _I, _P],
     "atl_head_norm_rotary_bwd_ws_bytes": [_I],
-    "atl_decay_attn_states": [_I, _I, _I],
-    "atl_decay_attn_ws_bytes": [_I, _I, _I, _C],
+    "atl_decay_attn_states": [_I, _I, _I, _I],
+    "atl_decay_attn_ws_bytes": [_I, _I, _I, _I, _C],
     "atl_decay_attn_fwd": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _I, _P, _P, _D, _P, _P, _P, _P, _I, _P],
     "atl_decay_attn_bwd": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _I, _P, _P, _P, _D, _P, _P, _P, _P,
                            _P, _P, _I, _P],

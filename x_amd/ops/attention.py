@@ -26,11 +26,19 @@ from .sequence import _CODE, _at, _float_type, _grads_wanted, _on, _plain, _rout
 MAX_ROTARY_WIDTH = 256
 MAX_ROTARY_AXES = 4
 MAX_ATTENTION_WIDTH = 128
+MAX_TOKEN_STRIDE = 2 ** 22
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """``t`` (N, H, D) with contiguous heads: itself where they are, else a copy."""
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _chunks(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (N, H, D) as the attention over windows takes it: contiguous heads, tokens that lie apart but within reach of the
+    32-bit offsets of 64 of them; else a copy."""
+    t = _heads(t)
+    return t if t.shape[0] < 2 or t.shape[2] <= t.stride(0) < MAX_TOKEN_STRIDE else t.contiguous()
 
 
 def _strides(t: torch.Tensor | None) -> tuple[int, int, int]:
@@ -159,8 +167,8 @@ def _decay_fwd(q, k, v, rate, start, dt, h0, scale):
     lib = load_library()
     y = torch.empty(N, H, D, dtype=q.dtype, device=dev)
     last = torch.empty(B, H, D, D, dtype=F32, device=dev)
-    held = int(lib.atl_decay_attn_states(N, H, D))
-    nbytes = int(lib.atl_decay_attn_ws_bytes(N, H, D, 0))
+    held = int(lib.atl_decay_attn_states(N, B, H, D))
+    nbytes = int(lib.atl_decay_attn_ws_bytes(N, B, H, D, 0))
     ws = _ws(nbytes, dev, "decay_attention")
     states = torch.empty(held, dtype=F32, device=dev) if held else None
     with on_device(dev):
@@ -186,11 +194,11 @@ class _Decay(torch.autograd.Function):
             return (None,) * 8
         N, H, D = q.shape
         B, dev = start.numel() - 1, q.device
-        gy = torch.zeros(N, H, D, dtype=q.dtype, device=dev) if gy is None else _heads(gy)
+        gy = torch.zeros(N, H, D, dtype=q.dtype, device=dev) if gy is None else _chunks(gy)
         glast = None if glast is None else glast.contiguous()
         gq, gk, gv = (torch.empty(N, H, D, dtype=q.dtype, device=dev) for _ in range(3))
         gh0 = torch.empty(B, H, D, D, dtype=F32, device=dev) if ctx.needs_input_grad[6] else None
-        nbytes = int(load_library().atl_decay_attn_ws_bytes(N, H, D, 1))
+        nbytes = int(load_library().atl_decay_attn_ws_bytes(N, B, H, D, 1))
         ws = _ws(nbytes, dev, "decay_attention")
         with on_device(dev):
             call("atl_decay_attn_bwd", *_strides(q), *_strides(k), *_strides(v), *_strides(gy), _CODE[q.dtype], N, H, D,
@@ -257,10 +265,12 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: tor
             raise ValueError(f"h0 must be ({B}, {H}, {D}, {D}), got {tuple(h0.shape)}")
     start = _plain(start, I64)
     through = _route(q, "decay_attention")
+    if H * D >= MAX_TOKEN_STRIDE:
+        raise ValueError(f"a token of fewer than {MAX_TOKEN_STRIDE} channels in all heads, got {H} x {D}")
     if through is None:
         return ref.decay_attention(q, k, v, rate, start, dt, h0, scale)
     h0 = None if h0 is None else _plain(h0, F32)
-    q, k, v = _heads(q), _heads(k), _heads(v)
+    q, k, v = _chunks(q), _chunks(k), _chunks(v)
     if through or _grads_wanted(q, k, v, h0):
         return _Decay.apply(q, k, v, rate, start, dt, h0, scale)
     return _decay_fwd(q, k, v, rate, start, dt, h0, scale)[:2]
