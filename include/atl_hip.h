@@ -558,8 +558,8 @@ int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void
                              void* yk, hipStream_t stream);
 /* Its backward from gyq, gyk (either may be null: zeros): gq, gk and gw (2,D: the weights' gradients, queries' first)
  * written, each unless null.  q, k may be null without norms.  ws (for gw): atl_head_norm_rotary_bwd_ws_bytes bytes (-1:
- * width unsupported). */
-int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t D);
+ * sizes unsupported). */
+int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t H, int64_t Hk, int64_t D);
 int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
                              const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
                              const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, const void* gyq,
@@ -569,20 +569,19 @@ int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void
 /* S_i = exp(-rate dt_i) S_{i-1} + k_i v_i^T, y_i = scale q_i S_i per head (dt null: ones; rate (H)) within each window of
  * tokens [start[b], start[b+1]) (start (B+1) ascends within [0, N]; empty windows allowed; tokens outside are in no window:
  * zeros), from h0 (B,H,D,D) or zero.  y (N,H,D) and last (B,H,D,D) = every window's last state (an empty window's: h0 or
- * zero) written.  states: atl_decay_attn_states floats (null where that is 0), kept for the backward.  ws:
- * atl_decay_attn_ws_bytes bytes (-1: sizes unsupported).  D <= 128, H D < 2^22; token strides (of two tokens or more) from
- * D to below 2^22. */
-int64_t atl_decay_attn_states(int64_t N, int64_t B, int64_t H, int64_t D);
-int64_t atl_decay_attn_ws_bytes(int64_t N, int64_t B, int64_t H, int64_t D, int backward);
+ * zero) written.  states: atl_decay_attn_states_bytes bytes (null where that is 0; -1: sizes unsupported), kept for the
+ * backward.  D <= 128, H D < 2^22; token strides (of two tokens or more) from D to below 2^22. */
+int64_t atl_decay_attn_states_bytes(int64_t N, int64_t B, int64_t H, int64_t D);
 int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate,
                        const int64_t* start, int64_t B, const float* dt, const float* h0, double scale, void* y, float* last,
-                       float* states, void* ws, int64_t ws_bytes, hipStream_t stream);
-/* Its backward from gy and glast (may be null): gq, gk, gv (N,H,D) and gh0 (B,H,D,D; may be null) written. */
+                       void* states, int64_t states_bytes, hipStream_t stream);
+/* Its backward from gy and glast (may be null): gq, gk, gv (N,H,D) and gh0 (B,H,D,D; may be null) written.  states: the
+ * forward's; ws: as many bytes. */
 int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, const void* gy, int64_t sgn, int64_t sgh, int dtype, int64_t N, int64_t H,
                        int64_t D, const float* rate, const int64_t* start, int64_t B, const float* dt, const float* h0,
-                       const float* glast, double scale, const float* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
+                       const float* glast, double scale, const void* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
                        int64_t ws_bytes, hipStream_t stream);
 /* One token of each of N streams: state (N,H,D,D) updated in place, y (N,H,D) = scale q state. */
 int atl_decay_attn_step(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,

@@ -211,29 +211,31 @@ def test_entries_reject_before_launch():
     refused(rot(eps=-1.0), b"bad sizes")
     refused(rot(pos=n), b"null")
     refused(rot(out=n), b"null")
-    need = L.atl_head_norm_rotary_bwd_ws_bytes(8)
-    assert need > 0 and L.atl_head_norm_rotary_bwd_ws_bytes(0) == -1 and L.atl_head_norm_rotary_bwd_ws_bytes(257) == -1
+    need = L.atl_head_norm_rotary_bwd_ws_bytes(2, 2, 8)
+    assert need > 0 and L.atl_head_norm_rotary_bwd_ws_bytes(2, 2, 0) == -1 and L.atl_head_norm_rotary_bwd_ws_bytes(2, 2, 257) == -1
     back = lambda ws=fake, bytes=need: L.atl_head_norm_rotary_bwd(*rows, *rows, 0, fake, fake, fake, 0, fake, 2, sec(2, 2), 5, 2, 2,
                                                                   8, 1e-6, *rows, *rows, fake, fake, fake, ws, bytes, n)
     refused(back(bytes=need - 1), b"workspace")
     refused(back(ws=n), b"null")
-    states = L.atl_decay_attn_states(100_000, 1, 2, 8)
-    assert states > 0 and L.atl_decay_attn_states(5, 1, 2, 8) == 0 and L.atl_decay_attn_states(5, 1, 2, 129) == -1
-    need, need2 = (L.atl_decay_attn_ws_bytes(100_000, 1, 2, 8, back) for back in (0, 1))
-    assert need2 >= need + 4 * states and L.atl_decay_attn_ws_bytes(-1, 1, 2, 8, 0) == -1
+    need = L.atl_decay_attn_states_bytes(100_000, 1, 2, 8)
+    assert need > 0 and L.atl_decay_attn_states_bytes(5, 1, 2, 8) == 0
+    assert L.atl_decay_attn_states_bytes(5, 1, 2, 129) == L.atl_decay_attn_states_bytes(-1, 1, 2, 8) == -1
     fwd = lambda N=100_000, D=8, dtype=0, B=1, held=fake, bytes=need, sn=16, start=fake: L.atl_decay_attn_fwd(
-        fake, sn, 8, *rows, *rows, dtype, N, 2, D, fake, start, B, n, n, 1.0, fake, fake, held, fake, bytes, n)
+        fake, sn, 8, *rows, *rows, dtype, N, 2, D, fake, start, B, n, n, 1.0, fake, fake, held, bytes, n)
     refused(fwd(N=-1), b"bad sizes")
     refused(fwd(D=0), b"bad sizes")
     refused(fwd(B=-1), b"bad sizes")
     refused(fwd(dtype=7), b"bad sizes")
     refused(fwd(sn=-1), b"bad sizes")
+    refused(fwd(sn=7), b"bad sizes")
+    refused(fwd(sn=2 ** 22), b"bad sizes")
     refused(fwd(held=n), b"null")
     refused(fwd(start=n), b"null")
-    refused(fwd(bytes=need - 1), b"workspace")
-    bwd = lambda gq=fake, bytes=need2: L.atl_decay_attn_bwd(*rows, *rows, *rows, *rows, 0, 100_000, 2, 8, fake, fake, 1, n, n, n, 1.0,
-                                                            fake, gq, fake, fake, n, fake, bytes, n)
+    refused(fwd(bytes=need - 1), b"states")
+    bwd = lambda gq=fake, ws=fake, bytes=need: L.atl_decay_attn_bwd(*rows, *rows, *rows, *rows, 0, 100_000, 2, 8, fake, fake, 1, n, n,
+                                                                    n, 1.0, fake, gq, fake, fake, n, ws, bytes, n)
     refused(bwd(gq=n), b"null")
-    refused(bwd(bytes=need2 - 1), b"workspace")
+    refused(bwd(ws=n), b"null")
+    refused(bwd(bytes=need - 1), b"workspace")
     refused(L.atl_decay_attn_step(*rows, *rows, *rows, 0, 5, 2, 200, fake, n, 1.0, fake, fake, n), b"bad sizes")
     refused(L.atl_decay_attn_step(*rows, *rows, *rows, 0, 5, 2, 8, fake, n, 1.0, n, fake, n), b"null")

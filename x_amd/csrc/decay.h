@@ -20,15 +20,20 @@ struct DecayFwd {
   Rows q, k, v;
   const float* h0;
   float scale;
-  void *y, *ws;
-  float *last, *states;
+  void* y;
+  float* last;
+  void* states;                            // spans of the stretches, and from span_bytes on their sums or states
+  int64_t span_bytes;
 };
 struct DecayBwd {
   Rows q, k, v, gy;
-  const float *h0, *glast, *states;
+  const float *h0, *glast;
   float scale;
-  void *gq, *gk, *gv, *ws;
-  float *gh0, *carry;
+  void *gq, *gk, *gv;
+  float* gh0;
+  const void* states;                      // the forward's
+  void* ws;                                // the same from the end
+  int64_t span_bytes;
 };
 struct DecayStep {
   Rows q, k, v;

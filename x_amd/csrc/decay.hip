@@ -7,15 +7,16 @@
 namespace atlhip {
 namespace {
 
-constexpr int kChunk = 64, kMaxHead = 128;
+constexpr int kMaxHead = 128;
 constexpr int64_t kMaxStride = (int64_t)1 << 22;
 
-// Tokens of a stretch: the stretches of all heads, and half a stretch for every window's last, fill the card once (eight,
-// four or two workgroups to a compute unit by the heads' width); where there are more windows than that, eight chunks.
-int64_t stretch_len(int64_t N, int64_t B, int64_t H, int64_t D) {
-  const int64_t groups = D <= 32 ? 2048 : D <= 64 ? 1024 : 512, left = std::max(groups - B * H / 2, groups / 2);
-  const int64_t chunks = (N * H / left + kChunk - 1) / kChunk;
-  return kChunk * std::min<int64_t>(std::max<int64_t>(chunks, 4), 512);
+// Tokens of a stretch: the stretches of all heads, and half a stretch for every window's last, are 1536 workgroups (768 and
+// 3072 were up to 20% slower, by the width), whole pairs of chunks, four pairs at least.
+int64_t stretch_len(int64_t N, int64_t B, int64_t H) {
+  constexpr int64_t kGroups = 1536, kPair = 64;
+  const int64_t left = std::max(kGroups - B * H / 2, kGroups / 2);
+  const int64_t pairs = (N * H / left + kPair - 1) / kPair;
+  return kPair * std::min<int64_t>(std::max<int64_t>(pairs, 4), 512);
 }
 
 bool decay_ok(int dtype, int64_t N, int64_t B, int64_t H, int64_t D) {
@@ -28,8 +29,8 @@ bool strides_ok(Rows& r, int64_t N, int64_t D) {
   return r.sh >= 0 && r.sn >= D && r.sn < kMaxStride;
 }
 
-int64_t decay_entries(int64_t N, int64_t B, int64_t H, int64_t D) { return N / stretch_len(N, B, H, D) + 1; }
-int64_t decay_span_bytes(int64_t N, int64_t B, int64_t H, int64_t D) { return (decay_entries(N, B, H, D) * H * 16 + 255) / 256 * 256; }
+int64_t decay_entries(int64_t N, int64_t B, int64_t H) { return N / stretch_len(N, B, H) + 1; }
+int64_t decay_span_bytes(int64_t N, int64_t B, int64_t H) { return (decay_entries(N, B, H) * H * 16 + 255) / 256 * 256; }
 
 template <typename F>
 void by_type(int dtype, F&& f) {
@@ -41,7 +42,7 @@ void by_type(int dtype, F&& f) {
 DecayGeo decay_geo(int64_t N, int64_t B, int64_t H, int64_t D, const int64_t* start, const float* dt, const float* rate) {
   DecayGeo d{};
   d.start = start; d.dt = dt; d.rate = rate;
-  d.N = N; d.B = B; d.L = stretch_len(N, B, H, D);
+  d.N = N; d.B = B; d.L = stretch_len(N, B, H);
   d.slots = N / d.L + B + 2;
   d.H = (int)H; d.D = (int)D;
   return d;
@@ -54,26 +55,22 @@ using namespace atlhip;
 
 extern "C" {
 
-int64_t atl_decay_attn_states(int64_t N, int64_t B, int64_t H, int64_t D) {
+int64_t atl_decay_attn_states_bytes(int64_t N, int64_t B, int64_t H, int64_t D) {
   if (!decay_ok(kF32, N, B, H, D)) return -1;
-  return N <= stretch_len(N, B, H, D) ? 0 : decay_entries(N, B, H, D) * H * D * D;
-}
-
-int64_t atl_decay_attn_ws_bytes(int64_t N, int64_t B, int64_t H, int64_t D, int backward) {
-  const int64_t n = atl_decay_attn_states(N, B, H, D);
-  return n < 0 ? -1 : decay_span_bytes(N, B, H, D) + (backward ? 4 * n : 0);
+  return N <= stretch_len(N, B, H) ? 0 : decay_span_bytes(N, B, H) + decay_entries(N, B, H) * H * D * D * 4;
 }
 
 int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate,
                        const int64_t* start, int64_t B, const float* dt, const float* h0, double scale, void* y, float* last,
-                       float* states, void* ws, int64_t ws_bytes, hipStream_t stream) {
+                       void* states, int64_t states_bytes, hipStream_t stream) {
   Rows rq{q, sqn, sqh}, rk{k, skn, skh}, rv{v, svn, svh};
   if (!decay_ok(dtype, N, B, H, D) || (N > 0 && !(strides_ok(rq, N, D) && strides_ok(rk, N, D) && strides_ok(rv, N, D)))) { set_error("decay_attn_fwd: bad sizes N=%lld B=%lld H=%lld D=%lld type %d", (long long)N, (long long)B, (long long)H, (long long)D, dtype); return 1; }
-  if (!start || !rate || !ws || (N > 0 && (!q || !k || !v || !y)) || (atl_decay_attn_states(N, B, H, D) && !states)) { set_error("decay_attn_fwd: null argument"); return 1; }
-  if (ws_bytes < atl_decay_attn_ws_bytes(N, B, H, D, 0)) { set_error("decay_attn_fwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_decay_attn_ws_bytes(N, B, H, D, 0)); return 1; }
+  const int64_t need = atl_decay_attn_states_bytes(N, B, H, D);
+  if (!start || !rate || (N > 0 && (!q || !k || !v || !y)) || (need && !states)) { set_error("decay_attn_fwd: null argument"); return 1; }
+  if (states_bytes < need) { set_error("decay_attn_fwd: states of %lld bytes, need %lld", (long long)states_bytes, (long long)need); return 1; }
   const DecayGeo d = decay_geo(N, B, H, D, start, dt, rate);
-  const DecayFwd a{rq, rk, rv, h0, (float)scale, y, ws, last, states};
+  const DecayFwd a{rq, rk, rv, h0, (float)scale, y, last, states, decay_span_bytes(N, B, H)};
   by_type(dtype, [&](auto t) { decay_fwd<decltype(t)>(d, a, stream); });
   return check_launch("decay_attn_fwd");
 }
@@ -81,15 +78,15 @@ int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, i
 int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, const void* gy, int64_t sgn, int64_t sgh, int dtype, int64_t N, int64_t H,
                        int64_t D, const float* rate, const int64_t* start, int64_t B, const float* dt, const float* h0,
-                       const float* glast, double scale, const float* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
+                       const float* glast, double scale, const void* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
                        int64_t ws_bytes, hipStream_t stream) {
   Rows rq{q, sqn, sqh}, rk{k, skn, skh}, rv{v, svn, svh}, rg{gy, sgn, sgh};
   if (!decay_ok(dtype, N, B, H, D) || (N > 0 && !(strides_ok(rq, N, D) && strides_ok(rk, N, D) && strides_ok(rv, N, D) && strides_ok(rg, N, D)))) { set_error("decay_attn_bwd: bad sizes N=%lld B=%lld H=%lld D=%lld type %d", (long long)N, (long long)B, (long long)H, (long long)D, dtype); return 1; }
-  if (!start || !rate || !ws || (N > 0 && (!q || !k || !v || !gy || !gq || !gk || !gv)) || (atl_decay_attn_states(N, B, H, D) && !states)) { set_error("decay_attn_bwd: null argument"); return 1; }
-  if (ws_bytes < atl_decay_attn_ws_bytes(N, B, H, D, 1)) { set_error("decay_attn_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_decay_attn_ws_bytes(N, B, H, D, 1)); return 1; }
+  const int64_t need = atl_decay_attn_states_bytes(N, B, H, D);
+  if (!start || !rate || (N > 0 && (!q || !k || !v || !gy || !gq || !gk || !gv)) || (need && (!states || !ws))) { set_error("decay_attn_bwd: null argument"); return 1; }
+  if (ws_bytes < need) { set_error("decay_attn_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const DecayGeo d = decay_geo(N, B, H, D, start, dt, rate);
-  const DecayBwd a{rq, rk, rv, rg, h0, glast, states, (float)scale, gq, gk, gv, ws, gh0,
-                   (float*)((char*)ws + decay_span_bytes(N, B, H, D))};
+  const DecayBwd a{rq, rk, rv, rg, h0, glast, (float)scale, gq, gk, gv, gh0, states, ws, decay_span_bytes(N, B, H)};
   by_type(dtype, [&](auto t) { decay_bwd<decltype(t)>(d, a, stream); });
   return check_launch("decay_attn_bwd");
 }

@@ -134,17 +134,6 @@ __device__ __forceinline__ void split(const float (&v)[8], Frag<T> (&f)[NS]) {
     }
   }
 }
-// The same where some values are not finite: those are one piece.
-template <typename T, int NS>
-__device__ __forceinline__ void split_any(const float (&v)[8], Frag<T> (&f)[NS]) {
-  float x[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] = fabsf(v[k]) < INFINITY ? v[k] : 0.f;
-  split<T, NS>(x, f);
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (!(fabsf(v[k]) < INFINITY)) f[0][k] = (T)v[k];
-}
 template <typename T>
 constexpr int pieces(int n) {
   return std::is_same<T, float>::value ? 1 : n;
@@ -177,6 +166,13 @@ __device__ __forceinline__ Fade fade_of(float z) {
   return Fade{keep ? expm1f(-z) : expf(-z), keep};
 }
 
+// A stretch's exponent (of two) and factor.
+struct Span {
+  double z;
+  Fade fade;
+};
+constexpr int kFew = 6;                                     // stretches of a window up to which a sweep adds up their sums
+
 // ------------------------------------------------------------------------------------------- windows
 // Stretch of a slot.  Windows are numbered with the tokens before the first (window -1) and behind the last (window B), which
 // are in none; window b begins at slot floor(first token / L) + b + 1, so every window has as many slots as stretches or
@@ -185,6 +181,7 @@ struct Stretch {
   int64_t window, lo, hi;                  // tokens of the stretch
   bool first, last, live;                  // of its window; live: there is one
   int64_t entry;                           // of the states after stretches: unlike for all but windows' last stretches
+  int64_t index, count;                    // of the window's stretches
 };
 
 __device__ __forceinline__ int64_t edge_of(const DecayGeo& d, int64_t e) {     // first token of window e - 1
@@ -217,6 +214,8 @@ __device__ __forceinline__ Stretch stretch_of(const DecayGeo& d, int64_t slot) {
   const int64_t k = slot - (begin / d.L + lo);
   s.window = lo - 1;
   s.entry = begin / d.L + k;
+  s.index = k;
+  s.count = (end - begin + d.L - 1) / d.L;
   s.lo = begin + k * d.L;
   s.hi = min(end, s.lo + d.L);
   s.first = k == 0;
@@ -340,6 +339,19 @@ struct Stage {
       }
     }
   }
+  // Whether some of the lane's elements are not finite (the exponent's bits are all ones).
+  __device__ __forceinline__ bool odd() const {
+    constexpr uint32_t kExp = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, f16_t>::value ? 0x7C007C00u : 0x7F807F80u;
+    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, f16_t>::value ? 0x04000400u : 0x00800080u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) {
+      const U4v w = *reinterpret_cast<const U4v*>(&v[n]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) any |= (w[k] & kExp) + kOne;
+    }
+    return any & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
+  }
   __device__ __forceinline__ void store(T* tile) const {
     T* to = tile + threadIdx.x / PER * tile_ld<T, DP>() + threadIdx.x % PER * V;
 #pragma unroll
@@ -347,17 +359,22 @@ struct Stage {
   }
 };
 
+// The Y channel of a lane's element r of block dt of a state.
+__device__ __forceinline__ int state_row(int dt, int r) {
+  return dt / 2 * 32 + ((threadIdx.x & (kWave - 1)) >> 4) * 8 + (dt & 1) * 4 + r;
+}
+
 // M = e^{-E} M + us sum_j e^{-(E - E_j)} Y_j W_j^T over the chunk; the wave holds the columns (W channels) of its CT tiles.  The
 // weighted W go in as three pieces, so a state is as good as one summed in single precision; the chunk's sum is taken
-// from zero and added once.  Returns whether some of the wave's W are not finite.
+// from zero and added once.
 template <typename T, int DP, int CT>
-__device__ __forceinline__ bool add_chunk(const Decays& s, const T* y, F4 (&M)[CT][DP / 16], const Frag<T> (&wf)[CT]) {
+__device__ __forceinline__ void add_chunk(const Decays& s, const T* y, F4 (&M)[CT][DP / 16], const Frag<T> (&wf)[CT]) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, NS = pieces<T>(3);
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   const int g = (threadIdx.x & (kWave - 1)) >> 4;
   const Pack<float, 4> we[2] = {load_pack<float, 4>(s.we + g * 4), load_pack<float, 4>(s.we + 16 + g * 4)};
   Frag<T> b[CT][NS];
-  float wv[CT][8], down[CT], odd = 0.f;
+  float wv[CT][8], down[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     float top = 0.f;
@@ -365,7 +382,6 @@ __device__ __forceinline__ bool add_chunk(const Decays& s, const T* y, F4 (&M)[C
     for (int k = 0; k < 8; ++k) {
       wv[ct][k] = we[k >> 2].e[k & 3] * (float)wf[ct][k];
       if (HALF) top = finite_top(top, wv[ct][k]);
-      odd = fmaf(wv[ct][k], 0.f, odd);
     }
     if (HALF) {
       const Fit f = fit_of(top_of_four(top));
@@ -374,14 +390,8 @@ __device__ __forceinline__ bool add_chunk(const Decays& s, const T* y, F4 (&M)[C
       for (int k = 0; k < 8; ++k) wv[ct][k] *= f.up;
     }
   }
-  const bool odds = __any(odd != 0.f);
-  if (!std::is_same<T, float>::value && odds) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) split_any<T, NS>(wv[ct], b[ct]);
-  } else {
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) split<T, NS>(wv[ct], b[ct]);
-  }
+  for (int ct = 0; ct < CT; ++ct) split<T, NS>(wv[ct], b[ct]);
   const Fade fade = s.fade;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
@@ -398,26 +408,56 @@ __device__ __forceinline__ bool add_chunk(const Decays& s, const T* y, F4 (&M)[C
       }
     }
   }
-  return odds;
 }
 
-// The Y channel of a lane's element r of block dt of a state.
-__device__ __forceinline__ int state_row(int dt, int r) {
-  return dt / 2 * 32 + ((threadIdx.x & (kWave - 1)) >> 4) * 8 + (dt & 1) * 4 + r;
-}
-// The lane's elements of a state (D x D at p, rows Y channels, or columns where flip), zeros past D.
-template <int DP, int CT>
-__device__ __forceinline__ void load_state(const float* p, bool flip, int D, int c0, F4 (&M)[CT][DP / 16]) {
-  const int i = threadIdx.x & 15, sy = flip ? 1 : D, sw = flip ? D : 1;
+// W that are not finite are left out of the products (their pieces would be NaNs, and so would zero weights times them) ...
+template <typename T, int CT>
+__device__ __forceinline__ void leave_out(Frag<T> (&wf)[CT]) {
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) wf[ct][k] = fabsf((float)wf[ct][k]) < INFINITY ? wf[ct][k] : (T)0.f;
+}
+// ... and added to the state behind them, one by one.
+template <typename T, int DP, int CT>
+__device__ __forceinline__ void add_odd(const Decays& s, const T* y, const T* w, int c0, F4 (&M)[CT][DP / 16]) {
+  constexpr int LD = tile_ld<T, DP>();
+#pragma unroll 1
+  for (int j = 0; j < kChunk; ++j)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float z = (float)w[j * LD + c0 + ct * 16 + (threadIdx.x & 15)];
+      const bool odd = !(fabsf(z) < INFINITY);
+      if (!__any(odd)) continue;
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float m = fmaf(s.we[j] * z, (float)y[j * LD + state_row(dt, r)], M[ct][dt][r]);
+          M[ct][dt][r] = odd ? m : M[ct][dt][r];
+        }
+    }
+}
+
+// M = e^{-z} M + the lane's elements of a state (D x D at p, rows Y channels, or columns where flip), zeros past D.
+template <int DP, int CT>
+__device__ __forceinline__ void add_state(const float* p, bool flip, int D, int c0, Fade fade, F4 (&M)[CT][DP / 16]) {
+  const auto buf = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, D * D * 4, 0x00020000);
+  const int sy = flip ? 1 : D, sw = flip ? D : 1;
+  int y0 = state_row(0, 0);
+  asm volatile("" : "+v"(y0));                              // (the elements' places, kept over a loop, would not fit the registers)
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int w = c0 + ct * 16 + (threadIdx.x & 15);
 #pragma unroll
     for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int y = state_row(dt, r), w = c0 + ct * 16 + i;
-        M[ct][dt][r] = p && y < D && w < D ? p[y * sy + w * sw] : 0.f;
+        const int y = y0 + dt / 2 * 32 + (dt & 1) * 4 + r;
+        const uint32_t off = y < D && w < D ? (uint32_t)(y * sy + w * sw) * 4 : kNoChannel;
+        M[ct][dt][r] = fade(M[ct][dt][r]) + __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, off, 0, 0));
       }
+  }
 }
 template <int DP, int CT>
 __device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&M)[CT][DP / 16]) {
@@ -436,12 +476,11 @@ __device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&
 // ------------------------------------------------------------------------------------------- the sweep
 constexpr int kLdsBytes = 160 * 1024, kSweepWaves = 2;
 
-// A workgroup of several waves has two buffers of tiles: it fills one while it works on the other, with one barrier a chunk.
-template <typename T, int DP, int NT, int THREADS>
+template <typename T, int DP, int NT>
 struct ChunkLds {
-  static constexpr int BUFS = THREADS > kWave ? 2 : 1;
-  T tile[BUFS][NT][kChunk * tile_ld<T, DP>()];
+  T tile[NT][kChunk * tile_ld<T, DP>()];
   Decays decay[2][2];                                       // of two chunks and of the next two
+  int odd[NT];                                              // done + 1 of the last chunk in which a tile had values that are not finite
 };
 // Waves to a SIMD that the shared memory leaves room for.
 template <typename LDS, int MOST>
@@ -455,7 +494,9 @@ constexpr int waves_of(int waves) {
 struct Sweep {
   Rows rows[4];
   void* out[2];                            // (N, H, D)
-  const float *carry, *given;              // states after stretches (entries, H, D, D); before the windows (B, H, D, D) or null
+  const float* carry;                      // sums of stretches, or in windows of more than kFew the states after them (entries, H, D, D)
+  const Span* spans;                       // (entries, H)
+  const float* given;                      // states before the windows (B, H, D, D), or null
   float* end;                              // behind the windows (B, H, D, D), or null (the first job's)
   int flip;                                // the states lie transposed (the first job's; the second's the other way)
   float ps, xs, us;
@@ -463,11 +504,11 @@ struct Sweep {
 
 constexpr int kTiles = 2;                  // blocks of 16 W channels of a wave
 
-// Goes through a stretch's chunks: chunk(done, len, tiles, decays) with its rows and exponents in shared memory.
-template <typename T, int DP, int NT, int THREADS, bool REV, bool WHOLE, typename Chunk>
-__device__ __forceinline__ double follow(ChunkLds<T, DP, NT, THREADS>& s, const DecayGeo& d, const Stretch& st, const Rows (&rows)[NT],
+// Goes through a stretch's chunks: chunk(done, len, decays) with its rows and exponents in shared memory.  W_TILES: the tiles
+// that are looked through for values that are not finite.
+template <typename T, int DP, int NT, int W_TILES, int THREADS, bool REV, bool WHOLE, typename Chunk>
+__device__ __forceinline__ double follow(ChunkLds<T, DP, NT>& s, const DecayGeo& d, const Stretch& st, const Rows (&rows)[NT],
                                          int head, float ps, float xs, float us, Chunk&& chunk) {
-  constexpr int BUFS = ChunkLds<T, DP, NT, THREADS>::BUFS;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const float rate = d.rate[head];
   const int tokens = (int)(st.hi - st.lo);
@@ -481,7 +522,10 @@ __device__ __forceinline__ double follow(ChunkLds<T, DP, NT, THREADS>& s, const 
   };
   auto put = [&](int done) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) stage[n].store(s.tile[BUFS == 1 ? 0 : done / kChunk & 1][n]);
+    for (int n = 0; n < NT; ++n) {
+      stage[n].store(s.tile[n]);
+      if ((W_TILES >> n & 1) && __any(stage[n].odd()) && lane == 0) s.odd[n] = done + 1;
+    }
   };
   // The last wave makes the exponents, two chunks at a time and two ahead.
   const bool decays = wave == THREADS / kWave - 1;
@@ -493,30 +537,23 @@ __device__ __forceinline__ double follow(ChunkLds<T, DP, NT, THREADS>& s, const 
     sum += exponents<REV>(s.decay[done / kWave & 1], gap, rate, tokens - done, ps, xs, us);
   };
   float gap = 1.f;
-  if (tokens > 0) fetch(0);
+  fetch(0);
   if (decays && tokens > 0) {
     make(0, gap_of(0));
     gap = gap_of(kWave);
   }
-  if (BUFS == 2 && tokens > 0) {
-    put(0);
-    fetch(kChunk);
-  }
+  if (threadIdx.x < NT) s.odd[threadIdx.x] = 0;
   for (int done = 0; done < tokens; done += kChunk) {
     __syncthreads();
-    if (BUFS == 1) {
-      put(done);
-      __syncthreads();
-    } else if (done + kChunk < tokens) {
-      put(done + kChunk);
-    }
-    fetch(done + BUFS * kChunk);
+    put(done);
+    __syncthreads();
+    fetch(done + kChunk);
     if (decays && done % kWave == 0 && done + kWave < tokens) {
       make(done + kWave, gap);
       gap = gap_of(done + 2 * kWave);
     }
     __builtin_amdgcn_sched_barrier(0);
-    chunk(done, min(kChunk, tokens - done), s.tile[BUFS == 1 ? 0 : done / kChunk & 1], s.decay[done / kWave & 1][done / kChunk & 1]);
+    chunk(done, min(kChunk, tokens - done), s.decay[done / kWave & 1][done / kChunk & 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
   return sum;
@@ -526,12 +563,12 @@ template <typename T, int DP, int JOBS>
 constexpr int sweep_threads() { return DP / 32 * JOBS * kWave; }
 
 template <typename T, int DP, int JOBS, bool REV, bool WHOLE>
-__global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<ChunkLds<T, DP, JOBS + 2, sweep_threads<T, DP, JOBS>()>, kSweepWaves>(DP / 32 * JOBS)))
+__global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<ChunkLds<T, DP, JOBS + 2>, kSweepWaves>(DP / 32 * JOBS)))
     k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, KD = DP / 32, THREADS = sweep_threads<T, DP, JOBS>();
   constexpr int NT = JOBS + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
   constexpr bool HALF = std::is_same<T, f16_t>::value;
-  __shared__ ChunkLds<T, DP, NT, THREADS> s;
+  __shared__ ChunkLds<T, DP, NT> s;
   const int64_t work = near_first(first + blockIdx.x, d.slots * d.H);
   if (work >= d.slots * d.H) return;
   const int64_t slot = work / d.H;
@@ -550,18 +587,32 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
   const bool begins = REV ? st.last : st.first, ends = REV ? st.first : st.last;
   const int64_t DD = (int64_t)d.D * d.D;
   F4 M[CT][DT];
-  load_state<DP, CT>(begins ? (a.given ? a.given + (st.window * d.H + head) * DD : nullptr)
-                            : a.carry + ((st.entry + (REV ? 1 : -1)) * d.H + head) * DD,
-                     (a.flip != 0) != (job != 0), d.D, c0, M);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
+  const bool flip = (a.flip != 0) != (job != 0);
+  // What is before the stretch: its window's given state and the sums of the stretches in between, or their joined state.
+  const int64_t dir = REV ? 1 : -1, past = begins ? 0 : st.count > kFew ? 1 : REV ? st.count - 1 - st.index : st.index;
+  const bool summed = begins || st.count <= kFew;
+#pragma unroll 1
+  for (int64_t k = past + (summed && a.given); k >= 1; --k) {
+    const int64_t e = (st.entry + dir * k) * d.H + head;
+    const bool given = k > past;
+    const float* p = given ? a.given + (st.window * d.H + head) * DD : a.carry + e * DD;
+    add_state<DP, CT>(p, flip, d.D, c0, !given && summed ? a.spans[e].fade : Fade{0.f, 1}, M);
+  }
   Rows rows[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) rows[n] = a.rows[n];
   const int out_stride = d.H * d.D * (int)sizeof(T);
   const int64_t from = REV ? st.hi - 1 : st.lo;
-  follow<T, DP, NT, THREADS, REV, WHOLE>(s, d, st, rows, head, a.ps, a.xs, a.us, [&](int done, int len, const auto& tile, const Decays& dec) {
-    const T* X = tile[JOBS == 1 ? 0 : job ? 2 : 1];
-    const T* Y = tile[JOBS == 1 ? 1 : job ? 3 : 0];
-    const T* W = tile[JOBS == 1 ? 2 : job ? 0 : 3];
+  follow<T, DP, NT, JOBS == 1 ? 4 : 9, THREADS, REV, WHOLE>(s, d, st, rows, head, a.ps, a.xs, a.us, [&](int done, int len, const Decays& dec) {
+    const int wt = JOBS == 1 ? 2 : job ? 0 : 3;
+    const T* X = s.tile[JOBS == 1 ? 0 : job ? 2 : 1];
+    const T* Y = s.tile[JOBS == 1 ? 1 : job ? 3 : 0];
+    const T* W = s.tile[wt];
+    const bool odd = __builtin_amdgcn_readfirstlane(s.odd[wt]) == done + 1;
     // What the rows take from the state before the chunk, M^T X^T: a lane holds four neighbouring channels of its row.
     F4 far[2][CT];
 #pragma unroll
@@ -581,12 +632,11 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
       for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
       fm = fit_of(top_of_four(top));
     }
-    Frag<T> xf[2][KD];
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
+      Frag<T> xf[2], sf[CT][NS];
 #pragma unroll
-      for (int it = 0; it < 2; ++it) xf[it][k] = frag_row<T, LD>(X, it * 16 + i16, k);
-      Frag<T> sf[CT][NS];
+      for (int it = 0; it < 2; ++it) xf[it] = frag_row<T, LD>(X, it * 16 + i16, k);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         float v[8];
@@ -599,8 +649,9 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int n = 0; n < NS; ++n) far[it][ct] = mma(sf[ct][n], xf[it][k], far[it][ct]);
+          for (int n = 0; n < NS; ++n) far[it][ct] = mma(sf[ct][n], xf[it], far[it][ct]);
     }
+    __builtin_amdgcn_sched_barrier(0);                      // (each part by itself: together they would not fit the registers)
     // The pairs, as Y X^T: a lane holds four neighbouring j of its i, in the order in which the next product sums them.
     // Rounded once: as far off as the output's own rounding.
     Frag<T> pf[2];
@@ -611,13 +662,15 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
       const Frag<T> y0 = frag_row<T, LD>(Y, i16, k), y1 = frag_row<T, LD>(Y, 16 + i16, k);
-      acc[0] = mma(y0, xf[0][k], acc[0]);
-      acc[1] = mma(y0, xf[1][k], acc[1]);
-      acc[2] = mma(y1, xf[1][k], acc[2]);
+      const Frag<T> x0 = frag_row<T, LD>(X, i16, k), x1 = frag_row<T, LD>(X, 16 + i16, k);
+      acc[0] = mma(y0, x0, acc[0]);
+      acc[1] = mma(y0, x1, acc[1]);
+      acc[2] = mma(y1, x1, acc[2]);
     }
     Frag<T> wf[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(W, c0 + ct * 16);
+    if (odd) leave_out<T, CT>(wf);
     {
       float v[3][4];
       const float row = dec.row[16 + i16];
@@ -654,71 +707,71 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
         pf[1][4 + r] = (T)v[2][r];
       }
     }
-    const bool odds = add_chunk<T, DP, CT>(dec, Y, M, wf);
-    // The outputs.  Rows past i have weight zero, and zero times an infinity or NaN would be a NaN: where there are any (ODD),
-    // the product is taken without such values, and those of the rows up to i are added, their weights taken anew.
-    const auto out_buf = chunk_buffer<REV>(out + ((REV ? from - done : from + done) * d.H + head) * d.D, out_stride, len, d.D * (int)sizeof(T));
-    auto emit = [&](auto is_odd) {
-      constexpr bool ODD = decltype(is_odd)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    add_chunk<T, DP, CT>(dec, Y, M, wf);
+    __builtin_amdgcn_sched_barrier(0);
+    T* to = out + ((REV ? from - done : from + done) * d.H + head) * d.D;
+    const auto out_buf = chunk_buffer<REV>(to, out_stride, len, d.D * (int)sizeof(T));
 #pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        const int i = it * 16 + i16;
-        const float xe = HALF ? dec.xe[i] * fm.down : dec.xe[i];
+    for (int it = 0; it < 2; ++it) {
+      const int i = it * 16 + i16;
+      const float xe = HALF ? dec.xe[i] * fm.down : dec.xe[i];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          Frag<T> w = wf[ct];
-          if (ODD)
+      for (int ct = 0; ct < CT; ++ct) {
+        const F4 pv = mma(wf[ct], pf[it], F4{0.f, 0.f, 0.f, 0.f});
+        const int c = c0 + ct * 16 + g * 4;
+        float o[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = fabsf((float)w[k]) < INFINITY ? w[k] : (T)0.f;
-          const F4 pv = mma(w, pf[it], F4{0.f, 0.f, 0.f, 0.f});
-          const int c = c0 + ct * 16 + g * 4;
-          float o[4];
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
+        if constexpr (WHOLE) {
+          const uint32_t off = row_offset<REV>(i, out_stride, len) + (c < d.D ? c * (uint32_t)sizeof(T) : kNoChannel);
+          Pack<T, 4> q;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
-          if (ODD)
-            for (int j = 0; j <= i; ++j)
-#pragma unroll 1
-              for (int r = 0; r < 4; ++r) {
-                const float z = (float)W[j * LD + c + r];
-                if (fabsf(z) < INFINITY) continue;
-                float dot = 0.f;
-#pragma unroll 1
-                for (int h = 0; h < DP; ++h) dot = fmaf((float)X[i * LD + h], (float)Y[j * LD + h], dot);
-                dot *= a.ps * exp2f((float)(dec.e[j] - dec.e[i]));
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  if (q == r) o[q] = fmaf(dot, z, o[q]);
-              }
-          if constexpr (WHOLE) {
-            const uint32_t off = row_offset<REV>(i, out_stride, len) + (c < d.D ? c * (uint32_t)sizeof(T) : kNoChannel);
-            Pack<T, 4> q;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) q.e[r] = (T)o[r];
-            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(*reinterpret_cast<const U2v*>(&q), out_buf, off, 0, 0);
-            else __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const U4v*>(&q), out_buf, off, 0, 0);
-          } else if (i < len && c < d.D) {
-            store_loose<4>(out + ((REV ? from - done - i : from + done + i) * d.H + head) * d.D + c, d.D - c, o);
-          }
+          for (int r = 0; r < 4; ++r) q.e[r] = (T)o[r];
+          if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(*reinterpret_cast<const U2v*>(&q), out_buf, off, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const U4v*>(&q), out_buf, off, 0, 0);
+        } else if (i < len && c < d.D) {
+          store_loose<4>(to + (int64_t)(REV ? -i : i) * d.H * d.D + c, d.D - c, o);
         }
       }
-    };
-    if (odds) emit(std::true_type{});
-    else emit(std::false_type{});
+    }
+    // What was left out, to the rows from its own on: their weights are taken anew.
+    if (odd) {
+      add_odd<T, DP, CT>(dec, Y, W, c0, M);
+      __threadfence_block();
+#pragma unroll 1
+      for (int q = 0; q < 2 * CT * 4; ++q) {
+        const int i = (q & 1) * 16 + i16, c = c0 + (q >> 3) * 16 + g * 4 + (q >> 1 & 3);
+        float sum = 0.f;
+        bool any = false;
+        if (i < len && c < d.D)
+#pragma unroll 1
+          for (int j = 0; j <= i; ++j) {
+            const float z = (float)W[j * LD + c];
+            if (fabsf(z) < INFINITY) continue;
+            float dot = 0.f;
+#pragma unroll 1
+            for (int h = 0; h < DP; ++h) dot = fmaf((float)X[i * LD + h], (float)Y[j * LD + h], dot);
+            sum = fmaf(dot * a.ps * exp2f((float)(dec.e[j] - dec.e[i])), z, sum);
+            any = true;
+          }
+        if (any) {
+          T* p = to + (int64_t)(REV ? -i : i) * d.H * d.D + c;
+          *p = (T)((float)*p + sum);
+        }
+      }
+    }
   });
   if (ends && a.end && job == 0) store_state<DP, CT>(a.end + (st.window * d.H + head) * DD, d.D, c0, M);
 }
 
 // A stretch's own sum from nothing (all but the last of a window, in the sweep's direction): carry (entries, H, D, D), and
 // its exponent and factor (entries, H).
-struct Span {
-  double z;
-  Fade fade;
-};
 template <typename T, int DP, bool REV, bool WHOLE>
-__global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2, DP / 32 * kWave>, kSweepWaves>(DP / 32)))
+__global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>, kSweepWaves>(DP / 32)))
     k_decay_local(DecayGeo d, Rows y, Rows w, float us, float* __restrict__ carry, Span* __restrict__ spans, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, THREADS = NW * kWave;
-  __shared__ ChunkLds<T, DP, 2, THREADS> s;
+  __shared__ ChunkLds<T, DP, 2> s;
   const int64_t work = near_first(first + blockIdx.x, d.slots * d.H);
   if (work >= d.slots * d.H) return;
   const int64_t slot = work / d.H;
@@ -732,42 +785,30 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2, 
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
   const Rows rows[2] = {y, w};
-  const double sum = follow<T, DP, 2, THREADS, REV, WHOLE>(s, d, st, rows, head, 1.f, 1.f, us,
-                                                           [&](int, int, const auto& tile, const Decays& dec) {
+  const double sum = follow<T, DP, 2, 2, THREADS, REV, WHOLE>(s, d, st, rows, head, 1.f, 1.f, us, [&](int done, int, const Decays& dec) {
     Frag<T> wf[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(tile[1], c0 + ct * 16);
-    add_chunk<T, DP, CT>(dec, tile[0], M, wf);
+    for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(s.tile[1], c0 + ct * 16);
+    const bool odd = __builtin_amdgcn_readfirstlane(s.odd[1]) == done + 1;
+    if (odd) leave_out<T, CT>(wf);
+    add_chunk<T, DP, CT>(dec, s.tile[0], M, wf);
+    if (odd) add_odd<T, DP, CT>(dec, s.tile[0], s.tile[1], c0, M);
   });
   store_state<DP, CT>(carry + (st.entry * d.H + head) * (int64_t)d.D * d.D, d.D, c0, M);
   if (threadIdx.x == THREADS - kWave) spans[st.entry * d.H + head] = Span{sum, fade_of((float)(sum * 0.6931471805599453))};
 }
 
-// The states after the stretches of every window (all but its last) from the stretches' own sums, in place: a thread an
-// element, for windows of fewer than kFew stretches.
-constexpr int kFew = 64, kAhead = 8;
+// The states after the stretches of every window of more than kFew stretches (all but the last) from the stretches' own sums, in
+// place; a sweep adds up fewer sums by itself.  A workgroup has EL elements of the state and cuts the stretches into runs: every
+// run's own sum, those joined, every run again from its begin (which the cache still holds).  A window is found by the first
+// multiple of kFew L in it, or with fewer windows than multiples by its number.
+constexpr int kAhead = 8;
 struct Join {
   float* p;                                // the element's sum of the first stretch in the sweep's direction
   const Span* z;
   int64_t n, step, zstep;                  // stretches but the last
-  float given;
   bool in;
 };
-template <bool REV>
-__device__ __forceinline__ Join join_of(const DecayGeo& d, const float* given, float* carry, const Span* spans, int64_t b, int head,
-                                        int64_t el) {
-  const int64_t DD = (int64_t)d.D * d.D, lo = edge_of(d, b + 1), hi = max(lo, edge_of(d, b + 2));
-  Join j;
-  j.n = (hi - lo + d.L - 1) / d.L - 1;
-  j.in = el < DD && j.n > 0;
-  const int64_t at = lo / d.L + (REV ? j.n : 0);
-  j.p = carry + (at * d.H + head) * DD + el;
-  j.z = spans + at * d.H + head;
-  j.step = (REV ? -1 : 1) * d.H * DD;
-  j.zstep = (REV ? -1 : 1) * d.H;
-  j.given = given && j.in ? given[(b * d.H + head) * DD + el] : 0.f;
-  return j;
-}
 template <bool WRITE>
 __device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1, float state) {
   for (int64_t k = k0; k < k1; k += kAhead) {
@@ -788,26 +829,13 @@ __device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1,
   }
   return state;
 }
-template <bool REV>
-__global__ void __launch_bounds__(kBlock) k_decay_join(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
-                                                       const Span* __restrict__ spans, int64_t first) {
-  const int64_t per = ((int64_t)d.D * d.D + kBlock - 1) / kBlock, block = first + blockIdx.x, bh = block / per;
-  const int64_t b = bh / d.H;
-  const Join j = join_of<REV>(d, given, carry, spans, b, (int)(bh - b * d.H), (block - bh * per) * kBlock + threadIdx.x);
-  if (j.n < 1 || j.n >= kFew || !j.in) return;
-  join_run<true>(j, 0, j.n, j.given);
-}
-
-// The same for windows of kFew stretches or more: a workgroup has EL elements of the state and cuts the stretches into runs:
-// every run's own sum, those joined, every run again from its begin (which the cache still holds).  A long window is found by
-// the first multiple of kFew L in it (or, with fewer windows than multiples, by its number).
 template <bool REV, int EL>
-__global__ void __launch_bounds__(1024) k_decay_join_long(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
-                                                          const Span* __restrict__ spans, int by_place, int64_t first) {
+__global__ void __launch_bounds__(1024) k_decay_join(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
+                                                     const Span* __restrict__ spans, int by_place, int parts, int64_t first) {
   constexpr int RUNS = 1024 / EL;
   __shared__ float end[RUNS][EL];
   __shared__ Fade fade[RUNS];
-  const int64_t per = ((int64_t)d.D * d.D + EL - 1) / EL, block = first + blockIdx.x, bh = block / per;
+  const int64_t block = first + blockIdx.x, bh = block / parts, DD = (int64_t)d.D * d.D;
   int64_t b = bh / d.H;
   const int head = (int)(bh - b * d.H);
   if (by_place) {
@@ -816,20 +844,31 @@ __global__ void __launch_bounds__(1024) k_decay_join_long(DecayGeo d, const floa
     if (e < 1 || e > d.B || edge_of(d, e) + kFew * d.L <= place) return;      // in no window, or not the first multiple in it
     b = e - 1;
   }
-  const int e = threadIdx.x % EL, run = threadIdx.x / EL;
-  const Join j = join_of<REV>(d, given, carry, spans, b, head, (block - bh * per) * EL + e);
+  const int64_t lo = edge_of(d, b + 1), hi = max(lo, edge_of(d, b + 2));
+  Join j;
+  j.n = (hi - lo + d.L - 1) / d.L - 1;
   if (j.n < kFew) return;
+  const int e = threadIdx.x % EL, run = threadIdx.x / EL;
+  const int64_t at = lo / d.L + (REV ? j.n : 0);
+  j.z = spans + at * d.H + head;
+  j.step = (REV ? -1 : 1) * d.H * DD;
+  j.zstep = (REV ? -1 : 1) * d.H;
   const int64_t len = (j.n + RUNS - 1) / RUNS, k0 = min(run * len, j.n), k1 = min(k0 + len, j.n);
-  end[run][e] = join_run<false>(j, k0, k1, 0.f);
   if (threadIdx.x < RUNS) {
     double total = 0;
     for (int64_t k = min(threadIdx.x * len, j.n); k < min((threadIdx.x + 1) * len, j.n); ++k) total += j.z[k * j.zstep].z;
     fade[threadIdx.x] = fade_of((float)(total * 0.6931471805599453));
   }
-  __syncthreads();
-  float state = j.given;
-  for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state) + end[r][e];
-  join_run<true>(j, k0, k1, state);
+  for (int64_t el = (block - bh * parts) * EL + e; el - e < DD; el += parts * EL) {
+    j.in = el < DD;
+    j.p = carry + (at * d.H + head) * DD + el;
+    __syncthreads();
+    end[run][e] = join_run<false>(j, k0, k1, 0.f);
+    __syncthreads();
+    float state = given && j.in ? given[(b * d.H + head) * DD + el] : 0.f;
+    for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state) + end[r][e];
+    join_run<true>(j, k0, k1, state);
+  }
 }
 
 // One token of every stream: M = e^{-z} M + k v^T in place, y = scale q M.  A wave a stream's head: lanes side by side along
@@ -891,7 +930,7 @@ bool rows_whole(const Rows& r, int64_t D) {
 }
 
 template <typename T, bool REV>
-void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const float* given, void* ws, float* carry,
+void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const float* given, Span* spans, float* carry,
                 hipStream_t stream) {
   if (d.N <= d.L) return;                                  // every window is one stretch at most
   const bool whole = rows_whole<T>(y, d.D) && rows_whole<T>(w, d.D);
@@ -900,31 +939,24 @@ void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const
     in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
       if (whole)
         hipLaunchKernelGGL((k_decay_local<T, DP, REV, true>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
-                           (Span*)ws, first);
+                           spans, first);
       else
         hipLaunchKernelGGL((k_decay_local<T, DP, REV, false>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
-                           (Span*)ws, first);
+                           spans, first);
     }, DP / 32 * kWave);
   });
-  const int64_t DD = (int64_t)d.D * d.D, entries = d.N / d.L + 1;
-  const Span* spans = (const Span*)ws;
-  if (d.B > 1 || entries <= kFew)
-    in_launches(d.B * d.H * ((DD + kBlock - 1) / kBlock), [&](int64_t first, unsigned count) {
-      hipLaunchKernelGGL((k_decay_join<REV>), dim3(count), dim3(kBlock), 0, stream, d, given, carry, spans, first);
-    });
-  if (entries > kFew) {
-    const int64_t places = d.N / (kFew * d.L) + 1;
-    const int by_place = places < d.B;
-    const int64_t of = (by_place ? places : d.B) * d.H;
-    if (DD * d.H <= 16384)                                 // few elements: more runs, for as many threads
-      in_launches(of * ((DD + 15) / 16), [&](int64_t first, unsigned count) {
-        hipLaunchKernelGGL((k_decay_join_long<REV, 16>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, first);
-      }, 1024);
-    else
-      in_launches(of * ((DD + 63) / 64), [&](int64_t first, unsigned count) {
-        hipLaunchKernelGGL((k_decay_join_long<REV, 64>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, first);
-      }, 1024);
-  }
+  if (d.N <= kFew * d.L) return;                           // no window has more than kFew stretches
+  const int64_t DD = (int64_t)d.D * d.D, places = d.N / (kFew * d.L) + 1;
+  const int by_place = places < d.B;
+  auto go = [&](auto el) {                                 // (most places find no window to join: few workgroups for each)
+    constexpr int EL = decltype(el)::value;
+    const int parts = (int)std::min<int64_t>((DD + EL - 1) / EL, by_place ? 8 : DD);
+    in_launches((by_place ? places : d.B) * d.H * parts, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL((k_decay_join<REV, EL>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, parts, first);
+    }, 1024);
+  };
+  if (DD * d.H * d.B <= 16384) go(std::integral_constant<int, 16>{});         // few elements: more runs, for as many threads
+  else go(std::integral_constant<int, 64>{});
 }
 
 template <typename T, int JOBS, bool REV>
@@ -945,14 +977,20 @@ void run_sweep(const DecayGeo& d, const Sweep& a, hipStream_t stream) {
 
 template <typename T>
 void run_fwd(const DecayGeo& d, const DecayFwd& a, hipStream_t stream) {
-  run_states<T, false>(d, a.k, a.v, 1.f, a.h0, a.ws, a.states, stream);
-  run_sweep<T, 1, false>(d, Sweep{{a.q, a.k, a.v}, {a.y}, a.states, a.h0, a.last, 0, a.scale, a.scale, 1.f}, stream);
+  Span* spans = (Span*)a.states;
+  float* carry = (float*)((char*)a.states + a.span_bytes);
+  run_states<T, false>(d, a.k, a.v, 1.f, a.h0, spans, carry, stream);
+  run_sweep<T, 1, false>(d, Sweep{{a.q, a.k, a.v}, {a.y}, carry, spans, a.h0, a.last, 0, a.scale, a.scale, 1.f}, stream);
 }
 template <typename T>
 void run_bwd(const DecayGeo& d, const DecayBwd& a, hipStream_t stream) {
-  run_states<T, true>(d, a.q, a.gy, a.scale, a.glast, a.ws, a.carry, stream);
-  run_sweep<T, 1, false>(d, Sweep{{a.gy, a.v, a.k}, {a.gq}, a.states, a.h0, nullptr, 1, a.scale, a.scale, 1.f}, stream);
-  run_sweep<T, 2, true>(d, Sweep{{a.q, a.k, a.v, a.gy}, {a.gv, a.gk}, a.carry, a.glast, a.gh0, 0, a.scale, 1.f, a.scale}, stream);
+  const Span* spans = (const Span*)a.states;
+  const float* held = (const float*)((const char*)a.states + a.span_bytes);
+  Span* own = (Span*)a.ws;
+  float* carry = (float*)((char*)a.ws + a.span_bytes);
+  run_states<T, true>(d, a.q, a.gy, a.scale, a.glast, own, carry, stream);
+  run_sweep<T, 1, false>(d, Sweep{{a.gy, a.v, a.k}, {a.gq}, held, spans, a.h0, nullptr, 1, a.scale, a.scale, 1.f}, stream);
+  run_sweep<T, 2, true>(d, Sweep{{a.q, a.k, a.v, a.gy}, {a.gv, a.gk}, carry, own, a.glast, a.gh0, 0, a.scale, 1.f, a.scale}, stream);
 }
 template <typename T>
 void run_step(const DecayStep& a, hipStream_t stream) {

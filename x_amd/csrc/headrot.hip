@@ -9,7 +9,8 @@
 //   gw = sum over tokens and heads of g x r,   gx = r (w g - x r mean(w g x r)).
 //
 // Angles are taken in turns in 64 bits and reduced to half a turn before they become single precision: a position of a
-// million with a frequency near one keeps its angle.  They are those of all the token's heads, so a group of lanes that
+// million with a frequency near one keeps its angle.  The hardware's sine and cosine take turns, and are off by 1.3e-7 at
+// most over the half turn (measured on 2^23 angles).  They are those of all the token's heads, so a group of lanes that
 // holds a row (16 bytes a lane) goes through several heads with them.  Bound by memory: a read and a write of the rows
 // forward, two reads and a write backward.
 #include "shares.h"
@@ -54,7 +55,8 @@ __device__ __forceinline__ void angles(const RotGeo& g, int64_t n, int c, float 
     const int64_t at = n * g.A + a;
     const double x = g.pos64 ? ((const double*)g.pos)[at] : (double)((const float*)g.pos)[at];
     const double turns = x * ((double)g.freq[p] * 0.15915494309189535);
-    sincospif(2.f * (float)(turns - rint(turns)), &si[m], &co[m]);
+    const float t = (float)(turns - rint(turns));
+    co[m] = __builtin_amdgcn_cosf(t), si[m] = __builtin_amdgcn_sinf(t);
   }
 }
 
@@ -70,15 +72,36 @@ __device__ __forceinline__ void turn(float (&v)[V], const float (&co)[V / 2], co
 
 // Sum over a row's lanes, returned to each.
 __device__ __forceinline__ float lanes_sum(float v, int cl2) {
-  for (int d = 1 << cl2 >> 1; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
+  if (cl2 >= 1) v += dppf<0xB1, 0xF>(v);                    // quad_perm [1, 0, 3, 2]
+  if (cl2 >= 2) v += dppf<0x4E, 0xF>(v);                    // quad_perm [2, 3, 0, 1]
+  if (cl2 >= 3) v += dppf<0x141, 0xF>(v);                   // row_half_mirror
+  if (cl2 >= 4) v += dppf<0x140, 0xF>(v);                   // row_mirror
+  if (cl2 >= 5) v += __shfl_xor(v, 16, kWave);
+  if (cl2 >= 6) v += __shfl_xor(v, 32, kWave);
   return v;
 }
 
 // A piece of a row of D channels, from column c < D on; zeros past it.
 template <bool WHOLE, int V, typename T>
+__device__ __forceinline__ Pack<T, V> fetch_part(const T* row, int c, int D) {
+  Pack<T, V> q;
+  if constexpr (WHOLE) {
+    q = load_pack<T, V>(row + c);
+  } else if (D - c >= V) {
+    const LoosePack<T, V> z = *reinterpret_cast<const LoosePack<T, V>*>(row + c);
+#pragma unroll
+    for (int k = 0; k < V; ++k) q.e[k] = z.e[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) q.e[k] = c + k < D ? row[c + k] : (T)0.f;
+  }
+  return q;
+}
+template <bool WHOLE, int V, typename T>
 __device__ __forceinline__ void load_part(const T* row, int c, int D, float (&v)[V]) {
-  if constexpr (WHOLE) load_f<V>(row + c, v);
-  else load_loose<V>(row + c, D - c, v);
+  const Pack<T, V> q = fetch_part<WHOLE, V>(row, c, D);
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = (float)q.e[k];
 }
 template <bool WHOLE, int V, typename T>
 __device__ __forceinline__ void store_part(T* row, int c, int D, const float (&v)[V]) {
@@ -86,44 +109,66 @@ __device__ __forceinline__ void store_part(T* row, int c, int D, const float (&v
   else store_loose<V>(row + c, D - c, v);
 }
 
+constexpr int kBatch = 2;             // rows whose loads are under way together (four: 5% slower, for the registers)
+
+// A row of a token: its head, and whether it is a key's.
+struct Row {
+  bool key;
+  int head;
+};
+__device__ __forceinline__ Row row_of(const RotGeo& g, int h) { return Row{h >= g.H, h >= g.H ? h - g.H : h}; }
+
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) k_headrot_fwd(RotGeo g, HeadRows q, HeadRows k, const float* __restrict__ wq,
                                                         const float* __restrict__ wk, T* __restrict__ yq, T* __restrict__ yk,
                                                         int64_t first) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & ((1 << g.cl2) - 1), c = lane * V;
-  const int64_t item = (first + blockIdx.x) * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
-  const int64_t n = item / g.blocks_of;
-  if (n >= g.N) return;                                   // a whole row's lanes
-  const int h0 = (int)(item - n * g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
+  const int64_t block = first + blockIdx.x, tokens = block / g.blocks_of;
+  const int64_t n = tokens * (kBlock >> g.cl2) + (threadIdx.x >> g.cl2);
+  if (n >= g.N) return;                                     // a whole row's lanes
+  const int h0 = (int)(block - tokens * g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
   const bool in = c < g.D;
-  float co[V / 2], si[V / 2];
-  angles<V>(g, n, c, co, si);
-  for (int h = h0; h < h1; ++h) {
-    const bool key = h >= g.H;
-    const HeadRows& r = key ? k : q;
-    const int head = key ? h - g.H : h;
-    const float* w = key ? wk : wq;
-    float v[V];
+  float co[V / 2], si[V / 2], wv[2][V];
+  if (wq && in) {
+    load_part<WHOLE, V>(wq, c, g.D, wv[0]);
+    load_part<WHOLE, V>(wk, c, g.D, wv[1]);
+  }
+  for (int h = h0; h < h1; h += kBatch) {
+    Pack<T, V> raw[kBatch];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = 0.f;
-    if (in) load_part<WHOLE, V>((const T*)r.p + n * r.sn + head * r.sh, c, g.D, v);
-    if (w) {
-      float ss = 0.f, wv[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss), wv[e] = 0.f;
-      if (in) load_part<WHOLE, V>(w, c, g.D, wv);
-      const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = v[e] * inv * wv[e];
+    for (int b = 0; b < kBatch; ++b) {
+      raw[b] = Pack<T, V>{};
+      if (h + b < h1 && in) {
+        const Row w = row_of(g, h + b);
+        const HeadRows& r = w.key ? k : q;
+        raw[b] = fetch_part<WHOLE, V>((const T*)r.p + n * r.sn + w.head * r.sh, c, g.D);
+      }
     }
-    turn<V>(v, co, si, 1.f);
-    if (in) store_part<WHOLE, V>((key ? yk + (n * g.Hk + head) * g.D : yq + (n * g.H + head) * g.D), c, g.D, v);
+    if (h == h0) angles<V>(g, n, c, co, si);                // while the rows are on their way
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (h + b >= h1) break;
+      const Row w = row_of(g, h + b);
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = (float)raw[b].e[e];
+      if (wq) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss);
+        const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = v[e] * inv * (w.key ? wv[1][e] : wv[0][e]);
+      }
+      turn<V>(v, co, si, 1.f);
+      if (in) store_part<WHOLE, V>((w.key ? yk + (n * g.Hk + w.head) * g.D : yq + (n * g.H + w.head) * g.D), c, g.D, v);
+    }
   }
 }
 
 // part (gridDim.x, 2, D): the workgroup's share of the weights' gradients, its rows added in a fixed order.  A null gradient
-// stands for zeros.
+// stands for zeros.  Workgroup b takes the heads' item b % blocks_of of tokens far apart.
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, HeadRows k, const float* __restrict__ wq,
                                                         const float* __restrict__ wk, HeadRows gq, HeadRows gk,
@@ -137,48 +182,42 @@ __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, He
   for (int e = 0; e < V; ++e) wv[0][e] = wv[1][e] = gw[0][e] = gw[1][e] = 0.f;
   if (in && wq) load_part<WHOLE, V>(wq, c, g.D, wv[0]);
   if (in && wk) load_part<WHOLE, V>(wk, c, g.D, wv[1]);
-  const int64_t items = g.N * g.blocks_of, step = (int64_t)gridDim.x * (kBlock >> g.cl2);
-  for (int64_t item = (int64_t)blockIdx.x * (kBlock >> g.cl2) + group; item < items; item += step) {
-    const int64_t n = item / g.blocks_of;
-    const int h0 = (int)(item - n * g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
+  const int64_t step = (int64_t)(gridDim.x / g.blocks_of) * (kBlock >> g.cl2);
+  const int h0 = (int)(blockIdx.x % g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
+  for (int64_t n = (int64_t)(blockIdx.x / g.blocks_of) * (kBlock >> g.cl2) + group; n < g.N; n += step) {
     float co[V / 2], si[V / 2];
-    angles<V>(g, n, c, co, si);
-    auto row = [&](int h, auto which) {
-      constexpr int K = decltype(which)::value;
-      const HeadRows &r = K ? k : q, &gr = K ? gk : gq;
-      const int head = K ? h - g.H : h;
-      const float* w = K ? wk : wq;
-      T* out = K ? dk : dq;
+    for (int h = h0; h < h1; ++h) {
+      const Row w = row_of(g, h);
+      const HeadRows &r = w.key ? k : q, &gr = w.key ? gk : gq;
+      Pack<T, V> xs{}, ys{};
+      if (in && gr.p) ys = fetch_part<WHOLE, V>((const T*)gr.p + n * gr.sn + w.head * gr.sh, c, g.D);
+      if (in && wq) xs = fetch_part<WHOLE, V>((const T*)r.p + n * r.sn + w.head * r.sh, c, g.D);
+      if (h == h0) angles<V>(g, n, c, co, si);              // while the rows are on their way
       float y[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = 0.f;
-      if (in && gr.p) load_part<WHOLE, V>((const T*)gr.p + n * gr.sn + head * gr.sh, c, g.D, y);
-      if (w) {
+      for (int e = 0; e < V; ++e) y[e] = (float)ys.e[e];
+      turn<V>(y, co, si, -1.f);
+      if (wq) {
         float x[V], ss = 0.f, dot = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = 0.f;
-        if (in) load_part<WHOLE, V>((const T*)r.p + n * r.sn + head * r.sh, c, g.D, x);
-        turn<V>(y, co, si, -1.f);
-#pragma unroll
         for (int e = 0; e < V; ++e) {
+          x[e] = (float)xs.e[e];
           ss = fmaf(x[e], x[e], ss);
-          dot = fmaf(wv[K][e] * y[e], x[e], dot);
+          dot = fmaf((w.key ? wv[1][e] : wv[0][e]) * y[e], x[e], dot);
         }
         const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
         const float mean = lanes_sum(dot, g.cl2) * inv * g.inv_d;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float hat = x[e] * inv;
-          gw[K][e] = fmaf(y[e], hat, gw[K][e]);
-          y[e] = inv * fmaf(wv[K][e], y[e], -hat * mean);
+          const float hat = x[e] * inv, part_of = y[e] * hat;
+          y[e] = inv * fmaf(w.key ? wv[1][e] : wv[0][e], y[e], -hat * mean);
+          gw[0][e] += w.key ? 0.f : part_of;
+          gw[1][e] += w.key ? part_of : 0.f;
         }
-      } else {
-        turn<V>(y, co, si, -1.f);
       }
-      if (in && out) store_part<WHOLE, V>(out + (n * (K ? g.Hk : g.H) + head) * g.D, c, g.D, y);
-    };
-    for (int h = h0; h < min(h1, g.H); ++h) row(h, std::integral_constant<int, 0>{});
-    for (int h = max(h0, g.H); h < h1; ++h) row(h, std::integral_constant<int, 1>{});
+      T* out = w.key ? dk : dq;
+      if (in && out) store_part<WHOLE, V>(out + (n * (w.key ? g.Hk : g.H) + w.head) * g.D, c, g.D, y);
+    }
   }
   if (!part) return;
 #pragma unroll
@@ -196,7 +235,7 @@ __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, He
 }
 
 // ------------------------------------------------------------------------------------------- host
-constexpr int64_t kRotBlocks = 2048;
+constexpr int64_t kRotBlocks = 2048;   // shares of the weights' gradients
 
 bool rot_ok(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t A, const int64_t* sections, double eps) {
   if (!dtype_ok(dtype) || N < 0 || N >= ((int64_t)1 << 40) || H < 1 || Hk < 1 || H > 65536 || Hk > 65536 || D < 1 ||
@@ -220,10 +259,13 @@ RotGeo rot_geo(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, const voi
   for (int a = 0; a < (int)A; ++a) g.bound[a] = g.pairs += (int)sections[a];
   const int64_t units = (D * dtype_size(dtype) + 15) / 16;
   while ((1 << g.cl2) < units) ++g.cl2;
-  // Heads that share a token's angles: all up to eight, fewer where that leaves the card without work.
-  g.per = (int)std::min<int64_t>(H + Hk, 8);
-  while (g.per > 1 && N * ((H + Hk + g.per - 1) / g.per) << g.cl2 < 256 * 1024) g.per = (g.per + 1) / 2;
-  g.blocks_of = (int)((H + Hk + g.per - 1) / g.per);
+  // Heads that share a token's angles: all up to 16, in even parts (100k tokens of 8 + 2 heads of 128: 114 us with ten, 155
+  // with eight and two), fewer where that leaves the card without work.
+  const int64_t heads = H + Hk;
+  g.blocks_of = (int)((heads + 15) / 16);
+  while (g.blocks_of < heads && N * g.blocks_of << g.cl2 < 256 * 1024) g.blocks_of = (int)std::min<int64_t>(2 * g.blocks_of, heads);
+  g.per = (int)((heads + g.blocks_of - 1) / g.blocks_of);
+  g.blocks_of = (int)((heads + g.per - 1) / g.per);
   return g;
 }
 
@@ -259,7 +301,7 @@ int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void
   if (!q || !k || !yq || !yk || (g.pairs && (!pos || !freqs))) { set_error("head_norm_rotary_fwd: null argument"); return 1; }
   const bool whole = rot_whole(dtype, D, sqn | sqh | skn | skh, {q, k, wq, wk, yq, yk});
   const HeadRows rq{q, sqn, sqh}, rk{k, skn, skh};
-  const int64_t blocks = (N * g.blocks_of + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2);
+  const int64_t blocks = (N + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2) * g.blocks_of;
   by_type(dtype, [&](auto t) {
     using T = decltype(t);
     in_launches(blocks, [&](int64_t first, unsigned count) {
@@ -272,7 +314,10 @@ int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void
   return check_launch("head_norm_rotary_fwd");
 }
 
-int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t D) { return D < 1 || D > kMaxHeadWidth ? -1 : kRotBlocks * 2 * D * 4; }
+int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t H, int64_t Hk, int64_t D) {
+  if (H < 1 || Hk < 1 || H > 65536 || Hk > 65536 || D < 1 || D > kMaxHeadWidth) return -1;
+  return std::max(kRotBlocks, H + Hk) * 2 * D * 4;
+}
 
 int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
                              const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
@@ -282,11 +327,12 @@ int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void
   if (!rot_ok(dtype, N, H, Hk, D, A, sections, eps) || (N > 0 && (sqn < 0 || sqh < 0 || skn < 0 || skh < 0 || sgqn < 0 || sgqh < 0 || sgkn < 0 || sgkh < 0))) { set_error("head_norm_rotary_bwd: bad sizes or settings N=%lld H=%lld, %lld D=%lld axes=%lld type %d eps=%g", (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)A, dtype, eps); return 1; }
   const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, pos64, freqs, A, sections, eps);
   if ((N > 0 && ((wq && !q) || (wk && !k) || (g.pairs && (!pos || !freqs)))) || (gw && !ws)) { set_error("head_norm_rotary_bwd: null argument"); return 1; }
-  if (gw && ws_bytes < atl_head_norm_rotary_bwd_ws_bytes(D)) { set_error("head_norm_rotary_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_head_norm_rotary_bwd_ws_bytes(D)); return 1; }
+  if (gw && ws_bytes < atl_head_norm_rotary_bwd_ws_bytes(H, Hk, D)) { set_error("head_norm_rotary_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_head_norm_rotary_bwd_ws_bytes(H, Hk, D)); return 1; }
   const bool whole = rot_whole(dtype, D, (wq ? sqn | sqh : 0) | (wk ? skn | skh : 0) | (gyq ? sgqn | sgqh : 0) | (gyk ? sgkn | sgkh : 0),
                                {wq ? q : nullptr, wk ? k : nullptr, wq, wk, gyq, gyk, gq, gk});
   const HeadRows rq{q, sqn, sqh}, rk{k, skn, skh}, rgq{gyq, sgqn, sgqh}, rgk{gyk, sgkn, sgkh};
-  const int nblk = (int)std::min<int64_t>((N * g.blocks_of + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2), kRotBlocks);
+  const int64_t each = std::max<int64_t>(kRotBlocks / g.blocks_of, 1);
+  const int nblk = (int)std::min<int64_t>((N + (kBlock >> g.cl2) - 1) / (kBlock >> g.cl2), each) * g.blocks_of;
   if (nblk > 0)
     by_type(dtype, [&](auto t) {
       using T = decltype(t);

@@ -140,10 +140,9 @@ _SIGS = {
     "atl_head_norm_rotary_fwd": [_P, _I, _I, _P, _I, _I, _C, _P, _P, _P, _C, _P, _I, _P, _I, _I, _I, _I, _D, _P, _P, _P],
     "atl_head_norm_rotary_bwd": [_P, _I, _I, _P, _I, _I, _C, _P, _P, _P, _C, _P, _I, _P, _I, _I, _I, _I, _D, _P, _I, _I, _P, _I, _I,
                                  _P, _P, _P, _P, _I, _P],
-    "atl_head_norm_rotary_bwd_ws_bytes": [_I],
-    "atl_decay_attn_states": [_I, _I, _I, _I],
-    "atl_decay_attn_ws_bytes": [_I, _I, _I, _I, _C],
-    "atl_decay_attn_fwd": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _I, _P, _P, _D, _P, _P, _P, _P, _I, _P],
+    "atl_head_norm_rotary_bwd_ws_bytes": [_I, _I, _I],
+    "atl_decay_attn_states_bytes": [_I, _I, _I, _I],
+    "atl_decay_attn_fwd": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _I, _P, _P, _D, _P, _P, _P, _I, _P],
     "atl_decay_attn_bwd": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _I, _P, _P, _P, _D, _P, _P, _P, _P,
                            _P, _P, _I, _P],
     "atl_decay_attn_step": [_P, _I, _I, _P, _I, _I, _P, _I, _I, _C, _I, _I, _I, _P, _P, _D, _P, _P, _P],
@@ -157,7 +156,7 @@ _RESTYPE = {"atl_scan_work_size": ctypes.c_int64, "atl_grid_plan_bytes": ctypes.
             "atl_image_variance_ws_bytes": ctypes.c_int64, "atl_embed_bwd_ws_bytes": ctypes.c_int64,
             "atl_rms_norm_bwd_ws_bytes": ctypes.c_int64, "atl_gated_scan_groups": ctypes.c_int64,
             "atl_gated_scan_ws_bytes": ctypes.c_int64, "atl_head_norm_rotary_bwd_ws_bytes": ctypes.c_int64,
-            "atl_decay_attn_states": ctypes.c_int64, "atl_decay_attn_ws_bytes": ctypes.c_int64,
+            "atl_decay_attn_states_bytes": ctypes.c_int64,
 "atl_last_error": ctypes.c_char_p, "atl_abi_version": ctypes.c_int}
 
 class FastGeometry(ctypes.Structure):

@@ -97,7 +97,7 @@ class _Rotary(torch.autograd.Function):
         gq = torch.empty(N, H, D, dtype=dtype, device=dev) if want[0] and gyq is not None else None
         gk = torch.empty(N, Hk, D, dtype=dtype, device=dev) if want[1] and gyk is not None else None
         gw = torch.empty(2, D, dtype=F32, device=dev) if want[2] or want[3] else None
-        nbytes = int(load_library().atl_head_norm_rotary_bwd_ws_bytes(D)) if gw is not None else 0
+        nbytes = int(load_library().atl_head_norm_rotary_bwd_ws_bytes(H, Hk, D)) if gw is not None else 0
         ws = _ws(nbytes, dev, "head_norm_rotary") if gw is not None else None
         with on_device(dev):
             call("atl_head_norm_rotary_bwd", *_strides(q), *_strides(k), _CODE[dtype], _at(wq), _at(wk), _at(pos),
@@ -164,16 +164,13 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | 
 def _decay_fwd(q, k, v, rate, start, dt, h0, scale):
     N, H, D = q.shape
     B, dev = start.numel() - 1, q.device
-    lib = load_library()
     y = torch.empty(N, H, D, dtype=q.dtype, device=dev)
     last = torch.empty(B, H, D, D, dtype=F32, device=dev)
-    held = int(lib.atl_decay_attn_states(N, B, H, D))
-    nbytes = int(lib.atl_decay_attn_ws_bytes(N, B, H, D, 0))
-    ws = _ws(nbytes, dev, "decay_attention")
-    states = torch.empty(held, dtype=F32, device=dev) if held else None
+    nbytes = int(load_library().atl_decay_attn_states_bytes(N, B, H, D))
+    states = _ws(nbytes, dev, "decay_attention") if nbytes else None
     with on_device(dev):
         call("atl_decay_attn_fwd", *_strides(q), *_strides(k), *_strides(v), _CODE[q.dtype], N, H, D, _at(rate), _at(start), B,
-             _at(dt), _at(h0), scale, _at(y), _at(last), _at(states), _at(ws), nbytes, raw_stream(dev))
+             _at(dt), _at(h0), scale, _at(y), _at(last), _at(states), nbytes, raw_stream(dev))
     return y, last, states
 
 
@@ -198,8 +195,8 @@ class _Decay(torch.autograd.Function):
         glast = None if glast is None else glast.contiguous()
         gq, gk, gv = (torch.empty(N, H, D, dtype=q.dtype, device=dev) for _ in range(3))
         gh0 = torch.empty(B, H, D, D, dtype=F32, device=dev) if ctx.needs_input_grad[6] else None
-        nbytes = int(load_library().atl_decay_attn_ws_bytes(N, B, H, D, 1))
-        ws = _ws(nbytes, dev, "decay_attention")
+        nbytes = 0 if states is None else states.numel()
+        ws = None if states is None else torch.empty_like(states)
         with on_device(dev):
             call("atl_decay_attn_bwd", *_strides(q), *_strides(k), *_strides(v), *_strides(gy), _CODE[q.dtype], N, H, D,
                  _at(rate), _at(start), B, _at(dt), _at(h0), _at(glast), ctx.scale, _at(states), _at(gq), _at(gk), _at(gv),
