@@ -157,13 +157,12 @@ __device__ __forceinline__ float top_of_four(float top) {
 
 // A state's factor e^{-z}: for small z by what it is less than one (else that would lose the factor's own bits).
 struct Fade {
-  float a;
-  int keep;
-  __device__ __forceinline__ float operator()(float m) const { return fmaf(m, a, keep ? m : 0.f); }
+  float a, keep;                           // m e^{-z} + u = m a + (m keep + u), keep 0 or 1
+  __device__ __forceinline__ float operator()(float m, float u) const { return fmaf(m, a, fmaf(m, keep, u)); }
 };
 __device__ __forceinline__ Fade fade_of(float z) {
   const bool keep = !(z > 0.5f);
-  return Fade{keep ? expm1f(-z) : expf(-z), keep};
+  return Fade{keep ? expm1f(-z) : expf(-z), keep ? 1.f : 0.f};
 }
 
 // A stretch's exponent (of two) and factor.
@@ -297,6 +296,9 @@ __device__ __forceinline__ uint32_t row_offset(int r, int stride, int len) {
   return (uint32_t)((REV ? len - 1 - r : r) * stride);
 }
 
+// How rows lie: in pieces of 16 bytes, in words of 32 bits (16 bytes at least), or anyhow.
+constexpr int kLoose = 0, kWords = 1, kWhole = 2;
+
 // Pieces of 16 bytes of a chunk's rows, in registers until the chunk's turn.
 template <typename T, int DP, int THREADS>
 struct Stage {
@@ -305,14 +307,14 @@ struct Stage {
   Pack<T, V> v[COUNT];
 
   // Row r of the chunk is token at + r (or at - r where REV); len rows are there, the others zero.
-  template <bool REV, bool WHOLE>
+  template <bool REV, int LAY>
   __device__ __forceinline__ void load(const Rows& rows, int64_t head, int64_t at, int len, int D) {
     const T* row0 = (const T*)rows.p + head * rows.sh + at * rows.sn;
     const int r0 = threadIdx.x / PER, c = threadIdx.x % PER * V;
-    if constexpr (WHOLE) {
+    if constexpr (LAY != kLoose) {                                  // a row's last piece ends with the row, and is moved up when it is stored
       const int stride = (int)rows.sn * (int)sizeof(T);
       const auto buf = chunk_buffer<REV>(row0, stride, len, D * (int)sizeof(T));
-      const uint32_t off = row_offset<REV>(r0, stride, len) + (c < D ? c * (uint32_t)sizeof(T) : kNoChannel);
+      const uint32_t off = row_offset<REV>(r0, stride, len) + (c < D ? (LAY == kWords ? min(c, D - V) : c) * (uint32_t)sizeof(T) : kNoChannel);
 #pragma unroll
       for (int n = 0; n < COUNT; ++n) {
         const U4v w = __builtin_amdgcn_raw_buffer_load_b128(buf, off + (uint32_t)((REV ? -n : n) * STEP * stride), 0, 0);
@@ -339,20 +341,43 @@ struct Stage {
       }
     }
   }
-  // Whether some of the lane's elements are not finite (the exponent's bits are all ones).
+  // Whether some of the lane's elements are not finite: magnitudes, as whole numbers, from the infinity's on.
   __device__ __forceinline__ bool odd() const {
-    constexpr uint32_t kExp = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, f16_t>::value ? 0x7C007C00u : 0x7F807F80u;
-    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, f16_t>::value ? 0x04000400u : 0x00800080u;
-    uint32_t any = 0;
+    if constexpr (sizeof(T) == 2) {
+      using H2 = uint16_t __attribute__((ext_vector_type(2)));
+      H2 top = {0, 0};
 #pragma unroll
-    for (int n = 0; n < COUNT; ++n) {
-      const U4v w = *reinterpret_cast<const U4v*>(&v[n]);
+      for (int n = 0; n < COUNT; ++n) {
+        const U4v w = *reinterpret_cast<const U4v*>(&v[n]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) any |= (w[k] & kExp) + kOne;
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t m = w[k] & 0x7FFF7FFFu;
+          top = __builtin_elementwise_max(top, *reinterpret_cast<const H2*>(&m));
+        }
+      }
+      return max(top[0], top[1]) >= (std::is_same<T, f16_t>::value ? 0x7C00 : 0x7F80);
+    } else {
+      uint32_t top = 0;
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n)
+#pragma unroll
+        for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(v[n].e[k]) & 0x7FFFFFFFu);
+      return top >= 0x7F800000u;
     }
-    return any & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
   }
-  __device__ __forceinline__ void store(T* tile) const {
+  template <int LAY>
+  __device__ __forceinline__ void store(T* tile, int D) {
+    if constexpr (LAY == kWords) {
+      const int c = threadIdx.x % PER * V, by = (V - D % V) * (int)sizeof(T) / 4;
+      const bool last = c < D && c + V > D;
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n) {
+        U4v w = *reinterpret_cast<U4v*>(&v[n]);
+        if (by & 1) w = last ? U4v{w[1], w[2], w[3], 0} : w;
+        if (by & 2) w = last ? U4v{w[2], w[3], 0, 0} : w;
+        v[n] = *reinterpret_cast<Pack<T, V>*>(&w);
+      }
+    }
     T* to = tile + threadIdx.x / PER * tile_ld<T, DP>() + threadIdx.x % PER * V;
 #pragma unroll
     for (int n = 0; n < COUNT; ++n) *reinterpret_cast<Pack<T, V>*>(to + n * STEP * tile_ld<T, DP>()) = v[n];
@@ -402,10 +427,7 @@ __device__ __forceinline__ void add_chunk(const Decays& s, const T* y, F4 (&M)[C
 #pragma unroll
       for (int n = 0; n < NS; ++n) u = mma(a, b[ct][n], u);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float m = fade(M[ct][dt][r]);
-        M[ct][dt][r] = HALF ? fmaf(u[r], down[ct], m) : m + u[r];
-      }
+      for (int r = 0; r < 4; ++r) M[ct][dt][r] = fade(M[ct][dt][r], HALF ? u[r] * down[ct] : u[r]);
     }
   }
 }
@@ -455,7 +477,7 @@ __device__ __forceinline__ void add_state(const float* p, bool flip, int D, int 
       for (int r = 0; r < 4; ++r) {
         const int y = y0 + dt / 2 * 32 + (dt & 1) * 4 + r;
         const uint32_t off = y < D && w < D ? (uint32_t)(y * sy + w * sw) * 4 : kNoChannel;
-        M[ct][dt][r] = fade(M[ct][dt][r]) + __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, off, 0, 0));
+        M[ct][dt][r] = fade(M[ct][dt][r], __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, off, 0, 0)));
       }
   }
 }
@@ -506,7 +528,7 @@ constexpr int kTiles = 2;                  // blocks of 16 W channels of a wave
 
 // Goes through a stretch's chunks: chunk(done, len, decays) with its rows and exponents in shared memory.  W_TILES: the tiles
 // that are looked through for values that are not finite.
-template <typename T, int DP, int NT, int W_TILES, int THREADS, bool REV, bool WHOLE, typename Chunk>
+template <typename T, int DP, int NT, int W_TILES, int THREADS, bool REV, int LAY, typename Chunk>
 __device__ __forceinline__ double follow(ChunkLds<T, DP, NT>& s, const DecayGeo& d, const Stretch& st, const Rows (&rows)[NT],
                                          int head, float ps, float xs, float us, Chunk&& chunk) {
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -518,12 +540,12 @@ __device__ __forceinline__ double follow(ChunkLds<T, DP, NT>& s, const DecayGeo&
     if (done >= tokens) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      stage[n].template load<REV, WHOLE>(rows[n], head, REV ? from - done : from + done, min(kChunk, tokens - done), d.D);
+      stage[n].template load<REV, LAY>(rows[n], head, REV ? from - done : from + done, min(kChunk, tokens - done), d.D);
   };
   auto put = [&](int done) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      stage[n].store(s.tile[n]);
+      stage[n].template store<LAY>(s.tile[n], d.D);
       if ((W_TILES >> n & 1) && __any(stage[n].odd()) && lane == 0) s.odd[n] = done + 1;
     }
   };
@@ -559,28 +581,33 @@ __device__ __forceinline__ double follow(ChunkLds<T, DP, NT>& s, const DecayGeo&
   return sum;
 }
 
+// Waves of a job: two at most, so the widest heads' columns are two workgroups' (which share their rows in the cache): a
+// workgroup of as many waves as a compute unit holds would wait for its own barriers.
+template <int DP>
+constexpr int sweep_waves() { return DP / 32 > 2 ? 2 : DP / 32; }
 template <typename T, int DP, int JOBS>
-constexpr int sweep_threads() { return DP / 32 * JOBS * kWave; }
+constexpr int sweep_threads() { return sweep_waves<DP>() * JOBS * kWave; }
 
-template <typename T, int DP, int JOBS, bool REV, bool WHOLE>
-__global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<ChunkLds<T, DP, JOBS + 2>, kSweepWaves>(DP / 32 * JOBS)))
+template <typename T, int DP, int JOBS, bool REV, int LAY>
+__global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<ChunkLds<T, DP, JOBS + 2>, kSweepWaves>(sweep_waves<DP>() * JOBS)))
     k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
-  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, KD = DP / 32, THREADS = sweep_threads<T, DP, JOBS>();
+  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = sweep_waves<DP>(), KD = DP / 32, THREADS = sweep_threads<T, DP, JOBS>();
+  constexpr int PARTS = DT / CT / NW;      // workgroups of a head
   constexpr int NT = JOBS + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   __shared__ ChunkLds<T, DP, NT> s;
-  const int64_t work = near_first(first + blockIdx.x, d.slots * d.H);
-  if (work >= d.slots * d.H) return;
-  const int64_t slot = work / d.H;
-  const int head = (int)(work - slot * d.H);
+  const int64_t work = near_first(first + blockIdx.x, d.slots * d.H * PARTS);
+  if (work >= d.slots * d.H * PARTS) return;
+  const int64_t slot = work / (d.H * PARTS);
+  const int place = (int)(work - slot * (d.H * PARTS)), head = place / PARTS;
   const Stretch st = stretch_of(d, slot);
   if (!st.live) return;
   const int every = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), job = every / NW, wave = every % NW;
   const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i16 = lane & 15;
-  const int c0 = wave * CT * 16;
+  const int c0 = (place % PARTS * NW + wave) * CT * 16;
   T* out = (T*)a.out[job];
   if (st.window < 0 || st.window >= d.B) {                  // tokens of no window
-    for (int64_t t = st.lo + wave; t < st.hi; t += NW)
+    for (int64_t t = st.lo + wave + place % PARTS * NW; t < st.hi; t += NW * PARTS)
       for (int c = lane; c < d.D; c += kWave) out[(t * d.H + head) * d.D + c] = (T)0.f;
     return;
   }
@@ -600,14 +627,14 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
     const int64_t e = (st.entry + dir * k) * d.H + head;
     const bool given = k > past;
     const float* p = given ? a.given + (st.window * d.H + head) * DD : a.carry + e * DD;
-    add_state<DP, CT>(p, flip, d.D, c0, !given && summed ? a.spans[e].fade : Fade{0.f, 1}, M);
+    add_state<DP, CT>(p, flip, d.D, c0, !given && summed ? a.spans[e].fade : Fade{0.f, 1.f}, M);
   }
   Rows rows[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) rows[n] = a.rows[n];
   const int out_stride = d.H * d.D * (int)sizeof(T);
   const int64_t from = REV ? st.hi - 1 : st.lo;
-  follow<T, DP, NT, JOBS == 1 ? 4 : 9, THREADS, REV, WHOLE>(s, d, st, rows, head, a.ps, a.xs, a.us, [&](int done, int len, const Decays& dec) {
+  follow<T, DP, NT, JOBS == 1 ? 4 : 9, THREADS, REV, LAY>(s, d, st, rows, head, a.ps, a.xs, a.us, [&](int done, int len, const Decays& dec) {
     const int wt = JOBS == 1 ? 2 : job ? 0 : 3;
     const T* X = s.tile[JOBS == 1 ? 0 : job ? 2 : 1];
     const T* Y = s.tile[JOBS == 1 ? 1 : job ? 3 : 0];
@@ -723,13 +750,20 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
         float o[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
-        if constexpr (WHOLE) {
-          const uint32_t off = row_offset<REV>(i, out_stride, len) + (c < d.D ? c * (uint32_t)sizeof(T) : kNoChannel);
+        if constexpr (LAY != kLoose) {
+          const uint32_t at_row = row_offset<REV>(i, out_stride, len) + c * (uint32_t)sizeof(T);
+          const uint32_t off = c + 4 <= d.D ? at_row : kNoChannel;
           Pack<T, 4> q;
 #pragma unroll
           for (int r = 0; r < 4; ++r) q.e[r] = (T)o[r];
           if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b64(*reinterpret_cast<const U2v*>(&q), out_buf, off, 0, 0);
           else __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const U4v*>(&q), out_buf, off, 0, 0);
+          if constexpr (LAY == kWords)                      // a row's end, word by word
+#pragma unroll
+            for (int r = 0; r < 4; r += 4 / (int)sizeof(T)) {
+              const uint32_t word = *reinterpret_cast<const uint32_t*>(&q.e[r]);
+              __builtin_amdgcn_raw_buffer_store_b32(word, out_buf, c + 4 > d.D && c + r < d.D ? at_row + r * (uint32_t)sizeof(T) : kNoChannel, 0, 0);
+            }
         } else if (i < len && c < d.D) {
           store_loose<4>(to + (int64_t)(REV ? -i : i) * d.H * d.D + c, d.D - c, o);
         }
@@ -767,7 +801,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
 
 // A stretch's own sum from nothing (all but the last of a window, in the sweep's direction): carry (entries, H, D, D), and
 // its exponent and factor (entries, H).
-template <typename T, int DP, bool REV, bool WHOLE>
+template <typename T, int DP, bool REV, int LAY>
 __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>, kSweepWaves>(DP / 32)))
     k_decay_local(DecayGeo d, Rows y, Rows w, float us, float* __restrict__ carry, Span* __restrict__ spans, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, THREADS = NW * kWave;
@@ -785,7 +819,7 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>,
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
   const Rows rows[2] = {y, w};
-  const double sum = follow<T, DP, 2, 2, THREADS, REV, WHOLE>(s, d, st, rows, head, 1.f, 1.f, us, [&](int done, int, const Decays& dec) {
+  const double sum = follow<T, DP, 2, 2, THREADS, REV, LAY>(s, d, st, rows, head, 1.f, 1.f, us, [&](int done, int, const Decays& dec) {
     Frag<T> wf[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(s.tile[1], c0 + ct * 16);
@@ -799,10 +833,10 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>,
 }
 
 // The states after the stretches of every window of more than kFew stretches (all but the last) from the stretches' own sums, in
-// place; a sweep adds up fewer sums by itself.  A workgroup has EL elements of the state and cuts the stretches into runs: every
-// run's own sum, those joined, every run again from its begin (which the cache still holds).  A window is found by the first
-// multiple of kFew L in it, or with fewer windows than multiples by its number.
-constexpr int kAhead = 8;
+// place; a sweep adds up fewer sums by itself.  Up to kMany stretches a thread follows an element.  Past that a workgroup has EL
+// elements and cuts the stretches into runs: every run's own sum, those joined, every run again from its begin (which the cache
+// still holds).  A window is found by the first multiple of kFew L in it, or with fewer windows than multiples by its number.
+constexpr int kAhead = 8, kMany = 64;
 struct Join {
   float* p;                                // the element's sum of the first stretch in the sweep's direction
   const Span* z;
@@ -823,7 +857,7 @@ __device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1,
 #pragma unroll
     for (int m = 0; m < kAhead; ++m) {
       if (k + m >= k1) break;
-      state = f[m](state) + u[m];
+      state = f[m](state, u[m]);
       if (WRITE && j.in) j.p[(k + m) * j.step] = state;
     }
   }
@@ -853,6 +887,14 @@ __global__ void __launch_bounds__(1024) k_decay_join(DecayGeo d, const float* __
   j.z = spans + at * d.H + head;
   j.step = (REV ? -1 : 1) * d.H * DD;
   j.zstep = (REV ? -1 : 1) * d.H;
+  if (j.n < kMany) {
+    j.in = true;
+    for (int64_t el = (block - bh * parts) * 1024 + threadIdx.x; el < DD; el += (int64_t)parts * 1024) {
+      j.p = carry + (at * d.H + head) * DD + el;
+      join_run<true>(j, 0, j.n, given ? given[(b * d.H + head) * DD + el] : 0.f);
+    }
+    return;
+  }
   const int64_t len = (j.n + RUNS - 1) / RUNS, k0 = min(run * len, j.n), k1 = min(k0 + len, j.n);
   if (threadIdx.x < RUNS) {
     double total = 0;
@@ -866,7 +908,7 @@ __global__ void __launch_bounds__(1024) k_decay_join(DecayGeo d, const float* __
     end[run][e] = join_run<false>(j, k0, k1, 0.f);
     __syncthreads();
     float state = given && j.in ? given[(b * d.H + head) * DD + el] : 0.f;
-    for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state) + end[r][e];
+    for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state, end[r][e]);
     join_run<true>(j, k0, k1, state);
   }
 }
@@ -901,7 +943,7 @@ __global__ void __launch_bounds__(kBlock) k_decay_step(Rows q, Rows k, Rows v, c
       const float kr = (float)kp[r], qr = (float)qp[r];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        m[e] = fmaf(kr, vv[e], fade(m[e]));
+        m[e] = fade(m[e], kr * vv[e]);
         acc[e] = fmaf(qr, m[e], acc[e]);
       }
       store_f<V>(M + r * D + c, m);
@@ -923,35 +965,42 @@ void by_head(int64_t D, F&& f) {
   else f(std::integral_constant<int, 128>{});
 }
 
+// How rows lie.  Words and pieces are read and written as buffers, loose rows element by element at their ends (251k tokens
+// of 3 x 45 in single precision forward + backward: 2079 us loose, 1223 as words; 1107 us of 3 x 48 as pieces).
 template <typename T>
-bool rows_whole(const Rows& r, int64_t D) {
-  const int v = 16 / (int)sizeof(T);
-  return D % v == 0 && r.sn % v == 0 && r.sh % v == 0 && aligned_to(r.p, 16);
+int layout(const Rows& r, int64_t D) {
+  const int64_t all = (D | r.sn | r.sh) * (int64_t)sizeof(T) | (int64_t)(uintptr_t)r.p;
+  return all % 16 == 0 ? kWhole : all % 4 == 0 && D * sizeof(T) >= 16 ? kWords : kLoose;
+}
+template <typename F>
+void by_layout(int lay, F&& f) {
+  if (lay == kWhole) f(std::integral_constant<int, kWhole>{});
+  else if (lay == kWords) f(std::integral_constant<int, kWords>{});
+  else f(std::integral_constant<int, kLoose>{});
 }
 
 template <typename T, bool REV>
 void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const float* given, Span* spans, float* carry,
                 hipStream_t stream) {
   if (d.N <= d.L) return;                                  // every window is one stretch at most
-  const bool whole = rows_whole<T>(y, d.D) && rows_whole<T>(w, d.D);
+  const int lay = std::min(layout<T>(y, d.D), layout<T>(w, d.D));
   by_head(d.D, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
-      if (whole)
-        hipLaunchKernelGGL((k_decay_local<T, DP, REV, true>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
-                           spans, first);
-      else
-        hipLaunchKernelGGL((k_decay_local<T, DP, REV, false>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us, carry,
-                           spans, first);
-    }, DP / 32 * kWave);
+    by_layout(lay, [&](auto l) {
+      in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
+        hipLaunchKernelGGL((k_decay_local<T, DP, REV, decltype(l)::value>), dim3(count), dim3(DP / 32 * kWave), 0, stream, d, y, w, us,
+                           carry, spans, first);
+      }, DP / 32 * kWave);
+    });
   });
   if (d.N <= kFew * d.L) return;                           // no window has more than kFew stretches
   const int64_t DD = (int64_t)d.D * d.D, places = d.N / (kFew * d.L) + 1;
   const int by_place = places < d.B;
-  auto go = [&](auto el) {                                 // (most places find no window to join: few workgroups for each)
+  const int64_t of = (by_place ? places : d.B) * d.H;
+  auto go = [&](auto el) {                                 // (many find no window to join: as few workgroups as fill the card)
     constexpr int EL = decltype(el)::value;
-    const int parts = (int)std::min<int64_t>((DD + EL - 1) / EL, by_place ? 8 : DD);
-    in_launches((by_place ? places : d.B) * d.H * parts, [&](int64_t first, unsigned count) {
+    const int parts = (int)std::min<int64_t>((DD + EL - 1) / EL, std::max<int64_t>(1024 / of, 1));
+    in_launches(of * parts, [&](int64_t first, unsigned count) {
       hipLaunchKernelGGL((k_decay_join<REV, EL>), dim3(count), dim3(1024), 0, stream, d, given, carry, spans, by_place, parts, first);
     }, 1024);
   };
@@ -961,17 +1010,16 @@ void run_states(const DecayGeo& d, const Rows& y, const Rows& w, float us, const
 
 template <typename T, int JOBS, bool REV>
 void run_sweep(const DecayGeo& d, const Sweep& a, hipStream_t stream) {
-  bool whole = true;
-  for (int n = 0; n < (JOBS == 1 ? 3 : 4); ++n) whole = whole && rows_whole<T>(a.rows[n], d.D);
-  for (int n = 0; n < JOBS; ++n) whole = whole && aligned_to(a.out[n], 16);
+  int lay = kWhole;
+  for (int n = 0; n < JOBS + 2; ++n) lay = std::min(lay, layout<T>(a.rows[n], d.D));
+  for (int n = 0; n < JOBS; ++n) lay = std::min(lay, layout<T>(Rows{a.out[n], d.D, d.D}, d.D));
   by_head(d.D, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    in_launches((d.slots * d.H + 7) / 8 * 8, [&](int64_t first, unsigned count) {
-      if (whole)
-        hipLaunchKernelGGL((k_decay_sweep<T, DP, JOBS, REV, true>), dim3(count), dim3(DP / 32 * JOBS * kWave), 0, stream, d, a, first);
-      else
-        hipLaunchKernelGGL((k_decay_sweep<T, DP, JOBS, REV, false>), dim3(count), dim3(DP / 32 * JOBS * kWave), 0, stream, d, a, first);
-    }, DP / 32 * JOBS * kWave);
+    constexpr int DP = decltype(dp)::value, THREADS = sweep_threads<T, DP, JOBS>();
+    by_layout(lay, [&](auto l) {
+      in_launches((d.slots * d.H * (DP / 32 / sweep_waves<DP>()) + 7) / 8 * 8, [&](int64_t first, unsigned count) {
+        hipLaunchKernelGGL((k_decay_sweep<T, DP, JOBS, REV, decltype(l)::value>), dim3(count), dim3(THREADS), 0, stream, d, a, first);
+      }, THREADS);
+    });
   });
 }
 
