@@ -132,6 +132,15 @@ class EventRecurrence(nn.Module):
             out.append(((w * (FP8_MAX / top)).to(torch.float8_e4m3fn), (top / FP8_MAX).t().contiguous()))
         return out
 
+    @staticmethod
+    def _projected(x, residual, weight, into, fp8):
+        """A layer's norm and input projection for one token of every stream, and the sum the norm is of."""
+        if fp8 is None:
+            y, s = residual_rms_norm(x, residual, weight)
+            return nn.functional.linear(y, into.to(y.dtype)), s
+        q, scale, s = residual_rms_norm_fp8(x, residual, weight)
+        return torch._scaled_mm(q, fp8[0].t(), scale_a=scale, scale_b=fp8[1], out_dtype=torch.bfloat16).to(s.dtype), s
+
     @torch.no_grad()
     def step(self, xy: torch.Tensor, p: torch.Tensor, dt: torch.Tensor, states: list, fp8=None) -> list:
         """One event of each of n streams (xy (n, 2), p (n,), dt (n,) gaps in units of tau): the layers' states, updated
@@ -140,13 +149,7 @@ class EventRecurrence(nn.Module):
         s = embed_tokens(self.tokens(xy, p), self.table, scale=math.sqrt(self.dim), dtype=self.dtype)
         x = None
         for k, (w, into) in enumerate(zip(self.norm, self.into)):
-            a, b = (s, None) if x is None else (x, s)
-            if fp8 is not None:
-                q, scale, s = residual_rms_norm_fp8(a, b, w)
-                y = torch._scaled_mm(q, fp8[k][0].t(), scale_a=scale, scale_b=fp8[k][1], out_dtype=torch.bfloat16).to(s.dtype)
-            else:
-                y, s = residual_rms_norm(a, b, w)
-                y = nn.functional.linear(y, into.to(y.dtype))
+            y, s = self._projected(*((s, None) if x is None else (x, s)), w, into, None if fp8 is None else fp8[k])
             x, gate = y.chunk(2, -1)
             h = gated_scan_step(x, gate, states[k], dt=dt)
             if k < len(self.out):
