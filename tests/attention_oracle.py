@@ -2,8 +2,8 @@
 helper, not part of the product.
 
 Every bound counts roundings in units of U = 2^-24 of sums of magnitudes: each fp32 operation behind a value adds half a unit of
-its result, the hardware's exponential a unit or two and its argument one per unit of the exponent.  Where operands are rounded to the
-16-bit type (the pairs' weights once, the states to two pieces), half a unit of that type is counted for them."""
+its result, the hardware's exponential a unit or two and its argument one per unit of the exponent.  Where operands go on as
+two pieces of a 16-bit type (the pairs' weights and the states), what is left behind both is counted for them."""
 import numpy as np
 
 from tests.sequence_oracle import HALF_ULP, U
@@ -12,7 +12,7 @@ from tests.sequence_oracle import HALF_ULP, U
 # neighbour is brought to 2^14 first (2^-25 / 2^14, and as much again).
 PIECES = {"float32": 0.0, "bfloat16": HALF_ULP["bfloat16"] ** 2, "float16": HALF_ULP["float16"] ** 2}
 FLOOR = {"float32": 0.0, "bfloat16": 0.0, "float16": 2.0 ** -38}
-PAIR = {"float32": 0.0, "bfloat16": HALF_ULP["bfloat16"], "float16": HALF_ULP["float16"]}
+PAIR = PIECES                                             # the weights of pairs too go on in two pieces
 FORGOTTEN = 400.0 * np.log(2.0)
 
 
@@ -98,6 +98,23 @@ def attention_bwd(q, k, v, rate, start, dt, h0, scale, gy, glast, dtype):
         o, _, bo, _ = _sweep(r(v), r(gy), r(q), zr, T(glast[b]), scale, 1.0, scale, dtype)
         out[1][s], bound[1][s] = o[::-1], bo[::-1]
     return (*out, g0), (*bound, b0)
+
+
+def follow(x, y, w, z, given, ps, xs, us):
+    """One long window's recurrence token by token, as _sweep's: out and end, and what the same comes to in magnitudes.  With
+    at most EXPONENT in any factor, a factor's own rounding is 1 + EXPONENT units of it."""
+    n, H, D = x.shape
+    out, mag = np.zeros((n, H, D)), np.zeros((n, H, D))
+    own, far = np.zeros((H, D, D)), given.astype(np.float64)
+    own_a, far_a = np.zeros((H, D, D)), np.abs(far)
+    for i in range(n):
+        a = np.exp(-z[i])[:, None, None]
+        new = y[i][:, :, None] * w[i][:, None, :]
+        own, far = a * own + new, a * far
+        own_a, far_a = a * own_a + np.abs(new), a * far_a
+        out[i] = ps * (x[i][:, None, :] @ own)[:, 0] + xs * (x[i][:, None, :] @ far)[:, 0]
+        mag[i] = abs(ps) * (np.abs(x[i])[:, None, :] @ own_a)[:, 0] + abs(xs) * (np.abs(x[i])[:, None, :] @ far_a)[:, 0]
+    return out, us * own + far, mag, abs(us) * own_a + far_a
 
 
 # ------------------------------------------------------------------------------------------- norm and rotation

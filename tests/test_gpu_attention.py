@@ -127,6 +127,58 @@ def test_attention_windows(kind, dtype, D, with_dt):
     _case(1100, 2, D, dtype, kind, with_dt=with_dt, seed=12)
 
 
+@pytest.mark.parametrize("N", [2500, 9000, 20_011])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("among", [False, True])
+def test_attention_of_long_windows(N, dtype, among):
+    """Windows of ten stretches, of 36 and of 79, alone and between many short ones: the states between stretches joined by one
+    thread, and in runs.  Exponents stay below 4, so a factor is off by 5 units of itself."""
+    H, D, scale = 1, 8, 0.5
+    rng = np.random.default_rng(N)
+    short = [3] * 60 if among else []
+    lo = sum(short)
+    start = np.concatenate([[0], np.cumsum(short + [N] + short)]).astype(int)
+    B, T = len(start) - 1, int(start[-1])
+    q, k, v, gy = (_t(a, dtype) for a in rng.normal(size=(4, T, H, D)))
+    h0, gl = (_t(a) for a in rng.normal(size=(2, B, H, D, D)))
+    dt, rate = _t(rng.random(T) * 8 / N), _t([0.9])
+    ins = [a.requires_grad_() for a in (q, k, v, h0)]
+    print(f"long windows N={N} {dtype} among={among}", flush=True)
+    y, last = ops.decay_attention(*ins[:3], rate, torch.tensor(start, device=DEV), dt=dt, h0=h0, scale=scale)
+    grads = torch.autograd.grad((y, last), ins, (gy, gl))
+    s, b = slice(lo, lo + N), len(short)
+    z = (_np(dt)[s] * _np(rate)[0])[:, None]
+    x, key, val, g = (_np(a)[s] for a in (q, k, v, gy))
+    units = (3 * D + 300 + 3 * (N // 32 + 1)) * 5 * O.U + O.PIECES[_name(dtype)]
+    T_ = lambda m: m.transpose(0, 2, 1)
+    out, end, mag, emag = O.follow(x, key, val, z, _np(h0)[b], scale, scale, 1.0)
+    _close(y[s], out, units * mag, "y")
+    _close(last[b], end, units * emag, "last")
+    out, _, mag, _ = O.follow(g, val, key, z, T_(_np(h0)[b]), scale, scale, 1.0)
+    _close(grads[0][s], out, units * mag, "gq")
+    r, zr = lambda a: a[::-1], np.concatenate([np.zeros((1, 1)), z[::-1][:-1]])
+    out, end, mag, emag = O.follow(r(key), r(x), r(g), zr, _np(gl)[b], scale, 1.0, scale)
+    _close(grads[2][s], out[::-1], units * mag[::-1], "gv")
+    f = np.exp(-z[0])[:, None, None]
+    _close(grads[3][b], f * end, units * f * emag, "gh0")
+    out, _, mag, _ = O.follow(r(val), r(g), r(x), zr, T_(_np(gl)[b]), scale, 1.0, scale)
+    _close(grads[1][s], out[::-1], units * mag[::-1], "gk")
+
+
+def test_attention_without_windows_and_of_plain_sums():
+    """No window: zeros.  32-bit starts, and the gradient of a plain sum (a scalar that is expanded)."""
+    q, k, v = (torch.randn(40, 2, 8, device=DEV, requires_grad=True) for _ in range(3))
+    rate = torch.ones(2, device=DEV)
+    y, last = ops.decay_attention(q, k, v, rate, torch.zeros(1, dtype=torch.int64, device=DEV))
+    assert not y.any() and last.shape == (0, 2, 8, 8)
+    assert not any(g.any() for g in torch.autograd.grad(y.sum(), (q, k, v)))
+    start = torch.tensor([0, 15, 40], device=DEV)
+    y, _ = ops.decay_attention(q, k, v, rate, start.int())
+    assert torch.equal(y, ops.decay_attention(q, k, v, rate, start)[0])
+    for a, b in zip(torch.autograd.grad(y.sum(), (q, k, v), retain_graph=True), torch.autograd.grad(y, (q, k, v), torch.ones_like(y))):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("H", [1, 2, 5, 16, 33])
 def test_attention_heads(H):
     _case(600, H, 16, BF16, "ragged", seed=H)

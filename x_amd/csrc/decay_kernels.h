@@ -679,9 +679,9 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
           for (int n = 0; n < NS; ++n) far[it][ct] = mma(sf[ct][n], xf[it], far[it][ct]);
     }
     __builtin_amdgcn_sched_barrier(0);                      // (each part by itself: together they would not fit the registers)
-    // The pairs, as Y X^T: a lane holds four neighbouring j of its i, in the order in which the next product sums them.
-    // Rounded once: as far off as the output's own rounding.
-    Frag<T> pf[2];
+    // The pairs, as Y X^T: a lane holds four neighbouring j of its i, in the order in which the next product sums them.  Their
+    // weights go on in two pieces: rounded to T once, they would be as far off as the output's own rounding.
+    Frag<T> pf[2][NS];
     Fit fp[2] = {{1.f, 1.f}, {1.f, 1.f}};
     F4 acc[3];                                              // blocks (0, 0), (1, 0), (1, 1)
 #pragma unroll
@@ -726,13 +726,14 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[n][r] *= fp[n > 0].up;
       }
+      float p[2][8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        pf[0][r] = (T)v[0][r];
-        pf[0][4 + r] = (T)0.f;
-        pf[1][r] = (T)v[1][r];
-        pf[1][4 + r] = (T)v[2][r];
+        p[0][r] = v[0][r], p[0][4 + r] = 0.f;
+        p[1][r] = v[1][r], p[1][4 + r] = v[2][r];
       }
+#pragma unroll
+      for (int it = 0; it < 2; ++it) split<T, NS>(p[it], pf[it]);
     }
     __builtin_amdgcn_sched_barrier(0);
     add_chunk<T, DP, CT>(dec, Y, M, wf);
@@ -745,7 +746,9 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, JOBS>()), (waves_of<Chun
       const float xe = HALF ? dec.xe[i] * fm.down : dec.xe[i];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const F4 pv = mma(wf[ct], pf[it], F4{0.f, 0.f, 0.f, 0.f});
+        F4 pv = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NS; ++n) pv = mma(wf[ct], pf[it][n], pv);
         const int c = c0 + ct * 16 + g * 4;
         float o[4];
 #pragma unroll
