@@ -186,13 +186,15 @@ __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, He
   const int h0 = (int)(blockIdx.x % g.blocks_of) * g.per, h1 = min(h0 + g.per, g.H + g.Hk);
   for (int64_t n = (int64_t)(blockIdx.x / g.blocks_of) * (kBlock >> g.cl2) + group; n < g.N; n += step) {
     float co[V / 2], si[V / 2];
-    for (int h = h0; h < h1; ++h) {
-      const Row w = row_of(g, h);
-      const HeadRows &r = w.key ? k : q, &gr = w.key ? gk : gq;
+    bool turned = false;
+    auto row = [&](int head, auto which) {
+      constexpr int K = decltype(which)::value;             // a key's row (the weights and their sums without a choice per element)
+      const HeadRows &r = K ? k : q, &gr = K ? gk : gq;
       Pack<T, V> xs{}, ys{};
-      if (in && gr.p) ys = fetch_part<WHOLE, V>((const T*)gr.p + n * gr.sn + w.head * gr.sh, c, g.D);
-      if (in && wq) xs = fetch_part<WHOLE, V>((const T*)r.p + n * r.sn + w.head * r.sh, c, g.D);
-      if (h == h0) angles<V>(g, n, c, co, si);              // while the rows are on their way
+      if (in && gr.p) ys = fetch_part<WHOLE, V>((const T*)gr.p + n * gr.sn + head * gr.sh, c, g.D);
+      if (in && wq) xs = fetch_part<WHOLE, V>((const T*)r.p + n * r.sn + head * r.sh, c, g.D);
+      if (!turned) angles<V>(g, n, c, co, si);              // while the rows are on their way
+      turned = true;
       float y[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) y[e] = (float)ys.e[e];
@@ -203,21 +205,22 @@ __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, He
         for (int e = 0; e < V; ++e) {
           x[e] = (float)xs.e[e];
           ss = fmaf(x[e], x[e], ss);
-          dot = fmaf((w.key ? wv[1][e] : wv[0][e]) * y[e], x[e], dot);
+          dot = fmaf(wv[K][e] * y[e], x[e], dot);
         }
         const float inv = rsqrtf(fmaf(lanes_sum(ss, g.cl2), g.inv_d, g.eps));
         const float mean = lanes_sum(dot, g.cl2) * inv * g.inv_d;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float hat = x[e] * inv, part_of = y[e] * hat;
-          y[e] = inv * fmaf(w.key ? wv[1][e] : wv[0][e], y[e], -hat * mean);
-          gw[0][e] += w.key ? 0.f : part_of;
-          gw[1][e] += w.key ? part_of : 0.f;
+          const float hat = x[e] * inv;
+          gw[K][e] = fmaf(y[e], hat, gw[K][e]);
+          y[e] = inv * fmaf(wv[K][e], y[e], -hat * mean);
         }
       }
-      T* out = w.key ? dk : dq;
-      if (in && out) store_part<WHOLE, V>(out + (n * (w.key ? g.Hk : g.H) + w.head) * g.D, c, g.D, y);
-    }
+      T* out = K ? dk : dq;
+      if (in && out) store_part<WHOLE, V>(out + (n * (K ? g.Hk : g.H) + head) * g.D, c, g.D, y);
+    };
+    for (int h = h0; h < min(h1, g.H); ++h) row(h, std::integral_constant<int, 0>{});
+    for (int h = max(h0, g.H); h < h1; ++h) row(h - g.H, std::integral_constant<int, 1>{});
   }
   if (!part) return;
 #pragma unroll
