@@ -10,8 +10,8 @@ namespace {
 constexpr int kMaxHead = 128;
 constexpr int64_t kMaxStride = (int64_t)1 << 22;
 
-// Tokens of a stretch: the stretches of all heads, and half a stretch for every window's last, are 1536 workgroups (768 and
-// 3072 were up to 20% slower, by the width), whole pairs of chunks, four pairs at least.
+// Tokens of a stretch: the stretches of all heads, and half a stretch for every window's last, are 1536 workgroups, six a
+// compute unit (half and twice as many were up to 20% slower, by the width), whole pairs of chunks, four pairs at least.
 int64_t stretch_len(int64_t N, int64_t B, int64_t H) {
   constexpr int64_t kGroups = 1536, kPair = 64;
   const int64_t left = std::max(kGroups - B * H / 2, kGroups / 2);

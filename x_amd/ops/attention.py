@@ -247,8 +247,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: tor
     views; their gradients come out per head and autograd adds them.  An endless gap forgets what was before it (with a
     positive rate), a negative one grows the state as the formula has it.  No gradient flows to rate and dt.
 
-    Products of 16-bit inputs run on the matrix cores: the pairs' weights are rounded to that type once, states to 16 bits of
-    mantissa where they meet a query, and states are kept and returned in single precision."""
+    Products run on the matrix cores.  With 16-bit inputs the pairs' weights and the states that meet a query go in as two
+    pieces of that type (16 bits of mantissa), tokens' shares of a state as three; states are kept and returned in single
+    precision."""
     rate, dt, scale = _attn_args(q, k, v, rate, dt, scale)
     N, H, D = q.shape
     _on(start, "start", q.device)
