@@ -132,8 +132,21 @@ def test_attention_windows(kind, dtype, D, with_dt):
 @pytest.mark.parametrize("among", [False, True])
 def test_attention_of_long_windows(N, dtype, among):
     """Windows of ten stretches, of 36 and of 79, alone and between many short ones: the states between stretches joined by one
-    thread, and in runs.  Exponents stay below 4, so a factor is off by 5 units of itself."""
-    H, D, scale = 1, 8, 0.5
+    thread, and in runs."""
+    _long_window(N, 8, dtype, among)
+
+
+@pytest.mark.parametrize("D", [32, 33, 72, 128])
+@pytest.mark.parametrize("N", [1300, 2500])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_attention_of_long_windows_and_wide_heads(N, D, dtype):
+    """Windows of six stretches, whose sums a sweep adds up, and of ten, whose sums are joined."""
+    _long_window(N, D, dtype, True)
+
+
+def _long_window(N, D, dtype, among):
+    """Exponents stay below 4, so a factor is off by 5 units of itself."""
+    H, scale = 1, 0.5
     rng = np.random.default_rng(N)
     short = [3] * 60 if among else []
     lo = sum(short)
@@ -143,7 +156,7 @@ def test_attention_of_long_windows(N, dtype, among):
     h0, gl = (_t(a) for a in rng.normal(size=(2, B, H, D, D)))
     dt, rate = _t(rng.random(T) * 8 / N), _t([0.9])
     ins = [a.requires_grad_() for a in (q, k, v, h0)]
-    print(f"long windows N={N} {dtype} among={among}", flush=True)
+    print(f"long windows N={N} D={D} {dtype} among={among}", flush=True)
     y, last = ops.decay_attention(*ins[:3], rate, torch.tensor(start, device=DEV), dt=dt, h0=h0, scale=scale)
     grads = torch.autograd.grad((y, last), ins, (gy, gl))
     s, b = slice(lo, lo + N), len(short)

@@ -10,11 +10,17 @@ namespace {
 constexpr int kMaxHead = 128;
 constexpr int64_t kMaxStride = (int64_t)1 << 22;
 
-// Tokens of a stretch: the stretches of all heads, and half a stretch for every window's last, are 1536 workgroups, six a
-// compute unit (half and twice as many were up to 20% slower, by the width), whole pairs of chunks, four pairs at least.
-int64_t stretch_len(int64_t N, int64_t B, int64_t H) {
-  constexpr int64_t kGroups = 1536, kPair = 64;
-  const int64_t left = std::max(kGroups - B * H / 2, kGroups / 2);
+// Tokens of a stretch: whole pairs of chunks, four pairs at least.  The stretches of all heads, and half a stretch for every
+// window's last, are whole rounds of workgroups: past 64 channels two rounds of two a compute unit (four waves each, two a
+// SIMD), past 32 two rounds of four, up to 32 one and a half a SIMD, all at once.  In microseconds, forward + backward in
+// bfloat16, by their number:
+//   65k x 8 x 128   512: 1195   768: 942   1024: 951   1536: 1010   2048: 1089
+//   180k x 6 x 64                          1024: 813   1800: 717    2048: 711    2200: 785
+//   1M x 2 x 32                 768: 657   1100: 643   1536: 572    1700: 676    2048: 648
+int64_t stretch_len(int64_t N, int64_t B, int64_t H, int64_t D) {
+  constexpr int64_t kPair = 64;
+  const int64_t groups = D <= 32 ? 1536 : D <= 64 ? 2048 : 1024;
+  const int64_t left = std::max(groups - B * H / 2, groups / 2);
   const int64_t pairs = (N * H / left + kPair - 1) / kPair;
   return kPair * std::min<int64_t>(std::max<int64_t>(pairs, 4), 512);
 }
@@ -29,8 +35,8 @@ bool strides_ok(Rows& r, int64_t N, int64_t D) {
   return r.sh >= 0 && r.sn >= D && r.sn < kMaxStride;
 }
 
-int64_t decay_entries(int64_t N, int64_t B, int64_t H) { return N / stretch_len(N, B, H) + 1; }
-int64_t decay_span_bytes(int64_t N, int64_t B, int64_t H) { return (decay_entries(N, B, H) * H * 16 + 255) / 256 * 256; }
+int64_t decay_entries(int64_t N, int64_t B, int64_t H, int64_t D) { return N / stretch_len(N, B, H, D) + 1; }
+int64_t decay_span_bytes(int64_t N, int64_t B, int64_t H, int64_t D) { return (decay_entries(N, B, H, D) * H * 16 + 255) / 256 * 256; }
 
 template <typename F>
 void by_type(int dtype, F&& f) {
@@ -42,7 +48,7 @@ void by_type(int dtype, F&& f) {
 DecayGeo decay_geo(int64_t N, int64_t B, int64_t H, int64_t D, const int64_t* start, const float* dt, const float* rate) {
   DecayGeo d{};
   d.start = start; d.dt = dt; d.rate = rate;
-  d.N = N; d.B = B; d.L = stretch_len(N, B, H);
+  d.N = N; d.B = B; d.L = stretch_len(N, B, H, D);
   d.slots = N / d.L + B + 2;
   d.H = (int)H; d.D = (int)D;
   return d;
@@ -57,7 +63,7 @@ extern "C" {
 
 int64_t atl_decay_attn_states_bytes(int64_t N, int64_t B, int64_t H, int64_t D) {
   if (!decay_ok(kF32, N, B, H, D)) return -1;
-  return N <= stretch_len(N, B, H) ? 0 : decay_span_bytes(N, B, H) + decay_entries(N, B, H) * H * D * D * 4;
+  return N <= stretch_len(N, B, H, D) ? 0 : decay_span_bytes(N, B, H, D) + decay_entries(N, B, H, D) * H * D * D * 4;
 }
 
 int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
@@ -70,7 +76,7 @@ int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, i
   if (!start || !rate || (N > 0 && (!q || !k || !v || !y)) || (need && !states)) { set_error("decay_attn_fwd: null argument"); return 1; }
   if (states_bytes < need) { set_error("decay_attn_fwd: states of %lld bytes, need %lld", (long long)states_bytes, (long long)need); return 1; }
   const DecayGeo d = decay_geo(N, B, H, D, start, dt, rate);
-  const DecayFwd a{rq, rk, rv, h0, (float)scale, y, last, states, decay_span_bytes(N, B, H)};
+  const DecayFwd a{rq, rk, rv, h0, (float)scale, y, last, states, decay_span_bytes(N, B, H, D)};
   by_type(dtype, [&](auto t) { decay_fwd<decltype(t)>(d, a, stream); });
   return check_launch("decay_attn_fwd");
 }
@@ -86,7 +92,7 @@ int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, i
   if (!start || !rate || (N > 0 && (!q || !k || !v || !gy || !gq || !gk || !gv)) || (need && (!states || !ws))) { set_error("decay_attn_bwd: null argument"); return 1; }
   if (ws_bytes < need) { set_error("decay_attn_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const DecayGeo d = decay_geo(N, B, H, D, start, dt, rate);
-  const DecayBwd a{rq, rk, rv, rg, h0, glast, (float)scale, gq, gk, gv, gh0, states, ws, decay_span_bytes(N, B, H)};
+  const DecayBwd a{rq, rk, rv, rg, h0, glast, (float)scale, gq, gk, gv, gh0, states, ws, decay_span_bytes(N, B, H, D)};
   by_type(dtype, [&](auto t) { decay_bwd<decltype(t)>(d, a, stream); });
   return check_launch("decay_attn_bwd");
 }
