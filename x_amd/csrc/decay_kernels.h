@@ -175,9 +175,9 @@ struct Span {
   double z;
   Fade fade;
 };
-// Stretches of a window up to which a sweep adds up their sums by itself: it reads half of them on average, and the join and
-// its launch (9 us where no window is left for it) are spared.  Windows of more stretches are joined: the sums that a sweep
-// would read grow with their square.
+// Stretches of a window up to which a sweep adds up their sums by itself: it reads half of them on average, and the join is
+// spared.  The sums that the sweeps read grow with the square of a window's stretches: up to 10 instead of 6 took 402 -> 441 us
+// (forward + backward of 60k tokens in 40 windows x 8 x 64), up to 16 took 512; up to 4 changed nothing by more than 2%.
 constexpr int kFew = 6;
 
 // ------------------------------------------------------------------------------------------- windows
@@ -882,6 +882,8 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>,
 // place; a sweep adds up fewer sums by itself.  Up to kMany stretches a thread follows an element.  Past that a workgroup has EL
 // elements and cuts the stretches into runs: every run's own sum, those joined, every run again from its begin (which the cache
 // still holds).  A window is found by the first multiple of kFew L in it, or with fewer windows than multiples by its number.
+// Bound by the states' traffic where there are many (65k tokens x 8 x 128: 27 us for 134 MB; with one workgroup a compute unit
+// instead of two 32), else by the latency of its searches and runs (1M x 2 x 32: 23 us; 11 where no window is to be joined).
 constexpr int kAhead = 8, kMany = 64;
 struct Join {
   float* p;                                // the element's sum of the first stretch in the sweep's direction
@@ -910,7 +912,7 @@ __device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1,
   return state;
 }
 template <bool REV, int EL>
-__global__ void __launch_bounds__(1024) k_decay_join(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
+__global__ void __launch_bounds__(1024, EL == kWave ? 8 : 4) k_decay_join(DecayGeo d, const float* __restrict__ given, float* __restrict__ carry,
                                                      const Span* __restrict__ spans, int by_place, int parts, int64_t first) {
   constexpr int RUNS = 1024 / EL;
   __shared__ float end[RUNS][EL];
@@ -928,7 +930,7 @@ __global__ void __launch_bounds__(1024) k_decay_join(DecayGeo d, const float* __
   Join j;
   j.n = (hi - lo + d.L - 1) / d.L - 1;
   if (j.n < kFew) return;
-  const int e = threadIdx.x % EL, run = threadIdx.x / EL;
+  const int e = threadIdx.x % EL, run = EL == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / EL) : threadIdx.x / EL;
   const int64_t at = lo / d.L + (REV ? j.n : 0);
   j.z = spans + at * d.H + head;
   j.step = (REV ? -1 : 1) * d.H * DD;
