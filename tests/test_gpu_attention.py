@@ -349,6 +349,34 @@ def test_attention_bad_gradients_stay_behind_their_token(bad, dtype):
         assert not torch.isfinite(a[430, 1, 3]), n
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_attention_bad_gradients_reach_the_stretches_before(bad, dtype, D):
+    """A bad gradient in a window's second stretch reaches its channel's values and its head's keys of the first one, and
+    changes no bit of the others."""
+    N, H, at = 900, 2, 700
+    start = torch.tensor([0, 200, 750, N], device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v, gy = torch.randn(4, N, H, D, device=DEV, generator=gen).to(dtype)
+    rate = torch.tensor([0.01, 0.02], device=DEV)
+    print(f"bad gradients {bad} {dtype} D={D}", flush=True)
+
+    def go(g):
+        ins = [a.clone().requires_grad_() for a in (q, k, v)]
+        return torch.autograd.grad(ops.decay_attention(*ins, rate, start)[0], ins, g)
+
+    clean = go(gy)
+    gy = gy.clone()
+    gy[at, 1, 3] = bad
+    got = go(gy)
+    hit = torch.zeros(3, N, H, D, dtype=torch.bool, device=DEV)
+    hit[0, at, 1] = hit[1, 200:at + 1, 1] = hit[2, 200:at + 1, 1, 3] = True
+    for n, (a, b) in enumerate(zip(got, clean)):
+        assert torch.equal(a[~hit[n]], b[~hit[n]]), n
+    assert not got[2][200:at + 1, 1, 3].isfinite().any() and not got[1][200:at + 1, 1].isfinite().any()
+
+
 def test_attention_bad_gaps_show():
     """A gap that is not a number makes its token's and the window's later outputs so, and the others' not."""
     N, H, D = 500, 2, 16
