@@ -1,5 +1,8 @@
 """The attention operators on the CPU: the definitions, gradients against differences, the single-token form, refusals."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -239,3 +242,24 @@ def test_entries_reject_before_launch():
     refused(bwd(bytes=need - 1), b"workspace")
     refused(L.atl_decay_attn_step(*rows, *rows, *rows, 0, 5, 2, 200, fake, n, 1.0, fake, fake, n), b"bad sizes")
     refused(L.atl_decay_attn_step(*rows, *rows, *rows, 0, 5, 2, 8, fake, n, 1.0, n, fake, n), b"null")
+
+
+_NO_WINDOW = """
+import ctypes
+from x_amd.ops import _ext
+L, fake, n = _ext.load_library(), ctypes.c_void_p(4096), None
+for D in (8, 64):
+    rows, held = (fake, 2 * D, D), L.atl_decay_attn_states_bytes({N}, {B}, 2, D)
+    print(L.atl_decay_attn_fwd(*rows, *rows, *rows, 0, {N}, 2, D, fake, fake, {B}, n, n, 1.0, fake, fake, fake, held, n),
+          L.atl_decay_attn_bwd(*rows, *rows, *rows, *rows, 0, {N}, 2, D, fake, fake, {B}, n, n, n, 1.0, fake, fake, fake, fake, n,
+                               fake, held, n))
+"""
+
+
+@pytest.mark.parametrize("N,B", [(1000, 0), (2000, 0), (20_000, 0), (20_000, 1)])
+def test_entries_return_without_windows(N, B):
+    """Tokens and no window, past the length from which stretches are joined: the entry points' host part returns (an error
+    here, since no device is visible to the process and nothing is launched)."""
+    env = {**os.environ, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1"}
+    run = subprocess.run([sys.executable, "-c", _NO_WINDOW.format(N=N, B=B)], env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.split() == ["1"] * 4, (run.returncode, run.stdout, run.stderr)

@@ -192,6 +192,19 @@ def test_attention_without_windows_and_of_plain_sums():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N", [2000, 20_000])
+@pytest.mark.parametrize("D", [8, 32, 64, 128])
+def test_attention_without_windows_past_the_joined_length(N, D):
+    """Tokens and no window, as long as windows whose stretches are joined: zeros, forward and backward."""
+    q, k, v = (torch.randn(N, 2, D, device=DEV, requires_grad=True) for _ in range(3))
+    h0 = torch.zeros(0, 2, D, D, device=DEV, requires_grad=True)
+    print(f"no window: N={N} D={D}", flush=True)
+    y, last = ops.decay_attention(q, k, v, torch.ones(2, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV), h0=h0)
+    assert not y.any() and last.shape == (0, 2, D, D)
+    *grads, g0 = torch.autograd.grad((y, last), (q, k, v, h0), (torch.randn_like(y), torch.zeros_like(last)))
+    assert not any(g.any() for g in grads) and g0.shape == h0.shape
+
+
 @pytest.mark.parametrize("H", [1, 2, 5, 16, 33])
 def test_attention_heads(H):
     _case(600, H, 16, BF16, "ragged", seed=H)

@@ -1030,7 +1030,7 @@ void by_layout(int lay, F&& f) {
 
 template <typename T, bool REV>
 void run_local(const DecayGeo& d, const Rows& y, const Rows& w, float us, Span* spans, float* carry, hipStream_t stream) {
-  if (d.N <= d.L) return;                                  // every window is one stretch at most
+  if (d.N <= d.L || d.B == 0) return;                      // every window is one stretch at most
   by_head(d.D, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     by_layout(std::min(layout<T>(y, d.D), layout<T>(w, d.D)), [&](auto l) {
@@ -1043,7 +1043,7 @@ void run_local(const DecayGeo& d, const Rows& y, const Rows& w, float us, Span* 
 }
 template <bool REV>
 void run_join(const DecayGeo& d, const float* given, const Span* spans, float* carry, hipStream_t stream) {
-  if (d.N <= kFew * d.L) return;                           // no window has more than kFew stretches
+  if (d.N <= kFew * d.L || d.B == 0) return;               // no window has more than kFew stretches
   const int64_t DD = (int64_t)d.D * d.D, places = d.N / (kFew * d.L) + 1;
   const int by_place = places < d.B;
   const int64_t of = (by_place ? places : d.B) * d.H;
