@@ -229,3 +229,14 @@ def test_entries_reject_before_launch():
     refused(L.atl_gated_scan_bwd(fake, 8, fake, 8, 0, 5, 8, fake, 1, n, n, n, fake, 8, n, fake, fake, n, fake, need, n),
             b"null")
     refused(L.atl_gated_scan_step(fake, -1, fake, 8, 0, 5, 8, n, fake, fake, n), b"bad sizes")
+
+
+@pytest.mark.parametrize("D", [3, 8, 33])
+def test_dropout_of_no_rows(D):
+    """No tokens: no rows, their norm and sum, with dropout too; the weight's gradient is zero."""
+    assert ref.dropout_keeps(0, D, 0.25, 1, 2).shape == (0, D)
+    x, w = torch.zeros(0, D, requires_grad=True), torch.ones(D, requires_grad=True)
+    y, s = ops.residual_rms_norm(x, torch.zeros(0, D), w, p=0.25, seed=1)
+    assert y.shape == s.shape == (0, D)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert gx.shape == (0, D) and not gw.any()

@@ -171,7 +171,7 @@ def dropout_keeps(rows, D, p, seed, offset, device="cpu"):
     words = philox4x32_10((row, group.expand_as(row), torch.full_like(row, offset & 0xFFFFFFFF),
                            torch.full_like(row, offset >> 32)), seed)
     bits = torch.stack([half for w in words for half in (w & 0xFFFF, w >> 16)], -1)
-    return bits.reshape(rows, -1)[:, :D] >= round(65536 * p)
+    return bits.flatten(1)[:, :D] >= round(65536 * p)
 
 
 def residual_rms_norm(x, residual, weight, eps, p, seed, offset):
