@@ -103,6 +103,27 @@ def test_positions_that_are_not_numbers_are_no_tokens(dev):
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_windows_without_events_and_no_streams(dev):
+    """A packet without events leaves the states as they were (zeros without any), its windows' whole length goes by, no stream
+    steps, and the packet's motion has gradients."""
+    net = _net(dev, torch.float32)
+    none = _packet(dev, n=60, B=2)
+    none = none.select(torch.zeros(0, dtype=torch.int64, device=none.device))
+    assert none.n == 0 and none.batch_size == 2
+    assert all(tuple(s.shape) == (2, 2, 16, 16) and not s.any() for s in net.states(none))
+    h0 = [torch.randn(2, 2, 16, 16, device=dev) for _ in net.norm]
+    since = torch.rand(2, device=dev)
+    for a, b in zip(net.states(none, h0=h0, p=0.1, since=since), h0):
+        assert torch.equal(a, b)
+    assert torch.equal(net.idle(none, since), since + 1)
+    net.coefficients(net.states(none, h0=h0)).sum().backward()
+    assert net.head.grad.isfinite().all() and net.read[0].grad.any()
+    empty = torch.zeros(0, device=dev)
+    states = net.step(torch.zeros(0, 2, device=dev), empty, empty, net.fresh_states(0))
+    assert [tuple(s.shape) for s in states] == [(0, 2, 16, 16)] * 2
+
+
 @pytest.mark.gpu
 def test_streams_in_8_bits():
     """e4m3 keeps three bits of mantissa: the projections of 64 terms are off by some percent of their size, and so are products

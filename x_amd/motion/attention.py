@@ -50,7 +50,7 @@ class EventAttention(EventRecurrence):
 
     def _heads(self, y, k, pos):
         """Queries, keys and values (n, heads, D) of a layer's projection, the first two normed and turned."""
-        *q, key, v = y.view(len(y), -1, self.heads, self.dim // self.heads).unbind(1)
+        *q, key, v = y.view(len(y), y.shape[1] // self.dim, self.heads, self.dim // self.heads).unbind(1)
         q, q_norm = (q[0], self.q_norm[k]) if q else (key, self.k_norm[k])
         return *head_norm_rotary(q, key, q_norm, self.k_norm[k], pos, self.freqs, self.sections), v
 
