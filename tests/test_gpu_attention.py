@@ -568,6 +568,44 @@ def test_rotary_of_zeros_and_bad_rows():
         assert torch.equal(a[~h], b[~h]) and a[9, :, :4].isnan().all()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D,sections", [(16, (1, 2)), (16, (3,)), (15, (2,)), (12, (0,))])
+def test_rotary_leaves_unturned_channels_alone(bad, dtype, D, sections):
+    """Without norms a channel past the sections is passed on as it is, whatever it holds, and so is its neighbour; in the
+    backward pass too, and a norm's weight gradient of the neighbour stays as it was."""
+    N, H, turned = 20, 2, 2 * sum(sections)
+    q, k, gq, gk = torch.randn(4, N, H, D, device=DEV).to(dtype)
+    w = torch.rand(D, device=DEV) + 0.5
+    pos, fr = torch.rand(N, len(sections), device=DEV), torch.rand(turned // 2, device=DEV)
+    print(f"unturned channels {bad} {dtype} D={D} {sections}", flush=True)
+
+    def go(q, gk):
+        ins = [t.clone().requires_grad_() for t in (q, k)]
+        out = ops.head_norm_rotary(*ins, None, None, pos, fr, sections)
+        return [*out, *torch.autograd.grad(out, ins, (gq, gk))]
+
+    clean, hit = go(q, gk), [torch.zeros(N, H, D, dtype=torch.bool, device=DEV) for _ in range(4)]
+    q, gk = q.clone(), gk.clone()
+    for n, c in enumerate(range(turned, D)):                 # of the even and of the odd channels, each in a row of its own
+        q[n, 0, c], gk[n, 1, c] = bad, bad
+        hit[0][n, 0, c] = hit[3][n, 1, c] = True
+    for a, b, h in zip(go(q, gk), clean, hit):
+        assert torch.equal(a[~h], b[~h]) and not a[h].isfinite().any()
+        assert bad != bad or bool((a[h] == bad).all())
+
+    def weights(g):
+        ins = [w.clone().requires_grad_() for _ in range(2)]
+        out = ops.head_norm_rotary(q0, k, *ins, pos, fr, sections)
+        return torch.autograd.grad(out, ins, (g, gk0))
+
+    q0, gk0 = torch.randn(2, N, H, D, device=DEV).to(dtype)
+    g = gq.clone()
+    g[4, 1, D - 1] = bad
+    (a, ak), (b, bk) = weights(g), weights(gq)
+    assert torch.equal(a[:-1], b[:-1]) and not a[-1].isfinite() and torch.equal(ak, bk)
+
+
 def test_rotary_gradients_of_some():
     """Each input's gradient alone, and from one output alone, is the one it has beside the others."""
     N, D = 30, 16

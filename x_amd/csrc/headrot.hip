@@ -62,13 +62,15 @@ __device__ __forceinline__ void angles(const RotGeo& g, int64_t n, int c, float 
   }
 }
 
+// The first `pairs` of the lane's; the others are passed on as they are (turned by zero, a NaN or an infinity would reach its
+// neighbour).
 template <int V>
-__device__ __forceinline__ void turn(float (&v)[V], const float (&co)[V / 2], const float (&si)[V / 2], float sign) {
+__device__ __forceinline__ void turn(float (&v)[V], const float (&co)[V / 2], const float (&si)[V / 2], float sign, int pairs) {
 #pragma unroll
   for (int m = 0; m < V / 2; ++m) {
     const float a = v[2 * m], b = v[2 * m + 1], s = sign * si[m];
-    v[2 * m] = fmaf(a, co[m], -b * s);
-    v[2 * m + 1] = fmaf(a, s, b * co[m]);
+    v[2 * m] = m < pairs ? fmaf(a, co[m], -b * s) : a;
+    v[2 * m + 1] = m < pairs ? fmaf(a, s, b * co[m]) : b;
   }
 }
 
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(kBlock) k_headrot_fwd(RotGeo g, HeadRows q, He
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = v[e] * inv * (w.key ? wv[1][e] : wv[0][e]);
       }
-      turn<V>(v, co, si, 1.f);
+      turn<V>(v, co, si, 1.f, g.pairs - c / 2);
       if (in) store_part<WHOLE, V>((w.key ? yk + (n * g.Hk + w.head) * g.D : yq + (n * g.H + w.head) * g.D), c, g.D, v);
     }
   }
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kBlock) k_headrot_bwd(RotGeo g, HeadRows q, He
       float y[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) y[e] = (float)ys.e[e];
-      turn<V>(y, co, si, -1.f);
+      turn<V>(y, co, si, -1.f, g.pairs - c / 2);
       if (wq) {
         float x[V], ss = 0.f, dot = 0.f;
 #pragma unroll
