@@ -157,3 +157,32 @@ def rotary_bwd(x, w, angle, eps, gy):
     big = r * (np.abs(w) * mag + np.abs(hat) * (np.abs(w) * mag * np.abs(hat)).mean(-1, keepdims=True))
     rows = x.shape[0] * x.shape[1]
     return (gx, (g * hat).sum((0, 1))), ((2 * D + 64) * U * big, (rows + D + 64) * U * (mag * np.abs(hat)).sum((0, 1)))
+
+
+def by_token(q, k, v, rate, start, dt, h0, scale, gy, glast):
+    """(y, last, gq, gk, gv, gh0) from the definitions one token after the other, and the same of magnitudes: no product is left
+    out or taken apart, so infinities and NaN go where the formulas take them."""
+    N, H, D = q.shape
+    B = len(start) - 1
+    a = np.exp(-(np.ones(N) if dt is None else dt)[:, None] * rate[None])[..., None, None]
+    with np.errstate(invalid="ignore", over="ignore"):
+        both = []
+        for f in (lambda t: t, np.abs):
+            Q, K, V, G0, GY, GL = (f(t) for t in (q, k, v, np.zeros((B, H, D, D)) if h0 is None else h0, gy, glast))
+            y, gq, gk, gv = (np.zeros((N, H, D)) for _ in range(4))
+            last, gh0 = np.zeros((B, H, D, D)), np.zeros((B, H, D, D))
+            for b in range(B):
+                S = G0[b]
+                for i in range(start[b], start[b + 1]):
+                    S = a[i] * S + K[i][:, :, None] * V[i][:, None, :]
+                    y[i] = f(scale) * (Q[i][:, :, None] * S).sum(1)
+                    gq[i] = f(scale) * (S * GY[i][:, None, :]).sum(2)
+                last[b], G = S, GL[b]
+                for i in reversed(range(start[b], start[b + 1])):
+                    G = G + f(scale) * Q[i][:, :, None] * GY[i][:, None, :]
+                    gv[i] = (K[i][:, :, None] * G).sum(1)
+                    gk[i] = (G * V[i][:, None, :]).sum(2)
+                    G = a[i] * G
+                gh0[b] = G
+            both.append((y, last, gq, gk, gv, gh0))
+    return both

@@ -390,6 +390,98 @@ def test_attention_bad_gradients_reach_the_stretches_before(bad, dtype, D):
     assert not got[2][200:at + 1, 1, 3].isfinite().any() and not got[1][200:at + 1, 1].isfinite().any()
 
 
+def _same_kinds(got, want, mag, units, dtype, what):
+    """Infinities with their signs and NaN where the definition has them, and finite values within its bound."""
+    want32 = want.astype(np.float32).astype(np.float64)      # what single precision can hold
+    for kind, of in (("NaN", np.isnan), ("+Inf", np.isposinf), ("-Inf", np.isneginf)):
+        a, b = of(_np(got)), of(want32)
+        assert (a == b).all(), f"{what}: {kind} in {int((a & ~b).sum())} places too many, {int((b & ~a).sum())} too few"
+    fine = np.isfinite(want32) & np.isfinite(mag)
+    tol = units * mag[fine] + rounding(dtype, np.abs(want[fine]) + units * mag[fine])
+    assert (np.abs(_np(got)[fine] - want[fine]) <= tol).all(), what
+
+
+def _by_token_case(x, rate, start, dt, dtype, where, scale=0.5, pieces=True):
+    """All outputs and gradients against the definition, exponents below 4 (5 units of a factor)."""
+    N, H, D = x["q"].shape
+    ins = [x[n].clone().requires_grad_() for n in ("q", "k", "v", "h0")]
+    y, last = ops.decay_attention(*ins[:3], rate, torch.tensor(start, device=DEV), dt=dt, h0=ins[3], scale=scale)
+    grads = torch.autograd.grad((y, last), ins, (x["gy"], x["glast"]))
+    want, mag = O.by_token(*(_np(x[n]) for n in "qkv"), _np(rate), start, _np(dt), _np(x["h0"]), scale, _np(x["gy"]), _np(x["glast"]))
+    units = (3 * D + 300 + 3 * (N // 32 + 1)) * 5 * O.U + O.PIECES[_name(dtype)]
+    for n, (name, got) in enumerate(zip(("y", "last", "gq", "gk", "gv", "gh0"), (y, last, *grads))):
+        _same_kinds(got, want[n], mag[n], units, got.dtype, f"{name} ({where})")
+
+
+@pytest.mark.parametrize("D", [1, 8, 32, 45, 64, 100, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_attention_infinities_go_where_the_formula_takes_them(D, dtype):
+    """An infinity in each of the inputs in turn, and in all: signed infinities and NaN are those of the definition, in the
+    token's chunk, later chunks, other stretches, states and gradients."""
+    N, H, start = 700, 2, [0, 100, 640, 700]
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    clean = {n: torch.randn(N, H, D, device=DEV, generator=gen).to(dtype) for n in ("q", "k", "v", "gy")}
+    clean.update({n: torch.randn(3, H, D, D, device=DEV, generator=gen) for n in ("h0", "glast")})
+    dt, rate = torch.rand(N, device=DEV, generator=gen) * 0.01, torch.tensor([1.0, 0.1], device=DEV)
+    c, inf = D // 2, float("inf")
+    bad = [("q", (150, 0, c), inf), ("k", (131, 1, c), -inf), ("v", (390, 0, D - 1), inf), ("gy", (420, 1, 0), -inf),
+           ("h0", (1, 0, c, 0), inf), ("glast", (1, 1, 0, c), -inf), ("k", (99, 0, 0), inf), ("v", (639, 1, c), -inf)]
+    for some in [[b] for b in bad] + [bad]:
+        print(f"infinities D={D} {dtype} {[b[0] for b in some]}", flush=True)
+        x = {n: t.clone() for n, t in clean.items()}
+        for name, at, value in some:
+            x[name][at] = value
+        _by_token_case(x, rate, start, dt, dtype, "+".join(b[0] for b in some))
+
+
+@pytest.mark.parametrize("N,D", [(2500, 8), (1600, 64), (17_000, 8)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_infinities_cross_joined_stretches(N, D, dtype):
+    """Windows whose stretches' sums are joined, by a thread an element and in runs."""
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    x = {n: torch.randn(N, 1, D, device=DEV, generator=gen).to(dtype) for n in ("q", "k", "v", "gy")}
+    x.update({n: torch.randn(1, 1, D, D, device=DEV, generator=gen) for n in ("h0", "glast")})
+    x["k"][40, 0, 1], x["gy"][N - 30, 0, 2] = float("inf"), float("-inf")
+    dt, rate = torch.rand(N, device=DEV, generator=gen) * 8 / N, torch.ones(1, device=DEV)
+    print(f"infinities across joins N={N} D={D} {dtype}", flush=True)
+    _by_token_case(x, rate, [0, N], dt, dtype, "joined")
+
+
+@pytest.mark.parametrize("D", [4, 64])
+def test_attention_of_products_past_single_precision(D):
+    """Queries and keys whose product is past float32, values so small that the outputs are not; and states past it."""
+    N, dtype = 400, F32
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    x = {n: torch.rand(N, 1, D, device=DEV, generator=gen) + 0.5 for n in ("q", "k", "v", "gy")}
+    x.update({n: torch.zeros(1, 1, D, D, device=DEV) for n in ("h0", "glast")})
+    x["q"][100:110] *= 1e25
+    x["k"][90:95] *= 1e20
+    x["v"][90:95] *= 1e-20
+    _by_token_case(x, torch.ones(1, device=DEV), [0, N], torch.full((N,), 0.001, device=DEV), dtype, "large products")
+    x["k"][300] = x["v"][300] = 1e25
+    x["q"][:], x["gy"][:] = 1.0, 1.0
+    _by_token_case(x, torch.ones(1, device=DEV), [0, N], torch.full((N,), 0.001, device=DEV), dtype, "large states")
+
+
+def test_step_of_infinite_states():
+    """An infinite state stays so, with its sign, until a factor of zero."""
+    N, H, D, inf = 3, 1, 8, float("inf")
+    q, k, v = torch.rand(3, N, H, D, device=DEV) + 0.5
+    state = torch.zeros(N, H, D, D, device=DEV)
+    state[0, 0, 2, 3], state[1, 0, 2, 3], k[2, 0, 1] = inf, -inf, inf
+    rate, dt = torch.ones(H, device=DEV), torch.tensor([0.1, 2.0, 1.0], device=DEV)
+    for _ in range(2):
+        want = torch.exp(-dt.double())[:, None, None, None] * state.double() + k.double()[..., None] * v.double()[:, :, None]
+        y = ops.decay_attention_step(q, k, v, rate, state, dt=dt, scale=1.0)
+        assert torch.equal(state.isposinf(), want.isposinf()) and torch.equal(state.isneginf(), want.isneginf())
+        assert torch.allclose(state, want.float(), rtol=1e-5) and not state.isnan().any()
+        out = (q.double()[..., None] * want).sum(2)
+        assert torch.equal(y.isposinf(), out.isposinf()) and torch.equal(y.isneginf(), out.isneginf())
+        assert torch.allclose(y, out.float(), rtol=1e-5)
+    ops.decay_attention_step(q, v, v, rate, state, dt=torch.full((N,), inf, device=DEV))
+    assert state[2].isfinite().sum() == 56 and state[0, 0, 2, 3].isnan()       # zero times an infinity
+
+
 def test_attention_bad_gaps_show():
     """A gap that is not a number makes its token's and the window's later outputs so, and the others' not."""
     N, H, D = 500, 2, 16

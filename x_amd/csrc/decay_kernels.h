@@ -164,6 +164,8 @@ __device__ __forceinline__ float top_of_four(float top) {
 struct Fade {
   float a, keep;                           // m e^{-z} + u = m a + (m keep + u), keep 0 or 1
   __device__ __forceinline__ float operator()(float m, float u) const { return fmaf(m, a, fmaf(m, keep, u)); }
+  // Of an infinite m too, of which the two parts would make a NaN.
+  __device__ __forceinline__ float any(float m, float u) const { return fabsf(m) < INFINITY ? (*this)(m, u) : fmaf(m, a + keep, u); }
 };
 __device__ __forceinline__ Fade fade_of(float z) {
   const bool keep = !(z > 0.5f);
@@ -444,7 +446,7 @@ __device__ __forceinline__ void add_chunk(const float* weight, Fade fade, float 
   }
 }
 
-// W that are not finite are left out of the products (their pieces would be NaNs, and so would zero weights times them) ...
+// W that are not finite are left out of the products: their pieces would be NaNs, and so would weights of zero times them ...
 template <typename T, int CT>
 __device__ __forceinline__ void leave_out(Frag<T> (&wf)[CT]) {
 #pragma unroll
@@ -452,24 +454,20 @@ __device__ __forceinline__ void leave_out(Frag<T> (&wf)[CT]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) wf[ct][k] = fabsf((float)wf[ct][k]) < INFINITY ? wf[ct][k] : (T)0.f;
 }
-// ... and added to the state behind them, one by one.
+// ... and what they have a part in is marked by a NaN, to be taken again by by_token: their columns of the state (and their
+// rows from their own on, where those are stored).
 template <typename T, int DP, int CT>
-__device__ __forceinline__ void add_odd(const float* weight, float times, const T* y, const T* w, int c0, F4 (&M)[CT][DP / 16]) {
-  constexpr int LD = tile_ld<T, DP>();
+__device__ __forceinline__ void mark(const T* w, int c0, F4 (&M)[CT][DP / 16]) {
 #pragma unroll 1
   for (int j = 0; j < kChunk; ++j)
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float z = (float)w[j * LD + c0 + ct * 16 + (threadIdx.x & 15)];
-      const bool odd = !(fabsf(z) < INFINITY);
+      const bool odd = !(fabsf((float)w[j * tile_ld<T, DP>() + c0 + ct * 16 + (threadIdx.x & 15)]) < INFINITY);
       if (!__any(odd)) continue;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float m = fmaf(weight[j] * times * z, (float)y[j * LD + state_row(dt, r)], M[ct][dt][r]);
-          M[ct][dt][r] = odd ? m : M[ct][dt][r];
-        }
+        for (int r = 0; r < 4; ++r) M[ct][dt][r] = odd ? NAN : M[ct][dt][r];
     }
 }
 
@@ -489,12 +487,13 @@ __device__ __forceinline__ void add_state(const float* p, bool flip, int D, int 
       for (int r = 0; r < 4; ++r) {
         const int y = y0 + dt / 2 * 32 + (dt & 1) * 4 + r;
         const uint32_t off = y < D && w < D ? (uint32_t)(y * sy + w * sw) * 4 : kNoChannel;
-        M[ct][dt][r] = fade(M[ct][dt][r], __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, off, 0, 0)));
+        M[ct][dt][r] = fade.any(M[ct][dt][r], __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buf, off, 0, 0)));
       }
   }
 }
+// (Where not `all`, over what is there and not finite.)
 template <int DP, int CT>
-__device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&M)[CT][DP / 16]) {
+__device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&M)[CT][DP / 16], bool all) {
   const int i = threadIdx.x & 15;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
@@ -503,8 +502,99 @@ __device__ __forceinline__ void store_state(float* p, int D, int c0, const F4 (&
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int y = state_row(dt, r), w = c0 + ct * 16 + i;
-        if (y < D && w < D) p[y * D + w] = M[ct][dt][r];
+        if (y < D && w < D && (all || !(fabsf(p[y * D + w]) < INFINITY))) p[y * D + w] = M[ct][dt][r];
       }
+}
+template <int DP, int CT>
+__device__ __forceinline__ void clear_state(F4 (&M)[CT][DP / 16]) {
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
+}
+template <int DP, int CT>
+__device__ __forceinline__ bool finite_state(const F4 (&M)[CT][DP / 16]) {
+  float check = 0.f;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) check = fmaf(M[ct][dt][r], 0.f, check);
+  return !__any(check != check);
+}
+
+// The recurrence as it is written, token by token in single precision, for a stretch with something in it that is not finite:
+// infinities do not come through the matrix products (an infinity's second piece is Inf - Inf, and weights of zero make NaNs of
+// them), nor do products past single precision on the way to a smaller result.  Only where the products left no finite result
+// is one written.  kAlong and kBack: the sweeps' directions, rows from the stretch's begin or end, with the gap before a row
+// taken before it or before the next; kFromEnd: the sum from the end's side, in the order of the tokens.  One wave waits for
+// every token's rows, about 2.5 us: 1M tokens x 2 x 32 in bfloat16 with one infinity take 13 ms forward + backward instead of 0.6.
+// What the check costs where all is finite, by the cases: 256 windows of 400 x 4 x 64 361 -> 366 us, 1M x 2 x 32 600 -> 606,
+// 251k x 3 x 45 in float32 1127 -> 1146, 65k x 8 x 128 960 -> 970, 100k x 8 x 64 in float16 forward 231 -> 235.
+enum Way : int { kAlong = 0, kBack = 1, kFromEnd = 2 };
+template <typename T, int DP, int CT, int WAY>
+__device__ __forceinline__ void by_token(const DecayGeo& d, const Stretch& st, int head, const Rows& x, const Rows& y, const Rows& w,
+                                         int c0, float xs, float us, F4 (&M)[CT][DP / 16], T* out) {
+  const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i16 = lane & 15;
+  const float rate = d.rate[head];
+  __threadfence();                                          // the results so far are read again
+  Fade pending{0.f, 1.f};
+  double gone = 0;
+#pragma unroll 1
+  for (int64_t n = st.hi - st.lo; n > 0; --n) {
+    const int64_t t = WAY == kBack ? st.lo + n - 1 : st.hi - n;
+    double z = (double)rate * (double)(d.dt ? d.dt[t] : 1.f) * 1.4426950408889634;
+    if (z > kForgotten) z = kForgotten;                     // a NaN stays
+    const Fade own = fade_of((float)(z * 0.6931471805599453));
+    gone += z;
+    const Fade f = WAY == kAlong ? own : pending;
+    if (WAY == kBack) pending = own;
+    const float weight = WAY == kFromEnd ? us * exp2f((float)-gone) : us;
+    const T* yr = (const T*)y.p + t * y.sn + head * y.sh;
+    const T* xr = (const T*)x.p + t * x.sn + head * x.sh;
+    const T* wr = (const T*)w.p + t * w.sn + head * w.sh;
+    float yv[DP / 16][4], xv[DP / 16][4], wv[CT], sum[CT];
+    bool odd[CT];                                           // (read with the rows: one wait a token)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+      const int row = state_row(dt, 0);
+      load_loose<4>(yr + row, d.D - row, yv[dt]);
+      if (out) load_loose<4>(xr + row, d.D - row, xv[dt]);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = c0 + ct * 16 + i16;
+      wv[ct] = c < d.D ? weight * (float)wr[c] : 0.f;
+      sum[ct] = 0.f;
+      odd[ct] = out && g == ct && c < d.D && !(fabsf((float)out[(t * d.H + head) * d.D + c]) < INFINITY);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (state_row(dt, r) >= d.D) continue;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          M[ct][dt][r] = f.any(M[ct][dt][r], yv[dt][r] * wv[ct]);
+          if (out) sum[ct] = fmaf(xv[dt][r], M[ct][dt][r], sum[ct]);
+        }
+      }
+    if (!out) continue;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      sum[ct] += __shfl_xor(sum[ct], 16, kWave);
+      sum[ct] += __shfl_xor(sum[ct], 32, kWave);
+      if (odd[ct]) out[(t * d.H + head) * d.D + c0 + ct * 16 + i16] = (T)(xs * sum[ct]);
+    }
+  }
+  if (WAY == kBack)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) M[ct][dt][r] = pending.any(M[ct][dt][r], 0.f);
 }
 
 // ------------------------------------------------------------------------------------------- the sweep
@@ -610,50 +700,77 @@ constexpr int jobs_of(int work) { return work == kSweep ? 1 : 2; }
 template <typename T, int DP, int WORK>
 constexpr int sweep_threads() { return sweep_waves<DP, WORK>() * jobs_of(WORK) * kWave; }
 
+// What a wave of a sweep goes through: its stretch (if `live`), head, job and columns.
+template <int DP, int WORK, bool REV>
+struct Part {
+  Stretch st;
+  int head, job, c0, lane0;                // lane0: the wave's first lane among those of a head's workgroups
+  bool live, summing, begins, ends;
+  __device__ __forceinline__ Part(const DecayGeo& d, int64_t block) {
+    constexpr int NW = sweep_waves<DP, WORK>(), PARTS = DP / 16 / kTiles / NW;         // workgroups of a head
+    const int64_t work = near_first(block, d.slots * d.H * PARTS);
+    live = work < d.slots * d.H * PARTS;
+    if (!live) return;
+    const int64_t slot = work / (d.H * PARTS);
+    const int place = (int)(work - slot * (d.H * PARTS)), every = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    head = place / PARTS;
+    st = stretch_of(d, slot);
+    live = st.live;
+    job = every / NW;
+    const int wave = place % PARTS * NW + every % NW;
+    c0 = wave * kTiles * 16;
+    lane0 = wave * kWave;
+    summing = WORK == kSweepAndSums && job == 1;
+    begins = REV ? st.last : st.first, ends = REV ? st.first : st.last;
+  }
+  // What is before the stretch: its window's given state and the sums of the stretches in between, or their joined state.
+  __device__ __forceinline__ void begin(const DecayGeo& d, const Sweep& a, F4 (&M)[kTiles][DP / 16]) const {
+    clear_state<DP, kTiles>(M);
+    const int64_t DD = (int64_t)d.D * d.D;
+    const bool flip = (a.flip != 0) != (job != 0);
+    const int64_t dir = REV ? 1 : -1, past = begins ? 0 : st.count > kFew ? 1 : REV ? st.count - 1 - st.index : st.index;
+    const bool summed = begins || st.count <= kFew;
+#pragma unroll 1
+    for (int64_t k = summing ? 0 : past + (summed && a.given); k >= 1; --k) {
+      const int64_t e = (st.entry + dir * k) * d.H + head;
+      const bool given = k > past;
+      const float* p = given ? a.given + (st.window * d.H + head) * DD : a.carry + e * DD;
+      add_state<DP, kTiles>(p, flip, d.D, c0, !given && summed ? a.spans[e].fade : Fade{0.f, 1.f}, M);
+    }
+  }
+  // The states behind the stretch that are kept.
+  __device__ __forceinline__ void store(const DecayGeo& d, const Sweep& a, const F4 (&M)[kTiles][DP / 16], bool all) const {
+    const int64_t DD = (int64_t)d.D * d.D;
+    if (ends && a.end && job == 0) store_state<DP, kTiles>(a.end + (st.window * d.H + head) * DD, d.D, c0, M, all);
+    if (summing && !st.first) store_state<DP, kTiles>(a.sums + (st.entry * d.H + head) * DD, d.D, c0, M, all);
+  }
+};
+
 template <typename T, int DP, int WORK, bool REV, int LAY>
-__global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<ChunkLds<T, DP, jobs_of(WORK) + 2>, kSweepWaves>(sweep_waves<DP, WORK>() * jobs_of(WORK))))
+__global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<ChunkLds<T, DP, jobs_of(WORK) + 2>, DP == 32 && WORK != kSweep && LAY == kWhole ? 3 : kSweepWaves>(sweep_waves<DP, WORK>() * jobs_of(WORK))))
     k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
-  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = sweep_waves<DP, WORK>(), KD = DP / 32, THREADS = sweep_threads<T, DP, WORK>();
-  constexpr int JOBS = jobs_of(WORK);
-  constexpr int PARTS = DT / CT / NW;      // workgroups of a head
-  constexpr int NT = JOBS + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
+  constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, KD = DP / 32, THREADS = sweep_threads<T, DP, WORK>();
+  constexpr int NT = jobs_of(WORK) + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   __shared__ ChunkLds<T, DP, NT> s;
-  const int64_t work = near_first(first + blockIdx.x, d.slots * d.H * PARTS);
-  if (work >= d.slots * d.H * PARTS) return;
-  const int64_t slot = work / (d.H * PARTS);
-  const int place = (int)(work - slot * (d.H * PARTS)), head = place / PARTS;
-  const Stretch st = stretch_of(d, slot);
-  if (!st.live) return;
-  const int every = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), job = every / NW, wave = every % NW;
+  const Part<DP, WORK, REV> part(d, first + blockIdx.x);
+  if (!part.live) return;
+  const Stretch& st = part.st;
   const int lane = threadIdx.x & (kWave - 1), g = lane >> 4, i16 = lane & 15;
-  const int c0 = (place % PARTS * NW + wave) * CT * 16;
+  const int head = part.head, job = part.job, c0 = part.c0;
   T* out = (T*)a.out[job];
-  const bool summing = WORK == kSweepAndSums && job == 1;
+  const bool summing = part.summing;
   if (st.window < 0 || st.window >= d.B) {                  // tokens of no window
     if (summing) return;
-    for (int64_t t = st.lo + wave + place % PARTS * NW; t < st.hi; t += NW * PARTS)
+    for (int64_t t = st.lo + part.lane0 / kWave; t < st.hi; t += DT / CT)
       for (int c = lane; c < d.D; c += kWave) out[(t * d.H + head) * d.D + c] = (T)0.f;
     return;
   }
-  const bool begins = REV ? st.last : st.first, ends = REV ? st.first : st.last;
-  const int64_t DD = (int64_t)d.D * d.D;
   F4 M[CT][DT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
-  const bool flip = (a.flip != 0) != (job != 0);
-  // What is before the stretch: its window's given state and the sums of the stretches in between, or their joined state.
-  const int64_t dir = REV ? 1 : -1, past = begins ? 0 : st.count > kFew ? 1 : REV ? st.count - 1 - st.index : st.index;
-  const bool summed = begins || st.count <= kFew;
-#pragma unroll 1
-  for (int64_t k = summing ? 0 : past + (summed && a.given); k >= 1; --k) {
-    const int64_t e = (st.entry + dir * k) * d.H + head;
-    const bool given = k > past;
-    const float* p = given ? a.given + (st.window * d.H + head) * DD : a.carry + e * DD;
-    add_state<DP, CT>(p, flip, d.D, c0, !given && summed ? a.spans[e].fade : Fade{0.f, 1.f}, M);
-  }
+  part.begin(d, a, M);
+  // Lanes in which a query or a pair's weight was not finite, of which no channel of its row's output is; what is not finite in Y, W
+  // or the state before shows in the state at the end.
+  uint64_t check = 0;
   Rows rows[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) rows[n] = a.rows[n];
@@ -675,7 +792,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
       for (int ct = 0; ct < CT; ++ct) wf[ct] = frag_col<T, LD, false>(W, c0 + ct * 16);
       if (odd) leave_out<T, CT>(wf);
       add_chunk<T, DP, CT>(dec.xe, Fade{0.f, 1.f}, times, Y, M, wf);
-      if (odd) add_odd<T, DP, CT>(dec.xe, times, Y, W, c0, M);
+      if (odd) mark<T, DP, CT>(W, c0, M);
       gone += dec.total;
       return;
     }
@@ -792,6 +909,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
         float o[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
+        if (ct == 0) check |= __ballot(!(fabsf(o[0]) < INFINITY));
         if constexpr (LAY != kLoose) {
           const uint32_t at_row = row_offset<REV>(i, out_stride, len) + c * (uint32_t)sizeof(T);
           const uint32_t off = c + 4 <= d.D ? at_row : kNoChannel;
@@ -811,44 +929,38 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
         }
       }
     }
-    // What was left out, to the rows from its own on: their weights are taken anew.
     if (odd) {
-      add_odd<T, DP, CT>(dec.we, 1.f, Y, W, c0, M);
-      __threadfence_block();
+      mark<T, DP, CT>(W, c0, M);
 #pragma unroll 1
       for (int q = 0; q < 2 * CT * 4; ++q) {
         const int i = (q & 1) * 16 + i16, c = c0 + (q >> 3) * 16 + g * 4 + (q >> 1 & 3);
-        float sum = 0.f;
-        bool any = false;
         if (i < len && c < d.D)
 #pragma unroll 1
-          for (int j = 0; j <= i; ++j) {
-            const float z = (float)W[j * LD + c];
-            if (fabsf(z) < INFINITY) continue;
-            float dot = 0.f;
-#pragma unroll 1
-            for (int h = 0; h < DP; ++h) dot = fmaf((float)X[i * LD + h], (float)Y[j * LD + h], dot);
-            sum = fmaf(dot * a.ps * exp2f((float)(dec.e[j] - dec.e[i])), z, sum);
-            any = true;
-          }
-        if (any) {
-          T* p = to + (int64_t)(REV ? -i : i) * d.H * d.D + c;
-          *p = (T)((float)*p + sum);
-        }
+          for (int j = 0; j <= i; ++j)
+            if (!(fabsf((float)W[j * LD + c]) < INFINITY)) to[(int64_t)(REV ? -i : i) * d.H * d.D + c] = (T)NAN;
       }
     }
   });
-  if (ends && a.end && job == 0) store_state<DP, CT>(a.end + (st.window * d.H + head) * DD, d.D, c0, M);
-  if (summing && !st.first) {
-    store_state<DP, CT>(a.sums + (st.entry * d.H + head) * DD, d.D, c0, M);
-    if (place % PARTS == 0 && wave == 0 && lane == 0) a.sum_spans[st.entry * d.H + head] = Span{gone, fade_of((float)(gone * 0.6931471805599453))};
-  }
+  part.store(d, a, M, true);
+  if (summing && !st.first && part.lane0 + lane == 0) a.sum_spans[st.entry * d.H + head] = Span{gone, fade_of((float)(gone * 0.6931471805599453))};
+  if (finite_state<DP, CT>(M) && !check) return;
+  int64_t block = first + blockIdx.x;
+  asm volatile("" : "+s"(block));                           // (all is found anew: kept until here, it would take registers from the sweep)
+  const Part<DP, WORK, REV> anew(d, block);
+  anew.begin(d, a, M);
+  if (anew.summing)
+    by_token<T, DP, CT, kFromEnd>(d, anew.st, anew.head, a.rows[0], a.rows[3], a.rows[0], anew.c0, 1.f, a.xs, M, nullptr);
+  else
+    by_token<T, DP, CT, REV ? kBack : kAlong>(d, anew.st, anew.head, a.rows[WORK != kSweepPair ? 0 : anew.job ? 2 : 1],
+                                              a.rows[WORK != kSweepPair ? 1 : anew.job ? 3 : 0],
+                                              a.rows[WORK != kSweepPair ? 2 : anew.job ? 0 : 3], anew.c0, a.xs, a.us, M, (T*)a.out[anew.job]);
+  anew.store(d, a, M, false);
 }
 
 // A stretch's own sum from nothing (all but the last of a window, in the sweep's direction): carry (entries, H, D, D), and
 // its exponent and factor (entries, H).
 template <typename T, int DP, bool REV, int LAY>
-__global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>, kSweepWaves>(DP / 32)))
+__global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>, LAY != kLoose && DP <= 64 ? 4 : kSweepWaves>(DP / 32)))
     k_decay_local(DecayGeo d, Rows y, Rows w, float us, float* __restrict__ carry, Span* __restrict__ spans, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, NW = DT / CT, THREADS = NW * kWave;
   __shared__ ChunkLds<T, DP, 2> s;
@@ -860,10 +972,7 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>,
   if (!st.live || (REV ? st.first : st.last) || st.window < 0 || st.window >= d.B) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), c0 = wave * CT * 16;
   F4 M[CT][DT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) M[ct][dt] = F4{0.f, 0.f, 0.f, 0.f};
+  clear_state<DP, CT>(M);
   const Rows rows[2] = {y, w};
   const double sum = follow<T, DP, 2, 2, THREADS, REV, LAY>(s, d, st, rows, head, 1.f, 1.f, us, [&](int done, int, const Decays& dec) {
     Frag<T> wf[CT];
@@ -872,10 +981,19 @@ __global__ void __launch_bounds__(DP / 32 * kWave, (waves_of<ChunkLds<T, DP, 2>,
     const bool odd = __builtin_amdgcn_readfirstlane(s.odd[1]) == done + 1;
     if (odd) leave_out<T, CT>(wf);
     add_chunk<T, DP, CT>(dec.we, dec.fade, 1.f, s.tile[0], M, wf);
-    if (odd) add_odd<T, DP, CT>(dec.we, 1.f, s.tile[0], s.tile[1], c0, M);
+    if (odd) mark<T, DP, CT>(s.tile[1], c0, M);
   });
-  store_state<DP, CT>(carry + (st.entry * d.H + head) * (int64_t)d.D * d.D, d.D, c0, M);
+  store_state<DP, CT>(carry + (st.entry * d.H + head) * (int64_t)d.D * d.D, d.D, c0, M, true);
   if (threadIdx.x == THREADS - kWave) spans[st.entry * d.H + head] = Span{sum, fade_of((float)(sum * 0.6931471805599453))};
+  if (finite_state<DP, CT>(M)) return;
+  int64_t anew = first + blockIdx.x;
+  asm volatile("" : "+s"(anew));                            // (as in the sweep)
+  anew = near_first(anew, d.slots * d.H);
+  const Stretch at = stretch_of(d, anew / d.H);
+  const int h = (int)(anew % d.H);
+  clear_state<DP, CT>(M);
+  by_token<T, DP, CT, REV ? kBack : kAlong>(d, at, h, y, y, w, c0, 1.f, us, M, nullptr);
+  store_state<DP, CT>(carry + (at.entry * d.H + h) * (int64_t)d.D * d.D, d.D, c0, M, false);
 }
 
 // The states after the stretches of every window of more than kFew stretches (all but the last) from the stretches' own sums, in
@@ -905,7 +1023,7 @@ __device__ __forceinline__ float join_run(const Join& j, int64_t k0, int64_t k1,
 #pragma unroll
     for (int m = 0; m < kAhead; ++m) {
       if (k + m >= k1) break;
-      state = f[m](state, u[m]);
+      state = f[m].any(state, u[m]);
       if (WRITE && j.in) j.p[(k + m) * j.step] = state;
     }
   }
@@ -956,7 +1074,7 @@ __global__ void __launch_bounds__(1024, EL == kWave ? 8 : 4) k_decay_join(DecayG
     end[run][e] = join_run<false>(j, k0, k1, 0.f);
     __syncthreads();
     float state = given && j.in ? given[(b * d.H + head) * DD + el] : 0.f;
-    for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r](state, end[r][e]);
+    for (int r = 0; r < run && r * len < j.n; ++r) state = fade[r].any(state, end[r][e]);
     join_run<true>(j, k0, k1, state);
   }
 }
@@ -992,7 +1110,7 @@ __global__ void __launch_bounds__(kBlock) k_decay_step(Rows q, Rows k, Rows v, c
       const float kr = (float)kp[r], qr = (float)qp[r];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        m[e] = fade(m[e], kr * vv[e]);
+        m[e] = fade.any(m[e], kr * vv[e]);
         acc[e] = fmaf(qr, m[e], acc[e]);
       }
       store_f<V>(M + r * D + c, m);

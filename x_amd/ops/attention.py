@@ -245,7 +245,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: tor
     [0, N], which is not checked on the device (no call reads past its tensors if it does not).  Tokens outside of it are in
     no window: zeros, and zero gradients.  Keys and values of fewer heads are given as ``k.unsqueeze(2).expand(...)``-like
     views; their gradients come out per head and autograd adds them.  An endless gap forgets what was before it (with a
-    positive rate), a negative one grows the state as the formula has it.  No gradient flows to rate and dt.
+    positive rate), a negative one grows the state as the formula has it.  NaN and infinities go where the formula takes them,
+    signs included, but a stretch of tokens that they reach is followed token by token, in some 20 times the time.  No
+    gradient flows to rate and dt.
 
     Products run on the matrix cores.  With 16-bit inputs the pairs' weights and the states that meet a query go in as two
     pieces of that type (16 bits of mantissa), tokens' shares of a state as three; states are kept and returned in single
