@@ -272,6 +272,40 @@ def test_attention_endless_gaps_forget():
     assert torch.equal(state[0, 0], k[0, 0, :, None] * v[0, 0, None])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [32, 64, 100, 128])
+def test_attention_rounds_outputs_on_the_right_side(dtype, D):
+    """States and pairs' weights meet an output within 2^-17 of themselves at most: next to the middle between two outputs, by 1.5
+    times that, each output is still rounded to its own side."""
+    step = torch.finfo(dtype).eps                            # between neighbours from one to two
+    odd = torch.arange(1, 2 * D, 2, device=DEV, dtype=torch.float64) * (step / 2) + 1
+    near = (odd[odd < 2][None, :] + torch.tensor([[-1.5], [1.5]], device=DEV, dtype=torch.float64) * 2.0 ** -17).flatten()
+    if dtype == F32:
+        near = 1 + torch.arange(2 * D, device=DEV, dtype=torch.float64) * step       # no pieces: the values themselves
+    n = len(near)
+    want = near.float().to(dtype)
+    assert (near.float().double() == near).all()
+    rate, start = torch.ones(1, device=DEV), torch.arange(n + 1, device=DEV)
+    zero = torch.zeros(n, 1, D, device=DEV, dtype=dtype)
+    # a state: every stream asks for its own row, next to other rows and columns of its size
+    h0 = near[:, None, None, None].expand(n, 1, D, D).float().contiguous()
+    q = zero.clone()
+    q[torch.arange(n, device=DEV), 0, torch.arange(n, device=DEV) % D] = 1
+    dt = torch.zeros(n, device=DEV)
+    y, last = ops.decay_attention(q, zero, zero, rate, start, dt=dt, h0=h0, scale=1.0)
+    assert torch.equal(last, h0) and torch.equal(y, want[:, None, None].expand(n, 1, D))
+    # a pair's weight: three products of a query and its key that add up to it, times a value of one
+    q, k, v = zero.clone(), zero.clone(), zero.clone()
+    high = torch.floor((near - 1) / step) * step + 1
+    half = torch.where(near - high > step / 4, step / 2, 0.0)
+    for c, part in enumerate((high, half, near - high - half)):
+        q[:, 0, c], k[:, 0, c] = part.to(dtype), 1
+        assert (q[:, 0, c].double() == part).all()
+    v[:, 0, 3] = 1
+    y, _ = ops.decay_attention(q, k, v, rate, start, dt=dt, scale=1.0)
+    assert torch.equal(y[:, 0, 3], want) and not y[:, 0, :3].any()
+
+
 def test_attention_without_decay_adds_up():
     ones = torch.ones(200, 1, 4, device=DEV)
     y, last = ops.decay_attention(ones, ones, ones, torch.zeros(1, device=DEV), torch.tensor([0, 200], device=DEV), scale=1.0)

@@ -101,32 +101,32 @@ __device__ __forceinline__ Frag<T> frag_col(const T* tile, int col0) {
   return f;
 }
 
-// Values in 32 bits as the sum of NS fragments of T, so that the products' sums are those of values in 24 bits (NS = 3), or
-// within 2^-16 (bfloat16, NS = 2).  Bfloat16 pieces but the last are the value's and the remainders' upper halves, cut
-// off: a mask and a subtraction, and one instruction that packs two.  Rounded pieces would need a conversion there and back.
-__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
+// Values in 32 bits as the sum of NS fragments of T, each piece the rounded rest of those before: three hold a value's 24 bits, two
+// the value within 2^-17 (bfloat16) or 2^-22 (half precision), a 256th of the output's own rounding or less.  The weights of
+// tokens in a state go in as three, since states are kept and handed on; the states and pairs' weights that meet a row's
+// output as two.  Three there take 2% more of the time at 32 channels, 7% at 64 and 10% at 128 (forward + backward: 1M x 2 x 32
+// 605 -> 619 us, 256 windows of 400 x 4 x 64 366 -> 397, 65k x 8 x 128 962 -> 1057); bfloat16 outputs are then 3.8e-5 instead of
+// 9.5e-5 from those of a plain form in single precision, and either way 1.66e-3 from the values before they are rounded,
+// as the plain form's own are.
 template <typename T, int NS>
 __device__ __forceinline__ void split(const float (&v)[8], Frag<T> (&f)[NS]) {
   if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[0][k] = v[k];
-  } else if constexpr (std::is_same<T, bf16_t>::value) {
+  } else if constexpr (std::is_same<T, bf16_t>::value) {     // two values an instruction, there and back
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = v[k];
 #pragma unroll
-    for (int s = 0; s + 1 < NS; ++s) {
+    for (int s = 0; s < NS; ++s) {
       union { uint32_t w[4]; Frag<T> f; } u;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u.w[k] = upper_halves(x[2 * k], x[2 * k + 1]);
+      for (int k = 0; k < 8; ++k) u.f[k] = (T)x[k];
       f[s] = u.f;
+      if (s + 1 < NS)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] -= __uint_as_float(__float_as_uint(x[k]) & 0xFFFF0000u);
+        for (int k = 0; k < 8; ++k) x[k] -= __uint_as_float(k & 1 ? u.w[k / 2] & 0xFFFF0000u : u.w[k / 2] << 16);
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[NS - 1][k] = (T)x[k];
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -750,7 +750,7 @@ template <typename T, int DP, int WORK, bool REV, int LAY>
 __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<ChunkLds<T, DP, jobs_of(WORK) + 2>, DP == 32 && WORK != kSweep && LAY == kWhole ? 3 : kSweepWaves>(sweep_waves<DP, WORK>() * jobs_of(WORK))))
     k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, KD = DP / 32, THREADS = sweep_threads<T, DP, WORK>();
-  constexpr int NT = jobs_of(WORK) + 2, NS = pieces<T>(2);           // the state within 2^-16 of its values: below the outputs' own rounding
+  constexpr int NT = jobs_of(WORK) + 2, NS = pieces<T>(2);
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   __shared__ ChunkLds<T, DP, NT> s;
   const Part<DP, WORK, REV> part(d, first + blockIdx.x);
