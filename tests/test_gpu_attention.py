@@ -306,6 +306,33 @@ def test_attention_rounds_outputs_on_the_right_side(dtype, D):
     assert torch.equal(y[:, 0, 3], want) and not y[:, 0, :3].any()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [8, 32, 64, 128])
+def test_attention_of_small_channels_beside_large_ones(dtype, D):
+    """A value channel keeps its bits next to one whose states are 2^35 times as large, in outputs and in the gradients that
+    have channels of such sizes; the large ones belong to a key channel that no query asks for."""
+    N, scale = 400, D ** -0.5
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    q, k, v, gy = (torch.randn(N, 1, D, device=DEV, generator=gen) for _ in range(4))
+    v *= 2.0 ** -12
+    gy[..., 1:] *= 2.0 ** 4
+    old = torch.arange(N, device=DEV) % 2 == 0               # half of the tokens have the large values
+    k[old], v[old] = 0, 0
+    k[old, 0, 0], v[old, 0, 0] = 1, 30000
+    k[~old, 0, 0], v[~old, 0, 0], q[..., 0], gy[..., 0] = 0, 0, 0, 0
+    q, k, v, gy = (t.to(dtype) for t in (q, k, v, gy))
+    rate, start = torch.full((1,), 1 / 256, device=DEV), [0, 70, N]
+    ins = [t.requires_grad_() for t in (q, k, v)]
+    y, last = ops.decay_attention(*ins, rate, torch.tensor(start, device=DEV), scale=scale)
+    got = (y, last, *torch.autograd.grad(y, ins, gy))
+    zero = np.zeros((2, 1, D, D))
+    want, mag = O.by_token(_np(q), _np(k), _np(v), _np(rate), start, None, None, scale, _np(gy), zero)
+    units = (3 * D + 300 + 3 * (N // 32 + 1)) * 5 * O.U + O.PIECES[_name(dtype)]
+    for name, a, b, c in zip(("y", "last", "gq", "gk", "gv"), got, want, mag):
+        _close(a, b, units * c, name)
+    assert np.abs(want[0]).max() < 1 and np.abs(want[1]).max() > 2.0 ** 20
+
+
 def test_attention_without_decay_adds_up():
     ones = torch.ones(200, 1, 4, device=DEV)
     y, last = ops.decay_attention(ones, ones, ones, torch.zeros(1, device=DEV), torch.tensor([0, 200], device=DEV), scale=1.0)

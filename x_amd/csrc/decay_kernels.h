@@ -145,7 +145,8 @@ constexpr int pieces(int n) {
 }
 
 // Half precision reaches from 6e-8 to 65504 only: what goes into it is brought to a largest value of 2^14 to 2^15 first, by
-// a power of two.
+// a power of two: a state column by column, pairs' weights row by row, weighted W column by column.  What lies 2^28 below the
+// largest of its column or row keeps fewer bits than the type's own.
 struct Fit {
   float up, down;
 };
@@ -802,19 +803,17 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
     for (int it = 0; it < 2; ++it)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) far[it][ct] = F4{0.f, 0.f, 0.f, 0.f};
-    Fit fm{1.f, 1.f};
-    if (HALF) {
-      float top = 0.f;
+    Fit fm[CT];                                             // of the lane's column: small channels beside large ones keep their bits
+    if (HALF)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < CT; ++ct) {
+        float top = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) top = finite_top(top, M[ct][dt][r]);
-#pragma unroll
-      for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
-      fm = fit_of(top_of_four(top));
-    }
+        fm[ct] = fit_of(top_of_four(top));
+      }
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
       Frag<T> xf[2], sf[CT][NS];
@@ -824,7 +823,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
       for (int ct = 0; ct < CT; ++ct) {
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = HALF ? M[ct][k * 2 + (e >> 2)][e & 3] * fm.up : M[ct][k * 2 + (e >> 2)][e & 3];
+        for (int e = 0; e < 8; ++e) v[e] = HALF ? M[ct][k * 2 + (e >> 2)][e & 3] * fm[ct].up : M[ct][k * 2 + (e >> 2)][e & 3];
         split<T, NS>(v, sf[ct]);
       }
 #pragma unroll
@@ -899,7 +898,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
       const int i = it * 16 + i16;
-      const float xe = HALF ? dec.xe[i] * fm.down : dec.xe[i];
+      const float xe = dec.xe[i];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         F4 pv = {0.f, 0.f, 0.f, 0.f};
@@ -908,7 +907,8 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
         const int c = c0 + ct * 16 + g * 4;
         float o[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = fmaf(far[it][ct][r], xe, HALF ? pv[r] * fp[it].down : pv[r]);
+        for (int r = 0; r < 4; ++r)
+          o[r] = HALF ? fmaf(far[it][ct][r] * __shfl(fm[ct].down, g * 4 + r, kWave), xe, pv[r] * fp[it].down) : fmaf(far[it][ct][r], xe, pv[r]);
         if (ct == 0) check |= __ballot(!(fabsf(o[0]) < INFINITY));
         if constexpr (LAY != kLoose) {
           const uint32_t at_row = row_offset<REV>(i, out_stride, len) + c * (uint32_t)sizeof(T);

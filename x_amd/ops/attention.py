@@ -250,8 +250,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: tor
     gradient flows to rate and dt.
 
     Products run on the matrix cores.  With 16-bit inputs the pairs' weights and the states that meet a query go in as two
-    pieces of that type (within 2^-17 of themselves, a 256th of a bfloat16 output's own rounding), tokens' shares of a state as
-    three; states are kept and returned in single precision."""
+    pieces of that type (within 2^-17 of themselves, a 256th of a bfloat16 output's own rounding; in half precision less of what
+    lies 2^28 below the largest of its value channel or token), tokens' shares of a state as three; states are kept and
+    returned in single precision."""
     rate, dt, scale = _attn_args(q, k, v, rate, dt, scale)
     N, H, D = q.shape
     _on(start, "start", q.device)
