@@ -333,6 +333,52 @@ def test_attention_of_small_channels_beside_large_ones(dtype, D):
     assert np.abs(want[0]).max() < 1 and np.abs(want[1]).max() > 2.0 ** 20
 
 
+def _states(x, dtype, start, dt, scale, rate):
+    """last and gh0 of a call in a type, from h0 of zeros."""
+    q, k, v, gy = (t.to(dtype) for t in x)
+    h0 = torch.zeros(len(start) - 1, q.shape[1], q.shape[2], q.shape[2], device=DEV, requires_grad=True)
+    y, last = ops.decay_attention(q, k, v, rate, torch.tensor(start, device=DEV), dt=dt, h0=h0, scale=scale)
+    return last.detach(), torch.autograd.grad(y, h0, gy)[0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [8, 32, 64, 128])
+def test_attention_states_hold_24_bits(dtype, D):
+    """A token's share of a state is its decay's 24 bits times its key and value: with powers of two for those, and one token a
+    window that has any, states and their gradients have the bits of the single-precision call, over chunks and stretches;
+    two pieces of the type could not hold them."""
+    sizes = [1, 2, 5, 20, 33, 40, 70, 200, 300, 700, 1200, 2000]
+    start = np.concatenate([[0], np.cumsum(sizes)]).tolist()
+    N, gen = start[-1], torch.Generator(device=DEV).manual_seed(D)
+    x = torch.zeros(4, N, 2, D, device=DEV)
+    for b, n in enumerate(sizes):
+        power = lambda: 2.0 ** torch.randint(-3, 4, (2, D), device=DEV, generator=gen)
+        first, end = start[b] + n // 3, start[b + 1] - 1 - n // 3
+        x[1, first], x[2, first], x[0, end], x[3, end] = power(), power(), power(), -power()
+    dt = torch.rand(N, device=DEV, generator=gen) * 0.01
+    rate = torch.tensor([0.9, 0.11], device=DEV)
+    wide = _states(x, F32, start, dt, 0.3, rate)
+    for a, b in zip(_states(x, dtype, start, dt, 0.3, rate), wide):
+        two = b.to(dtype).float()
+        two = two + (b - two).to(dtype).float()
+        assert torch.equal(a, b) and b.any() and not torch.equal(two, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,D", [(40, 16), (300, 32), (700, 45), (700, 64), (3000, 128)])
+def test_attention_states_are_as_good_as_single_precision(dtype, N, D):
+    """last and gh0 next to the definition in 64 bits: sums of N products in 32 bits are off by some 2^-24 times a small number's
+    root (2e-7), shares in two pieces of bfloat16 by 2^-17 or a third of it (3e-6) each and so in their root mean square."""
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    q, k, v, gy = torch.randn(4, N, 1, D, device=DEV, generator=gen).to(dtype)
+    dt, rate = torch.rand(N, device=DEV, generator=gen) * 0.01, torch.ones(1, device=DEV)
+    got = _states((q, k, v, gy), dtype, [0, N], dt, 0.5, rate)
+    zero = np.zeros((1, 1, D, D))
+    want, _ = O.by_token(_np(q), _np(k), _np(v), _np(rate), [0, N], _np(dt), None, 0.5, _np(gy), zero)
+    for a, b in zip(got, (want[1], want[5])):
+        assert np.sqrt(((_np(a) - b) ** 2).mean() / (b ** 2).mean()) < 1e-6
+
+
 def test_attention_without_decay_adds_up():
     ones = torch.ones(200, 1, 4, device=DEV)
     y, last = ops.decay_attention(ones, ones, ones, torch.zeros(1, device=DEV), torch.tensor([0, 200], device=DEV), scale=1.0)
