@@ -576,8 +576,8 @@ int atl_decay_attn_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, i
                        int64_t svn, int64_t svh, int dtype, int64_t N, int64_t H, int64_t D, const float* rate,
                        const int64_t* start, int64_t B, const float* dt, const float* h0, double scale, void* y, float* last,
                        void* states, int64_t states_bytes, hipStream_t stream);
-/* Its backward from gy and glast (may be null): gq, gk, gv (N,H,D) and gh0 (B,H,D,D; may be null) written.  states: the
- * forward's; ws: as many bytes. */
+/* Its backward from gy (null where nothing was made of y: gq is zeros, and q and y have no part in the others) and glast (may
+ * be null: zeros): gq, gk, gv (N,H,D) and gh0 (B,H,D,D; may be null) written.  states: the forward's; ws: as many bytes. */
 int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, const void* v,
                        int64_t svn, int64_t svh, const void* gy, int64_t sgn, int64_t sgh, int dtype, int64_t N, int64_t H,
                        int64_t D, const float* rate, const int64_t* start, int64_t B, const float* dt, const float* h0,

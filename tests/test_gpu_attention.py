@@ -216,6 +216,34 @@ def test_attention_partial_gradients(grads, dtype):
     _case(600, 2, 24, dtype, "ragged", seed=13, grads=grads)
 
 
+@pytest.mark.parametrize("D", [8, 32, 45, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N", [0, 50, 900, 2500])
+def test_attention_gradients_of_states_alone(N, D, dtype):
+    """Where nothing was made of the outputs, their products have no part in the gradients: queries get zeros, and infinities in
+    queries and in the states that they met change no bit of the others."""
+    gen = torch.Generator(device=DEV).manual_seed(N + D)
+    q, k, v = torch.randn(3, N, 2, D, device=DEV, generator=gen).to(dtype)
+    h0, gl = torch.randn(2, 3, 2, D, D, device=DEV, generator=gen)
+    rate, start = torch.tensor([0.01, 0.001], device=DEV), torch.tensor([N // 5, N // 5, N // 2, N], device=DEV)
+    print(f"gradients of states alone N={N} D={D} {dtype}", flush=True)
+
+    def go(q, h0):
+        ins = [t.clone().requires_grad_() for t in (q, k, v, h0)]
+        return torch.autograd.grad(ops.decay_attention(*ins[:3], rate, start, h0=ins[3])[1], ins, gl)
+
+    clean = go(q, h0)
+    assert not clean[0].any()
+    zeros = [t.clone().requires_grad_() for t in (q, k, v, h0)]
+    y, last = ops.decay_attention(*zeros[:3], rate, start, h0=zeros[3])
+    for a, b in zip(torch.autograd.grad((y, last), zeros, (torch.zeros_like(y), gl)), clean):
+        assert torch.equal(a, b)                             # finite inputs: as with a gradient of zeros
+    if N:
+        q, h0 = q.clone(), h0.clone()
+        q[N - N // 3, 0, D - 1], h0[1, 1, 0, D // 2], h0[2, 0, 0, 0] = float("inf"), float("-inf"), float("nan")
+        assert all(torch.equal(a, b) for a, b in zip(go(q, h0), clean))
+
+
 @pytest.mark.parametrize("gap", [1e-6, 1.0, 1e4])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_gaps(gap, dtype):

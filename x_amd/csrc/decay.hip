@@ -87,9 +87,9 @@ int atl_decay_attn_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, i
                        const float* glast, double scale, const void* states, void* gq, void* gk, void* gv, float* gh0, void* ws,
                        int64_t ws_bytes, hipStream_t stream) {
   Rows rq{q, sqn, sqh}, rk{k, skn, skh}, rv{v, svn, svh}, rg{gy, sgn, sgh};
-  if (!decay_ok(dtype, N, B, H, D) || (N > 0 && !(strides_ok(rq, N, D) && strides_ok(rk, N, D) && strides_ok(rv, N, D) && strides_ok(rg, N, D)))) { set_error("decay_attn_bwd: bad sizes N=%lld B=%lld H=%lld D=%lld type %d", (long long)N, (long long)B, (long long)H, (long long)D, dtype); return 1; }
+  if (!decay_ok(dtype, N, B, H, D) || (N > 0 && !(strides_ok(rq, N, D) && strides_ok(rk, N, D) && strides_ok(rv, N, D) && (!gy || strides_ok(rg, N, D))))) { set_error("decay_attn_bwd: bad sizes N=%lld B=%lld H=%lld D=%lld type %d", (long long)N, (long long)B, (long long)H, (long long)D, dtype); return 1; }
   const int64_t need = atl_decay_attn_states_bytes(N, B, H, D);
-  if (!start || !rate || (N > 0 && (!q || !k || !v || !gy || !gq || !gk || !gv)) || (need && (!states || !ws))) { set_error("decay_attn_bwd: null argument"); return 1; }
+  if (!start || !rate || (N > 0 && (!q || !k || !v || !gq || !gk || !gv)) || (need && (!states || !ws))) { set_error("decay_attn_bwd: null argument"); return 1; }
   if (ws_bytes < need) { set_error("decay_attn_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need); return 1; }
   const DecayGeo d = decay_geo(N, B, H, D, start, dt, rate);
   const DecayBwd a{rq, rk, rv, rg, h0, glast, (float)scale, gq, gk, gv, gh0, states, ws, decay_span_bytes(N, B, H, D)};

@@ -1203,12 +1203,30 @@ void run_fwd(const DecayGeo& d, const DecayFwd& a, hipStream_t stream) {
   run_sweep<T, kSweep, false>(d, Sweep{{a.q, a.k, a.v}, {a.y}, carry, spans, a.h0, a.last, 0, a.scale, a.scale, 1.f}, stream);
 }
 template <typename T>
-void run_bwd(const DecayGeo& d, const DecayBwd& a, hipStream_t stream) {
+__global__ void __launch_bounds__(kBlock) k_decay_zeros(T* __restrict__ p, int64_t n, int64_t first) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t at = ((first + blockIdx.x) * kBlock + threadIdx.x) * V;
+  const float zeros[V] = {};
+  store_loose<V>(p + at, n - at, zeros);
+}
+
+template <typename T>
+void run_bwd(const DecayGeo& d, DecayBwd a, hipStream_t stream) {
   Span* own = (Span*)a.ws;
   float* carry = (float*)((char*)a.ws + a.span_bytes);
+  const bool of_states = !a.gy.p;                          // alone: no query has met anything, so gq is zero, and stands for both
+  if (of_states) {
+    const int64_t n = d.N * d.H * d.D, each = kBlock * 16 / (int64_t)sizeof(T);
+    in_launches((n + each - 1) / each, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL((k_decay_zeros<T>), dim3(count), dim3(kBlock), 0, stream, (T*)a.gq, n, first);
+    });
+    a.q = a.gy = Rows{a.gq, (int64_t)d.H * d.D, d.D};
+  }
   const Sweep dq{{a.gy, a.v, a.k, a.q}, {a.gq}, (const float*)((const char*)a.states + a.span_bytes), (const Span*)a.states, a.h0, nullptr,
                  1, a.scale, a.scale, 1.f, carry, own};
-  if (d.D <= 32 && d.N > d.L) {                            // (a window of more than one stretch may be there)
+  if (of_states) {
+    run_local<T, true>(d, a.q, a.gy, a.scale, own, carry, stream);
+  } else if (d.D <= 32 && d.N > d.L) {                     // (a window of more than one stretch may be there)
     run_sweep<T, kSweepAndSums, false>(d, dq, stream);
   } else {
     run_local<T, true>(d, a.q, a.gy, a.scale, own, carry, stream);

@@ -191,7 +191,7 @@ class _Decay(torch.autograd.Function):
             return (None,) * 8
         N, H, D = q.shape
         B, dev = start.numel() - 1, q.device
-        gy = torch.zeros(N, H, D, dtype=q.dtype, device=dev) if gy is None else _chunks(gy)
+        gy = None if gy is None else _chunks(gy)
         glast = None if glast is None else glast.contiguous()
         gq, gk, gv = (torch.empty(N, H, D, dtype=q.dtype, device=dev) for _ in range(3))
         gh0 = torch.empty(B, H, D, D, dtype=F32, device=dev) if ctx.needs_input_grad[6] else None
