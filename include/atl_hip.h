@@ -550,10 +550,10 @@ int atl_gated_scan_step(const void* x, int64_t sx, const void* gate, int64_t sg,
 
 /* x / sqrt(mean_D(x^2) + eps) * w of every head of q (N,H,D) and k (N,Hk,D) (wq, wk (D) single precision; null: no norm),
  * then channel pairs (2p, 2p+1) turned by pos[n, a] * freqs[p], a the axis of p: sections (A, host memory) holds the pairs
- * of each axis, in order; channels past them are not turned.  pos (N,A) in double precision if pos64, else single.  yq
- * (N,H,D), yk (N,Hk,D) written.  D <= 256, A <= 4. */
+ * of each axis, in order; channels past them are not turned.  pos (N,A) and freqs in single precision, or in double: pos where
+ * doubles has 1, freqs where it has 2.  yq (N,H,D), yk (N,Hk,D) written.  D <= 256, A <= 4. */
 int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
-                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const float* wq, const float* wk, const void* pos, int doubles, const void* freqs, int64_t A,
                              const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, void* yq,
                              void* yk, hipStream_t stream);
 /* Its backward from gyq, gyk (either may be null: zeros): gq, gk and gw (2,D: the weights' gradients, queries' first)
@@ -561,7 +561,7 @@ int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void
  * sizes unsupported). */
 int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t H, int64_t Hk, int64_t D);
 int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
-                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const float* wq, const float* wk, const void* pos, int doubles, const void* freqs, int64_t A,
                              const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, const void* gyq,
                              int64_t sgqn, int64_t sgqh, const void* gyk, int64_t sgkn, int64_t sgkh, void* gq, void* gk,
                              float* gw, void* ws, int64_t ws_bytes, hipStream_t stream);

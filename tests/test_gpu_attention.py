@@ -774,6 +774,25 @@ def test_rotary_of_far_positions(far, pos_type):
     _rotary_case(60, 2, 2, 16, (3, 5), F32, seed=9, pos_type=pos_type, far=far)
 
 
+@pytest.mark.parametrize("pos_type", [F32, torch.float64, torch.int64])
+@pytest.mark.parametrize("freq_type", [F32, torch.float64, BF16])
+def test_rotary_frequency_types(pos_type, freq_type):
+    """Frequencies are taken as they are given: at a position of 2^24 one in 64 bits would be off by half a radian in 32."""
+    N, H, D = 40, 2, 12
+    gen = torch.Generator().manual_seed(3)
+    q, k, gq, gk = (torch.randn(N, H, D, generator=gen).to(DEV) for _ in range(4))
+    pos = (torch.rand(N, 2, generator=gen, dtype=torch.float64) * 2 ** 24).floor().to(pos_type).to(DEV)
+    fr = torch.rand(6, generator=gen, dtype=torch.float64).to(freq_type).to(DEV)
+    ins = [t.requires_grad_() for t in (q, k)]
+    got = ops.head_norm_rotary(*ins, None, None, pos, fr, (2, 4))
+    grads = torch.autograd.grad(got, ins, (gq, gk))
+    angle = O.angles(_np(pos), _np(fr), (2, 4))
+    for x, g, y, gx in zip((q, k), (gq, gk), got, grads):
+        _close(y, *O.rotary(_np(x), None, angle, 0.0), "y")
+        (want, _), (bound, _) = O.rotary_bwd(_np(x), None, angle, 0.0, _np(g))
+        _close(gx, want, bound, "gx")
+
+
 def test_rotary_of_zeros_and_bad_rows():
     """A row of zeros stays zero; a NaN or an infinity in a head or a position leaves the others alone."""
     N, D = 40, 16

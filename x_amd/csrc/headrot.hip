@@ -37,8 +37,8 @@ struct RotGeo {
   int H, Hk, D, A, pairs;             // heads of the queries and keys, channels, axes, turned pairs
   int bound[kMaxAxes];                // first pair behind each axis
   const void* pos;                    // (N, A)
-  int pos64;                          // in double precision
-  const float* freq;
+  int doubles;                        // 1: pos is in double precision, 2: freq is
+  const void* freq;
   float eps, inv_d;
   int cl2, per, blocks_of;            // log2 of a row's lanes, heads of an item, items of a token
 };
@@ -55,8 +55,9 @@ __device__ __forceinline__ void angles(const RotGeo& g, int64_t n, int c, float 
 #pragma unroll
     for (int k = 0; k < kMaxAxes - 1; ++k) a += k < g.A - 1 && p >= g.bound[k];
     const int64_t at = n * g.A + a;
-    const double x = g.pos64 ? ((const double*)g.pos)[at] : (double)((const float*)g.pos)[at];
-    const double turns = x * ((double)g.freq[p] * 0.15915494309189535);
+    const double x = g.doubles & 1 ? ((const double*)g.pos)[at] : (double)((const float*)g.pos)[at];
+    const double f = g.doubles & 2 ? ((const double*)g.freq)[p] : (double)((const float*)g.freq)[p];
+    const double turns = x * (f * 0.15915494309189535);
     const float t = (float)(turns - rint(turns));
     co[m] = __builtin_amdgcn_cosf(t), si[m] = __builtin_amdgcn_sinf(t);
   }
@@ -256,11 +257,11 @@ bool rot_ok(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t A, c
   return 2 * pairs <= D;
 }
 
-RotGeo rot_geo(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, const void* pos, int pos64, const float* freq, int64_t A,
+RotGeo rot_geo(int dtype, int64_t N, int64_t H, int64_t Hk, int64_t D, const void* pos, int doubles, const void* freq, int64_t A,
                const int64_t* sections, double eps) {
   RotGeo g{};
   g.N = N; g.H = (int)H; g.Hk = (int)Hk; g.D = (int)D; g.A = (int)A;
-  g.pos = pos; g.pos64 = pos64; g.freq = freq;
+  g.pos = pos; g.doubles = doubles; g.freq = freq;
   g.eps = (float)eps;
   g.inv_d = 1.f / (float)D;
   for (int a = 0; a < (int)A; ++a) g.bound[a] = g.pairs += (int)sections[a];
@@ -299,12 +300,12 @@ using namespace atlhip;
 extern "C" {
 
 int atl_head_norm_rotary_fwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
-                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const float* wq, const float* wk, const void* pos, int doubles, const void* freqs, int64_t A,
                              const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, void* yq,
                              void* yk, hipStream_t stream) {
   if (!rot_ok(dtype, N, H, Hk, D, A, sections, eps) || (N > 0 && (sqn < 0 || sqh < 0 || skn < 0 || skh < 0))) { set_error("head_norm_rotary_fwd: bad sizes or settings N=%lld H=%lld, %lld D=%lld axes=%lld type %d eps=%g", (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)A, dtype, eps); return 1; }
   if (N == 0) return 0;
-  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, pos64, freqs, A, sections, eps);
+  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, doubles, freqs, A, sections, eps);
   if (!q || !k || !yq || !yk || (g.pairs && (!pos || !freqs))) { set_error("head_norm_rotary_fwd: null argument"); return 1; }
   const bool whole = rot_whole(dtype, D, sqn | sqh | skn | skh, {q, k, wq, wk, yq, yk});
   const HeadRows rq{q, sqn, sqh}, rk{k, skn, skh};
@@ -327,12 +328,12 @@ int64_t atl_head_norm_rotary_bwd_ws_bytes(int64_t H, int64_t Hk, int64_t D) {
 }
 
 int atl_head_norm_rotary_bwd(const void* q, int64_t sqn, int64_t sqh, const void* k, int64_t skn, int64_t skh, int dtype,
-                             const float* wq, const float* wk, const void* pos, int pos64, const float* freqs, int64_t A,
+                             const float* wq, const float* wk, const void* pos, int doubles, const void* freqs, int64_t A,
                              const int64_t* sections, int64_t N, int64_t H, int64_t Hk, int64_t D, double eps, const void* gyq,
                              int64_t sgqn, int64_t sgqh, const void* gyk, int64_t sgkn, int64_t sgkh, void* gq, void* gk,
                              float* gw, void* ws, int64_t ws_bytes, hipStream_t stream) {
   if (!rot_ok(dtype, N, H, Hk, D, A, sections, eps) || (N > 0 && (sqn < 0 || sqh < 0 || skn < 0 || skh < 0 || sgqn < 0 || sgqh < 0 || sgkn < 0 || sgkh < 0))) { set_error("head_norm_rotary_bwd: bad sizes or settings N=%lld H=%lld, %lld D=%lld axes=%lld type %d eps=%g", (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)A, dtype, eps); return 1; }
-  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, pos64, freqs, A, sections, eps);
+  const RotGeo g = rot_geo(dtype, N, H, Hk, D, pos, doubles, freqs, A, sections, eps);
   if ((N > 0 && ((wq && !q) || (wk && !k) || (g.pairs && (!pos || !freqs)))) || (gw && !ws)) { set_error("head_norm_rotary_bwd: null argument"); return 1; }
   if (gw && ws_bytes < atl_head_norm_rotary_bwd_ws_bytes(H, Hk, D)) { set_error("head_norm_rotary_bwd: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)atl_head_norm_rotary_bwd_ws_bytes(H, Hk, D)); return 1; }
   const bool whole = rot_whole(dtype, D, (wq ? sqn | sqh : 0) | (wk ? skn | skh : 0) | (gyq ? sgqn | sgqh : 0) | (gyk ? sgkn | sgkh : 0),

@@ -64,6 +64,10 @@ def _sections(sections: tuple):
     return (ctypes.c_int64 * len(sections))(*sections)
 
 
+def _doubles(pos, freqs) -> int:
+    return (pos.dtype == torch.float64) + 2 * (freqs.dtype == torch.float64)
+
+
 def _rotary_fwd(q, k, wq, wk, pos, freqs, sections, eps):
     N, H, D = q.shape
     Hk, dev = k.shape[1], q.device
@@ -71,7 +75,7 @@ def _rotary_fwd(q, k, wq, wk, pos, freqs, sections, eps):
     yk = torch.empty(N, Hk, D, dtype=q.dtype, device=dev)
     with on_device(dev):
         call("atl_head_norm_rotary_fwd", *_strides(q), *_strides(k), _CODE[q.dtype], _at(wq), _at(wk), _at(pos),
-             int(pos.dtype == torch.float64), _at(freqs), len(sections), _sections(sections), N, H, Hk, D, eps, _at(yq), _at(yk),
+             _doubles(pos, freqs), _at(freqs), len(sections), _sections(sections), N, H, Hk, D, eps, _at(yq), _at(yk),
              raw_stream(dev))
     return yq, yk
 
@@ -101,7 +105,7 @@ class _Rotary(torch.autograd.Function):
         ws = _ws(nbytes, dev, "head_norm_rotary") if gw is not None else None
         with on_device(dev):
             call("atl_head_norm_rotary_bwd", *_strides(q), *_strides(k), _CODE[dtype], _at(wq), _at(wk), _at(pos),
-                 int(pos.dtype == torch.float64), _at(freqs), len(sections), _sections(sections), N, H, Hk, D, eps,
+                 _doubles(pos, freqs), _at(freqs), len(sections), _sections(sections), N, H, Hk, D, eps,
                  *_strides(gyq), *_strides(gyk), _at(gq), _at(gk), _at(gw), _at(ws), nbytes, raw_stream(dev))
         gwq = gw[0] if want[2] and gyq is not None else None
         gwk = gw[1] if want[3] and gyk is not None else None
@@ -116,7 +120,7 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | 
     ``pos`` (N, A) holds every token's position on up to four axes (time, row and column of an event; float32 or float64,
     integers are taken as float64), ``sections`` how many pairs turn with each axis, in order; channels past the last
     section's stay as the norm leaves them.  The product with a query of a key so turned depends on their distance along
-    every axis alone.  Angles are reduced in 64 bits, so far positions keep them.  Weights (D,), both None: no norm, the
+    every axis alone.  Angles are reduced in 64 bits, of float64 frequencies too, so far positions keep them.  Weights (D,), both None: no norm, the
     rotation alone.  Up to 256 channels; the outputs are contiguous.  No gradient flows to pos and freqs."""
     _head_args(q, "q", width=MAX_ROTARY_WIDTH)
     _head_args(k, "k", like=q)
@@ -152,7 +156,7 @@ def head_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | 
     pos = _plain(pos, F32 if pos.dtype in (F32, torch.float16, torch.bfloat16) else torch.float64)
     if through is None:
         return ref.head_norm_rotary(q, k, q_weight, k_weight, pos, freqs, sections, eps)
-    freqs = _plain(freqs, F32)
+    freqs = _plain(freqs, F32 if freqs.dtype in (F32, torch.float16, torch.bfloat16) else torch.float64)
     wq, wk = (None if w is None else _plain(w, F32) for w in (q_weight, k_weight))
     q, k = _heads(q), _heads(k)
     if through or _grads_wanted(q, k, wq, wk):
