@@ -437,6 +437,31 @@ def test_attention_of_shared_heads():
     assert torch.equal(y, ops.decay_attention(q, one[0].contiguous(), one[1].contiguous(), rate, start)[0])
 
 
+@pytest.mark.parametrize("Hk", [1, 2, 3])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_of_fewer_key_heads_as_documented(Hk, dtype):
+    """Keys and values of one head as views, of more as copies, behind a rotation that has Hk heads of keys: the results of
+    full heads, and gradients that are their sums."""
+    N, H, D = 300, 6, 32
+    gen = torch.Generator(device=DEV).manual_seed(Hk)
+    q, gy = torch.randn(2, N, H, D, device=DEV, generator=gen).to(dtype)
+    kv = torch.randn(2, N, Hk, D, device=DEV, generator=gen).to(dtype)
+    rate, start = torch.rand(H, device=DEV, generator=gen), torch.tensor([0, 100, N], device=DEV)
+    pos, fr = torch.rand(N, 1, device=DEV, generator=gen), torch.rand(8, device=DEV, generator=gen)
+    k, v = (t.clone().requires_grad_() for t in kv)
+    wide = (lambda t: t.expand(N, H, D)) if Hk == 1 else (lambda t: t.repeat_interleave(H // Hk, 1))
+    qr, kr = ops.head_norm_rotary(q, k, None, None, pos, fr, (8,))
+    y, last = ops.decay_attention(qr, wide(kr), wide(v), rate, start)
+    full = [t.detach().repeat_interleave(H // Hk, 1).requires_grad_() for t in (kr, v)]
+    y1, last1 = ops.decay_attention(qr, *full, rate, start)
+    assert torch.equal(y, y1) and torch.equal(last, last1)
+    got, per_head = torch.autograd.grad(y, (kr, v), gy, retain_graph=True), torch.autograd.grad(y1, full, gy)
+    for a, b in zip(got, per_head):                          # sums of H / Hk numbers, rounded to the type at most that often
+        parts = b.view(N, Hk, H // Hk, D).double()
+        assert ((a.double() - parts.sum(2)).abs() <= H // Hk * torch.finfo(dtype).eps / 2 * parts.abs().sum(2)).all()
+    assert all(g.any() for g in torch.autograd.grad(y, (k, v), gy))
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("which", ["q", "k", "v"])

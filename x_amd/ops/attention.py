@@ -35,8 +35,8 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 
 
 def _chunks(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (N, H, D) as the attention over windows takes it: contiguous heads, tokens that lie apart but within reach of the
-    32-bit offsets of 64 of them; else a copy."""
+    """``t`` (N, H, D) as the attention over windows takes it: contiguous heads, tokens that lie apart but within reach of a
+    chunk's 32-bit offsets (32 tokens); else a copy."""
     t = _heads(t)
     return t if t.shape[0] < 2 or t.shape[2] <= t.stride(0) < MAX_TOKEN_STRIDE else t.contiguous()
 
@@ -247,8 +247,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: tor
 
     ``start`` (B + 1) holds the windows' first tokens and the last one's end (``EventPacket.offsets``); it must ascend within
     [0, N], which is not checked on the device (no call reads past its tensors if it does not).  Tokens outside of it are in
-    no window: zeros, and zero gradients.  Keys and values of fewer heads are given as ``k.unsqueeze(2).expand(...)``-like
-    views; their gradients come out per head and autograd adds them.  An endless gap forgets what was before it (with a
+    no window: zeros, and zero gradients.  A key and a value that all heads share are given as views, ``k.expand(N, H, D)``
+    of (N, 1, D), which are read as they lie; those of Hk < H heads as copies, ``k.repeat_interleave(H // Hk, 1)``.  Their
+    gradients come out per head, each rounded to their type, and autograd adds them.  An endless gap forgets what was before it (with a
     positive rate), a negative one grows the state as the formula has it.  NaN and infinities go where the formula takes them,
     signs included, but a stretch of tokens that they reach is followed token by token, in some 20 times the time.  No
     gradient flows to rate and dt.
