@@ -747,8 +747,17 @@ struct Part {
   }
 };
 
+// Waves a SIMD that a sweep is to leave registers for.  Two jobs at 32 channels fit into three waves' registers; 128 channels of
+// bfloat16 in loose rows (odd widths) not into two waves': with one, 65k x 8 x 127 forward + backward take 3.12 ms instead of
+// 3.50; in float16 3.61 instead of 3.41, so there two it is.
+template <typename T, int DP, int WORK, int LAY>
+constexpr int wanted_waves() {
+  if (DP == 32 && WORK != kSweep && LAY == kWhole) return 3;
+  return DP == 128 && LAY == kLoose && std::is_same<T, bf16_t>::value ? 1 : kSweepWaves;
+}
+
 template <typename T, int DP, int WORK, bool REV, int LAY>
-__global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<ChunkLds<T, DP, jobs_of(WORK) + 2>, DP == 32 && WORK != kSweep && LAY == kWhole ? 3 : kSweepWaves>(sweep_waves<DP, WORK>() * jobs_of(WORK))))
+__global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<ChunkLds<T, DP, jobs_of(WORK) + 2>, (wanted_waves<T, DP, WORK, LAY>())>(sweep_waves<DP, WORK>() * jobs_of(WORK))))
     k_decay_sweep(DecayGeo d, Sweep a, int64_t first) {
   constexpr int LD = tile_ld<T, DP>(), DT = DP / 16, CT = kTiles, KD = DP / 32, THREADS = sweep_threads<T, DP, WORK>();
   constexpr int NT = jobs_of(WORK) + 2, NS = pieces<T>(2);
@@ -894,6 +903,8 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
     add_chunk<T, DP, CT>(dec.we, dec.fade, 1.f, Y, M, wf);
     __builtin_amdgcn_sched_barrier(0);
     T* to = out + ((REV ? from - done : from + done) * d.H + head) * d.D;
+    int from_lane = g * 4;
+    if (HALF) asm volatile("" : "+v"(from_lane));           // (the shuffles' addresses, kept over the loop, would take registers)
     const auto out_buf = chunk_buffer<REV>(to, out_stride, len, d.D * (int)sizeof(T));
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
@@ -908,7 +919,7 @@ __global__ void __launch_bounds__((sweep_threads<T, DP, WORK>()), (waves_of<Chun
         float o[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          o[r] = HALF ? fmaf(far[it][ct][r] * __shfl(fm[ct].down, g * 4 + r, kWave), xe, pv[r] * fp[it].down) : fmaf(far[it][ct][r], xe, pv[r]);
+          o[r] = HALF ? fmaf(far[it][ct][r] * __shfl(fm[ct].down, from_lane + r, kWave), xe, pv[r] * fp[it].down) : fmaf(far[it][ct][r], xe, pv[r]);
         if (ct == 0) check |= __ballot(!(fabsf(o[0]) < INFINITY));
         if constexpr (LAY != kLoose) {
           const uint32_t at_row = row_offset<REV>(i, out_stride, len) + c * (uint32_t)sizeof(T);
