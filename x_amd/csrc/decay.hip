@@ -12,11 +12,16 @@ constexpr int64_t kMaxStride = (int64_t)1 << 22;
 
 // Tokens of a stretch: whole pairs of chunks, four pairs at least.  The stretches of all heads, and half a stretch for every
 // window's last, are whole rounds of workgroups: past 64 channels two rounds of two a compute unit (four waves each, two a
-// SIMD), past 32 two rounds of four, up to 32 one and a half a SIMD, all at once.  In microseconds, forward + backward in
-// bfloat16, by their number:
-//   65k x 8 x 128   512: 1195   768: 942   1024: 951   1536: 1010   2048: 1089
-//   180k x 6 x 64                          1024: 813   1800: 717    2048: 711    2200: 785
-//   1M x 2 x 32                 768: 657   1100: 643   1536: 572    1700: 676    2048: 648
+// SIMD), past 32 two rounds of four, up to 32 one and a half a SIMD, all at once.  Chosen by bfloat16 cases; microseconds,
+// forward + backward, by their number:
+//   65k x 8 x 128   512: 1195   768: 942   1024: 951                 180k x 6 x 64   1024: 813   2048: 711   2900: 787
+//   30k x 16 x 128  512: 1059   768: 978   1024: 902                 102k x 4 x 64   1024: 422   2048: 361   2900: 364
+//   1M x 2 x 32     768: 657   1536: 572   2048: 648                 400k x 4 x 32    768: 640   1536: 509   2048: 554
+// The rule counts workgroups, not the states that stretches write, join and read, and so is off where there are few windows
+// of wide heads, and in other types:
+//   100k x 4 x 128, 3 windows           512: 695   1024: 826         250k x 4 x 64, 1 window        1024: 672   2048: 706
+//   40k x 6 x 100, float32              512: 1158  1024: 1238        251k x 3 x 45, float32         1024: 1100  2048: 1131
+//   90k x 8 x 96, float16               512: 1634  1024: 1687        100k x 8 x 32, float32         1536: 539   2048: 498
 int64_t stretch_len(int64_t N, int64_t B, int64_t H, int64_t D) {
   constexpr int64_t kPair = 64;
   const int64_t groups = D <= 32 ? 1536 : D <= 64 ? 2048 : 1024;

@@ -19,9 +19,9 @@
 // of one stretch need neither, and both return at once there.  Training so moves 18 tensors' worth of rows where 8 would do, each once
 // (forward 2 + 4, backward 2 + 4 + 6; 17 with heads of 32 channels, where the backward pass's own sums share a sweep).  What
 // bounds it: heads of 32 channels, memory (1M tokens x 2 x 32 in bfloat16: the sweeps move 3.7 to 4.1 TB/s, forward and backward
-// take 600 us); wider ones the vector instructions around the products and their latency at two waves a SIMD, whose
-// registers hold the states (65k x 8 x 128: a forward sweep's 207 us hold 91 us of vector and 41 of matrix instructions, and
-// 105 us of memory); single precision its matrix instructions (251k x 3 x 45: 1140 us).
+// take 605 us); wider ones the vector instructions around the products and their latency at two waves a SIMD, whose
+// registers hold the states (65k x 8 x 128: a forward sweep takes 215 to 228 us; its vector instructions' issue is 78, its matrix
+// instructions' 43 and its traffic at a copy's rate 105); single precision its matrix instructions (251k x 3 x 45: 1140 us).
 #pragma once
 #include "decay.h"
 
@@ -242,7 +242,7 @@ __device__ __forceinline__ int64_t near_first(int64_t block, int64_t blocks) {
 
 // ------------------------------------------------------------------------------------------- a chunk
 template <typename T, int DP>
-constexpr int tile_ld() { return DP + 16 / (int)sizeof(T); }                // rows a vector apart: no bank conflicts
+constexpr int tile_ld() { return DP + 16 / (int)sizeof(T); }                // rows a vector apart (bank conflicts: 32 to 54% of LDS cycles)
 
 // The exponents E_i of a chunk (in powers of two) and the factors made of them.  A pair's factor e^{-(E_i - E_j)} is taken from
 // the exponents inside a block of 16 rows, and between the two blocks as row_i col_j, from and to the first block's last
@@ -619,7 +619,8 @@ constexpr int waves_of(int waves) {
 // end, sum_i e^{-E_i} q_i gy_i^T, which those two begin with (the rows of gy are there already).  That one is for heads of one
 // tile of 32 channels: forward + backward of 1M tokens x 2 x 32 took 631 us with a pass over q and gy for those sums and 599
 // with them beside dq; 102k x 4 x 64 took 370 and 383, 65k x 8 x 128 1069 and 1113, 251k x 3 x 45 in float32 1191 and 1220:
-// the sums' waves have a third of the others' work and hold as many registers.
+// the sums' waves have a third of the others' work and hold as many registers.  (Heads of up to 32 channels in float32 and
+// float16 were not measured apart.)
 enum Work : int { kSweep = 0, kSweepPair = 1, kSweepAndSums = 2 };
 struct Sweep {
   Rows rows[4];

@@ -12,9 +12,11 @@
 // million with a frequency near one keeps its angle.  The hardware's sine and cosine take turns, and are off by 1.3e-7 at
 // most over the half turn (measured on 2^23 angles).  They are those of all the token's heads, so a group of lanes that
 // holds a row (16 bytes a lane) goes through several heads with them.  Bound by memory (a read and a write of the rows
-// forward, two reads and a write backward) and, where rows are short, by the angles: a token's are as much work for few
-// heads as for many.  100k tokens x (8 + 2) heads of 128 in float16 take 114 us forward, 4.5 TB/s; 1M x (2 + 2) heads of 32 in
-// bfloat16 124 us forward and 210 us backward (4.2 and 3.7 TB/s); 60k x (5 + 5) of 46 in float32 80 and 113 us.
+// forward, two reads and a write backward): 100k tokens x (8 + 2) heads of 128 in float16 take 114 us forward, 4.5 TB/s; 1M x
+// (2 + 2) heads of 32 in bfloat16 126 us forward and 215 us backward (4.1 and 3.6 TB/s), of which the vector instructions'
+// issue is 61 and 88.  Rows off 16 bytes wait longer: 60k x (5 + 5) of 46 in float32 take 74 and 114 us, of which issue, angles
+// of three axes among it, is 21 and 30; a row's last piece is read element by element, and 12 lanes of 16 have one (of 48
+// channels, from the cache, 41 us forward instead of 47).
 #include "shares.h"
 #include "typed.h"
 #include "../../include/atl_hip.h"
