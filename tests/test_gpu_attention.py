@@ -955,6 +955,40 @@ def test_operators_in_a_graph():
             assert all(torch.equal(a, b) for a, b in zip(out, want)), r
 
 
+def test_gradients_of_states_alone_in_a_graph():
+    """The zeros that stand for a gradient of y are made in every replay, also where infinities come and go between them."""
+    N, H, D = 1500, 2, 32
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    q, k, v = (torch.randn(N, H, D, device=DEV, generator=gen).to(BF16).requires_grad_() for _ in range(3))
+    gl, rate = torch.randn(1, H, D, D, device=DEV, generator=gen), torch.full((H,), 0.01, device=DEV)
+    start = torch.tensor([0, N], device=DEV)
+
+    def step():
+        last = ops.decay_attention(q, k, v, rate, start)[1]
+        return last, *torch.autograd.grad(last, (q, k, v), gl)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for r in range(4):
+        with torch.no_grad():
+            k.normal_(), v.normal_()
+            q[100 * r] = float("inf") if r % 2 else 1.0
+            v[700, 0, 3] = float("inf") if r == 2 else 0.5
+        want = step()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) or (a.isnan() == b.isnan()).all() and torch.equal(a.nan_to_num(), b.nan_to_num())
+                   for a, b in zip(out, want)), r
+        assert not out[1].any()
+
+
 def test_step_in_a_graph():
     """A recorded step follows its state from replay to replay."""
     N, H, D = 40, 2, 32
